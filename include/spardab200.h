@@ -402,6 +402,99 @@ SD_API int sd_decode_layer_offload(const void *qkv, int dtype, int64_t qkv_sb, c
                                    const float *cand_val, const int32_t *cand_slot, int32_t *sel_out,
                                    int32_t *cnt_out, int sel_cap, int32_t *err, void *stream);
 
+/* ---- ragged batches: packed prompts, paged caches, token scores ----
+ * Sequences of different lengths: prompts packed back to back into one row of
+ * tokens, and caches of pages that are scattered over a pool.  The reference
+ * runs batches of one length (model/attention/base.py:11-32,
+ * model/attention/dense.py); these are the same causal attention and loss
+ * without its padding.  Head size 64, as everywhere in this library.  Tensors
+ * of one call share a dtype, have 16-byte aligned rows and strides that are
+ * multiples of 16 bytes.  Lengths, bounds and page tables live on the device;
+ * every access is checked against the tensors' sizes there, so a malformed one
+ * gives wrong rows and, where noted, SD_KERR_BOUNDS in *err, never a fault. */
+
+/* Causal grouped-query attention of packed sequences.  q [total,Hq,64], k and
+ * v [total,Hkv,64]; sequence s holds the rows cu_seqlens[s] .. cu_seqlens[s+1]
+ * - 1 (device int32 [nseq + 1], ascending, within 0..total).  out [total,Hq,64]
+ * = softmax(scale q k^T over the sequence's tokens up to the query's own) v.
+ * Rows outside every sequence: zeros with zero_rest, else left as they are.
+ * lse (nullable): fp32 [Hq,total], log2 of each row's sum of exponentials, for
+ * the backward.  16-bit inputs run on the tensor cores, fp32 on CUDA cores.
+ * scale > 0. */
+SD_API int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, int64_t total, int64_t Hq,
+                               int64_t Hkv, int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                               int64_t v_st, int64_t v_sh, const int32_t *cu_seqlens, int nseq, float scale,
+                               void *out, int64_t o_st, int64_t o_sh, float *lse, int zero_rest, int32_t *err,
+                               void *stream);
+
+/* Its gradients for the output gradient dout [total,Hq,64]: dq [total,Hq,64],
+ * dk and dv [total,Hkv,64], contiguous, in the inputs' dtype (dk and dv summed
+ * over the query heads of their kv head; zeros outside every sequence).  out
+ * and lse are the forward's.  delta: fp32 [Hq,total] workspace of this call.
+ * Sums have a fixed order: equal inputs give equal bits. */
+SD_API int sd_packed_attention_backward(const void *q, const void *k, const void *v, const void *out,
+                                        const void *dout, int dtype, int64_t total, int64_t Hq, int64_t Hkv,
+                                        int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                                        int64_t v_st, int64_t v_sh, int64_t o_st, int64_t o_sh, int64_t g_st,
+                                        int64_t g_sh, const int32_t *cu_seqlens, int nseq, float scale,
+                                        const float *lse, float *delta, void *dq, void *dk, void *dv, int32_t *err,
+                                        void *stream);
+
+/* Paged KV append.  k_pages, v_pages: pools of `pages` pages [page][64] per kv
+ * head with element strides (p_sp, p_sh, p_st) for (page, head, token), the
+ * same for both.  Position t of sequence b is row t % page of page
+ * table[b][t / page] (device int32 [B][width], row stride t_sb).  lens[b]
+ * (device int32): tokens cached before the call.  xk, xv: [N,Hkv,64] rows.
+ * With cu_seqlens (device int32 [B + 1]) rows cu_seqlens[b] .. of sequence b
+ * take positions lens[b], lens[b] + 1, ..; without it N == B and row b is
+ * sequence b's one new token.  lens is not changed.  A row whose position or
+ * page is out of range is dropped and SD_KERR_BOUNDS is written to *err.  Two
+ * rows that name the same place leave either one's values there. */
+SD_API int sd_paged_append(const void *xk, const void *xv, int dtype, int64_t N, int64_t Hkv, int64_t D,
+                           int64_t k_sn, int64_t k_sh, int64_t v_sn, int64_t v_sh, void *k_pages, void *v_pages,
+                           int64_t pages, int page, int64_t p_sp, int64_t p_sh, int64_t p_st, const int32_t *table,
+                           int64_t t_sb, int width, const int32_t *lens, int B, const int32_t *cu_seqlens,
+                           int32_t *err, void *stream);
+
+/* Bytes of device workspace that sd_paged_decode_attention needs (16-byte
+ * aligned, contents arbitrary; not to be shared by calls that may overlap). */
+SD_API int sd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t *bytes);
+
+/* Attention of one query row per sequence, q [B,Hq,64] (strides q_sb, q_sh),
+ * over the first lens[b] positions of its pages (layout as sd_paged_append);
+ * out [B,Hq,64] (strides o_sb, o_sh).  lens[b] == 0 gives zeros.  Pages out of
+ * range count as absent and lengths past width * page are cut, with
+ * SD_KERR_BOUNDS in *err.  The cache's length is split over the SMs and the
+ * parts are joined in a fixed order. */
+SD_API int sd_paged_decode_attention(const void *q, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                     int64_t q_sb, int64_t q_sh, const void *k_pages, const void *v_pages,
+                                     int64_t pages, int page, int64_t p_sp, int64_t p_sh, int64_t p_st,
+                                     const int32_t *table, int64_t t_sb, int width, const int32_t *lens, float scale,
+                                     void *out, int64_t o_sb, int64_t o_sh, void *workspace, int64_t workspace_bytes,
+                                     int32_t *err, void *stream);
+
+/* Log probabilities of given tokens under softmax(logits), logits [rows,V]
+ * (row stride ld): logprobs[r] = logits[r][t] - lse(logits[r]) for t =
+ * targets[r] (int64), 0 where t == ignore_index; NaN and SD_KERR_BOUNDS for any
+ * other t outside 0..V-1.  entropy (nullable, fp32 [rows]): -sum p log p.  The
+ * top_k <= 64 likeliest tokens, best first (ties: lowest index; NaN above every
+ * number, as sd_argmax_rows): top_ids int64 and top_logprobs fp32
+ * [rows,top_k].  stats (nullable): fp32 [3,rows] for the backward.  Replaces
+ * the log-softmax of the reference's loss and perplexity
+ * (model/model.py:144-152, evaluation/perplexity.py). */
+SD_API int sd_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t V, int64_t ld,
+                             const int64_t *targets, int64_t ignore_index, float *logprobs, float *entropy,
+                             float *stats, int top_k, float *top_logprobs, int64_t *top_ids, int32_t *err,
+                             void *stream);
+
+/* Gradient of the logits (dlogits [rows,V], row stride d_ld, the logits'
+ * dtype) for the gradients g_logprobs and g_entropy (fp32 [rows], nullable) of
+ * the two sums above. */
+SD_API int sd_token_logprobs_backward(const void *logits, int dtype, int64_t rows, int64_t V, int64_t ld,
+                                      const int64_t *targets, int64_t ignore_index, const float *stats,
+                                      const float *g_logprobs, const float *g_entropy, void *dlogits, int64_t d_ld,
+                                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,9 @@ Drop-in for the reference's attention-backend / forecast API
 * ``B200SparseAttention``, ``gather_kv_blocks``      (model/attention/sparse.py)
 * ``B200KVCache``                                    (model/attention/base.py KVCache)
 * ``B200OffloadKVCache``                             (model/attention/offload.py, async_offload.py)
+* ``B200DenseAttention``, ``packed_attention``       (model/attention/dense.py, over packed sequences)
+* ``B200PagedKVCache``, ``paged_append``, ``paged_decode_attention`` (ragged batches' cache)
+* ``token_logprobs``                                 (the loss of model/model.py, evaluation/perplexity.py)
 * ``install(model)`` swaps the attention of every layer of a reference model.
 
 All compute runs in libspardab200.so (hand-written CUDA for sm_100a, C ABI in
@@ -14,18 +17,20 @@ include/spardab200.h).  There is no CPU path.
 """
 
 from .config import ModelConfig
-from .cache import B200KVCache
+from .cache import B200KVCache, B200PagedKVCache, PageTable
 from .offload import B200OffloadKVCache
 from .forecast import ForecastBlockSelector, ForecastProjection, KVBlockCompressor
-from .attention import B200SparseAttention, BaseAttention
-from .ops import gather_kv_blocks
+from .attention import B200DenseAttention, B200SparseAttention, BaseAttention, RaggedBatch, packed_attention
+from .ops import gather_kv_blocks, paged_append, paged_decode_attention
 from .rope import RotaryEmbedding
+from .scoring import TokenLogprobs, token_logprobs
 from . import ops
 from ._lib import SparDAError, load as load_library
 
 __all__ = ["ModelConfig", "B200KVCache", "B200OffloadKVCache", "ForecastBlockSelector", "ForecastProjection", "KVBlockCompressor",
            "B200SparseAttention", "BaseAttention", "gather_kv_blocks", "RotaryEmbedding", "ops", "SparDAError",
-           "load_library", "install"]
+           "load_library", "install", "B200DenseAttention", "RaggedBatch", "packed_attention", "B200PagedKVCache", "PageTable",
+           "paged_append", "paged_decode_attention", "TokenLogprobs", "token_logprobs"]
 
 
 def install(model, rule: str = "reference"):

@@ -19,6 +19,7 @@ SD_DTYPE_F32, SD_DTYPE_BF16, SD_DTYPE_F16 = 0, 1, 2
 SD_RULE_REFERENCE, SD_RULE_ABSOLUTE = 0, 1
 SD_SELECT_BEFORE_APPEND = 0x100
 SD_KERR_TIMEOUT = 1
+SD_KERR_BOUNDS = 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -75,6 +76,24 @@ _SIGS = {
                                 _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i32, _c_void_p, _i64,
                                 _i64, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _c_void_p, _i64, _c_void_p,
                                 _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p],
+    "sd_packed_attention": [_c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                            _i64, _i64, _c_void_p, _i32, _f32, _c_void_p, _i64, _i64, _c_void_p, _i32, _c_void_p,
+                            _c_void_p],
+    "sd_packed_attention_backward": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, _i64,
+                                     _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p,
+                                     _i32, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                     _c_void_p],
+    "sd_paged_append": [_c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p,
+                        _i64, _i32, _i64, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p, _i32, _c_void_p, _c_void_p,
+                        _c_void_p],
+    "sd_paged_decode_workspace": [_i64, _i64, _i64, _c_void_p],
+    "sd_paged_decode_attention": [_c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64,
+                                  _i32, _i64, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p, _f32, _c_void_p, _i64,
+                                  _i64, _c_void_p, _i64, _c_void_p, _c_void_p],
+    "sd_token_logprobs": [_c_void_p, _i32, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _i32,
+                          _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "sd_token_logprobs_backward": [_c_void_p, _i32, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p,
+                                   _c_void_p, _c_void_p, _i64, _c_void_p],
 }
 
 # entry points that return something other than an int status

@@ -8,9 +8,10 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
-from .cache import B200KVCache
+from .cache import B200KVCache, B200PagedKVCache
 from .offload import B200OffloadKVCache
 from .forecast import ForecastBlockSelector, KVBlockCompressor
 from .rope import apply_rotary_emb
@@ -59,6 +60,36 @@ class _SparseAttentionCore(torch.autograd.Function):
         return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype), None, None, None, None, None
 
 
+class _PackedAttention(torch.autograd.Function):
+    """ops.packed_attention with its backward."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, scale):
+        out, lse = ops.packed_attention(q, k, v, cu_seqlens, scale, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
+        dq, dk, dv = ops.packed_attention_backward(q, k, v, out, gout, lse, cu_seqlens, ctx.scale)
+        return dq, dk, dv, None, None
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Causal GQA attention over sequences packed back to back, differentiable
+    in q, k and v.  q [total,Hq,64], k, v [total,Hkv,64] (views of one packed
+    projection included); sequence s holds rows cu_seqlens[s] ..
+    cu_seqlens[s+1]-1 (device int32, not read by the host).  scale: 1/8 unless
+    given.  Returns [total,Hq,64], zeros outside every sequence."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, cu_seqlens, scale)
+    return ops.packed_attention(q, k, v, cu_seqlens, scale)
+
+
 class BaseAttention(nn.Module):
     """model/attention/base.py:35-52: owns wq, wk, wv, wo (same state-dict keys)."""
 
@@ -75,6 +106,17 @@ class BaseAttention(nn.Module):
         self.wk = nn.Linear(self.n_embd, self.n_kv_head * self.head_dim, bias=False)
         self.wv = nn.Linear(self.n_embd, self.n_kv_head * self.head_dim, bias=False)
         self.wo = nn.Linear(self.n_head * self.head_dim, self.n_embd, bias=False)
+        self._packed = None
+        self._packed_key = None
+
+    # -- fused projection weight [wq; wk; wv], rebuilt when any weight changes
+    def qkv_weight(self) -> torch.Tensor:
+        key = tuple((w.data_ptr(), w._version, w.dtype) for w in (self.wq.weight, self.wk.weight, self.wv.weight))
+        if self._packed is None or self._packed_key != key:
+            with torch.no_grad():
+                self._packed = torch.cat([self.wq.weight, self.wk.weight, self.wv.weight], dim=0).contiguous()
+            self._packed_key = key
+        return self._packed
 
 
 class B200SparseAttention(BaseAttention):
@@ -110,22 +152,11 @@ class B200SparseAttention(BaseAttention):
             raise ValueError(f"unknown selection timing {self.selection_timing!r}")
         self.compressor = KVBlockCompressor(self.block_size, self.head_dim, config.forecast_dim)
         self.selector = ForecastBlockSelector(self.block_size, config.forecast_dim)
-        self._packed = None
-        self._packed_key = None
         self.last_profile = {}
 
     @property
     def before_append(self) -> bool:
         return self.selection_timing == "before_append"
-
-    # -- fused projection weight [wq; wk; wv], rebuilt when any weight changes
-    def qkv_weight(self) -> torch.Tensor:
-        key = tuple((w.data_ptr(), w._version, w.dtype) for w in (self.wq.weight, self.wk.weight, self.wv.weight))
-        if self._packed is None or self._packed_key != key:
-            with torch.no_grad():
-                self._packed = torch.cat([self.wq.weight, self.wk.weight, self.wv.weight], dim=0).contiguous()
-            self._packed_key = key
-        return self._packed
 
     def forward(self, x: torch.Tensor, rotary_emb, kv_cache=None, mask: Optional[torch.Tensor] = None,
                 is_causal: bool = True, forecast_vector: Optional[torch.Tensor] = None, **kwargs):
@@ -296,3 +327,95 @@ class B200SparseAttention(BaseAttention):
         if grad:
             return _SparseAttentionCore.apply(xq, kh, vh, lists, counts, row_topk, self.block_size, causal)
         return ops.prefill_attention(xq, kh, vh, lists, counts, self.block_size, row_topk, causal)
+
+
+class RaggedBatch:
+    """What every layer of one ragged forward shares: the bounds of the packed
+    sequences, or for a decode step of one token each the lengths with that
+    token; and the RoPE rows of the tokens' own positions, fp32 [tokens, D/2]."""
+
+    def __init__(self, cos: torch.Tensor, sin: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                 lens_after: Optional[torch.Tensor] = None):
+        self.cos, self.sin, self.cu_seqlens, self.lens_after = cos, sin, cu_seqlens, lens_after
+
+    @classmethod
+    def prompts(cls, cu_seqlens: torch.Tensor, total: int, rotary_emb) -> "RaggedBatch":
+        """Packed prompts: the token at row r of sequence s has position
+        r - cu_seqlens[s].  Bounds stay on the device; no position can reach
+        ``total``, which the tables are grown to."""
+        rotary_emb.ensure(total)
+        rows = torch.arange(total, device=cu_seqlens.device)
+        bounds = cu_seqlens.to(torch.int64)
+        seq = torch.searchsorted(bounds, rows, right=True) - 1
+        pos = (rows - bounds[seq.clamp_min(0)]).clamp(0, max(total - 1, 0))
+        return cls(rotary_emb.cos[pos], rotary_emb.sin[pos], cu_seqlens=cu_seqlens)
+
+    @classmethod
+    def step(cls, lens: torch.Tensor, capacity: int, rotary_emb) -> "RaggedBatch":
+        """One new token per sequence, at the positions lens (device int32,
+        each below ``capacity``)."""
+        rotary_emb.ensure(capacity)
+        pos = lens.to(torch.int64).clamp(0, capacity - 1)
+        return cls(rotary_emb.cos[pos], rotary_emb.sin[pos], lens_after=lens + 1)
+
+
+class B200DenseAttention(BaseAttention):
+    """Exact causal GQA attention for ragged batches: the reference's dense
+    backend (model/attention/dense.py) over packed sequences of different
+    lengths, and over paged caches.  Same constructor, state-dict keys and
+    forward signature as the other backends; ``attention_backend="b200_dense"``
+    selects it in SparDAB200Model.
+
+    x is [B,T,C]: B sequences of T tokens, or with ``ragged`` (a RaggedBatch
+    with bounds) one row [1,total,C] of packed sequences.  ``kv_cache`` is a
+    B200PagedKVCache whose PageTable has the pages reserved: prompts (its
+    sequences empty so far) or, with T == 1 and no bounds, one decode step of
+    every sequence.  The caller advances the PageTable after the last layer."""
+
+    def forward(self, x: torch.Tensor, rotary_emb, kv_cache=None, mask: Optional[torch.Tensor] = None,
+                is_causal: bool = True, forecast_vector: Optional[torch.Tensor] = None,
+                ragged: Optional[RaggedBatch] = None, **kwargs):
+        b, t, _ = x.shape
+        # gradients reach wq, wk and wv through their own products
+        grad = torch.is_grad_enabled() and (x.requires_grad or self.wq.weight.requires_grad)
+        if grad:
+            heads = [w(x).view(b * t, -1, self.head_dim) for w in (self.wq, self.wk, self.wv)]
+        else:
+            rows = F.linear(x, self.qkv_weight()).view(b * t, -1, self.head_dim)
+            heads = rows.split([self.n_head, self.n_kv_head, self.n_kv_head], dim=1)
+        out = self.core(*heads, b, t, rotary_emb, kv_cache, mask, is_causal, ragged)
+        return self.wo(out.reshape(b, t, self.n_head * self.head_dim).to(x.dtype))
+
+    def core(self, xq, xk, xv, b: int, t: int, rotary_emb, kv_cache=None, mask=None, is_causal: bool = True,
+             ragged: Optional[RaggedBatch] = None) -> torch.Tensor:
+        """From the projections [B*T,H,64] to the attention output
+        [B*T,Hq,64]: RoPE, cache append, attention."""
+        if mask is not None or not is_causal:
+            raise NotImplementedError("the dense backend's attention is causal and takes no additive mask")
+        if kv_cache is not None and not isinstance(kv_cache, B200PagedKVCache):
+            raise NotImplementedError("the dense backend caches in a B200PagedKVCache")
+        grad = torch.is_grad_enabled() and (xq.requires_grad or xk.requires_grad or xv.requires_grad)
+        if grad and kv_cache is not None:
+            raise NotImplementedError("gradients through a KV cache are not supported: train without a cache")
+        step = kv_cache is not None and t == 1 and (any(kv_cache.pages.held) if ragged is None
+                                                    else ragged.cu_seqlens is None)
+        if ragged is None:
+            if step:
+                ragged = RaggedBatch.step(kv_cache.pages.lens, kv_cache.pages.capacity, rotary_emb)
+            else:
+                bounds = torch.arange(0, (b + 1) * t, t, dtype=torch.int32, device=xq.device)
+                ragged = RaggedBatch.prompts(bounds, b * t, rotary_emb)
+        if not step and b != 1 and ragged.cu_seqlens.numel() != b + 1:
+            raise ValueError(f"{ragged.cu_seqlens.numel() - 1} packed sequences do not fit {b} rows of {t} tokens")
+        rope = _RopeQK.apply if grad else ops.rope_qk
+        xq, xk = (y[0] for y in rope(xq[None], xk[None], ragged.cos, ragged.sin))
+        if kv_cache is None:
+            return packed_attention(xq, xk, xv, ragged.cu_seqlens)
+        pages = kv_cache.pages
+        if not step and any(pages.held):
+            raise NotImplementedError("prefill into a non-empty cache")
+        kv_cache.append(xk, xv, ragged.cu_seqlens)
+        if step:
+            return ops.paged_decode_attention(xq, kv_cache.k_pages, kv_cache.v_pages, pages.table,
+                                              ragged.lens_after)
+        return packed_attention(xq, xk, xv, ragged.cu_seqlens)

@@ -15,7 +15,7 @@ in the reference's [B, T, H, D] layout.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -73,3 +73,108 @@ class B200KVCache:
     def reset(self) -> None:
         self.current_len = 0
         self.len_dev.zero_()
+
+
+class PageTable:
+    """Which pages of a pool hold each sequence, shared by the layers' caches.
+
+      table  int32 [max_seqs, width] on the device: position t of sequence b
+             lies in page table[b, t // page_size]; -1 where none is held;
+      lens   int32 [max_seqs] on the device, tokens cached so far.
+
+    The host keeps the same lengths (``held``), each sequence's pages and the
+    free pages; ``reserve`` before a forward, ``advance`` after it."""
+
+    def __init__(self, max_seqs: int, max_seq_len: int, num_pages: int, device: torch.device, page_size: int = 64):
+        if min(max_seqs, max_seq_len, num_pages, page_size) < 1:
+            raise ValueError("max_seqs, max_seq_len, num_pages and page_size must be positive")
+        self.max_seqs, self.num_pages, self.page_size = max_seqs, num_pages, page_size
+        self.width = ops.num_blocks(max_seq_len, page_size)
+        self.capacity = self.width * page_size
+        self.table = torch.full((max_seqs, self.width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self.reset_host()
+
+    def reset_host(self) -> None:
+        self.held: List[int] = [0] * self.max_seqs
+        self.owned: List[List[int]] = [[] for _ in range(self.max_seqs)]
+        self.free: List[int] = list(range(self.num_pages - 1, -1, -1))
+
+    def _counts(self, counts) -> List[int]:
+        counts = [int(counts)] * self.max_seqs if isinstance(counts, int) else [int(c) for c in counts]
+        if len(counts) != self.max_seqs or min(counts) < 0:
+            raise ValueError(f"need {self.max_seqs} non-negative token counts, got {counts}")
+        return counts
+
+    def reserve(self, counts) -> None:
+        """Pages for counts[b] more tokens of every sequence b (or the same
+        number for all).  Raises, with nothing changed, when a sequence would
+        pass its longest or the pool has too few pages."""
+        counts = self._counts(counts)
+        need = []
+        for b, c in enumerate(counts):
+            if self.held[b] + c > self.capacity:
+                raise ValueError(f"cache overflow: sequence {b} would hold {self.held[b] + c} of {self.capacity}")
+            need.append(max(0, ops.num_blocks(self.held[b] + c, self.page_size) - len(self.owned[b])))
+        if sum(need) > len(self.free):
+            raise ValueError(f"out of pages: {sum(need)} needed, {len(self.free)} free")
+        rows, cols, pages = [], [], []
+        for b, n in enumerate(need):
+            for _ in range(n):
+                rows.append(b)
+                cols.append(len(self.owned[b]))
+                self.owned[b].append(self.free.pop())
+                pages.append(self.owned[b][-1])
+        if pages:
+            where = torch.tensor([rows, cols, pages], dtype=torch.int64).to(self.table.device)
+            self.table[where[0], where[1]] = where[2].to(torch.int32)
+
+    def advance(self, counts, device: bool = True) -> None:
+        """Counts the tokens of a finished forward: on the host and, unless a
+        captured step does that itself, on the device."""
+        counts = self._counts(counts)
+        for b, c in enumerate(counts):
+            if self.held[b] + c > len(self.owned[b]) * self.page_size:
+                raise ValueError(f"sequence {b} has no pages for {self.held[b] + c} tokens: reserve them first")
+        for b, c in enumerate(counts):
+            self.held[b] += c
+        if device:
+            if len(set(counts)) == 1:
+                self.lens.add_(counts[0])
+            else:
+                self.lens.add_(torch.tensor(counts, dtype=torch.int32).to(self.lens.device))
+
+    def release(self, seq: int) -> None:
+        """Frees a finished sequence's pages; its row starts empty again."""
+        if not 0 <= seq < self.max_seqs:
+            raise ValueError(f"no sequence {seq} of {self.max_seqs}")
+        self.free.extend(reversed(self.owned[seq]))
+        self.owned[seq], self.held[seq] = [], 0
+        self.table[seq].fill_(-1)
+        self.lens[seq] = 0
+
+    def reset(self) -> None:
+        self.reset_host()
+        self.table.fill_(-1)
+        self.lens.zero_()
+
+
+class B200PagedKVCache:
+    """One layer's pool of pages, k_pages and v_pages [num_pages, H, page, D]
+    (head-major: a head's page is one contiguous run), under a PageTable that
+    all layers share.  Sequences grow page by page, so a batch of ragged lengths
+    holds what it needs and not batch x longest (KVCache.update,
+    model/attention/base.py:11-32, reserves the longest for all)."""
+
+    def __init__(self, pages: PageTable, n_kv_head: int, head_dim: int, device: torch.device, dtype: torch.dtype):
+        self.pages = pages
+        shape = (pages.num_pages, n_kv_head, pages.page_size, head_dim)
+        self.k_pages = torch.zeros(shape, device=device, dtype=dtype)
+        self.v_pages = torch.zeros(shape, device=device, dtype=dtype)
+
+    def append(self, xk: torch.Tensor, xv: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> None:
+        """Writes rows xk, xv [N,H,D] behind the cached tokens of their
+        sequences (one row each, or packed by cu_seqlens); lengths are
+        advanced on the PageTable, once for all layers."""
+        ops.paged_append(xk.to(self.k_pages.dtype), xv.to(self.v_pages.dtype), self.k_pages, self.v_pages,
+                         self.pages.table, self.pages.lens, cu_seqlens)

@@ -1,0 +1,80 @@
+// Packed (ragged) sequences: how a CTA finds its tile, and the arguments that
+// the CUDA-core and tensor-core attention kernels share.
+#pragma once
+
+#include "sd_common.cuh"
+
+namespace sd {
+
+struct PackedArgs {
+  const void *q, *k, *v;                // [total][Hq|Hkv][64], element strides below
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  const int32_t *cu;                    // [S + 1] sequence bounds in the token rows
+  int S, Hq, Hkv;
+  int64_t total;
+  float scale_log2;                     // softmax scale times log2(e)
+  float scale;
+  void *out;                            // forward output, row strides o_st, o_sh
+  int64_t o_st, o_sh;
+  float *lse;                           // [Hq][total] log2 of the row's exponential sum (nullable in the forward)
+  int zero_rest;                        // write zeros to the rows outside every sequence
+  // backward
+  const void *dout;
+  int64_t g_st, g_sh;
+  float *delta;                         // [Hq][total] rowsum(dout * out)
+  void *dq, *dk, *dv;                   // contiguous
+};
+
+// A tile of kTile rows of one sequence.  start: first row of the sequence,
+// len: its rows, row0: the tile's first row within the sequence (row0 < len
+// where valid).  rest: the rows belong to no sequence (before cu[0] or from
+// cu[S] on).
+struct PackedTile {
+  int64_t start;
+  int len, row0;
+  bool valid, rest;
+};
+
+// Tile slots need no prefix sums over the sequences: with b_i the bounds
+// {0, cu[0], ..., cu[S], total} (S + 2 ranges, the first and the last holding
+// the rows outside every sequence), range i owns the slots from
+// floor(b_i / tile) + i, and ceil((b_{i+1} - b_i) / tile) of them are never
+// more than up to the next range's first.  So total / tile + S + 2 slots hold
+// every tile, and a warp finds a slot's range by a 32-way search (two rounds
+// of loads for a thousand sequences).  Bounds are clamped to [0, total]: a
+// malformed cu gives wrong rows but no access outside the tensors.
+__device__ __forceinline__ int64_t packed_bound(const int32_t *cu, int S, int64_t total, int i) {
+  if (i <= 0) return 0;
+  if (i > S + 1) return total;
+  const int64_t b = cu[i - 1];
+  return b < 0 ? 0 : (b > total ? total : b);
+}
+
+inline int64_t packed_slots(int64_t total, int S, int tile) { return total / tile + S + 2; }
+
+// Called by all 32 lanes of a warp with the same slot.
+__device__ __forceinline__ PackedTile packed_find(const int32_t *cu, int S, int64_t total, int64_t slot, int tile) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = S + 2;  // the range is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int i = lo + lane * step;
+    const bool le = lane * step < n && packed_bound(cu, S, total, i) / tile + i <= slot;
+    const unsigned hit = __ballot_sync(0xffffffffu, le);
+    const int top = hit ? 31 - __clz(hit) : 0;
+    const int end = lo + n;
+    lo += top * step;
+    n = min(step, end - lo);
+  }
+  const int64_t b = packed_bound(cu, S, total, lo), e = packed_bound(cu, S, total, lo + 1);
+  PackedTile t;
+  t.start = b;
+  t.len = e > b ? static_cast<int>(e - b) : 0;
+  const int64_t nth = slot - (b / tile + lo);
+  t.rest = lo == 0 || lo == S + 1;
+  t.valid = nth >= 0 && nth * tile < t.len;
+  t.row0 = t.valid ? static_cast<int>(nth * tile) : 0;
+  return t;
+}
+
+}  // namespace sd

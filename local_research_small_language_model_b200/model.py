@@ -17,12 +17,13 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
-from .attention import B200SparseAttention
-from .cache import B200KVCache
+from .attention import B200DenseAttention, B200SparseAttention, RaggedBatch
+from .cache import B200KVCache, B200PagedKVCache, PageTable
 from .offload import B200OffloadKVCache
 from .config import ModelConfig
 from .forecast import ForecastProjection
 from .rope import RotaryEmbedding
+from .scoring import TokenLogprobs, token_logprobs
 
 
 def _records_grad(x: torch.Tensor, module: nn.Module) -> bool:
@@ -93,7 +94,8 @@ class TransformerBlock(nn.Module):
         self.config = config
         self.layer_idx = layer_idx
         self.attn_norm = RMSNorm(config.n_embd, eps=config.norm_eps)
-        self.attention = B200SparseAttention(config, layer_idx)
+        dense = config.attention_backend == "b200_dense"
+        self.attention = (B200DenseAttention if dense else B200SparseAttention)(config, layer_idx)
         self.forecast = ForecastProjection(config)
         self.ffn_norm = RMSNorm(config.n_embd, eps=config.norm_eps)
         self.ffn = SwiGLU(config.n_embd, config.ffn_dim)
@@ -156,9 +158,25 @@ class TransformerBlock(nn.Module):
         gu = F.linear(self.ffn_norm(x2), self.packed_ffn_weight())
         return torch.addmm(x2, ops.silu_mul(gu), self.ffn.w_down.weight.t())
 
-    def forward(self, x, rotary_emb, kv_cache=None, mask=None, is_causal=True, prev_layer_forecast=None,
-                next_layer_block=None, next_kv_cache=None):
+    def _forward_dense(self, x, rotary_emb, kv_cache, mask, is_causal, ragged):
+        """The block around exact attention: no forecast (nothing selects
+        blocks by it)."""
+        a = self.attention
+        normed = self.attn_norm(x)
+        if _records_grad(x, self):
+            x = x + a(normed, rotary_emb, kv_cache, mask, is_causal, ragged=ragged)
+            return x + self.ffn(self.ffn_norm(x))
         b, t, c = x.shape
+        rows = F.linear(normed.reshape(b * t, c), a.qkv_weight()).unflatten(1, (-1, a.head_dim))
+        xq, xk, xv = rows.split([a.n_head, a.n_kv_head, a.n_kv_head], dim=1)
+        out = a.core(xq, xk, xv, b, t, rotary_emb, kv_cache, mask, is_causal, ragged)
+        return self._ffn_decode(x.reshape(b * t, c), out.flatten(1), False).view(b, t, c)
+
+    def forward(self, x, rotary_emb, kv_cache=None, mask=None, is_causal=True, prev_layer_forecast=None,
+                next_layer_block=None, next_kv_cache=None, ragged=None):
+        b, t, c = x.shape
+        if isinstance(self.attention, B200DenseAttention):
+            return self._forward_dense(x, rotary_emb, kv_cache, mask, is_causal, ragged), None
         if isinstance(kv_cache, (B200KVCache, B200OffloadKVCache)) and t == 1:
             # decode step: 8 launches per layer by default (norm, [wq;wk;wv;wf]
             # GEMM, fused attention kernel, wo GEMM with the residual add folded
@@ -365,9 +383,59 @@ class SparDAB200Model(nn.Module):
                 layer.side_stream = side
         return caches
 
-    def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
-                kv_caches: Optional[List] = None, return_forecasts: bool = False) -> Dict[str, torch.Tensor]:
+    def allocate_paged_caches(self, max_seqs: int, max_seq_len: int, num_pages: Optional[int] = None,
+                              page_size: int = 64, dtype: Optional[torch.dtype] = None, device=None) -> List:
+        """One B200PagedKVCache per layer under one PageTable
+        (``caches[0].pages``), for the "b200_dense" backend.  ``num_pages``
+        bounds the tokens held at once (default: every sequence at its
+        longest)."""
+        cfg = self.config
+        device = device or self.embeddings.weight.device
+        dtype = dtype or self.embeddings.weight.dtype
+        if num_pages is None:
+            num_pages = max_seqs * ops.num_blocks(max_seq_len, page_size)
+        pages = PageTable(max_seqs, max_seq_len, num_pages, device, page_size)
+        self.rotary_emb._extend_cache(pages.capacity, device)
+        return [B200PagedKVCache(pages, cfg.n_kv_head, cfg.head_dim, device, dtype) for _ in range(cfg.n_layer)]
+
+    def _ragged(self, input_ids, kv_caches, cu_seqlens, lengths):
+        """(RaggedBatch, PageTable or None, tokens to count) of a forward on
+        the dense backend."""
         b, t = input_ids.shape
+        pages = kv_caches[0].pages if kv_caches is not None else None
+        if pages is not None and cu_seqlens is None and b != pages.max_seqs:
+            raise ValueError(f"{b} rows for a cache of {pages.max_seqs} sequences")
+        if pages is not None and cu_seqlens is None and t == 1 and any(pages.held):
+            pages.reserve(1)
+            return RaggedBatch.step(pages.lens, pages.capacity, self.rotary_emb), pages, 1
+        if pages is not None and any(pages.held):
+            raise NotImplementedError("prefill into a non-empty cache")
+        if cu_seqlens is None:
+            cu_seqlens = torch.arange(0, (b + 1) * t, t, dtype=torch.int32, device=input_ids.device)
+            counts = [t] * b
+        elif b != 1:
+            raise ValueError(f"packed sequences are one row of tokens, got {b}")
+        else:
+            counts = lengths
+        if pages is not None:
+            if counts is None or sum(counts) != b * t:
+                raise ValueError("packed prompts into a cache need their lengths on the host too, "
+                                 "with the sum of the row's tokens")
+            pages.reserve(counts)
+        return RaggedBatch.prompts(cu_seqlens, b * t, self.rotary_emb), pages, counts
+
+    def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
+                kv_caches: Optional[List] = None, return_forecasts: bool = False,
+                cu_seqlens: Optional[torch.Tensor] = None,
+                lengths: Optional[List[int]] = None) -> Dict[str, torch.Tensor]:
+        """``cu_seqlens`` (device int32, "b200_dense" backend): input_ids
+        [1,total] holds sequences packed back to back; with paged caches also
+        their ``lengths`` as host numbers."""
+        b, t = input_ids.shape
+        if self.config.attention_backend == "b200_dense":
+            return self._forward_dense(input_ids, targets, kv_caches, cu_seqlens, lengths)
+        if cu_seqlens is not None:
+            raise NotImplementedError('packed sequences need attention_backend="b200_dense"')
         x = self.embeddings.embed(input_ids)
         forecasts = []
         prev = None
@@ -397,6 +465,34 @@ class SparDAB200Model(nn.Module):
             out["loss"] = F.cross_entropy(logits.view(-1, self.config.vocab_size), targets.view(-1),
                                           ignore_index=-100)
         return out
+
+    def _forward_dense(self, input_ids, targets, kv_caches, cu_seqlens, lengths) -> Dict[str, torch.Tensor]:
+        if kv_caches is not None and not all(isinstance(c, B200PagedKVCache) for c in kv_caches):
+            raise NotImplementedError("the dense backend caches in a B200PagedKVCache")
+        ragged, pages, counts = self._ragged(input_ids, kv_caches, cu_seqlens, lengths)
+        x = self.embeddings.embed(input_ids)
+        for i, layer in enumerate(self.layers):
+            x, _ = layer(x=x, rotary_emb=self.rotary_emb, kv_cache=kv_caches[i] if kv_caches is not None else None,
+                         ragged=ragged)
+        if pages is not None:
+            pages.advance(counts)
+        logits = self.embeddings.project(self.final_norm(x))
+        out = {"logits": logits}
+        if targets is not None:
+            # the mean over the scored tokens, as F.cross_entropy(ignore_index=-100)
+            flat = targets.reshape(-1)
+            scores = token_logprobs(logits.flatten(0, 1), flat)
+            out["loss"] = -scores.logprobs.sum() / (flat != -100).sum()
+        return out
+
+    def score(self, input_ids: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
+              cu_seqlens: Optional[torch.Tensor] = None) -> TokenLogprobs:
+        """Log probabilities of targets [B,T] (-100 = not scored) after the
+        prompt tokens input_ids [B,T], with the entropy and the top_k likeliest
+        tokens at every position: what evaluation/perplexity.py sums."""
+        more = {"cu_seqlens": cu_seqlens} if cu_seqlens is not None else {}
+        logits = self(input_ids, **more)["logits"]
+        return token_logprobs(logits.flatten(0, 1), targets.reshape(-1), top_k)
 
 
 class DecodeEngine:
