@@ -356,7 +356,6 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
                         int64_t v_sh, const int32_t *cu_seqlens, int nseq, float scale, void *out, int64_t o_st,
                         int64_t o_sh, float *lse, int zero_rest, int32_t *err, void *stream) {
   using namespace sd;
-  (void)err;
   PackedArgs a = {};
   a.q = q, a.k = k, a.v = v;
   a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
@@ -369,12 +368,11 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
   int rc = check_packed(a, dtype, D);
   if (rc != SD_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  SD_DISPATCH_DTYPE(dtype, T, {
-    const size_t smem = 4 * pk::kTileFloats * sizeof(float);
-    auto kern = packed_fwd_kernel<T>;
-    if (set_max_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
-    kern<<<dim3(static_cast<unsigned>(packed_slots(total, nseq, pk::kTile)), a.Hq), pk::kThreads, smem, s>>>(a);
-  });
+  if (dtype != SD_DTYPE_F32) return launch_packed_fwd_tc(a, dtype, err, s);
+  const size_t smem = 4 * pk::kTileFloats * sizeof(float);
+  auto kern = packed_fwd_kernel<float>;
+  if (set_max_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
+  kern<<<dim3(static_cast<unsigned>(packed_slots(total, nseq, pk::kTile)), a.Hq), pk::kThreads, smem, s>>>(a);
   return check_launch();
 }
 

@@ -77,4 +77,7 @@ __device__ __forceinline__ PackedTile packed_find(const int32_t *cu, int S, int6
   return t;
 }
 
+// The tensor-core kernels (16-bit types).
+int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s);
+
 }  // namespace sd

@@ -1,0 +1,362 @@
+// Causal attention over packed sequences on the 5th-generation tensor cores,
+// 16-bit inputs.
+//
+//   O_i = sum_{j <= i} exp2(c q_i.k_j - m_i) v_j / l_i,  c = scale log2(e)
+//
+// Forward.  One CTA per 256 query rows of one sequence and head, one per SM
+// (384 of the 512 tensor-memory columns).  The rows are two 128-row tiles;
+// for every 128 keys up to a tile's own diagonal
+//   S_x = Q_x K^T    4 MMAs M=128 N=128 K=16, fp32 in 128 columns
+//   P_x = exp2(..)   warpgroup x, one thread a row, 16-bit pairs written over
+//                    the first 64 columns of S_x
+//   O_x += P_x V     8 MMAs M=128 N=64 K=16, A from tensor memory
+// Warp 8 issues all MMAs, warp 9 all copies (K and V in a ring of 4 stages).
+// The two tiles alternate: while one warpgroup computes exponentials, the
+// other tile's two products run.  S_x(i + 1) is issued right behind O_x(i), so
+// its arrival also says that O_x(i) is done, and a row may rescale its O then
+// (rarely: a row keeps its reference maximum until a block exceeds it by 2^8).
+#include <type_traits>
+
+#include "sd_packed.cuh"
+#include "sd_tc.cuh"
+#include "sd_tma.cuh"
+
+namespace sd {
+
+namespace pt {
+
+using namespace tc;
+
+constexpr int kRows = 128;                   // MMA M, and keys of a block
+constexpr int kTileBytes = kRows * 128;      // 128 rows of 64 16-bit values
+constexpr int kStages = 4;
+constexpr int kFwdThreads = 320;             // 2 softmax warpgroups, MMA warp, copy warp
+
+struct FwdSmem {
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + 2 * kTileBytes;
+  static constexpr int kV = kK + kStages * kTileBytes;
+  static constexpr int kBar = kV + kStages * kTileBytes;
+  static constexpr int kBytes = kBar + 256;
+};
+
+// 32 consecutive columns of this thread's tensor-memory lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ void fma2(float &a, float &b, float c, float d) {  // {a, b} = {a, b} * c + d
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void add2(float &a, float &b, float c, float d) {  // {a, b} += {c, d}
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t tmem, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Zeros the rows from `first` on of a 128-row tile in shared memory (a warp):
+// the rows behind a sequence's end belong to others, and a masked weight of 0
+// times their NaN or infinity would show.
+__device__ __forceinline__ void clear_rows(char *tile, int first) {
+  const int lane = threadIdx.x & 31;
+  for (int e = first * 8 + lane; e < kRows * 8; e += 32)
+    *reinterpret_cast<uint4 *>(tile + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+  fence_async_smem();
+  __syncwarp();
+}
+
+// 64 fp32 values of one row, scaled, to 16-bit memory.
+template <typename T> __device__ __forceinline__ void store_row(T *dst, uint32_t taddr, float scale, bool write) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[32];
+    tmem_ld32(taddr + 32 * h, v);
+    tmem_wait_ld();
+    if (!write) continue;
+#pragma unroll
+    for (int c = 0; c < 32; c += 8)
+      *reinterpret_cast<uint4 *>(dst + 32 * h + c) =
+          make_uint4(pack2<T>(v[c] * scale, v[c + 1] * scale), pack2<T>(v[c + 2] * scale, v[c + 3] * scale),
+                     pack2<T>(v[c + 4] * scale, v[c + 5] * scale), pack2<T>(v[c + 6] * scale, v[c + 7] * scale));
+  }
+}
+
+template <typename T> __device__ __forceinline__ void zero_rows(T *dst, int64_t stride, int rows) {
+  for (int e = threadIdx.x; e < rows * 8; e += blockDim.x)
+    *reinterpret_cast<uint4 *>(dst + (e >> 3) * stride + (e & 7) * 8) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+}  // namespace pt
+
+template <typename T>
+__global__ void __launch_bounds__(pt::kFwdThreads, 1)
+    packed_fwd_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
+                         const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                         int32_t *err) {
+  using namespace pt;
+  constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  // heads fastest; the last tiles, which see the most keys, first
+  const int h = blockIdx.x % a.Hq;
+  const int64_t slots = gridDim.x / a.Hq;
+  const PackedTile t = packed_find(a.cu, a.S, a.total, slots - 1 - blockIdx.x / a.Hq, 2 * kRows);
+  if (!t.valid) return;
+  const int rows = min(2 * kRows, t.len - t.row0);
+  const int64_t first = t.start + t.row0;
+  T *out = static_cast<T *>(a.out) + first * a.o_st + h * a.o_sh;
+  if (t.rest) {
+    if (a.zero_rest) zero_rows(out, a.o_st, rows);
+    return;
+  }
+  extern __shared__ __align__(1024) char smem_raw[];
+  char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t *q_full = reinterpret_cast<uint64_t *>(sm + FwdSmem::kBar);
+  uint64_t *k_full = q_full + 1, *v_full = k_full + kStages, *kv_empty = v_full + kStages;
+  uint64_t *s_full = kv_empty + kStages, *p_full = s_full + 2, *o_full = p_full + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hk = h / (a.Hq / a.Hkv);
+  // key blocks of each tile: those up to its diagonal
+  const int n0 = t.row0 / kRows + 1, n1 = rows > kRows ? n0 + 1 : 0;
+  const int blocks = max(n0, n1);
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (tid == 288) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&o_full[x], 1);
+    }
+    mbar_init_fence();
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+  float l = 0.f, m = -INFINITY;
+
+  if (warp == 9) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(q_full, (n1 ? 2u : 1u) * kTileBytes);
+      for (int x = 0; x < (n1 ? 2 : 1); ++x)
+        tma_load_4d(sm + FwdSmem::kQ + x * kTileBytes, &tmq, 0, static_cast<int>(first) + x * kRows, h, 0, q_full);
+      for (int i = 0; i < blocks && ok; ++i) {
+        const int s = i % kStages;
+        if (i >= kStages) ok = mbar_wait_bounded(&kv_empty[s], (i / kStages - 1) & 1);
+        if (!ok) break;
+        const int row = static_cast<int>(t.start) + i * kRows;
+        mbar_arrive_expect_tx(&k_full[s], kTileBytes);
+        tma_load_4d(sm + FwdSmem::kK + s * kTileBytes, &tmk, 0, row, hk, 0, &k_full[s]);
+        mbar_arrive_expect_tx(&v_full[s], kTileBytes);
+        tma_load_4d(sm + FwdSmem::kV + s * kTileBytes, &tmv, 0, row, hk, 0, &v_full[s]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    const uint32_t id_s = idesc_f16(fmt, false, 128), id_o = idesc_f16(fmt, true, 64);
+    const uint32_t sq = smem_u32(sm + FwdSmem::kQ), sk = smem_u32(sm + FwdSmem::kK), sv = smem_u32(sm + FwdSmem::kV);
+    auto issue_s = [&](int x, int i) {
+      const int s = i % kStages;
+      ok = ok && mbar_wait_bounded(&k_full[s], (i / kStages) & 1);
+      fence_after_sync();
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_f16(tmem + 128 * x, umma_desc_sw128(sq + x * kTileBytes + 32 * k, 16, 1024),
+                umma_desc_sw128(sk + s * kTileBytes + 32 * k, 16, 1024), id_s, k > 0);
+      mma_commit(&s_full[x]);
+    };
+    if (lane == 0) {
+      ok = mbar_wait_bounded(q_full, 0);
+      issue_s(0, 0);
+      if (n1) issue_s(1, 0);
+    }
+    const int tail = t.len / kRows;  // the block that holds the sequence's end, if it ends inside one
+    for (int i = 0; i < blocks; ++i) {
+      const int s = i % kStages;
+      if (i == tail) {
+        if (lane == 0) ok = ok && mbar_wait_bounded(&v_full[s], (i / kStages) & 1);
+        __syncwarp();
+        clear_rows(sm + FwdSmem::kV + s * kTileBytes, t.len - tail * kRows);
+      }
+      if (lane == 0) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int n = x ? n1 : n0;
+          if (i >= n) continue;
+          ok = ok && mbar_wait_bounded(&v_full[s], (i / kStages) & 1);
+          ok = ok && mbar_wait_bounded(&p_full[x], i & 1);
+          fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_f16_ts(tmem + 256 + 64 * x, tmem + 128 * x + 8 * k,
+                       umma_desc_sw128(sv + s * kTileBytes + 2048 * k, kTileBytes, 1024), id_o, i > 0 || k > 0);
+          if (i + 1 < n)
+            issue_s(x, i + 1);
+          else
+            mma_commit(&o_full[x]);
+        }
+        if (i + kStages < blocks) mma_commit(&kv_empty[s]);
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+    }
+  } else {
+    const int x = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int n = x ? n1 : n0;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + 128 * x, t_o = tmem + lane_base + 256 + 64 * x;
+    const float c = a.scale_log2;
+    for (int i = 0; i < n; ++i) {
+      ok = mbar_wait_bounded(&s_full[x], i & 1);
+      if (__any_sync(0xffffffffu, !ok)) break;
+      fence_after_sync();
+      float s[128];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) tmem_ld32(t_s + 32 * u, s + 32 * u);
+      tmem_wait_ld();
+      if (i == n - 1) {  // the diagonal block: row r sees its first r + 1 keys
+#pragma unroll
+        for (int u = 0; u < 128; ++u) s[u] = u <= r ? s[u] : -INFINITY;
+      }
+      float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int u = 4; u < 128; u += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          top[e] = u + 4 + e < 128 ? fmaxf(top[e], fmaxf(s[u + e], s[u + 4 + e])) : fmaxf(top[e], s[u + e]);
+      }
+      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+      if (best > m + kRescaleLog2 || m == -INFINITY) {
+        const float alpha = m == -INFINITY ? 0.f : ex2(m - best);
+        m = best;
+        l *= alpha;
+        top[0] = alpha;
+      } else {
+        top[0] = 1.f;
+      }
+      if (i > 0 && __any_sync(0xffffffffu, top[0] != 1.f)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float o[32];
+          tmem_ld32(t_o + 32 * u, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= top[0];
+          tmem_st16(t_o + 32 * u, reinterpret_cast<float(&)[16]>(o[0]));
+          tmem_st16(t_o + 32 * u + 16, reinterpret_cast<float(&)[16]>(o[16]));
+        }
+      }
+      const float neg = m == -INFINITY ? 0.f : -m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float y0 = s[32 * u + 2 * e], y1 = s[32 * u + 2 * e + 1];
+          fma2(y0, y1, c, neg);
+          y0 = ex2(y0), y1 = ex2(y1);
+          add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], y0, y1);
+          p[e] = __uint_as_float(pack2<T>(y0, y1));
+        }
+        tmem_st16(t_s + 16 * u, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);
+    }
+    if (n > 0 && ok) {
+      ok = mbar_wait_bounded(&o_full[x], 0);
+      fence_after_sync();
+    }
+  }
+  const bool failed = __syncthreads_or(!ok);
+  if (failed) {  // a bounded wait expired: let copies in flight land, poison the rows
+    if (tid == 288)
+      for (int s = 0; s < kStages; ++s) {
+        mbar_wait_bounded(&k_full[s], 0, 1000000ull);
+        mbar_wait_bounded(&v_full[s], 0, 1000000ull);
+      }
+    l = __int_as_float(0x7fc00000);
+    if (tid == 0 && err) *err = SD_KERR_TIMEOUT;
+  }
+  if (warp < 8) {
+    const int x = warp >> 2, row = 32 * warp + lane;  // row of the CTA: tile x, row % 128
+    if (x == 0 || n1 > 0) {
+      const bool mine = row < rows;
+      fence_after_sync();
+      store_row(out + row * a.o_st, tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 + 64 * x, 1.0f / l,
+                mine);
+      if (mine && a.lse) a.lse[h * a.total + first + row] = m + log2f(l);
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Map of a packed tensor [total][H][64]: boxes of 128 rows of one head.
+static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total, int64_t H, int64_t st, int64_t sh) {
+  if (H == 1 && sh <= 0) sh = 64;
+  if (total == 1 && st <= 0) st = sh * H;
+  return encode_rows_map(map, p, dtype, 64, total, H, 1, st, sh, st, pt::kRows);
+}
+
+int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
+  CUtensorMap mq, mk, mv;
+  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh);
+  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh);
+  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh);
+  if (rc != SD_OK) return rc;
+  const int64_t ctas = packed_slots(a.total, a.S, 2 * pt::kRows) * a.Hq;
+  if (ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
+  const size_t smem = pt::FwdSmem::kBytes + 1024;
+  auto run = [&](auto *kern) {
+    if (set_max_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
+    kern<<<static_cast<unsigned>(ctas), pt::kFwdThreads, smem, s>>>(a, mq, mk, mv, err);
+    return check_launch();
+  };
+  return dtype == SD_DTYPE_BF16 ? run(packed_fwd_tc_kernel<__nv_bfloat16>) : run(packed_fwd_tc_kernel<__half>);
+}
+
+}  // namespace sd
