@@ -430,7 +430,7 @@ SD_API int sd_packed_attention(const void *q, const void *k, const void *v, int 
 /* Its gradients for the output gradient dout [total,Hq,64]: dq [total,Hq,64],
  * dk and dv [total,Hkv,64], contiguous, in the inputs' dtype (dk and dv summed
  * over the query heads of their kv head; zeros outside every sequence).  out
- * and lse are the forward's.  delta: fp32 [Hq,total] workspace of this call.
+ * and lse are the forward's.  delta: workspace of this call, fp32 [Hq*total + 1].
  * Sums have a fixed order: equal inputs give equal bits. */
 SD_API int sd_packed_attention_backward(const void *q, const void *k, const void *v, const void *out,
                                         const void *dout, int dtype, int64_t total, int64_t Hq, int64_t Hkv,

@@ -383,7 +383,6 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
                                  float scale, const float *lse, float *delta, void *dq, void *dk, void *dv,
                                  int32_t *err, void *stream) {
   using namespace sd;
-  (void)err;
   PackedArgs a = {};
   a.q = q, a.k = k, a.v = v;
   a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
@@ -401,17 +400,16 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   if (!lse || !delta || !dq || !dk || !dv) return SD_ERR_INVALID;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return SD_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  SD_DISPATCH_DTYPE(dtype, T, {
-    const unsigned slots = static_cast<unsigned>(packed_slots(total, nseq, pk::kTile));
-    const size_t smem_q = 5 * pk::kTileFloats * sizeof(float), smem_kv = 6 * pk::kTileFloats * sizeof(float);
-    auto kq = packed_bwd_dq_kernel<T>;
-    auto kkv = packed_bwd_dkv_kernel<T>;
-    if (set_max_smem(kq, smem_q) != SD_OK || set_max_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
-    kq<<<dim3(slots, a.Hq), pk::kThreads, smem_q, s>>>(a);
-    int rc2 = check_launch();
-    if (rc2 != SD_OK) return rc2;
-    kkv<<<dim3(slots, a.Hkv), pk::kThreads, smem_kv, s>>>(a);
-  });
+  if (dtype != SD_DTYPE_F32) return launch_packed_bwd_tc(a, dtype, err, s);
+  const unsigned slots = static_cast<unsigned>(packed_slots(total, nseq, pk::kTile));
+  const size_t smem_q = 5 * pk::kTileFloats * sizeof(float), smem_kv = 6 * pk::kTileFloats * sizeof(float);
+  auto kq = packed_bwd_dq_kernel<float>;
+  auto kkv = packed_bwd_dkv_kernel<float>;
+  if (set_max_smem(kq, smem_q) != SD_OK || set_max_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
+  kq<<<dim3(slots, a.Hq), pk::kThreads, smem_q, s>>>(a);
+  rc = check_launch();
+  if (rc != SD_OK) return rc;
+  kkv<<<dim3(slots, a.Hkv), pk::kThreads, smem_kv, s>>>(a);
   return check_launch();
 }
 

@@ -21,7 +21,7 @@ struct PackedArgs {
   // backward
   const void *dout;
   int64_t g_st, g_sh;
-  float *delta;                         // [Hq][total] rowsum(dout * out)
+  float *delta;                         // [Hq][total] rowsum(dout * out), and one word more
   void *dq, *dk, *dv;                   // contiguous
 };
 
@@ -79,5 +79,6 @@ __device__ __forceinline__ PackedTile packed_find(const int32_t *cu, int S, int6
 
 // The tensor-core kernels (16-bit types).
 int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s);
+int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s);
 
 }  // namespace sd

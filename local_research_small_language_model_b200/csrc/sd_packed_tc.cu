@@ -15,6 +15,20 @@
 // other tile's two products run.  S_x(i + 1) is issued right behind O_x(i), so
 // its arrival also says that O_x(i) is done, and a row may rescale its O then
 // (rarely: a row keeps its reference maximum until a block exceeds it by 2^8).
+//
+// Backward, two kernels of one shape: a CTA owns 128 rows, whose two operands
+// stay in tensor memory as A for all products, and walks 64-row blocks of the
+// other side, whose two operands arrive in shared memory and serve as B both
+// ways.  Block i belongs to warpgroup i mod 2, each with its own S and dP
+// columns, so one computes while the other's products run.
+//   dQ:    rows are queries (A: Q, dO), blocks are keys (B: K, V)
+//          S = Q K^T, dP = dO V^T;  dS = P (dP - delta);  dQ += dS K
+//   dK/dV: rows are keys (A: K, V), blocks are queries of every head of the
+//          group (B: Q, dO)
+//          S' = K Q^T, dP' = V dO^T;  dV += P' dO,  dK += dS' Q
+// S and dP are computed in both (7 products and 2 exponentials a pair instead
+// of 5 and 1): in return every gradient is summed in tensor memory in a fixed
+// order, with no atomics and no fp32 buffer to add into and convert.
 #include <type_traits>
 
 #include "sd_packed.cuh"
@@ -37,6 +51,18 @@ struct FwdSmem {
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kBar = kV + kStages * kTileBytes;
+  static constexpr int kBytes = kBar + 256;
+};
+
+constexpr int kBlock = 64;                   // rows of a block in the backward
+constexpr int kBlockBytes = kBlock * 128;
+constexpr int kBwdStages = 8;
+
+struct BwdSmem {
+  static constexpr int kA = 0;               // K or Q blocks
+  static constexpr int kB = kA + kBwdStages * kBlockBytes;  // V or dO blocks
+  static constexpr int kVec = kB + kBwdStages * kBlockBytes;  // 2 warpgroups x 2 x (64 lse, 64 delta)
+  static constexpr int kBar = kVec + 2048;
   static constexpr int kBytes = kBar + 256;
 };
 
@@ -70,6 +96,19 @@ __device__ __forceinline__ void add2(float &a, float &b, float c, float d) {  //
       : "f"(c), "f"(d));
 }
 
+__device__ __forceinline__ void fma2v(float &a, float &b, float c, float d, float e) {  // {a, b} = {a, b} * c + {d, e}
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %4};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d), "f"(e));
+}
+__device__ __forceinline__ void mul2(float &a, float &b, float c, float d) {  // {a, b} *= {c, d}
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -85,12 +124,12 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t tmem, uint32_t cols) {
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Zeros the rows from `first` on of a 128-row tile in shared memory (a warp):
-// the rows behind a sequence's end belong to others, and a masked weight of 0
-// times their NaN or infinity would show.
-__device__ __forceinline__ void clear_rows(char *tile, int first) {
+// Zeros the rows from `first` on of a tile in shared memory (a warp): the rows
+// behind a sequence's end belong to others, and a masked weight of 0 times
+// their NaN or infinity would show.
+__device__ __forceinline__ void clear_rows(char *tile, int first, int rows) {
   const int lane = threadIdx.x & 31;
-  for (int e = first * 8 + lane; e < kRows * 8; e += 32)
+  for (int e = first * 8 + lane; e < rows * 8; e += 32)
     *reinterpret_cast<uint4 *>(tile + e * 16) = make_uint4(0u, 0u, 0u, 0u);
   fence_async_smem();
   __syncwarp();
@@ -212,7 +251,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       if (i == tail) {
         if (lane == 0) ok = ok && mbar_wait_bounded(&v_full[s], (i / kStages) & 1);
         __syncwarp();
-        clear_rows(sm + FwdSmem::kV + s * kTileBytes, t.len - tail * kRows);
+        clear_rows(sm + FwdSmem::kV + s * kTileBytes, t.len - tail * kRows, kRows);
       }
       if (lane == 0) {
 #pragma unroll
@@ -335,18 +374,443 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
   }
 }
 
-// Map of a packed tensor [total][H][64]: boxes of 128 rows of one head.
-static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total, int64_t H, int64_t st, int64_t sh) {
+// ---------------------------------------------------------------- backward
+namespace pt {
+
+constexpr int kBwdThreads = 320;
+constexpr int kColS = 0, kColDp = 64, kColAcc = 256, kColAcc2 = 320, kColA = 384, kColB = 416;
+
+struct BwdBars {
+  uint64_t full[kBwdStages], empty[kBwdStages], sd_full[2], p_full[2], done;
+  uint32_t tmem;
+};
+
+__device__ __forceinline__ void bwd_init(BwdBars *bars) {
+  for (int s = 0; s < kBwdStages; ++s) {
+    mbar_init(&bars->full[s], 1);
+    mbar_init(&bars->empty[s], 1);
+  }
+  for (int b = 0; b < 2; ++b) {
+    mbar_init(&bars->sd_full[b], 1);
+    mbar_init(&bars->p_full[b], 4);
+  }
+  mbar_init(&bars->done, 1);
+  mbar_init_fence();
+}
+
+// This thread's row of 64 16-bit values (zeros where !held) into 32
+// tensor-memory columns, and a copy in registers.
+template <typename T>
+__device__ __forceinline__ void row_to_tmem(const T *src, bool held, uint32_t taddr, uint4 (&raw)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    raw[e] = held ? *reinterpret_cast<const uint4 *>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
+  tmem_st16(taddr, reinterpret_cast<const float(&)[16]>(raw[0]));
+  tmem_st16(taddr + 16, reinterpret_cast<const float(&)[16]>(raw[4]));
+  tmem_wait_st();
+}
+
+// The copy thread's loop over blocks [i0, i1): block i lies `i % per_head`
+// blocks behind row0, in head head0 + i / per_head.
+__device__ __forceinline__ bool bwd_copy(BwdBars *bars, char *sm, const CUtensorMap &ma, const CUtensorMap &mb, int i0,
+                                         int i1, int per_head, int row0, int head0) {
+  for (int i = i0; i < i1; ++i) {
+    const int s = i % kBwdStages;
+    if (i >= kBwdStages && !mbar_wait_bounded(&bars->empty[s], (i / kBwdStages - 1) & 1)) return false;
+    const int row = row0 + (i % per_head) * kBlock, head = head0 + i / per_head;
+    mbar_arrive_expect_tx(&bars->full[s], 2 * kBlockBytes);
+    tma_load_4d(sm + BwdSmem::kA + s * kBlockBytes, &ma, 0, row, head, 0, &bars->full[s]);
+    tma_load_4d(sm + BwdSmem::kB + s * kBlockBytes, &mb, 0, row, head, 0, &bars->full[s]);
+  }
+  return true;
+}
+
+// A bounded wait expired: copies in flight land before the CTA ends.
+__device__ __forceinline__ void bwd_failed(BwdBars *bars, int32_t *err) {
+  if (threadIdx.x == 288)
+    for (int s = 0; s < kBwdStages; ++s) mbar_wait_bounded(&bars->full[s], 0, 1000000ull);
+  if (threadIdx.x == 0 && err) *err = SD_KERR_TIMEOUT;
+}
+
+// The power of two that takes x into [1/2, 1) (1 for 0): fp16 holds dS scaled
+// by it, so that small output gradients (a loss averaged over many tokens)
+// keep their digits.
+__device__ __forceinline__ float unit_scale(float x) {
+  const int e = static_cast<int>(__float_as_uint(x) >> 23) - 126;
+  return x > 0.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 1.f;
+}
+
+// The MMA thread's loop, the same for both kernels: products of block i into
+// its warpgroup's columns, and the accumulation of block i once its weights are
+// there.  acc(i, stage): issues the accumulating MMAs.
+template <typename T, typename Acc>
+__device__ __forceinline__ bool bwd_mma(BwdBars *bars, char *sm, uint32_t tmem, int blocks, int first_row, int rows_end,
+                                        int per_head, bool clear_b, Acc acc) {
+  constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  constexpr uint32_t id = idesc_f16(fmt, false, 64);
+  const int lane = threadIdx.x & 31;
+  const uint32_t sa = smem_u32(sm + BwdSmem::kA), sb = smem_u32(sm + BwdSmem::kB);
+  bool ok = true;
+  auto products = [&](int i) {
+    const int s = i % kBwdStages;
+    if (lane == 0) ok = ok && mbar_wait_bounded(&bars->full[s], (i / kBwdStages) & 1);
+    const int left = rows_end - (first_row + (i % per_head) * kBlock);  // rows of the block within the sequence
+    if (left < kBlock) {
+      __syncwarp();
+      clear_rows(sm + BwdSmem::kA + s * kBlockBytes, left, kBlock);
+      if (clear_b) clear_rows(sm + BwdSmem::kB + s * kBlockBytes, left, kBlock);
+    }
+    if (lane == 0) {
+      fence_after_sync();
+      const uint32_t col = tmem + 128 * (i & 1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_f16_ts(col + kColS, tmem + kColA + 8 * k, umma_desc_sw128(sa + s * kBlockBytes + 32 * k, 16, 1024), id,
+                   k > 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_f16_ts(col + kColDp, tmem + kColB + 8 * k, umma_desc_sw128(sb + s * kBlockBytes + 32 * k, 16, 1024), id,
+                   k > 0);
+      mma_commit(&bars->sd_full[i & 1]);
+    }
+  };
+  products(0);
+  if (blocks > 1) products(1);
+  for (int i = 0; i < blocks; ++i) {
+    const int s = i % kBwdStages;
+    if (lane == 0) {
+      ok = ok && mbar_wait_bounded(&bars->p_full[i & 1], (i >> 1) & 1);
+      fence_after_sync();
+      acc(i, s);
+      if (i + kBwdStages < blocks) mma_commit(&bars->empty[s]);
+      if (i + 1 == blocks) mma_commit(&bars->done);
+    }
+    if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
+    if (i + 2 < blocks) products(i + 2);
+  }
+  return ok;
+}
+
+}  // namespace pt
+
+template <typename T>
+__global__ void __launch_bounds__(pt::kBwdThreads, 1)
+    packed_bwd_dq_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmk,
+                            const __grid_constant__ CUtensorMap tmv, unsigned *top, int32_t *err) {
+  using namespace pt;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr uint32_t fmt = kHalf ? 0u : 1u;
+  const int h = blockIdx.x % a.Hq;
+  const int64_t slots = gridDim.x / a.Hq;
+  const PackedTile t = packed_find(a.cu, a.S, a.total, slots - 1 - blockIdx.x / a.Hq, kRows);
+  if (!t.valid) return;
+  const int rows = min(kRows, t.len - t.row0);
+  const int64_t first = t.start + t.row0, c_st = static_cast<int64_t>(a.Hq) * 64;
+  T *dq = static_cast<T *>(a.dq) + first * c_st + h * 64;
+  if (t.rest) {
+    zero_rows(dq, c_st, rows);
+    return;
+  }
+  extern __shared__ __align__(1024) char smem_raw[];
+  char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float *vec = reinterpret_cast<float *>(sm + BwdSmem::kVec);  // [128] delta, [128] max |dout|
+  BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hk = h / (a.Hq / a.Hkv);
+  const int blocks = min((t.len + kBlock - 1) / kBlock, t.row0 / kBlock + 2);
+  if (warp == 8) tmem_alloc(&bars->tmem, 512);
+  if (tid == 288) bwd_init(bars);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = bars->tmem;
+  const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
+  const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  bool ok = true;
+  if (warp == 9 && lane == 0)
+    bwd_copy(bars, sm, tmk, tmv, 0, min(blocks, kBwdStages), blocks, static_cast<int>(t.start), hk);
+  if (warp < 8) {
+    // the tile's rows: warpgroup 0 brings Q, warpgroup 1 dO and with O delta
+    uint4 raw[8];
+    if (wg == 0) {
+      row_to_tmem(static_cast<const T *>(a.q) + (first + r) * a.q_st + h * a.q_sh, r < rows, tmem + lane_base + kColA,
+                  raw);
+    } else {
+      row_to_tmem(static_cast<const T *>(a.dout) + (first + r) * a.g_st + h * a.g_sh, r < rows,
+                  tmem + lane_base + kColB, raw);
+      float delta = 0.f, big = 0.f;
+      if (r < rows) {
+        const T *o = static_cast<const T *>(a.out) + (first + r) * a.o_st + h * a.o_sh;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(o + 8 * e);
+          const T *po = reinterpret_cast<const T *>(&x), *pg = reinterpret_cast<const T *>(&raw[e]);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            delta = fmaf(to_f(po[u]), to_f(pg[u]), delta);
+            if (kHalf) big = fmaxf(big, fabsf(to_f(pg[u])));
+          }
+        }
+        a.delta[h * a.total + first + r] = delta;
+      }
+      vec[r] = delta;
+      if (kHalf) {
+        big = big < INFINITY ? big : 0.f;
+        vec[128 + r] = big;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        if (lane == 0) atomicMax(top, __float_as_uint(big));
+      }
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+
+  if (warp == 9) {
+    if (lane == 0)
+      ok = bwd_copy(bars, sm, tmk, tmv, min(blocks, kBwdStages), blocks, blocks, static_cast<int>(t.start), hk);
+    __syncwarp();
+  } else if (warp == 8) {
+    constexpr uint32_t id = idesc_f16(fmt, true, 64);
+    const uint32_t sk = smem_u32(sm + BwdSmem::kA);
+    ok = bwd_mma<T>(bars, sm, tmem, blocks, 0, t.len, blocks, false, [&](int i, int s) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_f16_ts(tmem + kColAcc, tmem + 128 * (i & 1) + kColS + 8 * k,
+                   umma_desc_sw128(sk + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
+    });
+  } else {
+    const uint32_t t_s = tmem + lane_base + 128 * wg;
+    const float delta = vec[r], lse = r < rows ? a.lse[h * a.total + first + r] : 0.f;
+    const float f = kHalf ? unit_scale(vec[128 + r]) : 1.f;
+    for (int i = wg; i < blocks; i += 2) {
+      ok = mbar_wait_bounded(&bars->sd_full[wg], (i >> 1) & 1);
+      if (__any_sync(0xffffffffu, !ok)) break;
+      fence_after_sync();
+      float s[64], d[64];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        tmem_ld32(t_s + kColS + 32 * u, s + 32 * u);
+        tmem_ld32(t_s + kColDp + 32 * u, d + 32 * u);
+      }
+      tmem_wait_ld();
+#pragma unroll
+      for (int u = 0; u < 64; u += 2) {
+        fma2(s[u], s[u + 1], a.scale_log2, -lse);
+        s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
+        add2(d[u], d[u + 1], -delta, -delta);
+        if (kHalf) mul2(d[u], d[u + 1], f, f);
+        mul2(d[u], d[u + 1], s[u], s[u + 1]);
+      }
+      if (i * kBlock + kBlock - 1 > t.row0) {  // the diagonal's two blocks
+        const int seen = t.row0 + r + 1 - i * kBlock;
+#pragma unroll
+        for (int u = 0; u < 64; ++u) d[u] = u < seen ? d[u] : 0.f;
+      }
+      float w[32];
+#pragma unroll
+      for (int u = 0; u < 32; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
+      tmem_st16(t_s + kColS, reinterpret_cast<const float(&)[16]>(w[0]));
+      tmem_st16(t_s + kColS + 16, reinterpret_cast<const float(&)[16]>(w[16]));
+      tmem_wait_st();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->p_full[wg]);
+    }
+    if (ok) {
+      ok = mbar_wait_bounded(&bars->done, 0);
+      fence_after_sync();
+    }
+  }
+  const bool failed = __syncthreads_or(!ok);
+  if (failed) bwd_failed(bars, err);
+  if (warp < 4) {
+    fence_after_sync();
+    const float back = failed ? __int_as_float(0x7fc00000) : a.scale / (kHalf ? unit_scale(vec[128 + r]) : 1.f);
+    store_row(dq + r * c_st, tmem + lane_base + kColAcc, back, r < rows);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(pt::kBwdThreads, 1)
+    packed_bwd_dkv_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
+                             const __grid_constant__ CUtensorMap tmg, const unsigned *top, int32_t *err) {
+  using namespace pt;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr uint32_t fmt = kHalf ? 0u : 1u;
+  const int hk = blockIdx.x % a.Hkv, group = a.Hq / a.Hkv;
+  // a sequence's first keys are seen by the most queries: they start first
+  const PackedTile t = packed_find(a.cu, a.S, a.total, blockIdx.x / a.Hkv, kRows);
+  if (!t.valid) return;
+  const int keys = min(kRows, t.len - t.row0);
+  const int64_t first = t.start + t.row0, c_st = static_cast<int64_t>(a.Hkv) * 64;
+  T *dk = static_cast<T *>(a.dk) + first * c_st + hk * 64, *dv = static_cast<T *>(a.dv) + first * c_st + hk * 64;
+  if (t.rest) {
+    zero_rows(dk, c_st, keys);
+    zero_rows(dv, c_st, keys);
+    return;
+  }
+  extern __shared__ __align__(1024) char smem_raw[];
+  char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float *vec = reinterpret_cast<float *>(sm + BwdSmem::kVec);
+  BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per_head = (t.len - t.row0 + kBlock - 1) / kBlock, blocks = per_head * group;
+  if (warp == 8) tmem_alloc(&bars->tmem, 512);
+  if (tid == 288) bwd_init(bars);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = bars->tmem;
+  const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
+  const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  bool ok = true;
+  if (warp == 9 && lane == 0)
+    bwd_copy(bars, sm, tmq, tmg, 0, min(blocks, kBwdStages), per_head, static_cast<int>(first), hk * group);
+  if (warp < 8) {
+    uint4 raw[8];
+    const T *src = wg == 0 ? static_cast<const T *>(a.k) + (first + r) * a.k_st + hk * a.k_sh
+                           : static_cast<const T *>(a.v) + (first + r) * a.v_st + hk * a.v_sh;
+    row_to_tmem(src, r < keys, tmem + lane_base + (wg == 0 ? kColA : kColB), raw);
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const float f = kHalf ? unit_scale(__uint_as_float(*top)) : 1.f;
+  if (warp == 9) {
+    if (lane == 0)
+      ok = bwd_copy(bars, sm, tmq, tmg, min(blocks, kBwdStages), blocks, per_head, static_cast<int>(first), hk * group);
+    __syncwarp();
+  } else if (warp == 8) {
+    constexpr uint32_t id = idesc_f16(fmt, true, 64);
+    const uint32_t sq = smem_u32(sm + BwdSmem::kA), sg = smem_u32(sm + BwdSmem::kB);
+    ok = bwd_mma<T>(bars, sm, tmem, blocks, t.row0, t.len, per_head, true, [&](int i, int s) {
+      const uint32_t col = tmem + 128 * (i & 1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_f16_ts(tmem + kColAcc, col + kColS + 8 * k,
+                   umma_desc_sw128(sg + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_f16_ts(tmem + kColAcc2, col + kColDp + 8 * k,
+                   umma_desc_sw128(sq + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
+    });
+  } else {
+    const uint32_t t_s = tmem + lane_base + 128 * wg, bar_id = 1 + wg;
+    // the block's log sums and deltas, negated: thread r < 64 brings query r's sum, r >= 64 query r - 64's delta
+    const float *src = r < 64 ? a.lse : a.delta;
+    auto fetch = [&](int i) {
+      const int qr = t.row0 + (i % per_head) * kBlock + (r & 63);
+      return i < blocks && qr < t.len
+                 ? -src[(hk * group + i / per_head) * a.total + t.start + qr] : 0.f;
+    };
+    float next = fetch(wg);
+    for (int i = wg; i < blocks; i += 2) {
+      float *mine = vec + wg * 256 + ((i >> 1) & 1) * 128;
+      mine[r] = next;
+      // the vectors are there; and a wait that expired in one warp ends them all
+      uint32_t bad;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 128, q;\n\t"
+                   "selp.u32 %0, 1, 0, p;\n\t}"
+                   : "=r"(bad)
+                   : "r"(ok ? 0u : 1u), "r"(bar_id)
+                   : "memory");
+      if (bad) {
+        ok = false;
+        break;
+      }
+      next = fetch(i + 2);
+      ok = mbar_wait_bounded(&bars->sd_full[wg], (i >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      fence_after_sync();
+      const int q0 = (i % per_head) * kBlock;  // from the tile's first key
+      const bool edge = q0 < kRows || t.row0 + q0 + kBlock > t.len;
+      const int from = r - q0, to = t.len - t.row0 - q0;  // visible columns: from .. to - 1
+      float s[64], d[64];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        tmem_ld32(t_s + kColS + 32 * u, s + 32 * u);
+        tmem_ld32(t_s + kColDp + 32 * u, d + 32 * u);
+      }
+      tmem_wait_ld();
+#pragma unroll
+      for (int u = 0; u < 64; u += 4) {
+        const float4 l4 = *reinterpret_cast<const float4 *>(mine + u), d4 = *reinterpret_cast<const float4 *>(mine + 64 + u);
+        fma2v(s[u], s[u + 1], a.scale_log2, l4.x, l4.y);
+        fma2v(s[u + 2], s[u + 3], a.scale_log2, l4.z, l4.w);
+        add2(d[u], d[u + 1], d4.x, d4.y);
+        add2(d[u + 2], d[u + 3], d4.z, d4.w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u + e] = ex2(s[u + e]);
+        if (kHalf) {
+          mul2(d[u], d[u + 1], f, f);
+          mul2(d[u + 2], d[u + 3], f, f);
+        }
+        mul2(d[u], d[u + 1], s[u], s[u + 1]);
+        mul2(d[u + 2], d[u + 3], s[u + 2], s[u + 3]);
+      }
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < 64; ++u) {
+          const bool seen = u >= from && u < to;
+          s[u] = seen ? s[u] : 0.f;
+          d[u] = seen ? d[u] : 0.f;
+        }
+      }
+      float w[32];
+#pragma unroll
+      for (int u = 0; u < 32; ++u) w[u] = __uint_as_float(pack2<T>(s[2 * u], s[2 * u + 1]));
+      tmem_st16(t_s + kColS, reinterpret_cast<const float(&)[16]>(w[0]));
+      tmem_st16(t_s + kColS + 16, reinterpret_cast<const float(&)[16]>(w[16]));
+#pragma unroll
+      for (int u = 0; u < 32; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
+      tmem_st16(t_s + kColDp, reinterpret_cast<const float(&)[16]>(w[0]));
+      tmem_st16(t_s + kColDp + 16, reinterpret_cast<const float(&)[16]>(w[16]));
+      tmem_wait_st();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0 && ok) mbar_arrive(&bars->p_full[wg]);
+    }
+    if (ok) {
+      ok = mbar_wait_bounded(&bars->done, 0);
+      fence_after_sync();
+    }
+  }
+  const bool failed = __syncthreads_or(!ok);
+  if (failed) bwd_failed(bars, err);
+  if (warp < 8) {
+    fence_after_sync();
+    const float back = failed ? __int_as_float(0x7fc00000) : wg == 0 ? 1.f : a.scale / f;
+    store_row((wg == 0 ? dv : dk) + r * c_st, tmem + lane_base + (wg == 0 ? kColAcc : kColAcc2), back, r < keys);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Map of a packed tensor [total][H][64]: boxes of `box` rows of one head.
+static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total, int64_t H, int64_t st, int64_t sh,
+                      int box) {
   if (H == 1 && sh <= 0) sh = 64;
   if (total == 1 && st <= 0) st = sh * H;
-  return encode_rows_map(map, p, dtype, 64, total, H, 1, st, sh, st, pt::kRows);
+  return encode_rows_map(map, p, dtype, 64, total, H, 1, st, sh, st, box);
 }
 
 int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
   CUtensorMap mq, mk, mv;
-  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh);
-  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh);
-  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh);
+  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh, pt::kRows);
+  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kRows);
+  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh, pt::kRows);
   if (rc != SD_OK) return rc;
   const int64_t ctas = packed_slots(a.total, a.S, 2 * pt::kRows) * a.Hq;
   if (ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
@@ -357,6 +821,39 @@ int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
     return check_launch();
   };
   return dtype == SD_DTYPE_BF16 ? run(packed_fwd_tc_kernel<__nv_bfloat16>) : run(packed_fwd_tc_kernel<__half>);
+}
+
+int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
+  CUtensorMap mq, mk, mv, mg;
+  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh, pt::kBlock);
+  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kBlock);
+  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh, pt::kBlock);
+  if (rc == SD_OK) rc = packed_map(&mg, a.dout, dtype, a.total, a.Hq, a.g_st, a.g_sh, pt::kBlock);
+  if (rc != SD_OK) return rc;
+  const int64_t slots = packed_slots(a.total, a.S, pt::kRows);
+  if (slots * a.Hq > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
+  // fp16: the largest |dout|, in the word behind delta
+  unsigned *top = reinterpret_cast<unsigned *>(a.delta + a.Hq * a.total);
+  if (dtype == SD_DTYPE_F16) {
+    const cudaError_t e = cudaMemsetAsync(top, 0, sizeof(*top), s);
+    if (e != cudaSuccess) {
+      set_cuda_error(e);
+      cudaGetLastError();
+      return SD_ERR_CUDA;
+    }
+  }
+  const size_t smem = pt::BwdSmem::kBytes + 1024;
+  auto run = [&](auto *dq, auto *dkv) {
+    if (set_max_smem(dq, smem) != SD_OK || set_max_smem(dkv, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
+    dq<<<static_cast<unsigned>(slots * a.Hq), pt::kBwdThreads, smem, s>>>(a, mk, mv, top, err);
+    const int first = check_launch();
+    if (first != SD_OK) return first;
+    dkv<<<static_cast<unsigned>(slots * a.Hkv), pt::kBwdThreads, smem, s>>>(a, mq, mg, top, err);
+    return check_launch();
+  };
+  return dtype == SD_DTYPE_BF16
+             ? run(packed_bwd_dq_tc_kernel<__nv_bfloat16>, packed_bwd_dkv_tc_kernel<__nv_bfloat16>)
+             : run(packed_bwd_dq_tc_kernel<__half>, packed_bwd_dkv_tc_kernel<__half>);
 }
 
 }  // namespace sd

@@ -748,7 +748,7 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     dv = torch.empty_like(dk)
     if total:
         q, k, v, out, dout = (_rows16(t) for t in (q, k, v, out, dout))
-        delta = torch.empty_like(lse)
+        delta = torch.empty(hq * total + 1, dtype=torch.float32, device=q.device)
         with guard:
             L.call("sd_packed_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                    dout.data_ptr(), code, total, hq, hkv, d, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
