@@ -4,7 +4,7 @@
 // A pool holds pages of `page` tokens, k_pages and v_pages [P][Hkv][page][64]
 // (any strides with an innermost one of 1).  Position t of sequence b lies in
 // page table[b][t / page], row t % page.
-#include "sd_common.cuh"
+#include "sd_tma.cuh"
 
 namespace sd {
 
@@ -85,91 +85,426 @@ __global__ void __launch_bounds__(256)
   *reinterpret_cast<uint4 *>(v_pages + off + c) = *reinterpret_cast<const uint4 *>(xv + n * v_sn + h * v_sh + c);
 }
 
-// One CTA of 128 threads per (sequence, kv head, 16 query heads of it).
+// ---------------------------------------------------------------- decode
+//   out = sum_t exp2(c q.k_t - m) v_t / sum_t exp2(c q.k_t - m),  c = scale log2(e)
+//
+// HBM-bound: every cached K and V row is read once for all the query heads of
+// its kv head.  The work is cut into units (sequence, head group, 64 tokens;
+// 32 in fp32), numbered in that order, and each of 3 CTAs an SM takes an equal
+// run of them, whatever the lengths are: a CTA may end one sequence's head,
+// do several and begin another.  What a CTA holds of a head whole it writes out
+// itself; the other parts (running maximum, sum, weighted values) go to the
+// workspace, and a second kernel joins them in order.
+//
+// A warp owns a quarter of every unit's tokens with its own copies (cp.async,
+// 16 bytes a lane, kStages units ahead, page ids looked up one unit earlier
+// still) and its own softmax state, so the loop has no block barrier; the four
+// states meet at the end of a head.  16-bit products are mma.sync m16n8k16 with
+// up to 16 query heads as the rows (a kv head has few: a 128-row tcgen05 tile
+// would be mostly padding, and the tensor pipe is not what bounds this).
+namespace pg {
+
+constexpr int kThreads = 128, kWarps = 4, kStages = 4;
+constexpr int kMaxHeads = 16;                // query heads of a group
+constexpr int kCtas = 148 * 3;
+constexpr int kMaxSeqs = 2048;               // sequences of a launch (two ints each in shared memory)
+constexpr int kPart = 66;                    // m, l, 64 values
+constexpr int kWarpBytes = 4096;             // a warp's K and V rows of one unit
+template <typename T> constexpr int kUnit = sizeof(T) == 2 ? 64 : 32;
+
+struct DecodeArgs {
+  const void *q;
+  int64_t q_sb, q_sh;
+  const void *k, *v;
+  void *out;
+  int64_t o_sb, o_sh;
+  float scale_log2;
+  int G, Hh;           // query heads of a group, groups of all kv heads (Hkv x groups a kv head)
+  uint32_t page_inv;   // floor(2^32 / page), 2^32 - 1 for a page of 1
+  int32_t *plan;       // [B + 1] units before each sequence (of one head group), then units a CTA
+  float *parts;        // [kCtas][2][G][kPart]
+};
+
+struct Cursor {
+  int b, hh, tile;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool held) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(held ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// t / page: the estimate is never above and at most one below for t < 2^31.
+__device__ __forceinline__ int page_of(int t, int page, uint32_t inv) {
+  int p = static_cast<int>(__umulhi(static_cast<uint32_t>(t), inv));
+  return t - p * page >= page ? p + 1 : p;
+}
+
+// Joins (m, l) pairs: the factors of both sides.
+__device__ __forceinline__ float factor(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+
+}  // namespace pg
+
 template <typename T>
-__global__ void __launch_bounds__(128)
-    paged_decode_kernel(PagedArgs a, const T *q, int64_t q_sb, int64_t q_sh, const T *k_pages, const T *v_pages,
-                        float scale_log2, T *out, int64_t o_sb, int64_t o_sh) {
-  constexpr int kG = 16, kPitch = 68;
-  __shared__ float sq[kG][64], sp[kG][64], sm_[kG], sl[kG], sa[kG];
-  __shared__ float kv[64 * kPitch];
-  const int b = blockIdx.z, hk = blockIdx.y, g0 = blockIdx.x * kG;
-  const int group = a.Hq / a.Hkv, G = min(kG, group - g0), h0 = hk * group + g0;
+__global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const PagedArgs a, const pg::DecodeArgs d) {
+  using namespace pg;
+  constexpr bool k16 = sizeof(T) == 2;
+  constexpr int kTok = kUnit<T>, kMine = kTok / kWarps;  // tokens of a unit, and of a warp
+  constexpr int kRow = 64 * sizeof(T), kChunks = kRow / 16, kRowsAt = 32 / kChunks;  // rows of one copy of a warp
+  constexpr int kCopies = kMine / kRowsAt;
+  extern __shared__ __align__(128) char sm[];
+  char *ring = sm;                                                   // [warp][stage][K rows | V rows]
+  uint8_t *held = reinterpret_cast<uint8_t *>(sm + kWarps * kStages * kWarpBytes);  // [warp][stage][16]
+  float *merge = reinterpret_cast<float *>(held + kWarps * kStages * 16);           // [warp][G][kPart]
+  float *sq = merge + kWarps * d.G * kPart;                          // fp32: [G][64]
+  int *pre = reinterpret_cast<int *>(k16 ? sq : sq + d.G * 64), *len = pre + a.B + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int len = pg::seq_len(a, b);
-  for (int e = tid; e < G * 64; e += 128) sq[e >> 6][e & 63] = to_f(q[b * q_sb + (h0 + (e >> 6)) * q_sh + (e & 63)]);
-  if (tid < kG) sm_[tid] = -INFINITY, sl[tid] = 0.f;
-  float acc[kG] = {};
-  for (int t0 = 0; t0 < len; t0 += 64) {
-    const int n = min(64, len - t0);
-    auto load = [&](const T *src) {
-      constexpr int kVec = 16 / sizeof(T), kChunks = 64 / kVec;
-      for (int e = tid; e < 64 * kChunks; e += 128) {
-        const int r = e / kChunks, c = e % kChunks * kVec;
-        const int64_t off = r < n ? pg::row_of(a, b, hk, t0 + r) : -1;
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (off >= 0) raw = *reinterpret_cast<const uint4 *>(src + off + c);
-        const T *p = reinterpret_cast<const T *>(&raw);
-        for (int u = 0; u < kVec; ++u) kv[r * kPitch + c + u] = to_f(p[u]);
+
+  // ---- lengths, and the units before each sequence
+  {
+    __shared__ int sums[kWarps];
+    int run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+      const int b = b0 + tid;
+      const int n = b < a.B ? seq_len(a, b) : 0;
+      int x = (n + kTok - 1) / kTok;
+      const int own = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
       }
-    };
-    __syncthreads();
-    load(k_pages);
-    __syncthreads();
-    const int r = tid >> 1, d0 = (tid & 1) * 32;
-    bool held = r < n;
-    if (held && pg::row_of(a, b, hk, t0 + r) < 0) {
-      pg::report(a.err, SD_KERR_BOUNDS);
-      held = false;
+      if (lane == 31) sums[warp] = x;
+      __syncthreads();
+      int before = run, all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sums[w];
+        all += sums[w];
+      }
+      if (b < a.B) {
+        pre[b] = before + x - own;
+        len[b] = n;
+      }
+      run += all;
+      __syncthreads();
     }
-    for (int g = 0; g < G; ++g) {
-      float s = 0.f;
-      for (int d = 0; d < 32; ++d) s = fmaf(sq[g][d0 + d], kv[r * kPitch + d0 + d], s);
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      if (d0 == 0) sp[g][r] = held ? s * scale_log2 : -INFINITY;
-    }
+    if (tid == 0) pre[a.B] = run;
     __syncthreads();
-    load(v_pages);
-    for (int g = warp; g < G; g += 4) {
-      const float s0 = sp[g][lane], s1 = sp[g][lane + 32];
-      float mt = fmaxf(s0, s1);
-      for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-      const float mn = fmaxf(sm_[g], mt), ref = mn == -INFINITY ? 0.f : mn;
-      const float p0 = exp2f(s0 - ref), p1 = exp2f(s1 - ref);
-      float ps = p0 + p1;
-      for (int o = 16; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-      sp[g][lane] = p0, sp[g][lane + 32] = p1;
-      __syncwarp();
-      if (lane == 0) {
-        sa[g] = exp2f(sm_[g] - ref);
-        sl[g] = sl[g] * sa[g] + ps;
-        sm_[g] = mn;
+  }
+  const int64_t units = static_cast<int64_t>(pre[a.B]) * d.Hh;
+  const int64_t per = (units + gridDim.x - 1) / gridDim.x;
+  if (blockIdx.x == 0) {
+    for (int b = tid; b <= a.B; b += kThreads) d.plan[b] = pre[b];
+    if (tid == 0) d.plan[a.B + 1] = static_cast<int>(per);
+  }
+  const int64_t u0 = blockIdx.x * per, u1 = u0 + per < units ? u0 + per : units;
+  if (u0 >= u1) return;
+
+  // ---- the first unit
+  Cursor at;
+  {
+    int lo = 0, hi = a.B;  // the last b with pre[b] * Hh <= u0 that has units
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (static_cast<int64_t>(pre[mid]) * d.Hh <= u0) lo = mid; else hi = mid;
+    }
+    const int tiles = pre[lo + 1] - pre[lo];
+    const int64_t in = u0 - static_cast<int64_t>(pre[lo]) * d.Hh;
+    at = {lo, static_cast<int>(in / tiles), static_cast<int>(in % tiles)};
+  }
+  auto advance = [&](Cursor &c) {
+    if (++c.tile < pre[c.b + 1] - pre[c.b]) return;
+    c.tile = 0;
+    if (++c.hh < d.Hh) return;
+    c.hh = 0;
+    do ++c.b;
+    while (c.b < a.B && pre[c.b + 1] == pre[c.b]);
+  };
+  const int groups = d.Hh / a.Hkv;  // groups of a kv head
+
+  // ---- copies: this lane's rows of a unit
+  const int row0 = lane / kChunks, chunk = lane % kChunks;
+  Cursor ld = at;
+  int64_t left = u1 - u0;  // units not yet looked up
+  int page[kCopies];
+  bool more = false;
+  Cursor ld_at;
+  auto lookup = [&]() {  // the page ids of unit ld (used when it is copied, a unit later)
+    more = left > 0;
+    if (!more) return;
+    ld_at = ld;
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j) {
+      const int t = ld.tile * kTok + warp * kMine + row0 + kRowsAt * j;
+      page[j] = t < len[ld.b] ? a.table[ld.b * a.t_sb + page_of(t, a.page, d.page_inv)] : -1;
+    }
+    advance(ld);
+    --left;
+  };
+  char *mine = ring + warp * kStages * kWarpBytes;
+  uint8_t *mine_held = held + warp * kStages * 16;
+  auto copy = [&](int stage) {
+    if (more) {
+      const uint32_t dst = smem_u32(mine + stage * kWarpBytes);
+      const int hk = ld_at.hh / groups;
+#pragma unroll
+      for (int j = 0; j < kCopies; ++j) {
+        const int r = row0 + kRowsAt * j, t = ld_at.tile * kTok + warp * kMine + r;
+        const bool ok = page[j] >= 0 && page[j] < a.pages;
+        if (!ok && t < len[ld_at.b]) report(a.err, SD_KERR_BOUNDS);
+        const int64_t off =
+            ok ? page[j] * a.p_sp + hk * a.p_sh + (t - page_of(t, a.page, d.page_inv) * a.page) * a.p_st : 0;
+        // chunks change places by row so that a warp's reads meet no bank twice
+        const uint32_t to = dst + r * kRow + ((chunk ^ (k16 ? r & 7 : (r & 1) * 4)) << 4);
+        cp16(to, static_cast<const T *>(d.k) + off + chunk * (16 / sizeof(T)), ok);
+        cp16(to + kWarpBytes / 2, static_cast<const T *>(d.v) + off + chunk * (16 / sizeof(T)), ok);
+        if (chunk == 0) mine_held[stage * 16 + r] = ok;
       }
     }
-    __syncthreads();
-    const int d = tid & 63, k0 = (tid >> 6) * 32;
-    for (int g = 0; g < kG; ++g) {
-      if (g >= G) break;
-      float s = 0.f;
-      for (int k = k0; k < k0 + 32; ++k) s = fmaf(sp[g][k], kv[k * kPitch + d], s);
-      acc[g] = acc[g] * sa[g] + s;
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    lookup();
+    copy(s);
+  }
+  lookup();
+
+  // ---- state of the current head group
+  // 16-bit: fragments of m16n8k16, rows lane / 4 and lane / 4 + 8 are heads;
+  // fp32: every lane keeps all heads, columns 2 lane and 2 lane + 1
+  constexpr int kAcc = k16 ? 8 : kMaxHeads, kAccN = k16 ? 4 : 2, kStat = k16 ? 2 : kMaxHeads;
+  float o[kAcc][kAccN], m[kStat], l[kStat];
+  uint32_t qa[4][4];
+  const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+  auto begin = [&](const Cursor &c) {
+    const int h0 = (c.hh / groups) * (a.Hq / a.Hkv) + (c.hh % groups) * kMaxHeads;
+    const int n = min(d.G, (a.Hq / a.Hkv) - (c.hh % groups) * kMaxHeads);
+    const T *src = static_cast<const T *>(d.q) + c.b * d.q_sb + h0 * d.q_sh;
+    if constexpr (k16) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int g = r0 + (e & 1) * 8, col = 16 * k + c0 + (e >> 1) * 8;
+          qa[k][e] = g < n ? *reinterpret_cast<const uint32_t *>(src + g * d.q_sh + col) : 0u;
+        }
+    } else {
+      __syncthreads();
+      for (int e = tid; e < n * 64; e += kThreads) sq[e] = src[(e >> 6) * d.q_sh + (e & 63)];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kAcc; ++i)
+#pragma unroll
+      for (int e = 0; e < kAccN; ++e) o[i][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kStat; ++i) m[i] = -INFINITY, l[i] = 0.f;
+  };
+  begin(at);
+  int first_tile = at.tile;
+  const float c = d.scale_log2;
+
+  for (int64_t u = u0; u < u1; ++u) {
+    const int it = static_cast<int>(u - u0), stage = it % kStages;
+    copy((it + kStages - 1) % kStages);
+    lookup();
+    cp_wait<kStages - 1>();
+    __syncwarp();
+    const char *kt = mine + stage * kWarpBytes, *vt = kt + kWarpBytes / 2;
+    const uint8_t *ok = mine_held + stage * 16;
+    if constexpr (k16) {
+      float s[2][4];
+      const uint32_t kb = smem_u32(kt), vb = smem_u32(vt);
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+        uint32_t b0, b1, b2, b3;
+        const int key = 8 * nt + (lane & 7);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          ldsm_x4(kb + sw128(key, 4 * half + (lane >> 3)), b0, b1, b2, b3);
+          mma16816<T>(s[nt], qa[2 * half], b0, b1);
+          mma16816<T>(s[nt], qa[2 * half + 1], b2, b3);
+        }
+        const uint32_t flags = *reinterpret_cast<const uint16_t *>(ok + 8 * nt + c0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[nt][e] = (e & 1 ? flags >> 8 : flags & 0xff) ? s[nt][e] * c : -INFINITY;
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float best = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+        const float mn = fmaxf(m[half], best), ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = exp2f(m[half] - ref);
+        m[half] = mn;
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = exp2f(s[e >> 1][2 * half + (e & 1)] - ref);
+        l[half] = l[half] * alpha + ((p[0] + p[1]) + (p[2] + p[3]));
+        pa[half] = pack2<T>(p[0], p[1]);
+        pa[2 + half] = pack2<T>(p[2], p[3]);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          o[n][2 * half] *= alpha;
+          o[n][2 * half + 1] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4_t(vb + sw128(lane & 15, 2 * n + (lane >> 4)), b0, b1, b2, b3);
+        mma16816<T>(o[2 * n], pa, b0, b1);
+        mma16816<T>(o[2 * n + 1], pa, b2, b3);
+      }
+    } else {
+      const int key = lane >> 2, quarter = lane & 3, flip = (key & 1) * 4;
+      float4 kr[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        kr[i] = *reinterpret_cast<const float4 *>(kt + key * kRow + (((4 * i + quarter) ^ flip) << 4));
+      float2 vr[kMine];
+#pragma unroll
+      for (int r = 0; r < kMine; ++r)
+        vr[r] = *reinterpret_cast<const float2 *>(vt + r * kRow + (((lane >> 1) ^ ((r & 1) * 4)) << 4) + (lane & 1) * 8);
+      const bool seen = ok[key];
+#pragma unroll
+      for (int g = 0; g < kMaxHeads; ++g) {
+        if (g >= d.G) break;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 x = *reinterpret_cast<const float4 *>(sq + g * 64 + (4 * i + quarter) * 4);
+          s = fmaf(x.x, kr[i].x, fmaf(x.y, kr[i].y, fmaf(x.z, kr[i].z, fmaf(x.w, kr[i].w, s))));
+        }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        s = seen ? s * c : -INFINITY;
+        float best = s;
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, w));
+        const float mn = fmaxf(m[g], best), ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = exp2f(m[g] - ref), p = exp2f(s - ref);
+        float sum = p;
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        m[g] = mn;
+        l[g] = l[g] * alpha + sum;
+        o[g][0] *= alpha, o[g][1] *= alpha;
+#pragma unroll
+        for (int r = 0; r < kMine; ++r) {
+          const float w = __shfl_sync(0xffffffffu, p, 4 * r);
+          o[g][0] = fmaf(w, vr[r].x, o[g][0]);
+          o[g][1] = fmaf(w, vr[r].y, o[g][1]);
+        }
+      }
+    }
+    __syncwarp();
+    const int tiles = pre[at.b + 1] - pre[at.b];
+    const bool head_ends = at.tile + 1 == tiles;
+    if (head_ends || u + 1 == u1) {
+      // the four warps' states of this head group meet
+      float *to = merge + warp * d.G * kPart;
+      if constexpr (k16) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+          l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+          const int g = r0 + 8 * half;
+          if (g < d.G) {
+            if (c0 == 0) to[g * kPart] = m[half], to[g * kPart + 1] = l[half];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              to[g * kPart + 2 + 8 * n + c0] = o[n][2 * half];
+              to[g * kPart + 2 + 8 * n + c0 + 1] = o[n][2 * half + 1];
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kMaxHeads; ++g) {
+          if (g >= d.G) break;
+          if (lane == 0) to[g * kPart] = m[g], to[g * kPart + 1] = l[g];
+          to[g * kPart + 2 + 2 * lane] = o[g][0];
+          to[g * kPart + 2 + 2 * lane + 1] = o[g][1];
+        }
+      }
+      __syncthreads();
+      const bool whole = first_tile == 0 && head_ends;
+      const int sub = at.hh % groups, h0 = (at.hh / groups) * (a.Hq / a.Hkv) + sub * kMaxHeads;
+      const int n = min(d.G, (a.Hq / a.Hkv) - sub * kMaxHeads);
+      // a part that begins with the CTA's run is its slot 0, one that begins later slot 1
+      float *part = d.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (u - (at.tile - first_tile) == u0 ? 0 : 1)) *
+                                  d.G * kPart;
+      for (int g = tid >> 6; g < n; g += kThreads / 64) {
+        const int e = tid & 63;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, merge[(w * d.G + g) * kPart]);
+        float sum = 0.f, val = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float *p = merge + (w * d.G + g) * kPart;
+          const float f = factor(p[0], top);
+          sum = fmaf(f, p[1], sum);
+          val = fmaf(f, p[2 + e], val);
+        }
+        if (whole) {
+          static_cast<T *>(d.out)[at.b * d.o_sb + (h0 + g) * d.o_sh + e] = from_f<T>(sum == 0.f ? 0.f : val / sum);
+        } else {
+          if (e == 0) part[g * kPart] = top, part[g * kPart + 1] = sum;
+          part[g * kPart + 2 + e] = val;
+        }
+      }
+      __syncthreads();
+      advance(at);
+      if (u + 1 < u1) {
+        begin(at);
+        first_tile = 0;
+      }
+    } else {
+      ++at.tile;
     }
   }
-  __syncthreads();
-  for (int g = 0; g < kG; ++g)
-    if (g < G) sp[g][tid & 63] = 0.f;
-  __syncthreads();
-  if (tid >= 64)
-    for (int g = 0; g < kG; ++g)
-      if (g < G) sp[g][tid & 63] = acc[g];
-  __syncthreads();
-  if (tid < 64)
-    for (int g = 0; g < kG; ++g)
-      if (g < G) {
-        const float l = sl[g];
-        // a sequence without tokens gives zeros
-        out[b * o_sb + (h0 + g) * o_sh + tid] = from_f<T>(l == 0.f ? 0.f : (acc[g] + sp[g][tid]) / l);
-      }
+  cp_wait<0>();
+}
+
+// Joins the parts of the head groups that were split over CTAs, and zeros the
+// rows of sequences without tokens.  One CTA per (head group, sequence).
+template <typename T> __global__ void __launch_bounds__(64) paged_join_kernel(const PagedArgs a, const pg::DecodeArgs d) {
+  using namespace pg;
+  pdl_wait();
+  const int b = blockIdx.y, hh = blockIdx.x, groups = d.Hh / a.Hkv, e = threadIdx.x;
+  const int h0 = (hh / groups) * (a.Hq / a.Hkv) + (hh % groups) * kMaxHeads;
+  const int n = min(d.G, (a.Hq / a.Hkv) - (hh % groups) * kMaxHeads);
+  T *out = static_cast<T *>(d.out) + b * d.o_sb + h0 * d.o_sh;
+  const int64_t tiles = d.plan[b + 1] - d.plan[b], per = d.plan[a.B + 1];
+  if (tiles == 0) {
+    for (int g = 0; g < n; ++g) out[g * d.o_sh + e] = from_f<T>(0.f);
+    return;
+  }
+  const int64_t u0 = static_cast<int64_t>(d.plan[b]) * d.Hh + hh * tiles, u1 = u0 + tiles;
+  const int64_t c0 = u0 / per, c1 = (u1 - 1) / per;
+  if (c0 == c1) return;
+  for (int g = 0; g < n; ++g) {
+    float top = -INFINITY;
+    auto part = [&](int64_t i) { return d.parts + ((i * 2 + (i * per < u0 ? 1 : 0)) * d.G + g) * kPart; };
+    for (int64_t i = c0; i <= c1; ++i) top = fmaxf(top, part(i)[0]);
+    float sum = 0.f, val = 0.f;
+    for (int64_t i = c0; i <= c1; ++i) {
+      const float *p = part(i);
+      const float f = factor(p[0], top);
+      sum = fmaf(f, p[1], sum);
+      val = fmaf(f, p[2 + e], val);
+    }
+    out[g * d.o_sh + e] = from_f<T>(sum == 0.f ? 0.f : val / sum);
+  }
 }
 
 static int check_pool(const PagedArgs &a, int dtype, int64_t D, const void *k, const void *v) {
@@ -211,8 +546,11 @@ int sd_paged_append(const void *xk, const void *xv, int dtype, int64_t N, int64_
 }
 
 int sd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t *bytes) {
-  if (!bytes || B <= 0 || Hq <= 0 || Hkv <= 0) return SD_ERR_INVALID;
-  *bytes = 0;
+  using namespace sd;
+  if (!bytes || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return SD_ERR_INVALID;
+  const int64_t seqs = B < pg::kMaxSeqs ? B : pg::kMaxSeqs, group = Hq / Hkv;
+  const int64_t heads = group < pg::kMaxHeads ? group : pg::kMaxHeads;
+  *bytes = ((seqs + 2) * 4 + 15) / 16 * 16 + static_cast<int64_t>(pg::kCtas) * 2 * heads * pg::kPart * 4;
   return SD_OK;
 }
 
@@ -222,25 +560,54 @@ int sd_paged_decode_attention(const void *q, int dtype, int64_t B, int64_t Hq, i
                               int width, const int32_t *lens, float scale, void *out, int64_t o_sb, int64_t o_sh,
                               void *workspace, int64_t workspace_bytes, int32_t *err, void *stream) {
   using namespace sd;
-  (void)workspace, (void)workspace_bytes;
-  if (!q || !out || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || !(scale > 0.f) || scale > 3.0e38f)
+  if (!q || !out || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || !(scale > 0.f) || scale > 3.0e38f || !workspace)
     return SD_ERR_INVALID;
-  if (B > 65535 || Hq > 65535) return SD_ERR_UNSUPPORTED;
+  if (B > 0x7fffffff || Hq > 65535) return SD_ERR_UNSUPPORTED;
   PagedArgs a = {table, t_sb, width, lens, static_cast<int>(B), static_cast<int>(Hq), static_cast<int>(Hkv), page,
                  pages, p_sp, p_sh, p_st, err};
   int rc = check_pool(a, dtype, D, k_pages, v_pages);
   if (rc != SD_OK) return rc;
+  int64_t need = 0;
+  sd_paged_decode_workspace(B, Hq, Hkv, &need);
+  if (workspace_bytes < need) return SD_ERR_INVALID;
   const int64_t size = dtype_size(dtype);
-  if (!aligned16(q) || !aligned16(out) || (q_sb * size) % 16 || (q_sh * size) % 16 || (o_sb * size) % 16 ||
-      (o_sh * size) % 16)
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (q_sb * size) % 16 || (q_sh * size) % 16 ||
+      (o_sb * size) % 16 || (o_sh * size) % 16)
     return SD_ERR_ALIGN;
-  const unsigned heads = static_cast<unsigned>((Hq / Hkv + 15) / 16);
-  SD_DISPATCH_DTYPE(dtype, T, {
-    paged_decode_kernel<T><<<dim3(heads, a.Hkv, a.B), 128, 0, static_cast<cudaStream_t>(stream)>>>(
-        a, static_cast<const T *>(q), q_sb, q_sh, static_cast<const T *>(k_pages), static_cast<const T *>(v_pages),
-        scale * 1.4426950408889634f, static_cast<T *>(out), o_sb, o_sh);
-  });
-  return check_launch();
+  const int group = a.Hq / a.Hkv;
+  pg::DecodeArgs d = {};
+  d.q_sb = q_sb, d.q_sh = q_sh, d.k = k_pages, d.v = v_pages, d.o_sb = o_sb, d.o_sh = o_sh;
+  d.scale_log2 = scale * 1.4426950408889634f;
+  d.G = group < pg::kMaxHeads ? group : pg::kMaxHeads;
+  d.Hh = a.Hkv * ((group + pg::kMaxHeads - 1) / pg::kMaxHeads);
+  d.page_inv = page == 1 ? 0xffffffffu : static_cast<uint32_t>((1ull << 32) / static_cast<uint64_t>(page));
+  const int64_t tokens = static_cast<int64_t>(width) * page;
+  // more sequences than one launch plans: the launches follow each other on the stream
+  for (int64_t b0 = 0; b0 < B; b0 += pg::kMaxSeqs) {
+    a.B = static_cast<int>(B - b0 < pg::kMaxSeqs ? B - b0 : pg::kMaxSeqs);
+    a.table = table + b0 * t_sb;
+    a.lens = lens + b0;
+    d.plan = static_cast<int32_t *>(workspace);
+    d.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + ((a.B + 2) * 4 + 15) / 16 * 16);
+    SD_DISPATCH_DTYPE(dtype, T, {
+      d.q = static_cast<const T *>(q) + b0 * q_sb;
+      d.out = static_cast<T *>(out) + b0 * o_sb;
+      // the plan counts units of one head group in 32 bits
+      const int64_t most = static_cast<int64_t>(a.B) * ((tokens + pg::kUnit<T> - 1) / pg::kUnit<T>);
+      if (most > 0x3fffffffll) return SD_ERR_UNSUPPORTED;
+      const unsigned ctas = static_cast<unsigned>(most * d.Hh < pg::kCtas ? most * d.Hh : pg::kCtas);
+      const size_t smem = pg::kWarps * pg::kStages * (pg::kWarpBytes + 16) + pg::kWarps * d.G * pg::kPart * 4 +
+                          (sizeof(T) == 4 ? d.G * 256 : 0) + (2 * a.B + 1) * 4;
+      auto kern = paged_decode_kernel<T>;
+      if (set_max_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
+      kern<<<ctas, pg::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a, d);
+      rc = check_launch();
+      if (rc != SD_OK) return rc;
+      rc = launch(paged_join_kernel<T>, dim3(d.Hh, a.B), dim3(64), 0, static_cast<cudaStream_t>(stream), true, a, d);
+      if (rc != SD_OK) return rc;
+    });
+  }
+  return SD_OK;
 }
 
 }  // extern "C"
