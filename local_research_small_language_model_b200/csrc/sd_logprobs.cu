@@ -5,47 +5,79 @@
 //   log p_j = x_j - m - log s,   H = log s - w / s
 //   d/dx_j (g log p_t + h H) = g [j = t] - p_j (g + h (log p_j + H))
 //
-// m, s and w come from one pass over the row (s and w are rescaled when m
-// rises), in fp32.  A logit of -inf has probability 0 and adds nothing; a row
-// with a NaN, a +inf or nothing but -inf has NaN results, as log_softmax.
+// m, s and w come from one pass over the row in fp32 (s and w are rescaled when
+// m rises).  x - m is formed before it is scaled to base 2: with large common
+// offsets a rounded m log2(e) would cost digits.  A logit of -inf has
+// probability 0 and adds nothing; a row with a NaN, a +inf or nothing but -inf
+// has NaN results, as log_softmax.
+#include <type_traits>
+
 #include "sd_common.cuh"
 
 namespace sd {
 
 namespace lp {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kGroups = 128;            // of 4 threads: their maxima bound the top_k-th value (top_k <= 64)
+constexpr int kAbove = 4096;            // room for the values above that bound,
+constexpr int kTies = 4096 + 64;        // and for those equal to it: a step's 4096 and fewer than top_k before
+constexpr int kCandidates = kAbove + kTies;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFloor = -1e4f;         // stands for -inf: its exponential is 0 and 0 * kFloor is 0
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 
 struct Stat {
   float m, s, w;
 };
 
-__device__ __forceinline__ void add(Stat &a, float x) {
-  if (x == -INFINITY) return;
-  if (x > a.m) {
-    const float c = a.m == -INFINITY ? 0.f : __expf(a.m - x);
-    a.w = a.m == -INFINITY ? 0.f : c * (a.w + a.s * (a.m - x));
-    a.s *= c;
-    a.m = x;
+// m rises to (or stays at) top.
+__device__ __forceinline__ void raise(Stat &a, float top) {
+  if (!(top > a.m)) return;
+  if (a.m == -INFINITY) {
+    a.m = top;
+    return;  // s and w are 0, or NaN
   }
-  const float d = x - a.m, e = __expf(d);
-  a.s += e;
-  a.w = fmaf(e, d, a.w);
+  const float d = a.m - top, c = ex2(d * kLog2e);
+  a.w = c * fmaf(a.s, d, a.w);
+  a.s *= c;
+  a.m = top;
+}
+
+template <int N> __device__ __forceinline__ void add(Stat &a, const float (&x)[N]) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  raise(a, top);
+  const float ref = a.m == -INFINITY ? 0.f : a.m;
+  float s[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = max_nan(x[i] - ref, kFloor), e = ex2(d * kLog2e);
+    s[i & 1] += e;
+    w[i & 1] = fmaf(e, d, w[i & 1]);
+  }
+  a.s += s[0] + s[1];
+  a.w += w[0] + w[1];
 }
 
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
-  if (b.m > a.m) {
-    const Stat t = a;
-    a = b;
-    b = t;
-  }
-  if (b.m == -INFINITY) {  // an empty part (s = w = 0), or one that holds NaN only
-    a.s += b.s;
-    return a;
-  }
-  const float d = b.m - a.m, c = d == 0.f ? 1.f : __expf(d);
-  a.s += c * b.s;
-  a.w += c * (b.w + b.s * d);
+  const float top = fmaxf(a.m, b.m);
+  raise(a, top);
+  raise(b, top);
+  a.s += b.s;
+  a.w += b.w;
   return a;
 }
 
@@ -55,40 +87,109 @@ __device__ __forceinline__ uint32_t place(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// Larger for a larger value, for equal ones at the lower index.
+__device__ __forceinline__ unsigned long long key_of(float x, int64_t j) {
+  return static_cast<unsigned long long>(place(x)) << 32 | (0xfffffffeu - static_cast<uint32_t>(j));
+}
+
+template <typename T> struct Vec {
+  static constexpr int kN = 16 / sizeof(T);
+  static __device__ __forceinline__ void unpack(const uint4 &raw, float *x) {
+    if constexpr (sizeof(T) == 4) {
+      x[0] = __uint_as_float(raw.x), x[1] = __uint_as_float(raw.y);
+      x[2] = __uint_as_float(raw.z), x[3] = __uint_as_float(raw.w);
+    } else {
+      const T *p = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) x[i] = to_f(p[i]);
+    }
+  }
+};
+
+// A row in 16-byte pieces: `head` values up to the first aligned address, then
+// `vecs` pieces, then the rest.
+template <typename T> struct Row {
+  const T *p;
+  int64_t n;
+  int head;
+  int64_t vecs, tail;
+  __device__ __forceinline__ Row(const T *row, int64_t V) : p(row), n(V) {
+    const int64_t off = ((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T);
+    head = static_cast<int>(off < V ? off : V);
+    vecs = (V - head) / Vec<T>::kN;
+    tail = head + vecs * Vec<T>::kN;
+  }
+  __device__ __forceinline__ const uint4 *body() const { return reinterpret_cast<const uint4 *>(p + head); }
+};
 
 }  // namespace lp
 
-// stats [3][rows]: m, log s, H (kept for the gradient).
-template <typename T>
-__global__ void __launch_bounds__(lp::kThreads)
+// One CTA a row.  stats [3][rows]: m, log s, H (kept for the gradient).
+//
+// top_k: the top_k-th largest of the 128 thread groups' maxima bounds the
+// top_k-th largest value from below, so a second pass (the row is in L2, 64 KB
+// for 32000 16-bit logits) collects the values above that bound, and as many of
+// those equal to it, in index order, as can be needed; a candidate's rank among
+// them is its place in the answer.
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(lp::kThreads, 2)
     token_logprobs_kernel(const T *x, int64_t rows, int64_t V, int64_t ld, const int64_t *targets,
                           int64_t ignore_index, float *logprobs, float *entropy, float *stats, int top_k,
                           float *top_logprobs, int64_t *top_ids, int32_t *err) {
   using namespace lp;
-  __shared__ Stat part[kThreads / 32];
-  __shared__ unsigned long long best[kThreads / 32];
+  constexpr int kN = Vec<T>::kN, kUnroll = 4;
+  __shared__ Stat part[kWarps];
   const int64_t r = blockIdx.x;
-  const T *row = x + r * ld;
+  const Row<T> row(x + r * ld, V);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   Stat a = {-INFINITY, 0.f, 0.f};
-  for (int64_t j = tid; j < V; j += kThreads) add(a, to_f(row[j]));
+  float top = -INFINITY;  // largest value of this thread that is a number
+  {
+    float v[1];
+    if (tid < row.head) {
+      v[0] = to_f(row.p[tid]);
+      add(a, v);
+    }
+    if (row.tail + tid < V) {
+      v[0] = to_f(row.p[row.tail + tid]);
+      add(a, v);
+    }
+    const uint4 *body = row.body();
+    for (int64_t i = tid; i < row.vecs; i += kUnroll * kThreads) {
+      uint4 raw[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i + u * kThreads < row.vecs) raw[u] = __ldg(body + i + u * kThreads);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i + u * kThreads < row.vecs) {
+          float y[kN];
+          Vec<T>::unpack(raw[u], y);
+          add(a, y);
+        }
+    }
+    top = a.m;
+  }
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    Stat b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-              __shfl_xor_sync(0xffffffffu, a.w, o)};
-    a = join(a, b);
+    const Stat b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+                    __shfl_xor_sync(0xffffffffu, a.w, o)};
+    // both lanes of a pair join in the same order, so that all end with equal bits
+    a = lane & o ? join(b, a) : join(a, b);
   }
   if (lane == 0) part[warp] = a;
   __syncthreads();
   a = part[0];
-  for (int i = 1; i < kThreads / 32; ++i) a = join(a, part[i]);
-  const float logs = logf(a.s);
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) a = join(a, part[i]);
+  const float logs = a.s > 0.f ? logf(a.s) : __int_as_float(0x7fc00000);
   if (tid == 0) {
     const float h = logs - a.w / a.s;
     const int64_t t = targets[r];
     float v = 0.f;
     if (t != ignore_index) {
       if (t >= 0 && t < V) {
-        v = to_f(row[t]) - a.m - logs;
+        v = to_f(row.p[t]) - a.m - logs;
       } else {
         v = __int_as_float(0x7fc00000);
         if (err) *err = SD_KERR_BOUNDS;
@@ -98,46 +199,163 @@ __global__ void __launch_bounds__(lp::kThreads)
     if (entropy) entropy[r] = h;
     if (stats) stats[r] = a.m, stats[rows + r] = logs, stats[2 * rows + r] = h;
   }
-  unsigned long long prev = ~0ull;
-  for (int k = 0; k < top_k; ++k) {
-    unsigned long long b = 0;
-    for (int64_t j = tid; j < V; j += kThreads) {
-      const unsigned long long key =
-          static_cast<unsigned long long>(place(to_f(row[j]))) << 32 | (0xfffffffeu - static_cast<uint32_t>(j));
-      if (key < prev && key > b) b = key;
+  if constexpr (kTop) {
+    extern __shared__ unsigned long long cand[];  // [kCandidates]
+    __shared__ float group[kGroups];
+    __shared__ float bound;
+    __shared__ int above, ties;  // values above the bound, and equal to it
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if ((lane & 3) == 0) group[tid >> 2] = top;
+    if (tid == 0) above = ties = 0;
+    __syncthreads();
+    if (tid < kGroups) {
+      const float mine = group[tid];
+      int rank = 0;
+#pragma unroll 8
+      for (int i = 0; i < kGroups; ++i) rank += group[i] > mine || (group[i] == mine && i < tid);
+      if (rank == top_k - 1) bound = mine;
     }
-    for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
     __syncthreads();
-    if (lane == 0) best[warp] = b;
+    const float low = bound;
+    // candidates above the bound fill the buffer from its start, equal ones from
+    // its end; equal ones are taken in index order, piece by piece of the row,
+    // until there are top_k of them
+    auto take = [&](float v, int64_t j, bool equal_too) {
+      if (v < low) return;
+      if (v == low) {
+        if (!equal_too) return;
+        const int at = atomicAdd(&ties, 1);
+        cand[kCandidates - 1 - at] = key_of(v, j);
+      } else {
+        const int at = atomicAdd(&above, 1);
+        if (at < kAbove) cand[at] = key_of(v, j);
+      }
+    };
+    if (tid < row.head) take(to_f(row.p[tid]), tid, true);
     __syncthreads();
-    for (int i = 0; i < kThreads / 32; ++i) b = max(b, best[i]);
-    prev = b;
-    if (tid == 0) {
-      const int64_t j = 0xfffffffeu - static_cast<uint32_t>(b);
-      top_ids[r * top_k + k] = j;
-      top_logprobs[r * top_k + k] = to_f(row[j]) - a.m - logs;
+    const uint4 *body = row.body();
+    for (int64_t i0 = 0; i0 < row.vecs; i0 += kThreads) {
+      const bool equal_too = ties < top_k;
+      __syncthreads();  // all have read ties before any adds to it
+      if (i0 + tid < row.vecs) {
+        float y[kN];
+        Vec<T>::unpack(__ldg(body + i0 + tid), y);
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < kN; ++e) any = any || !(y[e] < low);
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < kN; ++e) take(y[e], row.head + (i0 + tid) * kN + e, equal_too);
+        }
+      }
+      __syncthreads();
+    }
+    {
+      const bool equal_too = ties < top_k;
+      __syncthreads();
+      if (row.tail + tid < V) take(to_f(row.p[row.tail + tid]), row.tail + tid, equal_too);
+      __syncthreads();
+    }
+    const int na = above, nt = ties, n = na + nt;
+    if (na <= kAbove) {
+      auto get = [&](int i) { return cand[i < na ? i : kCandidates - 1 - (i - na)]; };
+      for (int i = tid; i < n; i += kThreads) {
+        const unsigned long long mine = get(i);
+        int rank = 0;
+        for (int j = 0; j < na; ++j) rank += cand[j] > mine;
+        for (int j = 0; j < nt; ++j) rank += cand[kCandidates - 1 - j] > mine;
+        if (rank < top_k) {
+          const int64_t j = 0xfffffffeu - static_cast<uint32_t>(mine);
+          top_ids[r * top_k + rank] = j;
+          top_logprobs[r * top_k + rank] = to_f(row.p[j]) - a.m - logs;
+        }
+      }
+    } else {
+      // more than fit (many large values in few thread groups): one pass a place
+      unsigned long long prev = ~0ull;
+      for (int k = 0; k < top_k; ++k) {
+        unsigned long long b = 0;
+        for (int64_t j = tid; j < V; j += kThreads) {
+          const unsigned long long key = key_of(to_f(row.p[j]), j);
+          if (key < prev && key > b) b = key;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+        __syncthreads();
+        if (lane == 0) cand[warp] = b;
+        __syncthreads();
+        for (int i = 0; i < kWarps; ++i) b = max(b, cand[i]);
+        prev = b;
+        if (tid == 0) {
+          const int64_t j = 0xfffffffeu - static_cast<uint32_t>(b);
+          top_ids[r * top_k + k] = j;
+          top_logprobs[r * top_k + k] = to_f(row.p[j]) - a.m - logs;
+        }
+      }
     }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(lp::kThreads)
+// One CTA a row: one read of the logits, one write of their gradient.
+template <typename T, bool kEntropy>
+__global__ void __launch_bounds__(lp::kThreads, 2)
     token_logprobs_backward_kernel(const T *x, int64_t rows, int64_t V, int64_t ld, const int64_t *targets,
                                    int64_t ignore_index, const float *stats, const float *g_logprobs,
                                    const float *g_entropy, T *dx, int64_t d_ld) {
+  using namespace lp;
+  constexpr int kN = Vec<T>::kN, kUnroll = 4;
   const int64_t r = blockIdx.x;
-  const T *row = x + r * ld;
+  const Row<T> row(x + r * ld, V);
   T *d = dx + r * d_ld;
+  const int tid = threadIdx.x;
   const float m = stats[r], logs = stats[rows + r], h = stats[2 * rows + r];
   const int64_t t = targets[r];
   const float g = g_logprobs && t != ignore_index && t >= 0 && t < V ? g_logprobs[r] : 0.f;
-  const float ge = g_entropy ? g_entropy[r] : 0.f;
-  for (int64_t j = threadIdx.x; j < V; j += lp::kThreads) {
-    const float l = to_f(row[j]) - m - logs, p = __expf(l);
-    float v = j == t ? g : 0.f;
-    v -= p * g;
-    if (ge != 0.f && p > 0.f) v -= p * (ge * (l + h));
+  const float ge = kEntropy ? g_entropy[r] : 0.f;
+  auto grad = [&](float v) {
+    const float l = max_nan(v - m - logs, kFloor), p = ex2(l * kLog2e);
+    return kEntropy ? -p * fmaf(ge, l + h, g) : -p * g;
+  };
+  auto one = [&](int64_t j) {
+    float v = grad(to_f(row.p[j]));
+    if (j == t) v += g;
     d[j] = from_f<T>(v);
+  };
+  if ((reinterpret_cast<uintptr_t>(d + row.head) & 15) != 0) {  // the two rows are aligned differently
+    for (int64_t j = tid; j < V; j += kThreads) one(j);
+    return;
+  }
+  if (tid < row.head) one(tid);
+  if (row.tail + tid < V) one(row.tail + tid);
+  const uint4 *body = row.body();
+  uint4 *to = reinterpret_cast<uint4 *>(d + row.head);
+  // the piece that holds the target, and the place in it
+  const int64_t tv = t >= row.head && t < row.tail ? (t - row.head) / kN : -1;
+  for (int64_t i = tid; i < row.vecs; i += kUnroll * kThreads) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i + u * kThreads < row.vecs) raw[u] = __ldg(body + i + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t at = i + u * kThreads;
+      if (at >= row.vecs) continue;
+      float y[kN];
+      Vec<T>::unpack(raw[u], y);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) y[e] = grad(y[e]);
+      if (at == tv) {
+#pragma unroll
+        for (int e = 0; e < kN; ++e)
+          if (row.head + at * kN + e == t) y[e] += g;
+      }
+      uint4 out;
+      T *p = reinterpret_cast<T *>(&out);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) p[e] = from_f<T>(y[e]);
+      __stcs(to + at, out);
+    }
   }
 }
 
@@ -153,12 +371,19 @@ int sd_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t V, in
       (top_k > 0 && (!top_logprobs || !top_ids)) || ld < 0)
     return SD_ERR_INVALID;
   if (top_k > 64 || rows > 0x7fffffffll || V > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype)) return SD_ERR_ALIGN;
   SD_DISPATCH_DTYPE(dtype, T, {
-    token_logprobs_kernel<T><<<static_cast<unsigned>(rows), lp::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const T *>(logits), rows, V, ld, targets, ignore_index, logprobs, entropy, stats, top_k,
-        top_logprobs, top_ids, err);
+    auto run = [&](auto *kern, size_t smem) {
+      if (set_max_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
+      kern<<<static_cast<unsigned>(rows), lp::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
+          static_cast<const T *>(logits), rows, V, ld, targets, ignore_index, logprobs, entropy, stats, top_k,
+          top_logprobs, top_ids, err);
+      return check_launch();
+    };
+    return top_k > 0 ? run(token_logprobs_kernel<T, true>, lp::kCandidates * sizeof(unsigned long long))
+                     : run(token_logprobs_kernel<T, false>, 0);
   });
-  return check_launch();
+  return SD_OK;
 }
 
 int sd_token_logprobs_backward(const void *logits, int dtype, int64_t rows, int64_t V, int64_t ld,
@@ -169,11 +394,14 @@ int sd_token_logprobs_backward(const void *logits, int dtype, int64_t rows, int6
   if (!logits || !targets || !stats || !dlogits || !dtype_ok(dtype) || rows <= 0 || V <= 0 || ld < 0 || d_ld < V)
     return SD_ERR_INVALID;
   if (rows > 0x7fffffffll || V > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype) ||
+      reinterpret_cast<uintptr_t>(dlogits) % dtype_size(dtype))
+    return SD_ERR_ALIGN;
   SD_DISPATCH_DTYPE(dtype, T, {
-    token_logprobs_backward_kernel<T>
-        <<<static_cast<unsigned>(rows), lp::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const T *>(logits), rows, V, ld, targets, ignore_index, stats, g_logprobs, g_entropy,
-            static_cast<T *>(dlogits), d_ld);
+    auto kern = g_entropy ? token_logprobs_backward_kernel<T, true> : token_logprobs_backward_kernel<T, false>;
+    kern<<<static_cast<unsigned>(rows), lp::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const T *>(logits), rows, V, ld, targets, ignore_index, stats, g_logprobs, g_entropy,
+        static_cast<T *>(dlogits), d_ld);
   });
   return check_launch();
 }

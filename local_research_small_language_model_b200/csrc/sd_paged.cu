@@ -475,35 +475,55 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
   cp_wait<0>();
 }
 
-// Joins the parts of the head groups that were split over CTAs, and zeros the
-// rows of sequences without tokens.  One CTA per (head group, sequence).
-template <typename T> __global__ void __launch_bounds__(64) paged_join_kernel(const PagedArgs a, const pg::DecodeArgs d) {
+// Joins the parts of a head that was split over CTAs, in their order, and zeros
+// the rows of sequences without tokens.  One CTA per (sequence, query head):
+// eight runs of the parts side by side, then the eight.
+template <typename T>
+__global__ void __launch_bounds__(512) paged_join_kernel(const PagedArgs a, const pg::DecodeArgs d) {
   using namespace pg;
+  constexpr int kRuns = 8;
+  __shared__ float tops[16], sums[kRuns], vals[kRuns][64];
   pdl_wait();
-  const int b = blockIdx.y, hh = blockIdx.x, groups = d.Hh / a.Hkv, e = threadIdx.x;
-  const int h0 = (hh / groups) * (a.Hq / a.Hkv) + (hh % groups) * kMaxHeads;
-  const int n = min(d.G, (a.Hq / a.Hkv) - (hh % groups) * kMaxHeads);
-  T *out = static_cast<T *>(d.out) + b * d.o_sb + h0 * d.o_sh;
+  const int b = blockIdx.y, group = a.Hq / a.Hkv, groups = d.Hh / a.Hkv, tid = threadIdx.x;
+  const int h = blockIdx.x, hh = (h / group) * groups + h % group / kMaxHeads, g = h % group % kMaxHeads;
+  T *out = static_cast<T *>(d.out) + b * d.o_sb + h * d.o_sh;
   const int64_t tiles = d.plan[b + 1] - d.plan[b], per = d.plan[a.B + 1];
   if (tiles == 0) {
-    for (int g = 0; g < n; ++g) out[g * d.o_sh + e] = from_f<T>(0.f);
+    if (tid < 64) out[tid] = from_f<T>(0.f);
     return;
   }
   const int64_t u0 = static_cast<int64_t>(d.plan[b]) * d.Hh + hh * tiles, u1 = u0 + tiles;
-  const int64_t c0 = u0 / per, c1 = (u1 - 1) / per;
-  if (c0 == c1) return;
-  for (int g = 0; g < n; ++g) {
-    float top = -INFINITY;
-    auto part = [&](int64_t i) { return d.parts + ((i * 2 + (i * per < u0 ? 1 : 0)) * d.G + g) * kPart; };
-    for (int64_t i = c0; i <= c1; ++i) top = fmaxf(top, part(i)[0]);
-    float sum = 0.f, val = 0.f;
-    for (int64_t i = c0; i <= c1; ++i) {
-      const float *p = part(i);
-      const float f = factor(p[0], top);
-      sum = fmaf(f, p[1], sum);
-      val = fmaf(f, p[2 + e], val);
-    }
-    out[g * d.o_sh + e] = from_f<T>(sum == 0.f ? 0.f : val / sum);
+  const int c0 = static_cast<int>(u0 / per), n = static_cast<int>((u1 - 1) / per) - c0 + 1;
+  if (n == 1) return;
+  auto part = [&](int i) {
+    return d.parts + ((static_cast<int64_t>(c0 + i) * 2 + ((c0 + i) * per < u0 ? 1 : 0)) * d.G + g) * kPart;
+  };
+  float top = -INFINITY;  // n <= kCtas <= 512: one part a thread
+  if (tid < n) top = part(tid)[0];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((tid & 31) == 0) tops[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, tops[i]);
+  const int run = tid >> 6, e = tid & 63;
+  const int i0 = n * run / kRuns, i1 = n * (run + 1) / kRuns;
+  float sum = 0.f, val = 0.f;
+#pragma unroll 8
+  for (int i = i0; i < i1; ++i) {
+    const float *p = part(i);
+    const float f = factor(p[0], top);
+    sum = fmaf(f, p[1], sum);
+    val = fmaf(f, p[2 + e], val);
+  }
+  if (e == 0) sums[run] = sum;
+  vals[run][e] = val;
+  __syncthreads();
+  if (tid < 64) {
+    sum = val = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) sum += sums[i], val += vals[i][e];
+    out[e] = from_f<T>(sum == 0.f ? 0.f : val / sum);
   }
 }
 
@@ -603,7 +623,7 @@ int sd_paged_decode_attention(const void *q, int dtype, int64_t B, int64_t Hq, i
       kern<<<ctas, pg::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a, d);
       rc = check_launch();
       if (rc != SD_OK) return rc;
-      rc = launch(paged_join_kernel<T>, dim3(d.Hh, a.B), dim3(64), 0, static_cast<cudaStream_t>(stream), true, a, d);
+      rc = launch(paged_join_kernel<T>, dim3(a.Hq, a.B), dim3(512), 0, static_cast<cudaStream_t>(stream), true, a, d);
       if (rc != SD_OK) return rc;
     });
   }
