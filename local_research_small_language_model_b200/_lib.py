@@ -115,6 +115,8 @@ def exported_symbols():
 def load(path: str = LIB_PATH) -> ctypes.CDLL:
     """Loads the shared library once; raises if it was not built."""
     global _lib
+    if _lib is not None:  # set once, after every signature is in place
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -135,9 +137,14 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Calls an entry point and raises SparDAError on a non-zero status."""
-    lib = load()
-    code = getattr(lib, name)(*args)
+    code = getattr(load(), name)(*args)
     if code != SD_OK:
-        msg = lib.sd_strerror(code).decode()
-        extra = f" (cudaError {lib.sd_last_cuda_error()})" if code == -3 else ""
-        raise SparDAError(f"{name} failed: {msg}{extra}")
+        check(name, code)
+
+
+def check(name: str, code: int) -> None:
+    """Raises SparDAError for the non-zero status an entry point returned."""
+    lib = load()
+    msg = lib.sd_strerror(code).decode()
+    extra = f" (cudaError {lib.sd_last_cuda_error()})" if code == -3 else ""
+    raise SparDAError(f"{name} failed: {msg}{extra}")

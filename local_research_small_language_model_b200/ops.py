@@ -4,8 +4,8 @@ caching allocator and launches on the current CUDA stream."""
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -635,63 +635,93 @@ def swiglu_weight(w_gate: torch.Tensor, w_up: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- ragged batches
-_HERE = contextlib.nullcontext()
+# These calls are a few microseconds on the device, so their wrappers look at
+# each tensor once and keep to the cheap accessors.
+_err_ptrs = {}
 
 
-def _one_device(*ts):
-    """All tensors on one CUDA device (None is skipped); returns a guard that
-    makes it the current one, as a launch needs."""
-    _cuda(*ts)
-    first = next(t for t in ts if t is not None).device
+def _device(*ts) -> int:
+    """The one CUDA device index of the tensors (None is skipped)."""
+    dev = -1
     for t in ts:
-        if t is not None and t.device != first:
-            raise ValueError(f"tensors on {first} and {t.device}: one call needs one device")
-    return _HERE if first.index == torch.cuda.current_device() else torch.cuda.device(first)
+        if t is not None:
+            i = t.get_device()
+            if i < 0:
+                raise ValueError("the B200 kernels need CUDA tensors (this library has no CPU path)")
+            if dev < 0:
+                dev = i
+            elif dev != i:
+                raise ValueError(f"tensors on cuda:{dev} and cuda:{i}: one call needs one device")
+    return dev
+
+
+def _err_ptr(dev: int) -> int:
+    ptr = _err_ptrs.get(dev)
+    if ptr is None:
+        ptr = _err_ptrs[dev] = error_buffer(torch.device("cuda", dev)).data_ptr()
+    return ptr
+
+
+def _launch(name: str, dev: int, *args) -> None:
+    """L.call on the current stream of device ``dev``, which a launch needs as
+    the current device."""
+    if torch._C._cuda_getDevice() == dev:
+        code = getattr(L.load(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+        if code != L.SD_OK:
+            L.check(name, code)
+        return
+    with torch.cuda.device(dev):
+        L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t itself where its rows suit 16-byte loads and tensor copies (innermost
-    stride 1, aligned base and strides, no broadcast dimension), else a
-    contiguous copy."""
-    size = t.element_size()
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and \
-            all(s > 0 and s * size % 16 == 0 for s, n in zip(st[:-1], t.shape) if n > 1) and \
-            all(s * size % 16 == 0 for s in st[:-1]):
-        return t
+    """t itself where its rows of 64 values suit 16-byte loads and tensor copies
+    (innermost stride 1, aligned base and strides, no broadcast dimension),
+    else a contiguous copy."""
+    if not t.data_ptr() & 15:
+        if t.is_contiguous():
+            return t
+        *outer, inner = t.stride()
+        whole = 16 // t.element_size() - 1
+        if inner == 1 and not any(s & whole for s in outer) and all(s > 0 or n == 1 for s, n in zip(outer, t.shape)):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _index32(name: str, t: torch.Tensor, shape) -> torch.Tensor:
-    if tuple(t.shape) != tuple(shape) or t.dtype not in (torch.int32, torch.int64):
+    if t.shape != shape or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be {list(shape)} of int32, got {tuple(t.shape)} of {t.dtype}")
-    t = t if t.dtype == torch.int32 else t.to(torch.int32)
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    if t.dtype is not torch.int32:
+        t = t.to(torch.int32)
+    return t if t.stride(-1) == 1 else t.contiguous()
 
 
 def _scale(scale: Optional[float], d: int) -> float:
-    sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0.0 < sc < 3e38:
-        raise ValueError(f"the softmax scale must be positive and finite, got {sc}")
-    return sc
+    if scale is None:
+        return 1.0 / math.sqrt(d)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"the softmax scale must be positive and finite, got {scale}")
+    return float(scale)
 
 
 def _check_packed(q, k, v, cu_seqlens, **like_q):
-    if q.dim() != 3 or k.dim() != 3 or tuple(k.shape) != tuple(v.shape) or k.shape[0] != q.shape[0] \
-            or k.shape[2] != q.shape[2]:
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError(f"q must be [total, Hq, D] and k, v [total, Hkv, D], got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     if q.shape[2] != 64:
         raise ValueError(f"packed attention has head size 64, got {q.shape[2]}")
     if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"query heads ({q.shape[1]}) must be a multiple of kv heads ({k.shape[1]})")
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
         raise ValueError(f"cu_seqlens must hold a bound more than there are sequences, got {tuple(cu_seqlens.shape)}")
-    for t in (k, v, *like_q.values()):
-        if t is not None and t.dtype != q.dtype:
-            raise TypeError(f"the tensors of a call must share a dtype, got {q.dtype} and {t.dtype}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     for name, t in like_q.items():
-        if t is not None and tuple(t.shape) != tuple(q.shape):
+        if t is None:
+            continue
+        if t.dtype != q.dtype:
+            raise TypeError(f"{name} must have q's dtype {q.dtype}, got {t.dtype}")
+        if t.shape != q.shape:
             raise ValueError(f"{name} must have q's shape {tuple(q.shape)}, got {tuple(t.shape)}")
 
 
@@ -705,25 +735,22 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     they are in a caller's ``out``.  With ``return_lse`` also the fp32 [Hq,total]
     the backward needs."""
     _check_packed(q, k, v, cu_seqlens, out=out)
-    guard = _one_device(q, k, v, cu_seqlens, out)
+    dev = _device(q, k, v, cu_seqlens, out)
     total, hq, d = q.shape
-    hkv = k.shape[1]
     sc = _scale(scale, d)
     cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape)
     code = dtype_code(q)
     zero = out is None
     if zero:
-        out = torch.empty(total, hq, d, dtype=q.dtype, device=q.device)
+        out = q.new_empty((total, hq, d))
     elif _rows16(out) is not out:
         raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
     lse = torch.empty(hq, total, dtype=torch.float32, device=q.device) if return_lse else None
     if total:
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        with guard:
-            L.call("sd_packed_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, total, hq, hkv, d,
-                   q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), cu.data_ptr(),
-                   cu.numel() - 1, sc, out.data_ptr(), out.stride(0), out.stride(1),
-                   lse.data_ptr() if return_lse else None, int(zero), error_buffer(q.device).data_ptr(), _stream(q))
+        _launch("sd_packed_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, total, hq, k.shape[1], d,
+                *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, sc,
+                out.data_ptr(), *out.stride()[:2], lse.data_ptr() if return_lse else None, zero, _err_ptr(dev))
     return (out, lse) if return_lse else out
 
 
@@ -735,31 +762,29 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     the output gradient dout; out and lse are the forward's
     (sd_packed_attention_backward).  Equal inputs give equal bits."""
     _check_packed(q, k, v, cu_seqlens, out=out, dout=dout)
-    guard = _one_device(q, k, v, out, dout, lse, cu_seqlens)
+    dev = _device(q, k, v, out, dout, lse, cu_seqlens)
     total, hq, d = q.shape
     hkv = k.shape[1]
-    if tuple(lse.shape) != (hq, total) or lse.dtype != torch.float32 or not lse.is_contiguous():
+    if lse.shape != (hq, total) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError(f"lse must be the forward's fp32 [{hq}, {total}], got {tuple(lse.shape)} of {lse.dtype}")
     sc = _scale(scale, d)
     cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape)
     code = dtype_code(q)
-    dq = torch.empty(total, hq, d, dtype=q.dtype, device=q.device)
-    dk = torch.empty(total, hkv, d, dtype=q.dtype, device=q.device)
-    dv = torch.empty_like(dk)
+    dq = q.new_empty((total, hq, d))
+    dk = q.new_empty((total, hkv, d))
+    dv = q.new_empty((total, hkv, d))
     if total:
-        q, k, v, out, dout = (_rows16(t) for t in (q, k, v, out, dout))
-        delta = torch.empty(hq * total + 1, dtype=torch.float32, device=q.device)
-        with guard:
-            L.call("sd_packed_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                   dout.data_ptr(), code, total, hq, hkv, d, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                   v.stride(0), v.stride(1), out.stride(0), out.stride(1), dout.stride(0), dout.stride(1),
-                   cu.data_ptr(), cu.numel() - 1, sc, lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                   dv.data_ptr(), error_buffer(q.device).data_ptr(), _stream(q))
+        q, k, v, out, dout = _rows16(q), _rows16(k), _rows16(v), _rows16(out), _rows16(dout)
+        delta = lse.new_empty(hq * total + 1)
+        _launch("sd_packed_attention_backward", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                dout.data_ptr(), code, total, hq, hkv, d, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+                *out.stride()[:2], *dout.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, sc, lse.data_ptr(),
+                delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _err_ptr(dev))
     return dq, dk, dv
 
 
-def _check_pool(k_pages, v_pages, page_table, lens, heads_of, d):
-    if k_pages.dim() != 4 or tuple(k_pages.shape) != tuple(v_pages.shape) or 0 in k_pages.shape:
+def _check_pool(k_pages, v_pages, page_table, seqs, d):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or 0 in k_pages.shape:
         raise ValueError(f"k_pages and v_pages must be [pages, Hkv, page, D] alike, got {tuple(k_pages.shape)}, "
                          f"{tuple(v_pages.shape)}")
     if d != 64 or k_pages.shape[3] != 64:
@@ -768,8 +793,8 @@ def _check_pool(k_pages, v_pages, page_table, lens, heads_of, d):
         raise ValueError("k_pages and v_pages must share dtype and strides")
     if _rows16(k_pages) is not k_pages or _rows16(v_pages) is not v_pages:
         raise ValueError("pages must have 16-byte aligned rows and innermost stride 1")
-    if page_table.dim() != 2 or page_table.shape[0] != lens.shape[0] or page_table.shape[1] == 0:
-        raise ValueError(f"page_table must be [{lens.shape[0]}, width], got {tuple(page_table.shape)}")
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or page_table.shape[1] == 0:
+        raise ValueError(f"page_table must be [{seqs}, width], got {tuple(page_table.shape)}")
 
 
 def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -781,34 +806,37 @@ def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pa
     cu_seqlens[b+1]-1 go to positions lens[b], lens[b]+1, ..; without
     cu_seqlens row b is sequence b's one new token.  A row whose place is out
     of range is dropped and check_device_errors reports it."""
-    if xk.dim() != 3 or tuple(xk.shape) != tuple(xv.shape) or lens.dim() != 1:
+    if xk.dim() != 3 or xk.shape != xv.shape or lens.dim() != 1:
         raise ValueError(f"xk, xv must be [N, Hkv, D] alike and lens [B], got {tuple(xk.shape)}, "
                          f"{tuple(xv.shape)}, {tuple(lens.shape)}")
     n, hkv, d = xk.shape
     b = lens.shape[0]
-    _check_pool(k_pages, v_pages, page_table, lens, hkv, d)
+    _check_pool(k_pages, v_pages, page_table, b, d)
     if k_pages.shape[1] != hkv:
         raise ValueError(f"the pool has {k_pages.shape[1]} kv heads, the rows {hkv}")
     if xk.dtype != k_pages.dtype or xv.dtype != k_pages.dtype:
         raise TypeError(f"rows of {xk.dtype} do not fit pages of {k_pages.dtype}")
     if cu_seqlens is None and n != b:
         raise ValueError(f"without cu_seqlens every one of the {b} sequences has one row, got {n}")
-    guard = _one_device(xk, xv, k_pages, v_pages, page_table, lens, cu_seqlens)
+    dev = _device(xk, xv, k_pages, v_pages, page_table, lens, cu_seqlens)
     table = _index32("page_table", page_table, page_table.shape)
     ln = _index32("lens", lens, (b,))
     cu = _index32("cu_seqlens", cu_seqlens, (b + 1,)) if cu_seqlens is not None else None
     code = dtype_code(k_pages)
     if n == 0 or b == 0:
         return
-    if ln.stride(0) != 1:
-        ln = ln.contiguous()
     xk, xv = _rows16(xk), _rows16(xv)
-    with guard:
-        L.call("sd_paged_append", xk.data_ptr(), xv.data_ptr(), code, n, hkv, d, xk.stride(0), xk.stride(1),
-               xv.stride(0), xv.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
-               k_pages.shape[2], k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), table.data_ptr(),
-               table.stride(0), table.shape[1], ln.data_ptr(), b, cu.data_ptr() if cu is not None else None,
-               error_buffer(xk.device).data_ptr(), _stream(xk))
+    _launch("sd_paged_append", dev, xk.data_ptr(), xv.data_ptr(), code, n, hkv, d, *xk.stride()[:2],
+            *xv.stride()[:2], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], k_pages.shape[2],
+            *k_pages.stride()[:3], table.data_ptr(), table.stride(0), table.shape[1], ln.data_ptr(), b,
+            cu.data_ptr() if cu is not None else None, _err_ptr(dev))
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(b: int, hq: int, hkv: int) -> int:
+    need = ctypes.c_int64()
+    L.call("sd_paged_decode_workspace", b, hq, hkv, ctypes.byref(need))
+    return need.value
 
 
 def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -821,43 +849,38 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if q.dim() != 3 or lens.dim() != 1 or q.shape[0] != lens.shape[0]:
         raise ValueError(f"q must be [B, Hq, D] and lens [B], got {tuple(q.shape)}, {tuple(lens.shape)}")
     b, hq, d = q.shape
-    _check_pool(k_pages, v_pages, page_table, lens, hq, d)
-    hkv = k_pages.shape[1]
+    _check_pool(k_pages, v_pages, page_table, b, d)
+    pages, hkv, page, _ = k_pages.shape
     if hq == 0 or hq % hkv:
         raise ValueError(f"query heads ({hq}) must be a multiple of kv heads ({hkv})")
     if q.dtype != k_pages.dtype or (out is not None and out.dtype != q.dtype):
         raise TypeError(f"q of {q.dtype} does not fit pages of {k_pages.dtype}")
-    if out is not None and tuple(out.shape) != tuple(q.shape):
+    if out is not None and out.shape != q.shape:
         raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
-    guard = _one_device(q, k_pages, v_pages, page_table, lens, out)
+    dev = _device(q, k_pages, v_pages, page_table, lens, out)
     table = _index32("page_table", page_table, page_table.shape)
     ln = _index32("lens", lens, (b,))
     code = dtype_code(q)
     sc = _scale(scale, d)
     if out is None:
-        out = torch.empty(b, hq, d, dtype=q.dtype, device=q.device)
+        out = q.new_empty((b, hq, d))
     elif _rows16(out) is not out:
         raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
     if b == 0:
         return out
-    if ln.stride(0) != 1:
-        ln = ln.contiguous()
     q = _rows16(q)
-    need = ctypes.c_int64()
-    with guard:
-        L.call("sd_paged_decode_workspace", b, hq, hkv, ctypes.byref(need))
-        # from the caching allocator, so that calls on other streams and captured graphs have their own
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-        L.call("sd_paged_decode_attention", q.data_ptr(), code, b, hq, hkv, d, q.stride(0), q.stride(1),
-               k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], k_pages.shape[2], k_pages.stride(0),
-               k_pages.stride(1), k_pages.stride(2), table.data_ptr(), table.stride(0), table.shape[1],
-               ln.data_ptr(), sc, out.data_ptr(), out.stride(0), out.stride(1),
-               ws.data_ptr() if ws is not None else None, need.value, error_buffer(q.device).data_ptr(), _stream(q))
+    # from the caching allocator, so that calls on other streams and captured graphs have their own
+    need = _decode_workspace(b, hq, hkv)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch("sd_paged_decode_attention", dev, q.data_ptr(), code, b, hq, hkv, d, *q.stride()[:2],
+            k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *k_pages.stride()[:3], table.data_ptr(),
+            table.stride(0), table.shape[1], ln.data_ptr(), sc, out.data_ptr(), *out.stride()[:2], ws.data_ptr(),
+            need, _err_ptr(dev))
     return out
 
 
 def _check_scores(logits, targets):
-    if logits.dim() != 2 or logits.shape[1] == 0 or tuple(targets.shape) != (logits.shape[0],) \
+    if logits.dim() != 2 or logits.shape[1] == 0 or targets.shape != logits.shape[:1] \
             or targets.dtype != torch.int64:
         raise ValueError(f"logits must be [rows, V] and targets int64 [rows], got {tuple(logits.shape)} and "
                          f"{tuple(targets.shape)} of {targets.dtype}")
@@ -875,21 +898,19 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     rows, vocab = logits.shape
     if not 0 <= top_k <= min(64, vocab):
         raise ValueError(f"top_k must be within 0..{min(64, vocab)}, got {top_k}")
-    guard = _one_device(logits, targets)
+    dev = _device(logits, targets)
     code = dtype_code(logits)
     logits, targets = _inner1(logits), targets.contiguous()
-    dev = logits.device
-    logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    stats = torch.empty(3, rows, dtype=torch.float32, device=dev) if return_stats else None
-    top_lp = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
-    top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev)
+    where = logits.device
+    logprobs = torch.empty(rows, dtype=torch.float32, device=where)
+    entropy = torch.empty(rows, dtype=torch.float32, device=where)
+    stats = torch.empty(3, rows, dtype=torch.float32, device=where) if return_stats else None
+    top_lp = torch.empty(rows, top_k, dtype=torch.float32, device=where)
+    top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=where)
     if rows:
-        with guard:
-            L.call("sd_token_logprobs", logits.data_ptr(), code, rows, vocab, logits.stride(0), targets.data_ptr(),
-                   ignore_index, logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr() if return_stats else None,
-                   top_k, top_lp.data_ptr() if top_k else None, top_ids.data_ptr() if top_k else None,
-                   error_buffer(dev).data_ptr(), _stream(logits))
+        _launch("sd_token_logprobs", dev, logits.data_ptr(), code, rows, vocab, logits.stride(0), targets.data_ptr(),
+                ignore_index, logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr() if return_stats else None,
+                top_k, top_lp.data_ptr() if top_k else None, top_ids.data_ptr() if top_k else None, _err_ptr(dev))
     found = (logprobs, entropy, top_lp, top_ids)
     return found + (stats,) if return_stats else found
 
@@ -903,17 +924,16 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: 
     rows, vocab = logits.shape
     for name, t in (("stats", stats), ("g_logprobs", g_logprobs), ("g_entropy", g_entropy)):
         want = (3, rows) if name == "stats" else (rows,)
-        if t is not None and (tuple(t.shape) != want or t.dtype != torch.float32):
+        if t is not None and (t.shape != want or t.dtype != torch.float32):
             raise ValueError(f"{name} must be fp32 {list(want)}, got {tuple(t.shape)} of {t.dtype}")
-    guard = _one_device(logits, targets, stats, g_logprobs, g_entropy)
+    dev = _device(logits, targets, stats, g_logprobs, g_entropy)
     code = dtype_code(logits)
     logits, targets, stats = _inner1(logits), targets.contiguous(), stats.contiguous()
     gl = g_logprobs.contiguous() if g_logprobs is not None else None
     ge = g_entropy.contiguous() if g_entropy is not None else None
-    d = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+    d = logits.new_empty((rows, vocab))
     if rows:
-        with guard:
-            L.call("sd_token_logprobs_backward", logits.data_ptr(), code, rows, vocab, logits.stride(0),
-                   targets.data_ptr(), ignore_index, stats.data_ptr(), gl.data_ptr() if gl is not None else None,
-                   ge.data_ptr() if ge is not None else None, d.data_ptr(), d.stride(0), _stream(logits))
+        _launch("sd_token_logprobs_backward", dev, logits.data_ptr(), code, rows, vocab, logits.stride(0),
+                targets.data_ptr(), ignore_index, stats.data_ptr(), gl.data_ptr() if gl is not None else None,
+                ge.data_ptr() if ge is not None else None, d.data_ptr(), d.stride(0))
     return d
