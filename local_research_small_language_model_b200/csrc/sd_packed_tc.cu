@@ -3,18 +3,19 @@
 //
 //   O_i = sum_{j <= i} exp2(c q_i.k_j - m_i) v_j / l_i,  c = scale log2(e)
 //
-// Forward.  One CTA per 256 query rows of one sequence and head, one per SM
-// (384 of the 512 tensor-memory columns).  The rows are two 128-row tiles;
-// for every 128 keys up to a tile's own diagonal
-//   S_x = Q_x K^T    4 MMAs M=128 N=128 K=16, fp32 in 128 columns
+// Forward.  One CTA per 256 query rows of one sequence and head, one per SM.
+// The rows are two 128-row tiles, whose Q stays in tensor memory as A; for
+// every 64 keys up to a tile's own diagonal
+//   S_x = Q_x K^T    4 MMAs M=128 N=64 K=16, fp32 in 64 of two alternating
+//                    runs of 64 columns
 //   P_x = exp2(..)   warpgroup x, one thread a row, 16-bit pairs written over
-//                    the first 64 columns of S_x
-//   O_x += P_x V     8 MMAs M=128 N=64 K=16, A from tensor memory
-// Warp 8 issues all MMAs, warp 9 all copies (K and V in a ring of 4 stages).
-// The two tiles alternate: while one warpgroup computes exponentials, the
-// other tile's two products run.  S_x(i + 1) is issued right behind O_x(i), so
-// its arrival also says that O_x(i) is done, and a row may rescale its O then
-// (rarely: a row keeps its reference maximum until a block exceeds it by 2^8).
+//                    the first 32 columns of S_x
+//   O_x += P_x V     4 MMAs, A from tensor memory
+// Warp 8 issues all MMAs, warp 9 all copies (K and V in a ring of 8 stages).
+// S_x(i + 2) is issued right behind O_x(i), so a warpgroup finds the next
+// scores ready when it has written its weights, and both compute all the time.
+// A row keeps its reference maximum until a block exceeds it by 2^8; only then
+// does it wait for O_x(i - 1) and rescale it.
 //
 // Backward, two kernels of one shape: a CTA owns 128 rows, whose two operands
 // stay in tensor memory as A for all products, and walks 64-row blocks of the
@@ -41,21 +42,25 @@ namespace pt {
 
 using namespace tc;
 
-constexpr int kRows = 128;                   // MMA M, and keys of a block
-constexpr int kTileBytes = kRows * 128;      // 128 rows of 64 16-bit values
-constexpr int kStages = 4;
+constexpr int kRows = 128;                   // MMA M
+constexpr int kBlock = 64;                   // rows of a block of the other side
+constexpr int kBlockBytes = kBlock * 128;    // of 64 16-bit values
+constexpr int kStages = 8;
 constexpr int kFwdThreads = 320;             // 2 softmax warpgroups, MMA warp, copy warp
+constexpr int kFwdO = 256, kFwdQ = 384;      // tensor-memory columns; S of tile x from 128 x, two buffers
+
+struct FwdBars {
+  uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2][2];
+  uint32_t tmem;
+};
 
 struct FwdSmem {
-  static constexpr int kQ = 0;
-  static constexpr int kK = kQ + 2 * kTileBytes;
-  static constexpr int kV = kK + kStages * kTileBytes;
-  static constexpr int kBar = kV + kStages * kTileBytes;
+  static constexpr int kK = 0;
+  static constexpr int kV = kK + kStages * kBlockBytes;
+  static constexpr int kBar = kV + kStages * kBlockBytes;
   static constexpr int kBytes = kBar + 256;
 };
 
-constexpr int kBlock = 64;                   // rows of a block in the backward
-constexpr int kBlockBytes = kBlock * 128;
 constexpr int kBwdStages = 8;
 
 struct BwdSmem {
@@ -151,6 +156,18 @@ template <typename T> __device__ __forceinline__ void store_row(T *dst, uint32_t
   }
 }
 
+// This thread's row of 64 16-bit values (zeros where !held) into 32
+// tensor-memory columns, and a copy in registers.
+template <typename T>
+__device__ __forceinline__ void row_to_tmem(const T *src, bool held, uint32_t taddr, uint4 (&raw)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    raw[e] = held ? *reinterpret_cast<const uint4 *>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
+  tmem_st16(taddr, reinterpret_cast<const float(&)[16]>(raw[0]));
+  tmem_st16(taddr + 16, reinterpret_cast<const float(&)[16]>(raw[4]));
+  tmem_wait_st();
+}
+
 template <typename T> __device__ __forceinline__ void zero_rows(T *dst, int64_t stride, int rows) {
   for (int e = threadIdx.x; e < rows * 8; e += blockDim.x)
     *reinterpret_cast<uint4 *>(dst + (e >> 3) * stride + (e & 7) * 8) = make_uint4(0u, 0u, 0u, 0u);
@@ -160,9 +177,8 @@ template <typename T> __device__ __forceinline__ void zero_rows(T *dst, int64_t 
 
 template <typename T>
 __global__ void __launch_bounds__(pt::kFwdThreads, 1)
-    packed_fwd_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
-                         const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
-                         int32_t *err) {
+    packed_fwd_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmk,
+                         const __grid_constant__ CUtensorMap tmv, int32_t *err) {
   using namespace pt;
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   // heads fastest; the last tiles, which see the most keys, first
@@ -179,143 +195,152 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
   }
   extern __shared__ __align__(1024) char smem_raw[];
   char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t *q_full = reinterpret_cast<uint64_t *>(sm + FwdSmem::kBar);
-  uint64_t *k_full = q_full + 1, *v_full = k_full + kStages, *kv_empty = v_full + kStages;
-  uint64_t *s_full = kv_empty + kStages, *p_full = s_full + 2, *o_full = p_full + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+  FwdBars *bars = reinterpret_cast<FwdBars *>(sm + FwdSmem::kBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = h / (a.Hq / a.Hkv);
   // key blocks of each tile: those up to its diagonal
-  const int n0 = t.row0 / kRows + 1, n1 = rows > kRows ? n0 + 1 : 0;
+  const int all = (t.len + kBlock - 1) / kBlock;
+  const int n0 = min(all, t.row0 / kBlock + 2), n1 = rows > kRows ? min(all, n0 + 2) : 0;
   const int blocks = max(n0, n1);
-  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (warp == 8) tmem_alloc(&bars->tmem, 512);
   if (tid == 288) {
-    mbar_init(q_full, 1);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 4);
-      mbar_init(&o_full[x], 1);
+      mbar_init(&bars->s_full[x][0], 1);
+      mbar_init(&bars->s_full[x][1], 1);
+      mbar_init(&bars->p_full[x][0], 4);
+      mbar_init(&bars->p_full[x][1], 4);
+      mbar_init(&bars->o_full[x][0], 1);
+      mbar_init(&bars->o_full[x][1], 1);
     }
     mbar_init_fence();
   }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = bars->tmem;
   bool ok = true;
   float l = 0.f, m = -INFINITY;
+  const int x = warp >> 2, r = (warp & 3) * 32 + lane;  // of a softmax warp: tile and row
+  const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+
+  auto load = [&](int i) {
+    const int s = i % kStages, row = static_cast<int>(t.start) + i * kBlock;
+    mbar_arrive_expect_tx(&bars->full[s], 2 * kBlockBytes);
+    tma_load_4d(sm + FwdSmem::kK + s * kBlockBytes, &tmk, 0, row, hk, 0, &bars->full[s]);
+    tma_load_4d(sm + FwdSmem::kV + s * kBlockBytes, &tmv, 0, row, hk, 0, &bars->full[s]);
+  };
+  if (warp == 9 && lane == 0)
+    for (int i = 0; i < min(blocks, kStages); ++i) load(i);
+  if (warp < 8 && (x == 0 || n1 > 0)) {
+    uint4 raw[8];
+    row_to_tmem(static_cast<const T *>(a.q) + (first + x * kRows + r) * a.q_st + h * a.q_sh, x * kRows + r < rows,
+                tmem + lane_base + kFwdQ + 32 * x, raw);
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
 
   if (warp == 9) {
     if (lane == 0) {
-      mbar_arrive_expect_tx(q_full, (n1 ? 2u : 1u) * kTileBytes);
-      for (int x = 0; x < (n1 ? 2 : 1); ++x)
-        tma_load_4d(sm + FwdSmem::kQ + x * kTileBytes, &tmq, 0, static_cast<int>(first) + x * kRows, h, 0, q_full);
-      for (int i = 0; i < blocks && ok; ++i) {
-        const int s = i % kStages;
-        if (i >= kStages) ok = mbar_wait_bounded(&kv_empty[s], (i / kStages - 1) & 1);
+      for (int i = kStages; i < blocks; ++i) {
+        ok = mbar_wait(&bars->empty[i % kStages], (i / kStages - 1) & 1);
         if (!ok) break;
-        const int row = static_cast<int>(t.start) + i * kRows;
-        mbar_arrive_expect_tx(&k_full[s], kTileBytes);
-        tma_load_4d(sm + FwdSmem::kK + s * kTileBytes, &tmk, 0, row, hk, 0, &k_full[s]);
-        mbar_arrive_expect_tx(&v_full[s], kTileBytes);
-        tma_load_4d(sm + FwdSmem::kV + s * kTileBytes, &tmv, 0, row, hk, 0, &v_full[s]);
+        load(i);
       }
     }
     __syncwarp();
   } else if (warp == 8) {
-    const uint32_t id_s = idesc_f16(fmt, false, 128), id_o = idesc_f16(fmt, true, 64);
-    const uint32_t sq = smem_u32(sm + FwdSmem::kQ), sk = smem_u32(sm + FwdSmem::kK), sv = smem_u32(sm + FwdSmem::kV);
-    auto issue_s = [&](int x, int i) {
+    constexpr uint32_t id_s = idesc_f16(fmt, false, 64), id_o = idesc_f16(fmt, true, 64);
+    const uint32_t sk = smem_u32(sm + FwdSmem::kK), sv = smem_u32(sm + FwdSmem::kV);
+    auto issue_s = [&](int y, int i) {
       const int s = i % kStages;
-      ok = ok && mbar_wait_bounded(&k_full[s], (i / kStages) & 1);
+      ok = ok && mbar_wait(&bars->full[s], (i / kStages) & 1);
       fence_after_sync();
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mma_f16(tmem + 128 * x, umma_desc_sw128(sq + x * kTileBytes + 32 * k, 16, 1024),
-                umma_desc_sw128(sk + s * kTileBytes + 32 * k, 16, 1024), id_s, k > 0);
-      mma_commit(&s_full[x]);
+        for (int k = 0; k < 4; ++k)
+          mma_f16_ts(tmem + 128 * y + 64 * (i & 1), tmem + kFwdQ + 32 * y + 8 * k,
+                     umma_desc_sw128(sk + s * kBlockBytes + 32 * k, 16, 1024), id_s, k > 0);
+        mma_commit(&bars->s_full[y][i & 1]);
+      }
+      __syncwarp();
     };
-    if (lane == 0) {
-      ok = mbar_wait_bounded(q_full, 0);
-      issue_s(0, 0);
-      if (n1) issue_s(1, 0);
-    }
-    const int tail = t.len / kRows;  // the block that holds the sequence's end, if it ends inside one
+    for (int i = 0; i < 2; ++i)
+      for (int y = 0; y < 2; ++y)
+        if (i < (y ? n1 : n0)) issue_s(y, i);
+    const int tail = t.len / kBlock;  // the block that holds the sequence's end, if it ends inside one
     for (int i = 0; i < blocks; ++i) {
       const int s = i % kStages;
       if (i == tail) {
-        if (lane == 0) ok = ok && mbar_wait_bounded(&v_full[s], (i / kStages) & 1);
-        __syncwarp();
-        clear_rows(sm + FwdSmem::kV + s * kTileBytes, t.len - tail * kRows, kRows);
+        ok = ok && mbar_wait(&bars->full[s], (i / kStages) & 1);
+        clear_rows(sm + FwdSmem::kV + s * kBlockBytes, t.len - tail * kBlock, kBlock);
       }
-      if (lane == 0) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int n = x ? n1 : n0;
-          if (i >= n) continue;
-          ok = ok && mbar_wait_bounded(&v_full[s], (i / kStages) & 1);
-          ok = ok && mbar_wait_bounded(&p_full[x], i & 1);
-          fence_after_sync();
+      for (int y = 0; y < 2; ++y) {
+        const int n = y ? n1 : n0;
+        if (i >= n) continue;
+        ok = ok && mbar_wait(&bars->p_full[y][i & 1], (i >> 1) & 1);
+        fence_after_sync();
+        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_f16_ts(tmem + 256 + 64 * x, tmem + 128 * x + 8 * k,
-                       umma_desc_sw128(sv + s * kTileBytes + 2048 * k, kTileBytes, 1024), id_o, i > 0 || k > 0);
-          if (i + 1 < n)
-            issue_s(x, i + 1);
-          else
-            mma_commit(&o_full[x]);
+          for (int k = 0; k < 4; ++k)
+            mma_f16_ts(tmem + kFwdO + 64 * y, tmem + 128 * y + 64 * (i & 1) + 8 * k,
+                       umma_desc_sw128(sv + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id_o, i > 0 || k > 0);
+          mma_commit(&bars->o_full[y][i & 1]);
         }
-        if (i + kStages < blocks) mma_commit(&kv_empty[s]);
+        __syncwarp();
+        if (i + 2 < n) issue_s(y, i + 2);
       }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (i + kStages < blocks && elect_one()) mma_commit(&bars->empty[s]);
+      if (!__all_sync(0xffffffffu, ok)) break;
     }
   } else {
-    const int x = warp >> 2, r = (warp & 3) * 32 + lane;
-    const int n = x ? n1 : n0;
-    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_base + 128 * x, t_o = tmem + lane_base + 256 + 64 * x;
+    const int n = x ? n1 : n0, row = t.row0 + x * kRows + r;
+    const uint32_t t_o = tmem + lane_base + kFwdO + 64 * x;
     const float c = a.scale_log2;
     for (int i = 0; i < n; ++i) {
-      ok = mbar_wait_bounded(&s_full[x], i & 1);
+      const uint32_t t_s = tmem + lane_base + 128 * x + 64 * (i & 1);
+      ok = mbar_wait(&bars->s_full[x][i & 1], (i >> 1) & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
-      float s[128];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) tmem_ld32(t_s + 32 * u, s + 32 * u);
+      float s[64];
+      tmem_ld32(t_s, s);
+      tmem_ld32(t_s + 32, s + 32);
       tmem_wait_ld();
-      if (i == n - 1) {  // the diagonal block: row r sees its first r + 1 keys
+      if (i >= n - 2 && i * kBlock + kBlock - 1 > row - r) {  // the diagonal's two blocks
+        const int seen = row + 1 - i * kBlock;
 #pragma unroll
-        for (int u = 0; u < 128; ++u) s[u] = u <= r ? s[u] : -INFINITY;
+        for (int u = 0; u < 64; ++u) s[u] = u < seen ? s[u] : -INFINITY;
       }
-      float top[4] = {s[0], s[1], s[2], s[3]};
+      float top[4];
 #pragma unroll
-      for (int u = 4; u < 128; u += 8) {
+      for (int e = 0; e < 4; ++e) top[e] = fmaxf(s[e], s[e + 4]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          top[e] = u + 4 + e < 128 ? fmaxf(top[e], fmaxf(s[u + e], s[u + 4 + e])) : fmaxf(top[e], s[u + e]);
-      }
+      for (int u = 8; u < 64; u += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(s[u + e], s[u + 4 + e]));
       const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+      float alpha = 1.f;
       if (best > m + kRescaleLog2 || m == -INFINITY) {
-        const float alpha = m == -INFINITY ? 0.f : ex2(m - best);
+        alpha = m == -INFINITY ? 0.f : ex2(m - best);
         m = best;
         l *= alpha;
-        top[0] = alpha;
-      } else {
-        top[0] = 1.f;
       }
-      if (i > 0 && __any_sync(0xffffffffu, top[0] != 1.f)) {
+      if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        ok = mbar_wait(&bars->o_full[x][(i - 1) & 1], ((i - 1) >> 1) & 1);  // O up to block i - 1
+        if (__any_sync(0xffffffffu, !ok)) break;
+        fence_after_sync();
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float o[32];
           tmem_ld32(t_o + 32 * u, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= top[0];
+          for (int e = 0; e < 32; ++e) o[e] *= alpha;
           tmem_st16(t_o + 32 * u, reinterpret_cast<float(&)[16]>(o[0]));
           tmem_st16(t_o + 32 * u + 16, reinterpret_cast<float(&)[16]>(o[16]));
         }
@@ -323,7 +348,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       const float neg = m == -INFINITY ? 0.f : -m;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         float p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -339,32 +364,26 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+      // a barrier for each buffer: a warp may be a block ahead of its warpgroup's others
+      if (lane == 0) mbar_arrive(&bars->p_full[x][i & 1]);
     }
     if (n > 0 && ok) {
-      ok = mbar_wait_bounded(&o_full[x], 0);
+      ok = mbar_wait(&bars->o_full[x][(n - 1) & 1], ((n - 1) >> 1) & 1);
       fence_after_sync();
     }
   }
   const bool failed = __syncthreads_or(!ok);
   if (failed) {  // a bounded wait expired: let copies in flight land, poison the rows
     if (tid == 288)
-      for (int s = 0; s < kStages; ++s) {
-        mbar_wait_bounded(&k_full[s], 0, 1000000ull);
-        mbar_wait_bounded(&v_full[s], 0, 1000000ull);
-      }
+      for (int s = 0; s < kStages; ++s) mbar_wait(&bars->full[s], 0, 1000000ull);
     l = __int_as_float(0x7fc00000);
     if (tid == 0 && err) *err = SD_KERR_TIMEOUT;
   }
-  if (warp < 8) {
-    const int x = warp >> 2, row = 32 * warp + lane;  // row of the CTA: tile x, row % 128
-    if (x == 0 || n1 > 0) {
-      const bool mine = row < rows;
-      fence_after_sync();
-      store_row(out + row * a.o_st, tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 + 64 * x, 1.0f / l,
-                mine);
-      if (mine && a.lse) a.lse[h * a.total + first + row] = m + log2f(l);
-    }
+  if (warp < 8 && (x == 0 || n1 > 0)) {
+    const int row = x * kRows + r;
+    fence_after_sync();
+    store_row(out + row * a.o_st, tmem + lane_base + kFwdO + 64 * x, 1.0f / l, row < rows);
+    if (row < rows && a.lse) a.lse[h * a.total + first + row] = m + log2f(l);
   }
   fence_before_sync();
   __syncthreads();
@@ -398,25 +417,13 @@ __device__ __forceinline__ void bwd_init(BwdBars *bars) {
   mbar_init_fence();
 }
 
-// This thread's row of 64 16-bit values (zeros where !held) into 32
-// tensor-memory columns, and a copy in registers.
-template <typename T>
-__device__ __forceinline__ void row_to_tmem(const T *src, bool held, uint32_t taddr, uint4 (&raw)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    raw[e] = held ? *reinterpret_cast<const uint4 *>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
-  tmem_st16(taddr, reinterpret_cast<const float(&)[16]>(raw[0]));
-  tmem_st16(taddr + 16, reinterpret_cast<const float(&)[16]>(raw[4]));
-  tmem_wait_st();
-}
-
 // The copy thread's loop over blocks [i0, i1): block i lies `i % per_head`
 // blocks behind row0, in head head0 + i / per_head.
 __device__ __forceinline__ bool bwd_copy(BwdBars *bars, char *sm, const CUtensorMap &ma, const CUtensorMap &mb, int i0,
                                          int i1, int per_head, int row0, int head0) {
   for (int i = i0; i < i1; ++i) {
     const int s = i % kBwdStages;
-    if (i >= kBwdStages && !mbar_wait_bounded(&bars->empty[s], (i / kBwdStages - 1) & 1)) return false;
+    if (i >= kBwdStages && !mbar_wait(&bars->empty[s], (i / kBwdStages - 1) & 1)) return false;
     const int row = row0 + (i % per_head) * kBlock, head = head0 + i / per_head;
     mbar_arrive_expect_tx(&bars->full[s], 2 * kBlockBytes);
     tma_load_4d(sm + BwdSmem::kA + s * kBlockBytes, &ma, 0, row, head, 0, &bars->full[s]);
@@ -428,7 +435,7 @@ __device__ __forceinline__ bool bwd_copy(BwdBars *bars, char *sm, const CUtensor
 // A bounded wait expired: copies in flight land before the CTA ends.
 __device__ __forceinline__ void bwd_failed(BwdBars *bars, int32_t *err) {
   if (threadIdx.x == 288)
-    for (int s = 0; s < kBwdStages; ++s) mbar_wait_bounded(&bars->full[s], 0, 1000000ull);
+    for (int s = 0; s < kBwdStages; ++s) mbar_wait(&bars->full[s], 0, 1000000ull);
   if (threadIdx.x == 0 && err) *err = SD_KERR_TIMEOUT;
 }
 
@@ -440,7 +447,7 @@ __device__ __forceinline__ float unit_scale(float x) {
   return x > 0.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 1.f;
 }
 
-// The MMA thread's loop, the same for both kernels: products of block i into
+// The MMA warp's loop, the same for both kernels: products of block i into
 // its warpgroup's columns, and the accumulation of block i once its weights are
 // there.  acc(i, stage): issues the accumulating MMAs.
 template <typename T, typename Acc>
@@ -448,20 +455,18 @@ __device__ __forceinline__ bool bwd_mma(BwdBars *bars, char *sm, uint32_t tmem, 
                                         int per_head, bool clear_b, Acc acc) {
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t id = idesc_f16(fmt, false, 64);
-  const int lane = threadIdx.x & 31;
   const uint32_t sa = smem_u32(sm + BwdSmem::kA), sb = smem_u32(sm + BwdSmem::kB);
   bool ok = true;
   auto products = [&](int i) {
     const int s = i % kBwdStages;
-    if (lane == 0) ok = ok && mbar_wait_bounded(&bars->full[s], (i / kBwdStages) & 1);
+    ok = ok && mbar_wait(&bars->full[s], (i / kBwdStages) & 1);
     const int left = rows_end - (first_row + (i % per_head) * kBlock);  // rows of the block within the sequence
     if (left < kBlock) {
-      __syncwarp();
       clear_rows(sm + BwdSmem::kA + s * kBlockBytes, left, kBlock);
       if (clear_b) clear_rows(sm + BwdSmem::kB + s * kBlockBytes, left, kBlock);
     }
-    if (lane == 0) {
-      fence_after_sync();
+    fence_after_sync();
+    if (elect_one()) {
       const uint32_t col = tmem + 128 * (i & 1);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -473,19 +478,21 @@ __device__ __forceinline__ bool bwd_mma(BwdBars *bars, char *sm, uint32_t tmem, 
                    k > 0);
       mma_commit(&bars->sd_full[i & 1]);
     }
+    __syncwarp();
   };
   products(0);
   if (blocks > 1) products(1);
   for (int i = 0; i < blocks; ++i) {
     const int s = i % kBwdStages;
-    if (lane == 0) {
-      ok = ok && mbar_wait_bounded(&bars->p_full[i & 1], (i >> 1) & 1);
-      fence_after_sync();
+    ok = ok && mbar_wait(&bars->p_full[i & 1], (i >> 1) & 1);
+    fence_after_sync();
+    if (elect_one()) {
       acc(i, s);
       if (i + kBwdStages < blocks) mma_commit(&bars->empty[s]);
       if (i + 1 == blocks) mma_commit(&bars->done);
     }
-    if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
+    __syncwarp();
+    if (!__all_sync(0xffffffffu, ok)) return false;
     if (i + 2 < blocks) products(i + 2);
   }
   return ok;
@@ -585,7 +592,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     const float delta = vec[r], lse = r < rows ? a.lse[h * a.total + first + r] : 0.f;
     const float f = kHalf ? unit_scale(vec[128 + r]) : 1.f;
     for (int i = wg; i < blocks; i += 2) {
-      ok = mbar_wait_bounded(&bars->sd_full[wg], (i >> 1) & 1);
+      ok = mbar_wait(&bars->sd_full[wg], (i >> 1) & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
       float s[64], d[64];
@@ -619,7 +626,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
       if (lane == 0) mbar_arrive(&bars->p_full[wg]);
     }
     if (ok) {
-      ok = mbar_wait_bounded(&bars->done, 0);
+      ok = mbar_wait(&bars->done, 0);
       fence_after_sync();
     }
   }
@@ -727,7 +734,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
         break;
       }
       next = fetch(i + 2);
-      ok = mbar_wait_bounded(&bars->sd_full[wg], (i >> 1) & 1);
+      ok = mbar_wait(&bars->sd_full[wg], (i >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       fence_after_sync();
       const int q0 = (i % per_head) * kBlock;  // from the tile's first key
@@ -779,7 +786,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
       if (lane == 0 && ok) mbar_arrive(&bars->p_full[wg]);
     }
     if (ok) {
-      ok = mbar_wait_bounded(&bars->done, 0);
+      ok = mbar_wait(&bars->done, 0);
       fence_after_sync();
     }
   }
@@ -798,26 +805,24 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
 }
 
-// Map of a packed tensor [total][H][64]: boxes of `box` rows of one head.
-static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total, int64_t H, int64_t st, int64_t sh,
-                      int box) {
+// Map of a packed tensor [total][H][64]: boxes of 64 rows of one head.
+static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total, int64_t H, int64_t st, int64_t sh) {
   if (H == 1 && sh <= 0) sh = 64;
   if (total == 1 && st <= 0) st = sh * H;
-  return encode_rows_map(map, p, dtype, 64, total, H, 1, st, sh, st, box);
+  return encode_rows_map(map, p, dtype, 64, total, H, 1, st, sh, st, pt::kBlock);
 }
 
 int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
-  CUtensorMap mq, mk, mv;
-  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh, pt::kRows);
-  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kRows);
-  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh, pt::kRows);
+  CUtensorMap mk, mv;
+  int rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh);
+  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh);
   if (rc != SD_OK) return rc;
   const int64_t ctas = packed_slots(a.total, a.S, 2 * pt::kRows) * a.Hq;
   if (ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
   const size_t smem = pt::FwdSmem::kBytes + 1024;
   auto run = [&](auto *kern) {
     if (set_max_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
-    kern<<<static_cast<unsigned>(ctas), pt::kFwdThreads, smem, s>>>(a, mq, mk, mv, err);
+    kern<<<static_cast<unsigned>(ctas), pt::kFwdThreads, smem, s>>>(a, mk, mv, err);
     return check_launch();
   };
   return dtype == SD_DTYPE_BF16 ? run(packed_fwd_tc_kernel<__nv_bfloat16>) : run(packed_fwd_tc_kernel<__half>);
@@ -825,10 +830,10 @@ int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
 
 int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
   CUtensorMap mq, mk, mv, mg;
-  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh, pt::kBlock);
-  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kBlock);
-  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh, pt::kBlock);
-  if (rc == SD_OK) rc = packed_map(&mg, a.dout, dtype, a.total, a.Hq, a.g_st, a.g_sh, pt::kBlock);
+  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh);
+  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh);
+  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh);
+  if (rc == SD_OK) rc = packed_map(&mg, a.dout, dtype, a.total, a.Hq, a.g_st, a.g_sh);
   if (rc != SD_OK) return rc;
   const int64_t slots = packed_slots(a.total, a.S, pt::kRows);
   if (slots * a.Hq > 0x7fffffffll) return SD_ERR_UNSUPPORTED;

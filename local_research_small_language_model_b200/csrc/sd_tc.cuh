@@ -42,6 +42,18 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uin
       : "memory");
 }
 
+// One lane of a converged warp, always the same one.  MMAs behind this test
+// issue about three times as fast as behind a comparison of thread indexes
+// (67 against 208 cycles each): the compiler sees that one thread is active and
+// moves the descriptors to uniform registers without a loop over lanes.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
@@ -89,6 +101,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) 
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// mbar_wait_bounded with the clock read every 32 tries only: where a wait
+// stands in a chain of MMA and softmax, reading the timer costs more than the
+// wait.
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns = 2000000000ull) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1; i < (1u << 30); ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 31u) == 0) {
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > limit_ns) return false;
+    }
+  }
+  return false;
+}
 
 // Lazy rescaling: a row keeps its reference maximum m (log2 units) until a
 // block's maximum exceeds it by more than this; the exponentials are then at
