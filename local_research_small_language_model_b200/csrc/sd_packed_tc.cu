@@ -14,8 +14,11 @@
 // Warp 8 issues all MMAs, warp 9 all copies (K and V in a ring of 8 stages).
 // S_x(i + 2) is issued right behind O_x(i), so a warpgroup finds the next
 // scores ready when it has written its weights, and both compute all the time.
-// A row keeps its reference maximum until a block exceeds it by 2^8; only then
-// does it wait for O_x(i - 1) and rescale it.
+// A row's reference m is its first block's maximum, and stays while a block's
+// weights sum to at most 2^14 (16-bit weights and fp32 sums have the same
+// relative precision there), so the common path looks for no maximum: the sum,
+// needed anyway, tells.  Otherwise m moves to the block's maximum, the weights
+// are computed again, and O, once O_x(i - 1) is done, is rescaled.
 //
 // Backward, two kernels of one shape: a CTA owns 128 rows, whose two operands
 // stay in tensor memory as A for all products, and walks 64-row blocks of the
@@ -48,6 +51,8 @@ constexpr int kBlockBytes = kBlock * 128;    // of 64 16-bit values
 constexpr int kStages = 8;
 constexpr int kFwdThreads = 320;             // 2 softmax warpgroups, MMA warp, copy warp
 constexpr int kFwdO = 256, kFwdQ = 384;      // tensor-memory columns; S of tile x from 128 x, two buffers
+
+constexpr float kMostSum = 16384.f;          // of a block's weights against a row's reference
 
 struct FwdBars {
   uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2][2];
@@ -308,29 +313,49 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
       float s[64];
-      tmem_ld32(t_s, s);
-      tmem_ld32(t_s + 32, s + 32);
-      tmem_wait_ld();
-      if (i >= n - 2 && i * kBlock + kBlock - 1 > row - r) {  // the diagonal's two blocks
-        const int seen = row + 1 - i * kBlock;
-#pragma unroll
-        for (int u = 0; u < 64; ++u) s[u] = u < seen ? s[u] : -INFINITY;
-      }
-      float top[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top[e] = fmaxf(s[e], s[e + 4]);
-#pragma unroll
-      for (int u = 8; u < 64; u += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(s[u + e], s[u + 4 + e]));
-      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+      uint32_t w[32];
+      // this row's weights against the reference m, in w, and their sum; `raise`
+      // first moves m to the block's maximum
       float alpha = 1.f;
-      if (best > m + kRescaleLog2 || m == -INFINITY) {
-        alpha = m == -INFINITY ? 0.f : ex2(m - best);
-        m = best;
+      auto weights = [&](bool raise) {
+        tmem_ld32(t_s, s);
+        tmem_ld32(t_s + 32, s + 32);
+        tmem_wait_ld();
+        if (i >= n - 2 && i * kBlock + kBlock - 1 > row - r) {  // the diagonal's two blocks
+          const int seen = row + 1 - i * kBlock;
+#pragma unroll
+          for (int u = 0; u < 64; ++u) s[u] = u < seen ? s[u] : -INFINITY;
+        }
+        if (raise) {
+          float top[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = fmaxf(s[e], s[e + 4]);
+#pragma unroll
+          for (int u = 8; u < 64; u += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(s[u + e], s[u + 4 + e]));
+          const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+          if (best > m) {
+            alpha = m == -INFINITY ? 0.f : ex2(m - best);
+            m = best;
+          }
+        }
+        const float neg = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float y0 = s[2 * e], y1 = s[2 * e + 1];
+          fma2(y0, y1, c, neg);
+          y0 = ex2(y0), y1 = ex2(y1);
+          add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], y0, y1);
+          w[e] = pack2<T>(y0, y1);
+        }
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      };
+      float sum = weights(i == 0);
+      if (__any_sync(0xffffffffu, !(sum <= kMostSum)) && i > 0) {
+        sum = weights(true);
         l *= alpha;
-      }
-      if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
         ok = mbar_wait(&bars->o_full[x][(i - 1) & 1], ((i - 1) >> 1) & 1);  // O up to block i - 1
         if (__any_sync(0xffffffffu, !ok)) break;
         fence_after_sync();
@@ -345,22 +370,9 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
           tmem_st16(t_o + 32 * u + 16, reinterpret_cast<float(&)[16]>(o[16]));
         }
       }
-      const float neg = m == -INFINITY ? 0.f : -m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float y0 = s[32 * u + 2 * e], y1 = s[32 * u + 2 * e + 1];
-          fma2(y0, y1, c, neg);
-          y0 = ex2(y0), y1 = ex2(y1);
-          add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], y0, y1);
-          p[e] = __uint_as_float(pack2<T>(y0, y1));
-        }
-        tmem_st16(t_s + 16 * u, p);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += sum;
+      tmem_st16(t_s, reinterpret_cast<const float(&)[16]>(w[0]));
+      tmem_st16(t_s + 16, reinterpret_cast<const float(&)[16]>(w[16]));
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
