@@ -3,22 +3,22 @@
 //
 //   O_i = sum_{j <= i} exp2(c q_i.k_j - m_i) v_j / l_i,  c = scale log2(e)
 //
-// Forward.  One CTA per 256 query rows of one sequence and head, one per SM.
-// The rows are two 128-row tiles, whose Q stays in tensor memory as A; for
-// every 64 keys up to a tile's own diagonal
-//   S_x = Q_x K^T    4 MMAs M=128 N=64 K=16, fp32 in 64 of two alternating
-//                    runs of 64 columns
+// Forward.  One CTA per 256 query rows of one sequence and head, two per SM.
+// The rows are two 128-row tiles; for every 64 keys up to a tile's own diagonal
+//   S_x = Q_x K^T    4 MMAs M=128 N=64 K=16, fp32 in 64 columns
 //   P_x = exp2(..)   warpgroup x, one thread a row, 16-bit pairs written over
 //                    the first 32 columns of S_x
 //   O_x += P_x V     4 MMAs, A from tensor memory
-// Warp 8 issues all MMAs, warp 9 all copies (K and V in a ring of 8 stages).
-// S_x(i + 2) is issued right behind O_x(i), so a warpgroup finds the next
-// scores ready when it has written its weights, and both compute all the time.
+// Warp 8 issues all MMAs, warp 9 all copies (K and V in a ring of 4 stages).
+// The four tiles of an SM take turns: while one's products run, the others
+// compute exponentials, which are the bound (64 a row and block at 16 a cycle
+// and SM; the products need 320 of those 512 cycles).  S_x(i + 1) is issued right
+// behind O_x(i), so its arrival also says that O_x(i) is done.
 // A row's reference m is its first block's maximum, and stays while a block's
 // weights sum to at most 2^14 (16-bit weights and fp32 sums have the same
 // relative precision there), so the common path looks for no maximum: the sum,
 // needed anyway, tells.  Otherwise m moves to the block's maximum, the weights
-// are computed again, and O, once O_x(i - 1) is done, is rescaled.
+// are computed again, and O is rescaled.
 //
 // Backward, two kernels of one shape: a CTA owns 128 rows, whose two operands
 // stay in tensor memory as A for all products, and walks 64-row blocks of the
@@ -48,19 +48,21 @@ using namespace tc;
 constexpr int kRows = 128;                   // MMA M
 constexpr int kBlock = 64;                   // rows of a block of the other side
 constexpr int kBlockBytes = kBlock * 128;    // of 64 16-bit values
-constexpr int kStages = 8;
+constexpr int kStages = 4;
 constexpr int kFwdThreads = 320;             // 2 softmax warpgroups, MMA warp, copy warp
-constexpr int kFwdO = 256, kFwdQ = 384;      // tensor-memory columns; S of tile x from 128 x, two buffers
+constexpr int kFwdCols = 256, kFwdO = 128;   // tensor-memory columns: S of tile x from 64 x, O_x from 128 + 64 x
+constexpr int kTileBytes = kRows * 128;
 
 constexpr float kMostSum = 16384.f;          // of a block's weights against a row's reference
 
 struct FwdBars {
-  uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2][2];
+  uint64_t full[kStages], empty[kStages], s_full[2], p_full[2], o_full[2];
   uint32_t tmem;
 };
 
 struct FwdSmem {
-  static constexpr int kK = 0;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kBlockBytes;
   static constexpr int kBar = kV + kStages * kBlockBytes;
   static constexpr int kBytes = kBar + 256;
@@ -181,7 +183,7 @@ template <typename T> __device__ __forceinline__ void zero_rows(T *dst, int64_t 
 }  // namespace pt
 
 template <typename T>
-__global__ void __launch_bounds__(pt::kFwdThreads, 1)
+__global__ void __launch_bounds__(pt::kFwdThreads, 2)
     packed_fwd_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmk,
                          const __grid_constant__ CUtensorMap tmv, int32_t *err) {
   using namespace pt;
@@ -207,19 +209,16 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
   const int all = (t.len + kBlock - 1) / kBlock;
   const int n0 = min(all, t.row0 / kBlock + 2), n1 = rows > kRows ? min(all, n0 + 2) : 0;
   const int blocks = max(n0, n1);
-  if (warp == 8) tmem_alloc(&bars->tmem, 512);
+  if (warp == 8) tmem_alloc(&bars->tmem, kFwdCols);
   if (tid == 288) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&bars->s_full[x][0], 1);
-      mbar_init(&bars->s_full[x][1], 1);
-      mbar_init(&bars->p_full[x][0], 4);
-      mbar_init(&bars->p_full[x][1], 4);
-      mbar_init(&bars->o_full[x][0], 1);
-      mbar_init(&bars->o_full[x][1], 1);
+      mbar_init(&bars->s_full[x], 1);
+      mbar_init(&bars->p_full[x], 4);
+      mbar_init(&bars->o_full[x], 1);
     }
     mbar_init_fence();
   }
@@ -241,9 +240,14 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
   if (warp == 9 && lane == 0)
     for (int i = 0; i < min(blocks, kStages); ++i) load(i);
   if (warp < 8 && (x == 0 || n1 > 0)) {
-    uint4 raw[8];
-    row_to_tmem(static_cast<const T *>(a.q) + (first + x * kRows + r) * a.q_st + h * a.q_sh, x * kRows + r < rows,
-                tmem + lane_base + kFwdQ + 32 * x, raw);
+    // this thread's row of Q, swizzled as the copies swizzle (zeros behind the sequence)
+    const T *src = static_cast<const T *>(a.q) + (first + x * kRows + r) * a.q_st + h * a.q_sh;
+    const bool held = x * kRows + r < rows;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<uint4 *>(sm + FwdSmem::kQ + x * kTileBytes + sw128(r, e)) =
+          held ? *reinterpret_cast<const uint4 *>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
+    fence_async_smem();
   }
   fence_before_sync();
   __syncthreads();
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
     __syncwarp();
   } else if (warp == 8) {
     constexpr uint32_t id_s = idesc_f16(fmt, false, 64), id_o = idesc_f16(fmt, true, 64);
-    const uint32_t sk = smem_u32(sm + FwdSmem::kK), sv = smem_u32(sm + FwdSmem::kV);
+    const uint32_t sq = smem_u32(sm + FwdSmem::kQ), sk = smem_u32(sm + FwdSmem::kK), sv = smem_u32(sm + FwdSmem::kV);
     auto issue_s = [&](int y, int i) {
       const int s = i % kStages;
       ok = ok && mbar_wait(&bars->full[s], (i / kStages) & 1);
@@ -268,15 +272,14 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mma_f16_ts(tmem + 128 * y + 64 * (i & 1), tmem + kFwdQ + 32 * y + 8 * k,
-                     umma_desc_sw128(sk + s * kBlockBytes + 32 * k, 16, 1024), id_s, k > 0);
-        mma_commit(&bars->s_full[y][i & 1]);
+          mma_f16(tmem + 64 * y, umma_desc_sw128(sq + y * kTileBytes + 32 * k, 16, 1024),
+                  umma_desc_sw128(sk + s * kBlockBytes + 32 * k, 16, 1024), id_s, k > 0);
+        mma_commit(&bars->s_full[y]);
       }
       __syncwarp();
     };
-    for (int i = 0; i < 2; ++i)
-      for (int y = 0; y < 2; ++y)
-        if (i < (y ? n1 : n0)) issue_s(y, i);
+    issue_s(0, 0);
+    if (n1 > 0) issue_s(1, 0);
     const int tail = t.len / kBlock;  // the block that holds the sequence's end, if it ends inside one
     for (int i = 0; i < blocks; ++i) {
       const int s = i % kStages;
@@ -288,53 +291,54 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       for (int y = 0; y < 2; ++y) {
         const int n = y ? n1 : n0;
         if (i >= n) continue;
-        ok = ok && mbar_wait(&bars->p_full[y][i & 1], (i >> 1) & 1);
+        ok = ok && mbar_wait(&bars->p_full[y], i & 1);
         fence_after_sync();
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_f16_ts(tmem + kFwdO + 64 * y, tmem + 128 * y + 64 * (i & 1) + 8 * k,
+            mma_f16_ts(tmem + kFwdO + 64 * y, tmem + 64 * y + 8 * k,
                        umma_desc_sw128(sv + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id_o, i > 0 || k > 0);
-          mma_commit(&bars->o_full[y][i & 1]);
+          if (i + 1 == n) mma_commit(&bars->o_full[y]);
         }
         __syncwarp();
-        if (i + 2 < n) issue_s(y, i + 2);
+        if (i + 1 < n) issue_s(y, i + 1);
       }
       if (i + kStages < blocks && elect_one()) mma_commit(&bars->empty[s]);
       if (!__all_sync(0xffffffffu, ok)) break;
     }
   } else {
     const int n = x ? n1 : n0, row = t.row0 + x * kRows + r;
-    const uint32_t t_o = tmem + lane_base + kFwdO + 64 * x;
+    const uint32_t t_s = tmem + lane_base + 64 * x, t_o = tmem + lane_base + kFwdO + 64 * x;
     const float c = a.scale_log2;
     for (int i = 0; i < n; ++i) {
-      const uint32_t t_s = tmem + lane_base + 128 * x + 64 * (i & 1);
-      ok = mbar_wait(&bars->s_full[x][i & 1], (i >> 1) & 1);
+      ok = mbar_wait(&bars->s_full[x], i & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
-      float s[64];
       uint32_t w[32];
       // this row's weights against the reference m, in w, and their sum; `raise`
       // first moves m to the block's maximum
       float alpha = 1.f;
-      auto weights = [&](bool raise) {
-        tmem_ld32(t_s, s);
-        tmem_ld32(t_s + 32, s + 32);
+      const bool edge = i * kBlock + kBlock - 1 > row - r;  // the diagonal's two blocks
+      auto scores = [&](int half, float (&s)[32]) {
+        tmem_ld32(t_s + 32 * half, s);
         tmem_wait_ld();
-        if (i >= n - 2 && i * kBlock + kBlock - 1 > row - r) {  // the diagonal's two blocks
-          const int seen = row + 1 - i * kBlock;
+        if (edge) {
+          const int seen = row + 1 - i * kBlock - 32 * half;
 #pragma unroll
-          for (int u = 0; u < 64; ++u) s[u] = u < seen ? s[u] : -INFINITY;
+          for (int u = 0; u < 32; ++u) s[u] = u < seen ? s[u] : -INFINITY;
         }
+      };
+      auto weights = [&](bool raise) {
+        float s[32];
         if (raise) {
-          float top[4];
+          float best = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = fmaxf(s[e], s[e + 4]);
+          for (int half = 0; half < 2; ++half) {
+            scores(half, s);
 #pragma unroll
-          for (int u = 8; u < 64; u += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(s[u + e], s[u + 4 + e]));
-          const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+            for (int u = 0; u < 32; ++u) best = fmaxf(best, s[u]);
+          }
+          best *= c;
           if (best > m) {
             alpha = m == -INFINITY ? 0.f : ex2(m - best);
             m = best;
@@ -343,12 +347,16 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
         const float neg = m == -INFINITY ? 0.f : -m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float y0 = s[2 * e], y1 = s[2 * e + 1];
-          fma2(y0, y1, c, neg);
-          y0 = ex2(y0), y1 = ex2(y1);
-          add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], y0, y1);
-          w[e] = pack2<T>(y0, y1);
+        for (int half = 0; half < 2; ++half) {
+          scores(half, s);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float y0 = s[2 * e], y1 = s[2 * e + 1];
+            fma2(y0, y1, c, neg);
+            y0 = ex2(y0), y1 = ex2(y1);
+            add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], y0, y1);
+            w[16 * half + e] = pack2<T>(y0, y1);
+          }
         }
         return (sum[0] + sum[1]) + (sum[2] + sum[3]);
       };
@@ -356,9 +364,6 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       if (__any_sync(0xffffffffu, !(sum <= kMostSum)) && i > 0) {
         sum = weights(true);
         l *= alpha;
-        ok = mbar_wait(&bars->o_full[x][(i - 1) & 1], ((i - 1) >> 1) & 1);  // O up to block i - 1
-        if (__any_sync(0xffffffffu, !ok)) break;
-        fence_after_sync();
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float o[32];
@@ -376,11 +381,10 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
-      // a barrier for each buffer: a warp may be a block ahead of its warpgroup's others
-      if (lane == 0) mbar_arrive(&bars->p_full[x][i & 1]);
+      if (lane == 0) mbar_arrive(&bars->p_full[x]);
     }
     if (n > 0 && ok) {
-      ok = mbar_wait(&bars->o_full[x][(n - 1) & 1], ((n - 1) >> 1) & 1);
+      ok = mbar_wait(&bars->o_full[x], 0);
       fence_after_sync();
     }
   }
@@ -401,7 +405,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 1)
   __syncthreads();
   if (warp == 8) {
     fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, kFwdCols);
   }
 }
 
