@@ -121,6 +121,31 @@ __device__ __forceinline__ void mul2(float &a, float &b, float c, float d) {  //
       : "f"(c), "f"(d));
 }
 
+// 2^a and 2^b on the FMA pipe, to 2^-22, for a, b <= 127 (above: 2^127; a NaN
+// too).  n = round(x) by adding 1.5 2^23, f = x - n in [-1/2, 1/2], 2^f by its
+// degree-5 polynomial of least relative error (fitted for this use), n added to
+// the exponent.  Below -126: at most 2^-126.
+__device__ __forceinline__ void exp2_fma(float &a, float &b) {
+  a = fmaxf(fminf(a, 127.f), -126.f);
+  b = fmaxf(fminf(b, 127.f), -126.f);
+  asm("{\n\t.reg .b64 x, t, n, f, p, c;\n\t.reg .b32 t0, t1, p0, p1;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b32 t0, 0f4B400000;\n\tmov.b64 c, {t0, t0};\n\tadd.rn.f32x2 t, x, c;\n\t"
+      "mov.b32 t1, 0fCB400000;\n\tmov.b64 c, {t1, t1};\n\tadd.rn.f32x2 n, t, c;\n\t"
+      "mov.b32 t1, 0fBF800000;\n\tmov.b64 c, {t1, t1};\n\tfma.rn.f32x2 f, n, c, x;\n\t"
+      "mov.b64 p, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%4, %4};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 {t0, t1}, t;\n\tmov.b64 {p0, p1}, p;\n\t"
+      "shl.b32 t0, t0, 23;\n\tshl.b32 t1, t1, 23;\n\t"
+      "add.u32 p0, p0, t0;\n\tadd.u32 p1, p1, t1;\n\tmov.b32 %0, p0;\n\tmov.b32 %1, p1;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(0.001327647129073739f), "f"(0.009675540961325169f), "f"(0.05550713092088699f), "f"(0.24022120237350464f),
+        "f"(0.6931469440460205f), "f"(1.0000001192092896f));
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -314,10 +339,6 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
       ok = mbar_wait(&bars->s_full[x], i & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
-      uint32_t w[32];
-      // this row's weights against the reference m, in w, and their sum; `raise`
-      // first moves m to the block's maximum
-      float alpha = 1.f;
       const bool edge = i * kBlock + kBlock - 1 > row - r;  // the diagonal's two blocks
       auto scores = [&](int half, float (&s)[32]) {
         tmem_ld32(t_s + 32 * half, s);
@@ -328,52 +349,65 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
           for (int u = 0; u < 32; ++u) s[u] = u < seen ? s[u] : -INFINITY;
         }
       };
-      auto weights = [&](bool raise) {
-        float s[32];
-        if (raise) {
-          float best = -INFINITY;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            scores(half, s);
-#pragma unroll
-            for (int u = 0; u < 32; ++u) best = fmaxf(best, s[u]);
-          }
-          best *= c;
-          if (best > m) {
-            alpha = m == -INFINITY ? 0.f : ex2(m - best);
-            m = best;
-          }
-        }
+      uint32_t w[32];
+      auto weights = [&](auto poly) {
+        constexpr bool kPoly = decltype(poly)::value;
         const float neg = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
+          float s[32];
           scores(half, s);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float y0 = s[2 * e], y1 = s[2 * e + 1];
             fma2(y0, y1, c, neg);
-            y0 = ex2(y0), y1 = ex2(y1);
-            add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], y0, y1);
+            // every fourth pair's exponentials on the FMA pipe: the special-function unit is the bound
+            if (kPoly && (e & 3) == 3)
+              exp2_fma(y0, y1);
+            else
+              y0 = ex2(y0), y1 = ex2(y1);
+            add2(part[2 * (e & 1)], part[2 * (e & 1) + 1], y0, y1);
             w[16 * half + e] = pack2<T>(y0, y1);
           }
         }
-        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        return (part[0] + part[1]) + (part[2] + part[3]);
       };
-      float sum = weights(i == 0);
-      if (__any_sync(0xffffffffu, !(sum <= kMostSum)) && i > 0) {
-        sum = weights(true);
-        l *= alpha;
+      float sum;
+      for (bool raise = i == 0;;) {
+        if (raise) {  // the reference moves to this block's maximum, what is summed so far with it
+          float best = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float o[32];
-          tmem_ld32(t_o + 32 * u, o);
-          tmem_wait_ld();
+          for (int half = 0; half < 2; ++half) {
+            float s[32];
+            scores(half, s);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= alpha;
-          tmem_st16(t_o + 32 * u, reinterpret_cast<float(&)[16]>(o[0]));
-          tmem_st16(t_o + 32 * u + 16, reinterpret_cast<float(&)[16]>(o[16]));
+            for (int u = 0; u < 32; ++u) best = fmaxf(best, s[u]);
+          }
+          best *= c;
+          float alpha = 1.f;
+          if (best > m) {
+            alpha = m == -INFINITY ? 0.f : ex2(m - best);
+            m = best;
+          }
+          l *= alpha;
+          if (i > 0) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              float o[16];
+              tmem_ld16(t_o + 16 * u, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              tmem_st16(t_o + 16 * u, o);
+            }
+          }
         }
+        // masked and first blocks, and what the polynomial's range does not hold (a NaN, an infinity, a weight
+        // past 2^127: the sum tells), take the special-function unit for all
+        sum = raise || edge ? weights(std::false_type()) : weights(std::true_type());
+        if (raise || !__any_sync(0xffffffffu, !(sum <= kMostSum))) break;
+        raise = true;
       }
       l += sum;
       tmem_st16(t_s, reinterpret_cast<const float(&)[16]>(w[0]));
