@@ -23,8 +23,9 @@
 // Backward, two kernels of one shape: a CTA owns 128 rows, whose two operands
 // stay in tensor memory as A for all products, and walks 64-row blocks of the
 // other side, whose two operands arrive in shared memory and serve as B both
-// ways.  Block i belongs to warpgroup i mod 2, each with its own S and dP
-// columns, so one computes while the other's products run.
+// ways.  Blocks alternate between two runs of S and dP columns; two warpgroups
+// share a run, 32 columns each, so eight warps compute while the other run's
+// products are under way.
 //   dQ:    rows are queries (A: Q, dO), blocks are keys (B: K, V)
 //          S = Q K^T, dP = dO V^T;  dS = P (dP - delta);  dQ += dS K
 //   dK/dV: rows are keys (A: K, V), blocks are queries of every head of the
@@ -73,7 +74,7 @@ constexpr int kBwdStages = 8;
 struct BwdSmem {
   static constexpr int kA = 0;               // K or Q blocks
   static constexpr int kB = kA + kBwdStages * kBlockBytes;  // V or dO blocks
-  static constexpr int kVec = kB + kBwdStages * kBlockBytes;  // 2 warpgroups x 2 x (64 lse, 64 delta)
+  static constexpr int kVec = kB + kBwdStages * kBlockBytes;  // 4 warpgroups x 2 x (32 lse, 32 delta)
   static constexpr int kBar = kVec + 2048;
   static constexpr int kBytes = kBar + 256;
 };
@@ -446,7 +447,8 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
 // ---------------------------------------------------------------- backward
 namespace pt {
 
-constexpr int kBwdThreads = 320;
+constexpr int kBwdMma = 16, kBwdCopy = 17;    // warps; 0 to 15 compute
+constexpr int kBwdThreads = 576;
 constexpr int kColS = 0, kColDp = 64, kColAcc = 256, kColAcc2 = 320, kColA = 384, kColB = 416;
 
 struct BwdBars {
@@ -461,7 +463,7 @@ __device__ __forceinline__ void bwd_init(BwdBars *bars) {
   }
   for (int b = 0; b < 2; ++b) {
     mbar_init(&bars->sd_full[b], 1);
-    mbar_init(&bars->p_full[b], 4);
+    mbar_init(&bars->p_full[b], 8);
   }
   mbar_init(&bars->done, 1);
   mbar_init_fence();
@@ -484,10 +486,14 @@ __device__ __forceinline__ bool bwd_copy(BwdBars *bars, char *sm, const CUtensor
 
 // A bounded wait expired: copies in flight land before the CTA ends.
 __device__ __forceinline__ void bwd_failed(BwdBars *bars, int32_t *err) {
-  if (threadIdx.x == 288)
+  if (threadIdx.x == 32 * kBwdCopy)
     for (int s = 0; s < kBwdStages; ++s) mbar_wait(&bars->full[s], 0, 1000000ull);
   if (threadIdx.x == 0 && err) *err = SD_KERR_TIMEOUT;
 }
+
+// Where the 16-bit weights of 16 rows of a block lie from their score columns
+// on: each half of the 64 score columns holds its own, in its first 16.
+__device__ __forceinline__ constexpr int weight_col(int k) { return 8 * (k & 1) + 32 * (k >> 1); }
 
 // The power of two that takes x into [1/2, 1) (1 for 0): fp16 holds dS scaled
 // by it, so that small output gradients (a loss averaged over many tokens)
@@ -575,8 +581,8 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = h / (a.Hq / a.Hkv);
   const int blocks = min((t.len + kBlock - 1) / kBlock, t.row0 / kBlock + 2);
-  if (warp == 8) tmem_alloc(&bars->tmem, 512);
-  if (tid == 288) bwd_init(bars);
+  if (warp == kBwdMma) tmem_alloc(&bars->tmem, 512);
+  if (tid == 32 * kBwdCopy) bwd_init(bars);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -584,7 +590,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
   bool ok = true;
-  if (warp == 9 && lane == 0)
+  if (warp == kBwdCopy && lane == 0)
     bwd_copy(bars, sm, tmk, tmv, 0, min(blocks, kBwdStages), blocks, static_cast<int>(t.start), hk);
   if (warp < 8) {
     // the tile's rows: warpgroup 0 brings Q, warpgroup 1 dO and with O delta
@@ -624,36 +630,34 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   __syncthreads();
   fence_after_sync();
 
-  if (warp == 9) {
+  if (warp == kBwdCopy) {
     if (lane == 0)
       ok = bwd_copy(bars, sm, tmk, tmv, min(blocks, kBwdStages), blocks, blocks, static_cast<int>(t.start), hk);
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == kBwdMma) {
     constexpr uint32_t id = idesc_f16(fmt, true, 64);
     const uint32_t sk = smem_u32(sm + BwdSmem::kA);
     ok = bwd_mma<T>(bars, sm, tmem, blocks, 0, t.len, blocks, false, [&](int i, int s) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tmem + kColAcc, tmem + 128 * (i & 1) + kColS + 8 * k,
+        mma_f16_ts(tmem + kColAcc, tmem + 128 * (i & 1) + kColS + weight_col(k),
                    umma_desc_sw128(sk + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
     });
   } else {
-    const uint32_t t_s = tmem + lane_base + 128 * wg;
+    const int buf = wg >> 1, half = wg & 1;  // score columns: of blocks buf, buf + 2, .., 32 from 32 half on
+    const uint32_t t_s = tmem + lane_base + 128 * buf + 32 * half;
     const float delta = vec[r], lse = r < rows ? a.lse[h * a.total + first + r] : 0.f;
     const float f = kHalf ? unit_scale(vec[128 + r]) : 1.f;
-    for (int i = wg; i < blocks; i += 2) {
-      ok = mbar_wait(&bars->sd_full[wg], (i >> 1) & 1);
+    for (int i = buf; i < blocks; i += 2) {
+      ok = mbar_wait(&bars->sd_full[buf], (i >> 1) & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
-      float s[64], d[64];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        tmem_ld32(t_s + kColS + 32 * u, s + 32 * u);
-        tmem_ld32(t_s + kColDp + 32 * u, d + 32 * u);
-      }
+      float s[32], d[32];
+      tmem_ld32(t_s + kColS, s);
+      tmem_ld32(t_s + kColDp, d);
       tmem_wait_ld();
 #pragma unroll
-      for (int u = 0; u < 64; u += 2) {
+      for (int u = 0; u < 32; u += 2) {
         fma2(s[u], s[u + 1], a.scale_log2, -lse);
         s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
         add2(d[u], d[u + 1], -delta, -delta);
@@ -661,19 +665,18 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
         mul2(d[u], d[u + 1], s[u], s[u + 1]);
       }
       if (i * kBlock + kBlock - 1 > t.row0) {  // the diagonal's two blocks
-        const int seen = t.row0 + r + 1 - i * kBlock;
+        const int seen = t.row0 + r + 1 - i * kBlock - 32 * half;
 #pragma unroll
-        for (int u = 0; u < 64; ++u) d[u] = u < seen ? d[u] : 0.f;
+        for (int u = 0; u < 32; ++u) d[u] = u < seen ? d[u] : 0.f;
       }
-      float w[32];
+      float w[16];
 #pragma unroll
-      for (int u = 0; u < 32; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
-      tmem_st16(t_s + kColS, reinterpret_cast<const float(&)[16]>(w[0]));
-      tmem_st16(t_s + kColS + 16, reinterpret_cast<const float(&)[16]>(w[16]));
+      for (int u = 0; u < 16; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
+      tmem_st16(t_s + kColS, w);
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full[wg]);
+      if (lane == 0) mbar_arrive(&bars->p_full[buf]);
     }
     if (ok) {
       ok = mbar_wait(&bars->done, 0);
@@ -689,7 +692,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kBwdMma) {
     fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
@@ -720,8 +723,8 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per_head = (t.len - t.row0 + kBlock - 1) / kBlock, blocks = per_head * group;
-  if (warp == 8) tmem_alloc(&bars->tmem, 512);
-  if (tid == 288) bwd_init(bars);
+  if (warp == kBwdMma) tmem_alloc(&bars->tmem, 512);
+  if (tid == 32 * kBwdCopy) bwd_init(bars);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -729,7 +732,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
   bool ok = true;
-  if (warp == 9 && lane == 0)
+  if (warp == kBwdCopy && lane == 0)
     bwd_copy(bars, sm, tmq, tmg, 0, min(blocks, kBwdStages), per_head, static_cast<int>(first), hk * group);
   if (warp < 8) {
     uint4 raw[8];
@@ -741,37 +744,39 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   __syncthreads();
   fence_after_sync();
   const float f = kHalf ? unit_scale(__uint_as_float(*top)) : 1.f;
-  if (warp == 9) {
+  if (warp == kBwdCopy) {
     if (lane == 0)
       ok = bwd_copy(bars, sm, tmq, tmg, min(blocks, kBwdStages), blocks, per_head, static_cast<int>(first), hk * group);
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == kBwdMma) {
     constexpr uint32_t id = idesc_f16(fmt, true, 64);
     const uint32_t sq = smem_u32(sm + BwdSmem::kA), sg = smem_u32(sm + BwdSmem::kB);
     ok = bwd_mma<T>(bars, sm, tmem, blocks, t.row0, t.len, per_head, true, [&](int i, int s) {
       const uint32_t col = tmem + 128 * (i & 1);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tmem + kColAcc, col + kColS + 8 * k,
+        mma_f16_ts(tmem + kColAcc, col + kColS + weight_col(k),
                    umma_desc_sw128(sg + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tmem + kColAcc2, col + kColDp + 8 * k,
+        mma_f16_ts(tmem + kColAcc2, col + kColDp + weight_col(k),
                    umma_desc_sw128(sq + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
     });
   } else {
-    const uint32_t t_s = tmem + lane_base + 128 * wg, bar_id = 1 + wg;
-    // the block's log sums and deltas, negated: thread r < 64 brings query r's sum, r >= 64 query r - 64's delta
-    const float *src = r < 64 ? a.lse : a.delta;
+    const int buf = wg >> 1, half = wg & 1;
+    const uint32_t t_s = tmem + lane_base + 128 * buf + 32 * half, bar_id = 1 + wg;
+    // its 32 queries' log sums and deltas, negated, come through shared memory: thread r < 32 brings query r's
+    // sum, the next 32 the deltas
+    const float *src = r < 32 ? a.lse : a.delta;
     auto fetch = [&](int i) {
-      const int qr = t.row0 + (i % per_head) * kBlock + (r & 63);
-      return i < blocks && qr < t.len
+      const int qr = t.row0 + (i % per_head) * kBlock + 32 * half + (r & 31);
+      return r < 64 && i < blocks && qr < t.len
                  ? -src[(hk * group + i / per_head) * a.total + t.start + qr] : 0.f;
     };
-    float next = fetch(wg);
-    for (int i = wg; i < blocks; i += 2) {
-      float *mine = vec + wg * 256 + ((i >> 1) & 1) * 128;
-      mine[r] = next;
+    float next = fetch(buf);
+    for (int i = buf; i < blocks; i += 2) {
+      float *mine = vec + wg * 128 + ((i >> 1) & 1) * 64;
+      if (r < 64) mine[r] = next;
       // the vectors are there; and a wait that expired in one warp ends them all
       uint32_t bad;
       asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 128, q;\n\t"
@@ -784,22 +789,19 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
         break;
       }
       next = fetch(i + 2);
-      ok = mbar_wait(&bars->sd_full[wg], (i >> 1) & 1);
+      ok = mbar_wait(&bars->sd_full[buf], (i >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       fence_after_sync();
       const int q0 = (i % per_head) * kBlock;  // from the tile's first key
       const bool edge = q0 < kRows || t.row0 + q0 + kBlock > t.len;
-      const int from = r - q0, to = t.len - t.row0 - q0;  // visible columns: from .. to - 1
-      float s[64], d[64];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        tmem_ld32(t_s + kColS + 32 * u, s + 32 * u);
-        tmem_ld32(t_s + kColDp + 32 * u, d + 32 * u);
-      }
+      const int from = r - q0 - 32 * half, to = t.len - t.row0 - q0 - 32 * half;  // visible columns: from .. to - 1
+      float s[32], d[32];
+      tmem_ld32(t_s + kColS, s);
+      tmem_ld32(t_s + kColDp, d);
       tmem_wait_ld();
 #pragma unroll
-      for (int u = 0; u < 64; u += 4) {
-        const float4 l4 = *reinterpret_cast<const float4 *>(mine + u), d4 = *reinterpret_cast<const float4 *>(mine + 64 + u);
+      for (int u = 0; u < 32; u += 4) {
+        const float4 l4 = *reinterpret_cast<const float4 *>(mine + u), d4 = *reinterpret_cast<const float4 *>(mine + 32 + u);
         fma2v(s[u], s[u + 1], a.scale_log2, l4.x, l4.y);
         fma2v(s[u + 2], s[u + 3], a.scale_log2, l4.z, l4.w);
         add2(d[u], d[u + 1], d4.x, d4.y);
@@ -815,25 +817,23 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
       }
       if (edge) {
 #pragma unroll
-        for (int u = 0; u < 64; ++u) {
+        for (int u = 0; u < 32; ++u) {
           const bool seen = u >= from && u < to;
           s[u] = seen ? s[u] : 0.f;
           d[u] = seen ? d[u] : 0.f;
         }
       }
-      float w[32];
+      float w[16];
 #pragma unroll
-      for (int u = 0; u < 32; ++u) w[u] = __uint_as_float(pack2<T>(s[2 * u], s[2 * u + 1]));
-      tmem_st16(t_s + kColS, reinterpret_cast<const float(&)[16]>(w[0]));
-      tmem_st16(t_s + kColS + 16, reinterpret_cast<const float(&)[16]>(w[16]));
+      for (int u = 0; u < 16; ++u) w[u] = __uint_as_float(pack2<T>(s[2 * u], s[2 * u + 1]));
+      tmem_st16(t_s + kColS, w);
 #pragma unroll
-      for (int u = 0; u < 32; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
-      tmem_st16(t_s + kColDp, reinterpret_cast<const float(&)[16]>(w[0]));
-      tmem_st16(t_s + kColDp + 16, reinterpret_cast<const float(&)[16]>(w[16]));
+      for (int u = 0; u < 16; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
+      tmem_st16(t_s + kColDp, w);
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
-      if (lane == 0 && ok) mbar_arrive(&bars->p_full[wg]);
+      if (lane == 0 && ok) mbar_arrive(&bars->p_full[buf]);
     }
     if (ok) {
       ok = mbar_wait(&bars->done, 0);
@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kBwdMma) {
     fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
