@@ -201,6 +201,11 @@ __device__ __forceinline__ void row_to_tmem(const T *src, bool held, uint32_t ta
   tmem_wait_st();
 }
 
+// A value that the warp's lanes share, in a form the compiler knows to be shared:
+// descriptors and columns derived from it stay in uniform registers, where MMAs
+// take them from.
+template <typename V> __device__ __forceinline__ V shared_value(V v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 template <typename T> __device__ __forceinline__ void zero_rows(T *dst, int64_t stride, int rows) {
   for (int e = threadIdx.x; e < rows * 8; e += blockDim.x)
     *reinterpret_cast<uint4 *>(dst + (e >> 3) * stride + (e & 7) * 8) = make_uint4(0u, 0u, 0u, 0u);
@@ -290,7 +295,11 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
     __syncwarp();
   } else if (warp == 8) {
     constexpr uint32_t id_s = idesc_f16(fmt, false, 64), id_o = idesc_f16(fmt, true, 64);
-    const uint32_t sq = smem_u32(sm + FwdSmem::kQ), sk = smem_u32(sm + FwdSmem::kK), sv = smem_u32(sm + FwdSmem::kV);
+    const uint64_t dq = umma_desc_sw128(smem_u32(sm + FwdSmem::kQ), 16, 1024);
+    const uint64_t dk = umma_desc_sw128(smem_u32(sm + FwdSmem::kK), 16, 1024);
+    const uint64_t dv = umma_desc_sw128(smem_u32(sm + FwdSmem::kV), kBlockBytes, 1024);
+    const uint32_t tm = shared_value(tmem);
+    const int u0 = shared_value(n0), u1 = shared_value(n1), last = max(u0, u1);
     auto issue_s = [&](int y, int i) {
       const int s = i % kStages;
       ok = ok && mbar_wait(&bars->full[s], (i / kStages) & 1);
@@ -298,16 +307,15 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mma_f16(tmem + 64 * y, umma_desc_sw128(sq + y * kTileBytes + 32 * k, 16, 1024),
-                  umma_desc_sw128(sk + s * kBlockBytes + 32 * k, 16, 1024), id_s, k > 0);
+          mma_f16(tm + 64 * y, dq + y * (kTileBytes >> 4) + 2 * k, dk + s * (kBlockBytes >> 4) + 2 * k, id_s, k > 0);
         mma_commit(&bars->s_full[y]);
       }
       __syncwarp();
     };
     issue_s(0, 0);
-    if (n1 > 0) issue_s(1, 0);
-    const int tail = t.len / kBlock;  // the block that holds the sequence's end, if it ends inside one
-    for (int i = 0; i < blocks; ++i) {
+    if (u1 > 0) issue_s(1, 0);
+    const int tail = shared_value(t.len) / kBlock;  // the block that holds the sequence's end, if it ends inside one
+    for (int i = 0; i < last; ++i) {
       const int s = i % kStages;
       if (i == tail) {
         ok = ok && mbar_wait(&bars->full[s], (i / kStages) & 1);
@@ -315,21 +323,21 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
       }
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int n = y ? n1 : n0;
+        const int n = y ? u1 : u0;
         if (i >= n) continue;
         ok = ok && mbar_wait(&bars->p_full[y], i & 1);
         fence_after_sync();
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_f16_ts(tmem + kFwdO + 64 * y, tmem + 64 * y + 8 * k,
-                       umma_desc_sw128(sv + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id_o, i > 0 || k > 0);
+            mma_f16_ts(tm + kFwdO + 64 * y, tm + 64 * y + 8 * k, dv + s * (kBlockBytes >> 4) + 128 * k, id_o,
+                       i > 0 || k > 0);
           if (i + 1 == n) mma_commit(&bars->o_full[y]);
         }
         __syncwarp();
         if (i + 1 < n) issue_s(y, i + 1);
       }
-      if (i + kStages < blocks && elect_one()) mma_commit(&bars->empty[s]);
+      if (i + kStages < last && elect_one()) mma_commit(&bars->empty[s]);
       if (!__all_sync(0xffffffffu, ok)) break;
     }
   } else {
@@ -503,35 +511,38 @@ __device__ __forceinline__ float unit_scale(float x) {
   return x > 0.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 1.f;
 }
 
-// The MMA warp's loop, the same for both kernels: products of block i into
-// its warpgroup's columns, and the accumulation of block i once its weights are
-// there.  acc(i, stage): issues the accumulating MMAs.
+// The MMA warp's loop, the same for both kernels: products of block i into its
+// run of columns, and the accumulation of block i once its weights are there.
+// Blocks come in runs of per_head, each over rows first_row .. rows_end - 1.
+// acc(b, off, first): issues the accumulating MMAs of the run of columns b with
+// shared-memory blocks `off` (in descriptor units) behind the first stage's.
 template <typename T, typename Acc>
 __device__ __forceinline__ bool bwd_mma(BwdBars *bars, char *sm, uint32_t tmem, int blocks, int first_row, int rows_end,
                                         int per_head, bool clear_b, Acc acc) {
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t id = idesc_f16(fmt, false, 64);
-  const uint32_t sa = smem_u32(sm + BwdSmem::kA), sb = smem_u32(sm + BwdSmem::kB);
+  const uint64_t da = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), 16, 1024);
+  const uint64_t db = umma_desc_sw128(smem_u32(sm + BwdSmem::kB), 16, 1024);
+  const int whole = (rows_end - first_row) / kBlock;  // a run's blocks that end within the sequence
   bool ok = true;
+  int nth = 0;  // of the next block in its run
   auto products = [&](int i) {
     const int s = i % kBwdStages;
     ok = ok && mbar_wait(&bars->full[s], (i / kBwdStages) & 1);
-    const int left = rows_end - (first_row + (i % per_head) * kBlock);  // rows of the block within the sequence
-    if (left < kBlock) {
+    if (nth >= whole) {
+      const int left = (rows_end - first_row) - nth * kBlock;
       clear_rows(sm + BwdSmem::kA + s * kBlockBytes, left, kBlock);
       if (clear_b) clear_rows(sm + BwdSmem::kB + s * kBlockBytes, left, kBlock);
     }
+    nth = nth + 1 == per_head ? 0 : nth + 1;
     fence_after_sync();
     if (elect_one()) {
       const uint32_t col = tmem + 128 * (i & 1);
+      const uint32_t off = s * (kBlockBytes >> 4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mma_f16_ts(col + kColS, tmem + kColA + 8 * k, umma_desc_sw128(sa + s * kBlockBytes + 32 * k, 16, 1024), id,
-                   k > 0);
+      for (int k = 0; k < 4; ++k) mma_f16_ts(col + kColS, tmem + kColA + 8 * k, da + off + 2 * k, id, k > 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mma_f16_ts(col + kColDp, tmem + kColB + 8 * k, umma_desc_sw128(sb + s * kBlockBytes + 32 * k, 16, 1024), id,
-                   k > 0);
+      for (int k = 0; k < 4; ++k) mma_f16_ts(col + kColDp, tmem + kColB + 8 * k, db + off + 2 * k, id, k > 0);
       mma_commit(&bars->sd_full[i & 1]);
     }
     __syncwarp();
@@ -543,7 +554,7 @@ __device__ __forceinline__ bool bwd_mma(BwdBars *bars, char *sm, uint32_t tmem, 
     ok = ok && mbar_wait(&bars->p_full[i & 1], (i >> 1) & 1);
     fence_after_sync();
     if (elect_one()) {
-      acc(i, s);
+      acc(i & 1, static_cast<uint32_t>(s * (kBlockBytes >> 4)), i == 0);
       if (i + kBwdStages < blocks) mma_commit(&bars->empty[s]);
       if (i + 1 == blocks) mma_commit(&bars->done);
     }
@@ -636,12 +647,13 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     __syncwarp();
   } else if (warp == kBwdMma) {
     constexpr uint32_t id = idesc_f16(fmt, true, 64);
-    const uint32_t sk = smem_u32(sm + BwdSmem::kA);
-    ok = bwd_mma<T>(bars, sm, tmem, blocks, 0, t.len, blocks, false, [&](int i, int s) {
+    const uint64_t dk = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), kBlockBytes, 1024);
+    const uint32_t tm = shared_value(tmem);
+    const int n = shared_value(blocks);
+    ok = bwd_mma<T>(bars, sm, tm, n, 0, shared_value(t.len), n, false, [&](int b, uint32_t off, bool first) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tmem + kColAcc, tmem + 128 * (i & 1) + kColS + weight_col(k),
-                   umma_desc_sw128(sk + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
+        mma_f16_ts(tm + kColAcc, tm + 128 * b + kColS + weight_col(k), dk + off + 128 * k, id, !first || k > 0);
     });
   } else {
     const int buf = wg >> 1, half = wg & 1;  // score columns: of blocks buf, buf + 2, .., 32 from 32 half on
@@ -750,17 +762,17 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     __syncwarp();
   } else if (warp == kBwdMma) {
     constexpr uint32_t id = idesc_f16(fmt, true, 64);
-    const uint32_t sq = smem_u32(sm + BwdSmem::kA), sg = smem_u32(sm + BwdSmem::kB);
-    ok = bwd_mma<T>(bars, sm, tmem, blocks, t.row0, t.len, per_head, true, [&](int i, int s) {
-      const uint32_t col = tmem + 128 * (i & 1);
+    const uint64_t dq = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), kBlockBytes, 1024);
+    const uint64_t dg = umma_desc_sw128(smem_u32(sm + BwdSmem::kB), kBlockBytes, 1024);
+    const uint32_t tm = shared_value(tmem);
+    ok = bwd_mma<T>(bars, sm, tm, shared_value(blocks), shared_value(t.row0), shared_value(t.len),
+                    shared_value(per_head), true, [&](int b, uint32_t off, bool first) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tmem + kColAcc, col + kColS + weight_col(k),
-                   umma_desc_sw128(sg + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
+        mma_f16_ts(tm + kColAcc, tm + 128 * b + kColS + weight_col(k), dg + off + 128 * k, id, !first || k > 0);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tmem + kColAcc2, col + kColDp + weight_col(k),
-                   umma_desc_sw128(sq + s * kBlockBytes + 2048 * k, kBlockBytes, 1024), id, i > 0 || k > 0);
+        mma_f16_ts(tm + kColAcc2, tm + 128 * b + kColDp + weight_col(k), dq + off + 128 * k, id, !first || k > 0);
     });
   } else {
     const int buf = wg >> 1, half = wg & 1;
