@@ -20,17 +20,18 @@
 // needed anyway, tells.  Otherwise m moves to the block's maximum, the weights
 // are computed again, and O is rescaled.
 //
-// Backward, two kernels of one shape: a CTA owns 128 rows, whose two operands
-// stay in tensor memory as A for all products, and walks 64-row blocks of the
-// other side, whose two operands arrive in shared memory and serve as B both
-// ways.  Blocks alternate between two runs of S and dP columns; two warpgroups
-// share a run, 32 columns each, so eight warps compute while the other run's
-// products are under way.
+// Backward, two kernels of one shape: a CTA owns 128 rows, the A operands of its
+// products, and walks 128-row blocks of the other side, which serve as B both
+// ways.
 //   dQ:    rows are queries (A: Q, dO), blocks are keys (B: K, V)
 //          S = Q K^T, dP = dO V^T;  dS = P (dP - delta);  dQ += dS K
 //   dK/dV: rows are keys (A: K, V), blocks are queries of every head of the
 //          group (B: Q, dO)
 //          S' = K Q^T, dP' = V dO^T;  dV += P' dO,  dK += dS' Q
+// Sixteen warps compute, 32 rows x 32 columns each.  They read a block's S and dP
+// into registers at once, which frees the columns for the next block's products,
+// and write their 16-bit weights to columns of their own: products, exponentials
+// and accumulation of neighbouring blocks run side by side.
 // S and dP are computed in both (7 products and 2 exponentials a pair instead
 // of 5 and 1): in return every gradient is summed in tensor memory in a fixed
 // order, with no atomics and no fp32 buffer to add into and convert.
@@ -66,16 +67,6 @@ struct FwdSmem {
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kBlockBytes;
   static constexpr int kBar = kV + kStages * kBlockBytes;
-  static constexpr int kBytes = kBar + 256;
-};
-
-constexpr int kBwdStages = 8;
-
-struct BwdSmem {
-  static constexpr int kA = 0;               // K or Q blocks
-  static constexpr int kB = kA + kBwdStages * kBlockBytes;  // V or dO blocks
-  static constexpr int kVec = kB + kBwdStages * kBlockBytes;  // 4 warpgroups x 2 x (32 lse, 32 delta)
-  static constexpr int kBar = kVec + 2048;
   static constexpr int kBytes = kBar + 256;
 };
 
@@ -122,13 +113,13 @@ __device__ __forceinline__ void mul2(float &a, float &b, float c, float d) {  //
       : "f"(c), "f"(d));
 }
 
-// 2^a and 2^b on the FMA pipe, to 2^-22, for a, b <= 127 (above: 2^127; a NaN
-// too).  n = round(x) by adding 1.5 2^23, f = x - n in [-1/2, 1/2], 2^f by its
+// 2^a and 2^b on the FMA pipe, to 2^-22, for a, b <= 127; with kUpper 2^127 for
+// what is above and for a NaN.  n = round(x) by adding 1.5 2^23, f = x - n in [-1/2, 1/2], 2^f by its
 // degree-5 polynomial of least relative error (fitted for this use), n added to
 // the exponent.  Below -126: at most 2^-126.
-__device__ __forceinline__ void exp2_fma(float &a, float &b) {
-  a = fmaxf(fminf(a, 127.f), -126.f);
-  b = fmaxf(fminf(b, 127.f), -126.f);
+template <bool kUpper> __device__ __forceinline__ void exp2_fma(float &a, float &b) {
+  a = fmaxf(kUpper ? fminf(a, 127.f) : a, -126.f);
+  b = fmaxf(kUpper ? fminf(b, 127.f) : b, -126.f);
   asm("{\n\t.reg .b64 x, t, n, f, p, c;\n\t.reg .b32 t0, t1, p0, p1;\n\t"
       "mov.b64 x, {%0, %1};\n\t"
       "mov.b32 t0, 0f4B400000;\n\tmov.b64 c, {t0, t0};\n\tadd.rn.f32x2 t, x, c;\n\t"
@@ -187,18 +178,6 @@ template <typename T> __device__ __forceinline__ void store_row(T *dst, uint32_t
           make_uint4(pack2<T>(v[c] * scale, v[c + 1] * scale), pack2<T>(v[c + 2] * scale, v[c + 3] * scale),
                      pack2<T>(v[c + 4] * scale, v[c + 5] * scale), pack2<T>(v[c + 6] * scale, v[c + 7] * scale));
   }
-}
-
-// This thread's row of 64 16-bit values (zeros where !held) into 32
-// tensor-memory columns, and a copy in registers.
-template <typename T>
-__device__ __forceinline__ void row_to_tmem(const T *src, bool held, uint32_t taddr, uint4 (&raw)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    raw[e] = held ? *reinterpret_cast<const uint4 *>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
-  tmem_st16(taddr, reinterpret_cast<const float(&)[16]>(raw[0]));
-  tmem_st16(taddr + 16, reinterpret_cast<const float(&)[16]>(raw[4]));
-  tmem_wait_st();
 }
 
 // A value that the warp's lanes share, in a form the compiler knows to be shared:
@@ -373,7 +352,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
             fma2(y0, y1, c, neg);
             // every fourth pair's exponentials on the FMA pipe: the special-function unit is the bound
             if (kPoly && (e & 3) == 3)
-              exp2_fma(y0, y1);
+              exp2_fma<true>(y0, y1);
             else
               y0 = ex2(y0), y1 = ex2(y1);
             add2(part[2 * (e & 1)], part[2 * (e & 1) + 1], y0, y1);
@@ -457,51 +436,71 @@ namespace pt {
 
 constexpr int kBwdMma = 16, kBwdCopy = 17;    // warps; 0 to 15 compute
 constexpr int kBwdThreads = 576;
-constexpr int kColS = 0, kColDp = 64, kColAcc = 256, kColAcc2 = 320, kColA = 384, kColB = 416;
+constexpr int kBwdStages = 4;
+
+struct BwdSmem {
+  static constexpr int kRowsA = 0;                              // the CTA's rows: Q or K
+  static constexpr int kRowsB = kRowsA + kTileBytes;            // dO or V
+  static constexpr int kA = kRowsB + kTileBytes;                // the other side's blocks: K or Q
+  static constexpr int kB = kA + kBwdStages * kTileBytes;       // V or dO
+  static constexpr int kVec = kB + kBwdStages * kTileBytes;     // dQ: [128] delta, [128] max |dout|;
+  static constexpr int kBar = kVec + 4096;                      // dK/dV: 16 warps x (32 lse, 32 delta)
+  static constexpr int kBytes = kBar + 256;
+};
+
+// Tensor-memory columns: scores, dP, 16-bit weights (dS; for dK/dV P then dS), accumulators.
+constexpr int kColS = 0, kColDp = 128, kColW = 256, kColW2 = 320;
+constexpr int kDqAcc = 320, kDkvAcc = 384, kDkvAcc2 = 448;
 
 struct BwdBars {
-  uint64_t full[kBwdStages], empty[kBwdStages], sd_full[2], p_full[2], done;
+  uint64_t rows, full[kBwdStages], empty[kBwdStages];
+  uint64_t sd_full, sd_free;  // S and dP computed; read
+  uint64_t w_full, w_free;    // weights written; consumed
   uint32_t tmem;
 };
 
 __device__ __forceinline__ void bwd_init(BwdBars *bars) {
+  mbar_init(&bars->rows, 1);
   for (int s = 0; s < kBwdStages; ++s) {
     mbar_init(&bars->full[s], 1);
     mbar_init(&bars->empty[s], 1);
   }
-  for (int b = 0; b < 2; ++b) {
-    mbar_init(&bars->sd_full[b], 1);
-    mbar_init(&bars->p_full[b], 8);
-  }
-  mbar_init(&bars->done, 1);
+  mbar_init(&bars->sd_full, 1);
+  mbar_init(&bars->sd_free, 16);
+  mbar_init(&bars->w_full, 16);
+  mbar_init(&bars->w_free, 1);
   mbar_init_fence();
 }
 
-// The copy thread's loop over blocks [i0, i1): block i lies `i % per_head`
-// blocks behind row0, in head head0 + i / per_head.
-__device__ __forceinline__ bool bwd_copy(BwdBars *bars, char *sm, const CUtensorMap &ma, const CUtensorMap &mb, int i0,
-                                         int i1, int per_head, int row0, int head0) {
-  for (int i = i0; i < i1; ++i) {
+// The copy thread: the CTA's rows, then the blocks; block i lies i % per_head
+// blocks behind block_row, in head head0 + i / per_head.
+__device__ __forceinline__ bool bwd_copy(BwdBars *bars, char *sm, const CUtensorMap &rows_a, const CUtensorMap &rows_b,
+                                         int row, int head, const CUtensorMap &ma, const CUtensorMap &mb, int blocks,
+                                         int per_head, int block_row, int head0) {
+  mbar_arrive_expect_tx(&bars->rows, 2 * kTileBytes);
+  tma_load_4d(sm + BwdSmem::kRowsA, &rows_a, 0, row, head, 0, &bars->rows);
+  tma_load_4d(sm + BwdSmem::kRowsB, &rows_b, 0, row, head, 0, &bars->rows);
+  int nth = 0;
+  for (int i = 0; i < blocks; ++i) {
     const int s = i % kBwdStages;
     if (i >= kBwdStages && !mbar_wait(&bars->empty[s], (i / kBwdStages - 1) & 1)) return false;
-    const int row = row0 + (i % per_head) * kBlock, head = head0 + i / per_head;
-    mbar_arrive_expect_tx(&bars->full[s], 2 * kBlockBytes);
-    tma_load_4d(sm + BwdSmem::kA + s * kBlockBytes, &ma, 0, row, head, 0, &bars->full[s]);
-    tma_load_4d(sm + BwdSmem::kB + s * kBlockBytes, &mb, 0, row, head, 0, &bars->full[s]);
+    const int at = block_row + nth * kRows;
+    mbar_arrive_expect_tx(&bars->full[s], 2 * kTileBytes);
+    tma_load_4d(sm + BwdSmem::kA + s * kTileBytes, &ma, 0, at, head0, 0, &bars->full[s]);
+    tma_load_4d(sm + BwdSmem::kB + s * kTileBytes, &mb, 0, at, head0, 0, &bars->full[s]);
+    if (++nth == per_head) nth = 0, ++head0;
   }
   return true;
 }
 
 // A bounded wait expired: copies in flight land before the CTA ends.
 __device__ __forceinline__ void bwd_failed(BwdBars *bars, int32_t *err) {
-  if (threadIdx.x == 32 * kBwdCopy)
+  if (threadIdx.x == 32 * kBwdCopy) {
+    mbar_wait(&bars->rows, 0, 1000000ull);
     for (int s = 0; s < kBwdStages; ++s) mbar_wait(&bars->full[s], 0, 1000000ull);
+  }
   if (threadIdx.x == 0 && err) *err = SD_KERR_TIMEOUT;
 }
-
-// Where the 16-bit weights of 16 rows of a block lie from their score columns
-// on: each half of the 64 score columns holds its own, in its first 16.
-__device__ __forceinline__ constexpr int weight_col(int k) { return 8 * (k & 1) + 32 * (k >> 1); }
 
 // The power of two that takes x into [1/2, 1) (1 for 0): fp16 holds dS scaled
 // by it, so that small output gradients (a loss averaged over many tokens)
@@ -511,65 +510,83 @@ __device__ __forceinline__ float unit_scale(float x) {
   return x > 0.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 1.f;
 }
 
-// The MMA warp's loop, the same for both kernels: products of block i into its
-// run of columns, and the accumulation of block i once its weights are there.
-// Blocks come in runs of per_head, each over rows first_row .. rows_end - 1.
-// acc(b, off, first): issues the accumulating MMAs of the run of columns b with
-// shared-memory blocks `off` (in descriptor units) behind the first stage's.
+// The MMA warp's loop, the same for both kernels: the products of block i + 1
+// as soon as block i's are read, then the accumulation of block i once its
+// weights are there.  Blocks come in runs of per_head, each over
+// rows_left rows.  acc(off, first): issues the accumulating MMAs with the
+// block's shared memory `off` (in descriptor units) behind the first stage's.
 template <typename T, typename Acc>
-__device__ __forceinline__ bool bwd_mma(BwdBars *bars, char *sm, uint32_t tmem, int blocks, int first_row, int rows_end,
-                                        int per_head, bool clear_b, Acc acc) {
+__device__ __forceinline__ bool bwd_mma(BwdBars *bars, char *sm, uint32_t tmem, int blocks, int rows_left, int per_head,
+                                        bool clear_b, Acc acc) {
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  constexpr uint32_t id = idesc_f16(fmt, false, 64);
+  constexpr uint32_t id = idesc_f16(fmt, false, 128);
+  const uint64_t ra = umma_desc_sw128(smem_u32(sm + BwdSmem::kRowsA), 16, 1024);
+  const uint64_t rb = umma_desc_sw128(smem_u32(sm + BwdSmem::kRowsB), 16, 1024);
   const uint64_t da = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), 16, 1024);
   const uint64_t db = umma_desc_sw128(smem_u32(sm + BwdSmem::kB), 16, 1024);
-  const int whole = (rows_end - first_row) / kBlock;  // a run's blocks that end within the sequence
-  bool ok = true;
-  int nth = 0;  // of the next block in its run
+  const int whole = rows_left / kRows;  // a run's blocks that end within the sequence
+  int nth = 0;                          // of the next block in its run
+  bool ok = mbar_wait(&bars->rows, 0);
   auto products = [&](int i) {
     const int s = i % kBwdStages;
     ok = ok && mbar_wait(&bars->full[s], (i / kBwdStages) & 1);
     if (nth >= whole) {
-      const int left = (rows_end - first_row) - nth * kBlock;
-      clear_rows(sm + BwdSmem::kA + s * kBlockBytes, left, kBlock);
-      if (clear_b) clear_rows(sm + BwdSmem::kB + s * kBlockBytes, left, kBlock);
+      const int left = rows_left - nth * kRows;
+      clear_rows(sm + BwdSmem::kA + s * kTileBytes, left, kRows);
+      if (clear_b) clear_rows(sm + BwdSmem::kB + s * kTileBytes, left, kRows);
     }
     nth = nth + 1 == per_head ? 0 : nth + 1;
     fence_after_sync();
     if (elect_one()) {
-      const uint32_t col = tmem + 128 * (i & 1);
-      const uint32_t off = s * (kBlockBytes >> 4);
+      const uint32_t off = s * (kTileBytes >> 4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mma_f16_ts(col + kColS, tmem + kColA + 8 * k, da + off + 2 * k, id, k > 0);
+      for (int k = 0; k < 4; ++k) mma_f16(tmem + kColS, ra + 2 * k, da + off + 2 * k, id, k > 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mma_f16_ts(col + kColDp, tmem + kColB + 8 * k, db + off + 2 * k, id, k > 0);
-      mma_commit(&bars->sd_full[i & 1]);
+      for (int k = 0; k < 4; ++k) mma_f16(tmem + kColDp, rb + 2 * k, db + off + 2 * k, id, k > 0);
+      mma_commit(&bars->sd_full);
     }
     __syncwarp();
   };
   products(0);
-  if (blocks > 1) products(1);
   for (int i = 0; i < blocks; ++i) {
+    if (i + 1 < blocks) {
+      ok = ok && mbar_wait(&bars->sd_free, i & 1);
+      products(i + 1);
+    }
     const int s = i % kBwdStages;
-    ok = ok && mbar_wait(&bars->p_full[i & 1], (i >> 1) & 1);
+    ok = ok && mbar_wait(&bars->w_full, i & 1);
     fence_after_sync();
     if (elect_one()) {
-      acc(i & 1, static_cast<uint32_t>(s * (kBlockBytes >> 4)), i == 0);
+      acc(static_cast<uint32_t>(s * (kTileBytes >> 4)), i == 0);
+      mma_commit(&bars->w_free);
       if (i + kBwdStages < blocks) mma_commit(&bars->empty[s]);
-      if (i + 1 == blocks) mma_commit(&bars->done);
     }
     __syncwarp();
     if (!__all_sync(0xffffffffu, ok)) return false;
-    if (i + 2 < blocks) products(i + 2);
   }
   return ok;
+}
+
+// A compute warp says that it has read its scores, or written its weights.
+__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
+  fence_before_sync();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+template <typename T> __device__ __forceinline__ void store_weights(uint32_t taddr, const float (&x)[32]) {
+  float w[16];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) w[u] = __uint_as_float(pack2<T>(x[2 * u], x[2 * u + 1]));
+  tmem_st16(taddr, w);
 }
 
 }  // namespace pt
 
 template <typename T>
 __global__ void __launch_bounds__(pt::kBwdThreads, 1)
-    packed_bwd_dq_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmk,
+    packed_bwd_dq_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
+                            const __grid_constant__ CUtensorMap tmg, const __grid_constant__ CUtensorMap tmk,
                             const __grid_constant__ CUtensorMap tmv, unsigned *top, int32_t *err) {
   using namespace pt;
   constexpr bool kHalf = std::is_same<T, __half>::value;
@@ -587,111 +604,106 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
   extern __shared__ __align__(1024) char smem_raw[];
   char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float *vec = reinterpret_cast<float *>(sm + BwdSmem::kVec);  // [128] delta, [128] max |dout|
+  float *vec = reinterpret_cast<float *>(sm + BwdSmem::kVec);
   BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = h / (a.Hq / a.Hkv);
-  const int blocks = min((t.len + kBlock - 1) / kBlock, t.row0 / kBlock + 2);
+  const int blocks = t.row0 / kRows + 1;  // keys up to the tile's diagonal
   if (warp == kBwdMma) tmem_alloc(&bars->tmem, 512);
   if (tid == 32 * kBwdCopy) bwd_init(bars);
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
-  const uint32_t tmem = bars->tmem;
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  bool ok = true;
-  if (warp == kBwdCopy && lane == 0)
-    bwd_copy(bars, sm, tmk, tmv, 0, min(blocks, kBwdStages), blocks, static_cast<int>(t.start), hk);
-  if (warp < 8) {
-    // the tile's rows: warpgroup 0 brings Q, warpgroup 1 dO and with O delta
-    uint4 raw[8];
-    if (wg == 0) {
-      row_to_tmem(static_cast<const T *>(a.q) + (first + r) * a.q_st + h * a.q_sh, r < rows, tmem + lane_base + kColA,
-                  raw);
-    } else {
-      row_to_tmem(static_cast<const T *>(a.dout) + (first + r) * a.g_st + h * a.g_sh, r < rows,
-                  tmem + lane_base + kColB, raw);
-      float delta = 0.f, big = 0.f;
-      if (r < rows) {
-        const T *o = static_cast<const T *>(a.out) + (first + r) * a.o_st + h * a.o_sh;
+  if (warp < 4) {  // delta, and for fp16 the largest |dout|, of row r
+    float delta = 0.f, big = 0.f;
+    if (r < rows) {
+      const T *o = static_cast<const T *>(a.out) + (first + r) * a.o_st + h * a.o_sh;
+      const T *g = static_cast<const T *>(a.dout) + (first + r) * a.g_st + h * a.g_sh;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(o + 8 * e);
-          const T *po = reinterpret_cast<const T *>(&x), *pg = reinterpret_cast<const T *>(&raw[e]);
+      for (int e = 0; e < 8; ++e) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(o + 8 * e), y = *reinterpret_cast<const uint4 *>(g + 8 * e);
+        const T *po = reinterpret_cast<const T *>(&x), *pg = reinterpret_cast<const T *>(&y);
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            delta = fmaf(to_f(po[u]), to_f(pg[u]), delta);
-            if (kHalf) big = fmaxf(big, fabsf(to_f(pg[u])));
-          }
+        for (int u = 0; u < 8; ++u) {
+          delta = fmaf(to_f(po[u]), to_f(pg[u]), delta);
+          if (kHalf) big = fmaxf(big, fabsf(to_f(pg[u])));
         }
-        a.delta[h * a.total + first + r] = delta;
       }
-      vec[r] = delta;
-      if (kHalf) {
-        big = big < INFINITY ? big : 0.f;
-        vec[128 + r] = big;
+      a.delta[h * a.total + first + r] = delta;
+    }
+    vec[r] = delta;
+    if (kHalf) {
+      big = big < INFINITY ? big : 0.f;
+      vec[128 + r] = big;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        if (lane == 0) atomicMax(top, __float_as_uint(big));
-      }
+      for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      if (lane == 0) atomicMax(top, __float_as_uint(big));
     }
   }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
-
+  const uint32_t tmem = bars->tmem;
+  bool ok = true;
   if (warp == kBwdCopy) {
     if (lane == 0)
-      ok = bwd_copy(bars, sm, tmk, tmv, min(blocks, kBwdStages), blocks, blocks, static_cast<int>(t.start), hk);
+      ok = bwd_copy(bars, sm, tmq, tmg, static_cast<int>(first), h, tmk, tmv, blocks, blocks,
+                    static_cast<int>(t.start), hk);
     __syncwarp();
   } else if (warp == kBwdMma) {
     constexpr uint32_t id = idesc_f16(fmt, true, 64);
-    const uint64_t dk = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), kBlockBytes, 1024);
+    const uint64_t dk = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), kTileBytes, 1024);
     const uint32_t tm = shared_value(tmem);
     const int n = shared_value(blocks);
-    ok = bwd_mma<T>(bars, sm, tm, n, 0, shared_value(t.len), n, false, [&](int b, uint32_t off, bool first) {
+    ok = bwd_mma<T>(bars, sm, tm, n, shared_value(t.len), n + 1, false, [&](uint32_t off, bool start) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tm + kColAcc, tm + 128 * b + kColS + weight_col(k), dk + off + 128 * k, id, !first || k > 0);
+      for (int k = 0; k < 8; ++k)
+        mma_f16_ts(tm + kDqAcc, tm + kColW + 8 * k, dk + off + 128 * k, id, !start || k > 0);
     });
   } else {
-    const int buf = wg >> 1, half = wg & 1;  // score columns: of blocks buf, buf + 2, .., 32 from 32 half on
-    const uint32_t t_s = tmem + lane_base + 128 * buf + 32 * half;
+    const uint32_t t_s = tmem + lane_base + kColS + 32 * wg;
     const float delta = vec[r], lse = r < rows ? a.lse[h * a.total + first + r] : 0.f;
     const float f = kHalf ? unit_scale(vec[128 + r]) : 1.f;
-    for (int i = buf; i < blocks; i += 2) {
-      ok = mbar_wait(&bars->sd_full[buf], (i >> 1) & 1);
+    for (int i = 0; i < blocks; ++i) {
+      ok = mbar_wait(&bars->sd_full, i & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
       float s[32], d[32];
-      tmem_ld32(t_s + kColS, s);
+      tmem_ld32(t_s, s);
       tmem_ld32(t_s + kColDp, d);
       tmem_wait_ld();
+      warp_arrive(&bars->sd_free);
+      // every fourth pair of exponentials on the FMA pipe where nothing is masked (scores are at most lse; a NaN
+      // there is in delta too)
+      auto weights = [&](auto poly) {
 #pragma unroll
-      for (int u = 0; u < 32; u += 2) {
-        fma2(s[u], s[u + 1], a.scale_log2, -lse);
-        s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
-        add2(d[u], d[u + 1], -delta, -delta);
-        if (kHalf) mul2(d[u], d[u + 1], f, f);
-        mul2(d[u], d[u + 1], s[u], s[u + 1]);
-      }
-      if (i * kBlock + kBlock - 1 > t.row0) {  // the diagonal's two blocks
-        const int seen = t.row0 + r + 1 - i * kBlock - 32 * half;
+        for (int u = 0; u < 32; u += 2) {
+          fma2(s[u], s[u + 1], a.scale_log2, -lse);
+          if (decltype(poly)::value && u % 8 == 6)
+            exp2_fma<false>(s[u], s[u + 1]);
+          else
+            s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
+          add2(d[u], d[u + 1], -delta, -delta);
+          if (kHalf) mul2(d[u], d[u + 1], f, f);
+          mul2(d[u], d[u + 1], s[u], s[u + 1]);
+        }
+      };
+      if (i + 1 < blocks) {
+        weights(std::true_type());
+      } else {  // the diagonal block
+        weights(std::false_type());
+        const int seen = r + 1 - 32 * wg;
 #pragma unroll
         for (int u = 0; u < 32; ++u) d[u] = u < seen ? d[u] : 0.f;
       }
-      float w[16];
-#pragma unroll
-      for (int u = 0; u < 16; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
-      tmem_st16(t_s + kColS, w);
+      if (i > 0) ok = mbar_wait(&bars->w_free, (i - 1) & 1);
+      if (__any_sync(0xffffffffu, !ok)) break;
+      fence_after_sync();
+      store_weights<T>(tmem + lane_base + kColW + 16 * wg, d);
       tmem_wait_st();
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full[buf]);
+      warp_arrive(&bars->w_full);
     }
     if (ok) {
-      ok = mbar_wait(&bars->done, 0);
+      ok = mbar_wait(&bars->w_free, (blocks - 1) & 1);
       fence_after_sync();
     }
   }
@@ -700,7 +712,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (warp < 4) {
     fence_after_sync();
     const float back = failed ? __int_as_float(0x7fc00000) : a.scale / (kHalf ? unit_scale(vec[128 + r]) : 1.f);
-    store_row(dq + r * c_st, tmem + lane_base + kColAcc, back, r < rows);
+    store_row(dq + r * c_st, tmem + lane_base + kDqAcc, back, r < rows);
   }
   fence_before_sync();
   __syncthreads();
@@ -713,7 +725,8 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
 template <typename T>
 __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     packed_bwd_dkv_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
-                             const __grid_constant__ CUtensorMap tmg, const unsigned *top, int32_t *err) {
+                             const __grid_constant__ CUtensorMap tmg, const __grid_constant__ CUtensorMap tmk,
+                             const __grid_constant__ CUtensorMap tmv, const unsigned *top, int32_t *err) {
   using namespace pt;
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr uint32_t fmt = kHalf ? 0u : 1u;
@@ -734,7 +747,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   float *vec = reinterpret_cast<float *>(sm + BwdSmem::kVec);
   BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int per_head = (t.len - t.row0 + kBlock - 1) / kBlock, blocks = per_head * group;
+  const int per_head = (t.len - t.row0 + kRows - 1) / kRows, blocks = per_head * group;
   if (warp == kBwdMma) tmem_alloc(&bars->tmem, 512);
   if (tid == 32 * kBwdCopy) bwd_init(bars);
   fence_before_sync();
@@ -743,91 +756,86 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   const uint32_t tmem = bars->tmem;
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  bool ok = true;
-  if (warp == kBwdCopy && lane == 0)
-    bwd_copy(bars, sm, tmq, tmg, 0, min(blocks, kBwdStages), per_head, static_cast<int>(first), hk * group);
-  if (warp < 8) {
-    uint4 raw[8];
-    const T *src = wg == 0 ? static_cast<const T *>(a.k) + (first + r) * a.k_st + hk * a.k_sh
-                           : static_cast<const T *>(a.v) + (first + r) * a.v_st + hk * a.v_sh;
-    row_to_tmem(src, r < keys, tmem + lane_base + (wg == 0 ? kColA : kColB), raw);
-  }
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
   const float f = kHalf ? unit_scale(__uint_as_float(*top)) : 1.f;
+  bool ok = true;
   if (warp == kBwdCopy) {
     if (lane == 0)
-      ok = bwd_copy(bars, sm, tmq, tmg, min(blocks, kBwdStages), blocks, per_head, static_cast<int>(first), hk * group);
+      ok = bwd_copy(bars, sm, tmk, tmv, static_cast<int>(first), hk, tmq, tmg, blocks, per_head,
+                    static_cast<int>(first), hk * group);
     __syncwarp();
   } else if (warp == kBwdMma) {
     constexpr uint32_t id = idesc_f16(fmt, true, 64);
-    const uint64_t dq = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), kBlockBytes, 1024);
-    const uint64_t dg = umma_desc_sw128(smem_u32(sm + BwdSmem::kB), kBlockBytes, 1024);
+    const uint64_t dq = umma_desc_sw128(smem_u32(sm + BwdSmem::kA), kTileBytes, 1024);
+    const uint64_t dg = umma_desc_sw128(smem_u32(sm + BwdSmem::kB), kTileBytes, 1024);
     const uint32_t tm = shared_value(tmem);
-    ok = bwd_mma<T>(bars, sm, tm, shared_value(blocks), shared_value(t.row0), shared_value(t.len),
-                    shared_value(per_head), true, [&](int b, uint32_t off, bool first) {
+    ok = bwd_mma<T>(bars, sm, tm, shared_value(blocks), shared_value(t.len - t.row0), shared_value(per_head), true,
+                    [&](uint32_t off, bool start) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tm + kColAcc, tm + 128 * b + kColS + weight_col(k), dg + off + 128 * k, id, !first || k > 0);
+      for (int k = 0; k < 8; ++k)
+        mma_f16_ts(tm + kDkvAcc, tm + kColW + 8 * k, dg + off + 128 * k, id, !start || k > 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mma_f16_ts(tm + kColAcc2, tm + 128 * b + kColDp + weight_col(k), dq + off + 128 * k, id, !first || k > 0);
+      for (int k = 0; k < 8; ++k)
+        mma_f16_ts(tm + kDkvAcc2, tm + kColW2 + 8 * k, dq + off + 128 * k, id, !start || k > 0);
     });
   } else {
-    const int buf = wg >> 1, half = wg & 1;
-    const uint32_t t_s = tmem + lane_base + 128 * buf + 32 * half, bar_id = 1 + wg;
-    // its 32 queries' log sums and deltas, negated, come through shared memory: thread r < 32 brings query r's
-    // sum, the next 32 the deltas
-    const float *src = r < 32 ? a.lse : a.delta;
+    const uint32_t t_s = tmem + lane_base + kColS + 32 * wg;
+    // the warp's 32 queries' log sums and deltas, negated: a lane brings one of each, all read them from shared memory
+    float *mine = vec + warp * 64;
+    const int left = t.len - t.row0 - 32 * wg - lane;  // the lane's query is held up to this many rows behind the tile
+    const int64_t at = static_cast<int64_t>(hk) * group * a.total + first + 32 * wg + lane;
+    const float *lse = a.lse + at, *delta = a.delta + at;
+    int nth = 0;  // of the next block in its run of one head
+    float next_l = 0.f, next_d = 0.f;
     auto fetch = [&](int i) {
-      const int qr = t.row0 + (i % per_head) * kBlock + 32 * half + (r & 31);
-      return r < 64 && i < blocks && qr < t.len
-                 ? -src[(hk * group + i / per_head) * a.total + t.start + qr] : 0.f;
+      const bool held = i < blocks && nth * kRows < left;
+      next_l = held ? -lse[nth * kRows] : 0.f;
+      next_d = held ? -delta[nth * kRows] : 0.f;
+      if (++nth == per_head) nth = 0, lse += a.total, delta += a.total;
     };
-    float next = fetch(buf);
-    for (int i = buf; i < blocks; i += 2) {
-      float *mine = vec + wg * 128 + ((i >> 1) & 1) * 64;
-      if (r < 64) mine[r] = next;
-      // the vectors are there; and a wait that expired in one warp ends them all
-      uint32_t bad;
-      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 128, q;\n\t"
-                   "selp.u32 %0, 1, 0, p;\n\t}"
-                   : "=r"(bad)
-                   : "r"(ok ? 0u : 1u), "r"(bar_id)
-                   : "memory");
-      if (bad) {
-        ok = false;
-        break;
-      }
-      next = fetch(i + 2);
-      ok = mbar_wait(&bars->sd_full[buf], (i >> 1) & 1);
-      ok = __all_sync(0xffffffffu, ok);
+    fetch(0);
+    int q0 = 0;  // the block's first query, from the tile's first key
+    for (int i = 0; i < blocks; ++i) {
+      __syncwarp();
+      mine[lane] = next_l;
+      mine[32 + lane] = next_d;
+      const bool nan = __any_sync(0xffffffffu, next_l != next_l);
+      __syncwarp();
+      fetch(i + 1);
+      ok = mbar_wait(&bars->sd_full, i & 1);
+      if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
-      const int q0 = (i % per_head) * kBlock;  // from the tile's first key
-      const bool edge = q0 < kRows || t.row0 + q0 + kBlock > t.len;
-      const int from = r - q0 - 32 * half, to = t.len - t.row0 - q0 - 32 * half;  // visible columns: from .. to - 1
       float s[32], d[32];
-      tmem_ld32(t_s + kColS, s);
+      tmem_ld32(t_s, s);
       tmem_ld32(t_s + kColDp, d);
       tmem_wait_ld();
+      warp_arrive(&bars->sd_free);
+      auto weights = [&](auto poly) {
 #pragma unroll
-      for (int u = 0; u < 32; u += 4) {
-        const float4 l4 = *reinterpret_cast<const float4 *>(mine + u), d4 = *reinterpret_cast<const float4 *>(mine + 32 + u);
-        fma2v(s[u], s[u + 1], a.scale_log2, l4.x, l4.y);
-        fma2v(s[u + 2], s[u + 3], a.scale_log2, l4.z, l4.w);
-        add2(d[u], d[u + 1], d4.x, d4.y);
-        add2(d[u + 2], d[u + 3], d4.z, d4.w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[u + e] = ex2(s[u + e]);
-        if (kHalf) {
-          mul2(d[u], d[u + 1], f, f);
-          mul2(d[u + 2], d[u + 3], f, f);
+        for (int u = 0; u < 32; u += 4) {
+          const float4 l4 = *reinterpret_cast<const float4 *>(mine + u);
+          const float4 d4 = *reinterpret_cast<const float4 *>(mine + 32 + u);
+          fma2v(s[u], s[u + 1], a.scale_log2, l4.x, l4.y);
+          fma2v(s[u + 2], s[u + 3], a.scale_log2, l4.z, l4.w);
+          add2(d[u], d[u + 1], d4.x, d4.y);
+          add2(d[u + 2], d[u + 3], d4.z, d4.w);
+          s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
+          if (decltype(poly)::value && u % 8 == 4)
+            exp2_fma<false>(s[u + 2], s[u + 3]);
+          else
+            s[u + 2] = ex2(s[u + 2]), s[u + 3] = ex2(s[u + 3]);
+          if (kHalf) {
+            mul2(d[u], d[u + 1], f, f);
+            mul2(d[u + 2], d[u + 3], f, f);
+          }
+          mul2(d[u], d[u + 1], s[u], s[u + 1]);
+          mul2(d[u + 2], d[u + 3], s[u + 2], s[u + 3]);
         }
-        mul2(d[u], d[u + 1], s[u], s[u + 1]);
-        mul2(d[u + 2], d[u + 3], s[u + 2], s[u + 3]);
-      }
-      if (edge) {
+      };
+      const int from = r - q0 - 32 * wg, to = t.len - t.row0 - q0 - 32 * wg;  // visible columns: from .. to - 1
+      if (q0 > 0 && to >= 32 && !nan) {
+        weights(std::true_type());
+      } else {
+        weights(std::false_type());
 #pragma unroll
         for (int u = 0; u < 32; ++u) {
           const bool seen = u >= from && u < to;
@@ -835,20 +843,18 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
           d[u] = seen ? d[u] : 0.f;
         }
       }
-      float w[16];
-#pragma unroll
-      for (int u = 0; u < 16; ++u) w[u] = __uint_as_float(pack2<T>(s[2 * u], s[2 * u + 1]));
-      tmem_st16(t_s + kColS, w);
-#pragma unroll
-      for (int u = 0; u < 16; ++u) w[u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
-      tmem_st16(t_s + kColDp, w);
+      q0 += kRows;
+      if (q0 >= t.len - t.row0) q0 = 0;
+      if (i > 0) ok = mbar_wait(&bars->w_free, (i - 1) & 1);
+      if (__any_sync(0xffffffffu, !ok)) break;
+      fence_after_sync();
+      store_weights<T>(tmem + lane_base + kColW + 16 * wg, s);
+      store_weights<T>(tmem + lane_base + kColW2 + 16 * wg, d);
       tmem_wait_st();
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0 && ok) mbar_arrive(&bars->p_full[buf]);
+      warp_arrive(&bars->w_full);
     }
     if (ok) {
-      ok = mbar_wait(&bars->done, 0);
+      ok = mbar_wait(&bars->w_free, (blocks - 1) & 1);
       fence_after_sync();
     }
   }
@@ -857,7 +863,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (warp < 8) {
     fence_after_sync();
     const float back = failed ? __int_as_float(0x7fc00000) : wg == 0 ? 1.f : a.scale / f;
-    store_row((wg == 0 ? dv : dk) + r * c_st, tmem + lane_base + (wg == 0 ? kColAcc : kColAcc2), back, r < keys);
+    store_row((wg == 0 ? dv : dk) + r * c_st, tmem + lane_base + (wg == 0 ? kDkvAcc : kDkvAcc2), back, r < keys);
   }
   fence_before_sync();
   __syncthreads();
@@ -867,17 +873,18 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
 }
 
-// Map of a packed tensor [total][H][64]: boxes of 64 rows of one head.
-static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total, int64_t H, int64_t st, int64_t sh) {
+// Map of a packed tensor [total][H][64]: boxes of `box` rows of one head.
+static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total, int64_t H, int64_t st, int64_t sh,
+                      int box) {
   if (H == 1 && sh <= 0) sh = 64;
   if (total == 1 && st <= 0) st = sh * H;
-  return encode_rows_map(map, p, dtype, 64, total, H, 1, st, sh, st, pt::kBlock);
+  return encode_rows_map(map, p, dtype, 64, total, H, 1, st, sh, st, box);
 }
 
 int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
   CUtensorMap mk, mv;
-  int rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh);
-  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh);
+  int rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kBlock);
+  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh, pt::kBlock);
   if (rc != SD_OK) return rc;
   const int64_t ctas = packed_slots(a.total, a.S, 2 * pt::kRows) * a.Hq;
   if (ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
@@ -892,10 +899,10 @@ int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
 
 int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
   CUtensorMap mq, mk, mv, mg;
-  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh);
-  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh);
-  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh);
-  if (rc == SD_OK) rc = packed_map(&mg, a.dout, dtype, a.total, a.Hq, a.g_st, a.g_sh);
+  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh, pt::kRows);
+  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kRows);
+  if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh, pt::kRows);
+  if (rc == SD_OK) rc = packed_map(&mg, a.dout, dtype, a.total, a.Hq, a.g_st, a.g_sh, pt::kRows);
   if (rc != SD_OK) return rc;
   const int64_t slots = packed_slots(a.total, a.S, pt::kRows);
   if (slots * a.Hq > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
@@ -912,10 +919,10 @@ int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
   const size_t smem = pt::BwdSmem::kBytes + 1024;
   auto run = [&](auto *dq, auto *dkv) {
     if (set_max_smem(dq, smem) != SD_OK || set_max_smem(dkv, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
-    dq<<<static_cast<unsigned>(slots * a.Hq), pt::kBwdThreads, smem, s>>>(a, mk, mv, top, err);
+    dq<<<static_cast<unsigned>(slots * a.Hq), pt::kBwdThreads, smem, s>>>(a, mq, mg, mk, mv, top, err);
     const int first = check_launch();
     if (first != SD_OK) return first;
-    dkv<<<static_cast<unsigned>(slots * a.Hkv), pt::kBwdThreads, smem, s>>>(a, mq, mg, top, err);
+    dkv<<<static_cast<unsigned>(slots * a.Hkv), pt::kBwdThreads, smem, s>>>(a, mq, mg, mk, mv, top, err);
     return check_launch();
   };
   return dtype == SD_DTYPE_BF16
