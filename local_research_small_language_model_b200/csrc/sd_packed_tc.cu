@@ -781,26 +781,26 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     const uint32_t t_s = tmem + lane_base + kColS + 32 * wg;
     // the warp's 32 queries' log sums and deltas, negated: a lane brings one of each, all read them from shared memory
     float *mine = vec + warp * 64;
-    const int left = t.len - t.row0 - 32 * wg - lane;  // the lane's query is held up to this many rows behind the tile
-    const int64_t at = static_cast<int64_t>(hk) * group * a.total + first + 32 * wg + lane;
-    const float *lse = a.lse + at, *delta = a.delta + at;
-    int nth = 0;  // of the next block in its run of one head
-    float next_l = 0.f, next_d = 0.f;
-    auto fetch = [&](int i) {
-      const bool held = i < blocks && nth * kRows < left;
-      next_l = held ? -lse[nth * kRows] : 0.f;
-      next_d = held ? -delta[nth * kRows] : 0.f;
-      if (++nth == per_head) nth = 0, lse += a.total, delta += a.total;
+    const int span = t.len - t.row0 - 32 * wg;  // rows of a head from this warpgroup's first query on
+    int64_t at = static_cast<int64_t>(hk) * group * a.total + first + 32 * wg + lane;
+    int qn = 0;  // the next block's first query, from the tile's first key
+    float next_l, next_d;
+    auto fetch = [&](bool more) {
+      const bool held = more && qn + lane < span;
+      next_l = held ? -a.lse[at + qn] : 0.f;
+      next_d = held ? -a.delta[at + qn] : 0.f;
+      qn += kRows;
+      if (qn >= span + 32 * wg) qn = 0, at += a.total;
     };
-    fetch(0);
-    int q0 = 0;  // the block's first query, from the tile's first key
+    fetch(true);
     for (int i = 0; i < blocks; ++i) {
       __syncwarp();
       mine[lane] = next_l;
       mine[32 + lane] = next_d;
       const bool nan = __any_sync(0xffffffffu, next_l != next_l);
       __syncwarp();
-      fetch(i + 1);
+      const int q0 = qn == 0 ? (span + 32 * wg - 1) / kRows * kRows : qn - kRows;  // this block's
+      fetch(i + 1 < blocks);
       ok = mbar_wait(&bars->sd_full, i & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
           mul2(d[u + 2], d[u + 3], s[u + 2], s[u + 3]);
         }
       };
-      const int from = r - q0 - 32 * wg, to = t.len - t.row0 - q0 - 32 * wg;  // visible columns: from .. to - 1
+      const int from = r - q0 - 32 * wg, to = span - q0;  // visible columns: from .. to - 1
       if (q0 > 0 && to >= 32 && !nan) {
         weights(std::true_type());
       } else {
@@ -843,8 +843,6 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
           d[u] = seen ? d[u] : 0.f;
         }
       }
-      q0 += kRows;
-      if (q0 >= t.len - t.row0) q0 = 0;
       if (i > 0) ok = mbar_wait(&bars->w_free, (i - 1) & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
