@@ -18,10 +18,14 @@ namespace sd {
 
 namespace lp {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kGroups = 128;            // of 4 threads: their maxima bound the top_k-th value (top_k <= 64)
+// From four rows an SM on, small CTAs win: one's loads cover another's joining
+// of its threads (8192 x 32000 bf16: 105 us with 128 threads, 127 with 256, 189
+// with 512; the gradient 165 us with 256, 168 with 128, 177 with 512).  With
+// fewer rows a row's own latency counts (64 rows: 5.5 us with 512 threads).
+constexpr int64_t kManyRows = 4 * 148;
+constexpr int kGroups = 128;            // of threads: their maxima bound the top_k-th value (top_k <= 64)
 constexpr int kAbove = 4096;            // room for the values above that bound,
-constexpr int kTies = 4096 + 64;        // and for those equal to it: a step's 4096 and fewer than top_k before
+constexpr int kTies = 8192 + 64;        // and for those equal to it: a step's and fewer than top_k before
 constexpr int kCandidates = kAbove + kTies;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e4f;         // stands for -inf: its exponential is 0 and 0 * kFloor is 0
@@ -55,21 +59,47 @@ __device__ __forceinline__ void raise(Stat &a, float top) {
   a.m = top;
 }
 
-template <int N> __device__ __forceinline__ void add(Stat &a, const float (&x)[N]) {
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 y;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return y;
+}
+
+// N values (N even) with their largest and smallest (NaNs left out).  Nearly
+// always none is -inf, and its guard is left out for all.
+template <int N> __device__ __forceinline__ void add(Stat &a, const float (&x)[N], float top, float least) {
   raise(a, top);
   const float ref = a.m == -INFINITY ? 0.f : a.m;
-  float s[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
+  const float2 neg = {-ref, -ref}, log2e = {kLog2e, kLog2e}, zero = {0.f, 0.f};
+  float2 s[2] = {}, w[2] = {};
+  const bool guard = least == -INFINITY;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = max_nan(x[i] - ref, kFloor), e = ex2(d * kLog2e);
-    s[i & 1] += e;
-    w[i & 1] = fmaf(e, d, w[i & 1]);
+  for (int i = 0; i < N; i += 2) {
+    float2 d = add2({x[i], x[i + 1]}, neg);
+    if (guard) d.x = max_nan(d.x, kFloor), d.y = max_nan(d.y, kFloor);
+    float2 e = fma2(d, log2e, zero);
+    e.x = ex2(e.x), e.y = ex2(e.y);
+    s[(i >> 1) & 1] = add2(s[(i >> 1) & 1], e);
+    w[(i >> 1) & 1] = fma2(e, d, w[(i >> 1) & 1]);
   }
-  a.s += s[0] + s[1];
-  a.w += w[0] + w[1];
+  a.s += (s[0].x + s[0].y) + (s[1].x + s[1].y);
+  a.w += (w[0].x + w[0].y) + (w[1].x + w[1].y);
+}
+__device__ __forceinline__ void add_one(Stat &a, float x) {
+  const float pair[2] = {x, -INFINITY};
+  add(a, pair, x, -INFINITY);
 }
 
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
@@ -104,6 +134,27 @@ template <typename T> struct Vec {
       for (int i = 0; i < kN; ++i) x[i] = to_f(p[i]);
     }
   }
+  // Largest and smallest of n pieces: 16-bit types two values an instruction.
+  template <int n> static __device__ __forceinline__ void range(const uint4 (&raw)[n], float &top, float &least) {
+    if constexpr (sizeof(T) == 4) {
+      top = -INFINITY, least = INFINITY;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        float x[4];
+        unpack(raw[i], x);
+        top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        least = fminf(least, fminf(fminf(x[0], x[1]), fminf(x[2], x[3])));
+      }
+    } else {
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      const T2 *p = reinterpret_cast<const T2 *>(&raw[0]);
+      T2 hi = p[0], lo = p[0];
+#pragma unroll
+      for (int i = 1; i < 4 * n; ++i) hi = __hmax2(hi, p[i]), lo = __hmin2(lo, p[i]);
+      top = fmaxf(to_f(hi.x), to_f(hi.y));
+      least = fminf(to_f(lo.x), to_f(lo.y));
+    }
+  }
 };
 
 // A row in 16-byte pieces: `head` values up to the first aligned address, then
@@ -131,13 +182,13 @@ template <typename T> struct Row {
 // for 32000 16-bit logits) collects the values above that bound, and as many of
 // those equal to it, in index order, as can be needed; a candidate's rank among
 // them is its place in the answer.
-template <typename T, bool kTop>
-__global__ void __launch_bounds__(lp::kThreads, 2)
+template <typename T, bool kTop, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     token_logprobs_kernel(const T *x, int64_t rows, int64_t V, int64_t ld, const int64_t *targets,
                           int64_t ignore_index, float *logprobs, float *entropy, float *stats, int top_k,
                           float *top_logprobs, int64_t *top_ids, int32_t *err) {
   using namespace lp;
-  constexpr int kN = Vec<T>::kN, kUnroll = 4;
+  constexpr int kN = Vec<T>::kN, kUnroll = 4, kWarps = kThreads / 32;
   __shared__ Stat part[kWarps];
   const int64_t r = blockIdx.x;
   const Row<T> row(x + r * ld, V);
@@ -145,28 +196,26 @@ __global__ void __launch_bounds__(lp::kThreads, 2)
   Stat a = {-INFINITY, 0.f, 0.f};
   float top = -INFINITY;  // largest value of this thread that is a number
   {
-    float v[1];
-    if (tid < row.head) {
-      v[0] = to_f(row.p[tid]);
-      add(a, v);
-    }
-    if (row.tail + tid < V) {
-      v[0] = to_f(row.p[row.tail + tid]);
-      add(a, v);
-    }
+    if (tid < row.head) add_one(a, to_f(row.p[tid]));
+    if (row.tail + tid < V) add_one(a, to_f(row.p[row.tail + tid]));
     const uint4 *body = row.body();
-    for (int64_t i = tid; i < row.vecs; i += kUnroll * kThreads) {
+    int64_t i = tid;
+    for (; i + (kUnroll - 1) * kThreads < row.vecs; i += kUnroll * kThreads) {
       uint4 raw[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (i + u * kThreads < row.vecs) raw[u] = __ldg(body + i + u * kThreads);
+      for (int u = 0; u < kUnroll; ++u) raw[u] = __ldg(body + i + u * kThreads);
+      float y[kUnroll * kN], hi, lo;
+      Vec<T>::range(raw, hi, lo);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (i + u * kThreads < row.vecs) {
-          float y[kN];
-          Vec<T>::unpack(raw[u], y);
-          add(a, y);
-        }
+      for (int u = 0; u < kUnroll; ++u) Vec<T>::unpack(raw[u], y + kN * u);
+      add(a, y, hi, lo);
+    }
+    for (; i < row.vecs; i += kThreads) {
+      uint4 raw[1] = {__ldg(body + i)};
+      float y[kN], hi, lo;
+      Vec<T>::range(raw, hi, lo);
+      Vec<T>::unpack(raw[0], y);
+      add(a, y, hi, lo);
     }
     top = a.m;
   }
@@ -204,9 +253,10 @@ __global__ void __launch_bounds__(lp::kThreads, 2)
     __shared__ float group[kGroups];
     __shared__ float bound;
     __shared__ int above, ties;  // values above the bound, and equal to it
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if ((lane & 3) == 0) group[tid >> 2] = top;
+    constexpr int kGroup = kThreads / kGroups;  // threads of a group
+#pragma unroll
+    for (int o = 1; o < kGroup; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (tid % kGroup == 0) group[tid / kGroup] = top;
     if (tid == 0) above = ties = 0;
     __syncthreads();
     if (tid < kGroups) {
@@ -298,8 +348,8 @@ __global__ void __launch_bounds__(lp::kThreads, 2)
 }
 
 // One CTA a row: one read of the logits, one write of their gradient.
-template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(lp::kThreads, 2)
+template <typename T, bool kEntropy, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     token_logprobs_backward_kernel(const T *x, int64_t rows, int64_t V, int64_t ld, const int64_t *targets,
                                    int64_t ignore_index, const float *stats, const float *g_logprobs,
                                    const float *g_entropy, T *dx, int64_t d_ld) {
@@ -373,15 +423,16 @@ int sd_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t V, in
   if (top_k > 64 || rows > 0x7fffffffll || V > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype)) return SD_ERR_ALIGN;
   SD_DISPATCH_DTYPE(dtype, T, {
-    auto run = [&](auto *kern, size_t smem) {
+    auto run = [&](auto *kern, int threads, size_t smem) {
       if (set_max_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
-      kern<<<static_cast<unsigned>(rows), lp::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
+      kern<<<static_cast<unsigned>(rows), threads, smem, static_cast<cudaStream_t>(stream)>>>(
           static_cast<const T *>(logits), rows, V, ld, targets, ignore_index, logprobs, entropy, stats, top_k,
           top_logprobs, top_ids, err);
       return check_launch();
     };
-    return top_k > 0 ? run(token_logprobs_kernel<T, true>, lp::kCandidates * sizeof(unsigned long long))
-                     : run(token_logprobs_kernel<T, false>, 0);
+    if (top_k > 0) return run(token_logprobs_kernel<T, true, 512>, 512, lp::kCandidates * sizeof(unsigned long long));
+    return rows >= lp::kManyRows ? run(token_logprobs_kernel<T, false, 128>, 128, 0)
+                                 : run(token_logprobs_kernel<T, false, 512>, 512, 0);
   });
   return SD_OK;
 }
@@ -398,8 +449,11 @@ int sd_token_logprobs_backward(const void *logits, int dtype, int64_t rows, int6
       reinterpret_cast<uintptr_t>(dlogits) % dtype_size(dtype))
     return SD_ERR_ALIGN;
   SD_DISPATCH_DTYPE(dtype, T, {
-    auto kern = g_entropy ? token_logprobs_backward_kernel<T, true> : token_logprobs_backward_kernel<T, false>;
-    kern<<<static_cast<unsigned>(rows), lp::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+    const bool many = rows >= lp::kManyRows;
+    auto kern = g_entropy ? many ? token_logprobs_backward_kernel<T, true, 256> : token_logprobs_backward_kernel<T, true, 512>
+                : many    ? token_logprobs_backward_kernel<T, false, 256>
+                          : token_logprobs_backward_kernel<T, false, 512>;
+    kern<<<static_cast<unsigned>(rows), many ? 256 : 512, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const T *>(logits), rows, V, ld, targets, ignore_index, stats, g_logprobs, g_entropy,
         static_cast<T *>(dlogits), d_ld);
   });
