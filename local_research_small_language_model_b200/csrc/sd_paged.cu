@@ -141,12 +141,21 @@ __device__ __forceinline__ int page_of(int t, int page, uint32_t inv) {
   return t - p * page >= page ? p + 1 : p;
 }
 
-// Joins (m, l) pairs: the factors of both sides.
-__device__ __forceinline__ float factor(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a part with maximum m weighs under the common maximum.
+__device__ __forceinline__ float factor(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
 
 }  // namespace pg
 
-template <typename T>
+// kWhole: a warp's tokens of a unit lie in one page (the page size is a multiple
+// of them), so a unit takes one look-up and its rows follow each other; kWide:
+// more than 8 query heads a group (the fragments' second 8 rows hold heads too).
+template <typename T, bool kWhole, bool kWide>
 __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const PagedArgs a, const pg::DecodeArgs d) {
   using namespace pg;
   constexpr bool k16 = sizeof(T) == 2;
@@ -194,12 +203,15 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
     __syncthreads();
   }
   const int64_t units = static_cast<int64_t>(pre[a.B]) * d.Hh;
-  const int64_t per = (units + gridDim.x - 1) / gridDim.x;
+  const int64_t per = units <= 0x7fffffff - kCtas ? (static_cast<uint32_t>(units) + gridDim.x - 1) / gridDim.x
+                                                  : (units + gridDim.x - 1) / gridDim.x;
   if (blockIdx.x == 0) {
     for (int b = tid; b <= a.B; b += kThreads) d.plan[b] = pre[b];
     if (tid == 0) d.plan[a.B + 1] = static_cast<int>(per);
   }
   const int64_t u0 = blockIdx.x * per, u1 = u0 + per < units ? u0 + per : units;
+  // the joining kernel may be brought in from here on; it waits for this one's end before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (u0 >= u1) return;
 
   // ---- the first unit
@@ -212,7 +224,10 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
     }
     const int tiles = pre[lo + 1] - pre[lo];
     const int64_t in = u0 - static_cast<int64_t>(pre[lo]) * d.Hh;
-    at = {lo, static_cast<int>(in / tiles), static_cast<int>(in % tiles)};
+    if (in <= 0x7fffffff)
+      at = {lo, static_cast<int>(in) / tiles, static_cast<int>(in) % tiles};
+    else
+      at = {lo, static_cast<int>(in / tiles), static_cast<int>(in % tiles)};
   }
   auto advance = [&](Cursor &c) {
     if (++c.tile < pre[c.b + 1] - pre[c.b]) return;
@@ -226,41 +241,63 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
 
   // ---- copies: this lane's rows of a unit
   const int row0 = lane / kChunks, chunk = lane % kChunks;
-  Cursor ld = at;
-  int64_t left = u1 - u0;  // units not yet looked up
-  int page[kCopies];
+  Cursor ld = at, ld_at = at;
+  int left = static_cast<int>(u1 - u0);  // units not yet looked up
+  int page[kWhole ? 1 : kCopies];
   bool more = false;
-  Cursor ld_at;
+  const int64_t lane_off = chunk * (16 / static_cast<int>(sizeof(T))) + (kWhole ? row0 * a.p_st : 0);
   auto lookup = [&]() {  // the page ids of unit ld (used when it is copied, a unit later)
     more = left > 0;
     if (!more) return;
     ld_at = ld;
+    const int n = len[ld.b], t0 = ld.tile * kTok + warp * kMine;
 #pragma unroll
-    for (int j = 0; j < kCopies; ++j) {
-      const int t = ld.tile * kTok + warp * kMine + row0 + kRowsAt * j;
-      page[j] = t < len[ld.b] ? a.table[ld.b * a.t_sb + page_of(t, a.page, d.page_inv)] : -1;
+    for (int j = 0; j < (kWhole ? 1 : kCopies); ++j) {
+      const int t = kWhole ? t0 : t0 + row0 + kRowsAt * j;
+      page[j] = t < n ? a.table[ld.b * a.t_sb + page_of(t, a.page, d.page_inv)] : -1;
     }
     advance(ld);
     --left;
   };
   char *mine = ring + warp * kStages * kWarpBytes;
   uint8_t *mine_held = held + warp * kStages * 16;
+  // chunks change places by row so that a warp's reads meet no bank twice
+  auto place = [&](int r) { return r * kRow + ((chunk ^ (k16 ? r & 7 : (r & 1) * 4)) << 4); };
+  const uint32_t ring_at = smem_u32(mine);
   auto copy = [&](int stage) {
     if (more) {
-      const uint32_t dst = smem_u32(mine + stage * kWarpBytes);
-      const int hk = ld_at.hh / groups;
+      const uint32_t dst = ring_at + stage * kWarpBytes;
+      const int hk = groups == 1 ? ld_at.hh : ld_at.hh / groups;
+      const int t0 = ld_at.tile * kTok + warp * kMine, n = len[ld_at.b];
+      if constexpr (kWhole) {
+        const bool ok = page[0] >= 0 && page[0] < a.pages;
+        const int here = ok ? min(n - t0, kMine) : 0;  // rows held (lane 0 tells the readers)
+        if (!ok && t0 < n) report(a.err, SD_KERR_BOUNDS);
+        const int64_t off = ok ? page[0] * a.p_sp + hk * a.p_sh +
+                                     (t0 - page_of(t0, a.page, d.page_inv) * a.page) * a.p_st + lane_off
+                               : lane_off;
+        const T *ks = static_cast<const T *>(d.k) + off, *vs = static_cast<const T *>(d.v) + off;
 #pragma unroll
-      for (int j = 0; j < kCopies; ++j) {
-        const int r = row0 + kRowsAt * j, t = ld_at.tile * kTok + warp * kMine + r;
-        const bool ok = page[j] >= 0 && page[j] < a.pages;
-        if (!ok && t < len[ld_at.b]) report(a.err, SD_KERR_BOUNDS);
-        const int64_t off =
-            ok ? page[j] * a.p_sp + hk * a.p_sh + (t - page_of(t, a.page, d.page_inv) * a.page) * a.p_st : 0;
-        // chunks change places by row so that a warp's reads meet no bank twice
-        const uint32_t to = dst + r * kRow + ((chunk ^ (k16 ? r & 7 : (r & 1) * 4)) << 4);
-        cp16(to, static_cast<const T *>(d.k) + off + chunk * (16 / sizeof(T)), ok);
-        cp16(to + kWarpBytes / 2, static_cast<const T *>(d.v) + off + chunk * (16 / sizeof(T)), ok);
-        if (chunk == 0) mine_held[stage * 16 + r] = ok;
+        for (int j = 0; j < kCopies; ++j) {
+          const bool in = row0 + kRowsAt * j < here;
+          const int64_t step = in ? kRowsAt * j * a.p_st : 0;
+          cp16(dst + place(row0 + kRowsAt * j), in ? ks + step : static_cast<const T *>(d.k), in);
+          cp16(dst + place(row0 + kRowsAt * j) + kWarpBytes / 2, in ? vs + step : static_cast<const T *>(d.v), in);
+        }
+        if (lane == 0) mine_held[stage * 16] = here > 0 ? here : 0;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+          const int r = row0 + kRowsAt * j, t = t0 + r;
+          const bool ok = page[j] >= 0 && page[j] < a.pages;
+          if (!ok && t < n) report(a.err, SD_KERR_BOUNDS);
+          const int64_t off = ok ? page[j] * a.p_sp + hk * a.p_sh +
+                                       (t - page_of(t, a.page, d.page_inv) * a.page) * a.p_st + lane_off
+                                 : 0;
+          cp16(dst + place(r), static_cast<const T *>(d.k) + off, ok);
+          cp16(dst + place(r) + kWarpBytes / 2, static_cast<const T *>(d.v) + off, ok);
+          if (chunk == 0) mine_held[stage * 16 + r] = ok;
+        }
       }
     }
     cp_commit();
@@ -275,7 +312,8 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
   // ---- state of the current head group
   // 16-bit: fragments of m16n8k16, rows lane / 4 and lane / 4 + 8 are heads;
   // fp32: every lane keeps all heads, columns 2 lane and 2 lane + 1
-  constexpr int kAcc = k16 ? 8 : kMaxHeads, kAccN = k16 ? 4 : 2, kStat = k16 ? 2 : kMaxHeads;
+  constexpr int kHalves = kWide ? 2 : 1;
+  constexpr int kAcc = k16 ? 8 : kMaxHeads, kAccN = k16 ? 4 : 2, kStat = k16 ? kHalves : kMaxHeads;
   float o[kAcc][kAccN], m[kStat], l[kStat];
   uint32_t qa[4][4];
   const int r0 = lane >> 2, c0 = (lane & 3) * 2;
@@ -289,7 +327,7 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int g = r0 + (e & 1) * 8, col = 16 * k + c0 + (e >> 1) * 8;
-          qa[k][e] = g < n ? *reinterpret_cast<const uint32_t *>(src + g * d.q_sh + col) : 0u;
+          qa[k][e] = (kWide || !(e & 1)) && g < n ? *reinterpret_cast<const uint32_t *>(src + g * d.q_sh + col) : 0u;
         }
     } else {
       __syncthreads();
@@ -307,8 +345,9 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
   int first_tile = at.tile;
   const float c = d.scale_log2;
 
-  for (int64_t u = u0; u < u1; ++u) {
-    const int it = static_cast<int>(u - u0), stage = it % kStages;
+  const int count = static_cast<int>(u1 - u0);
+  for (int it = 0; it < count; ++it) {
+    const int stage = it % kStages;
     copy((it + kStages - 1) % kStages);
     lookup();
     cp_wait<kStages - 1>();
@@ -330,31 +369,49 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
           mma16816<T>(s[nt], qa[2 * half], b0, b1);
           mma16816<T>(s[nt], qa[2 * half + 1], b2, b3);
         }
-        const uint32_t flags = *reinterpret_cast<const uint16_t *>(ok + 8 * nt + c0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          s[nt][e] = (e & 1 ? flags >> 8 : flags & 0xff) ? s[nt][e] * c : -INFINITY;
       }
-      uint32_t pa[4];
+      if constexpr (kWhole) {
+        const int here = ok[0];
+        if (here < kMine) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (8 * nt + c0 + (e & 1) >= here) s[nt][e] = -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const uint32_t flags = *reinterpret_cast<const uint16_t *>(ok + 8 * nt + c0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(e & 1 ? flags >> 8 : flags & 0xff)) s[nt][e] = -INFINITY;
+        }
+      }
+      uint32_t pa[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int half = 0; half < kHalves; ++half) {
         float best = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
         best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
         best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-        const float mn = fmaxf(m[half], best), ref = mn == -INFINITY ? 0.f : mn;
-        const float alpha = exp2f(m[half] - ref);
-        m[half] = mn;
+        best *= c;
+        if (__any_sync(0xffffffffu, best > m[half])) {  // some head's maximum rises
+          const float mn = fmaxf(m[half], best), alpha = m[half] == -INFINITY ? 0.f : ex2(m[half] - mn);
+          m[half] = mn;
+          l[half] *= alpha;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            o[n][2 * half] *= alpha;
+            o[n][2 * half + 1] *= alpha;
+          }
+        }
+        const float neg = m[half] == -INFINITY ? 0.f : -m[half];
         float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = exp2f(s[e >> 1][2 * half + (e & 1)] - ref);
-        l[half] = l[half] * alpha + ((p[0] + p[1]) + (p[2] + p[3]));
+        for (int e = 0; e < 4; ++e) p[e] = ex2(fmaf(s[e >> 1][2 * half + (e & 1)], c, neg));
+        l[half] += (p[0] + p[1]) + (p[2] + p[3]);
         pa[half] = pack2<T>(p[0], p[1]);
         pa[2 + half] = pack2<T>(p[2], p[3]);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          o[n][2 * half] *= alpha;
-          o[n][2 * half + 1] *= alpha;
-        }
       }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -373,7 +430,7 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
 #pragma unroll
       for (int r = 0; r < kMine; ++r)
         vr[r] = *reinterpret_cast<const float2 *>(vt + r * kRow + (((lane >> 1) ^ ((r & 1) * 4)) << 4) + (lane & 1) * 8);
-      const bool seen = ok[key];
+      const bool seen = kWhole ? key < ok[0] : ok[key];
 #pragma unroll
       for (int g = 0; g < kMaxHeads; ++g) {
         if (g >= d.G) break;
@@ -390,7 +447,7 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, w));
         const float mn = fmaxf(m[g], best), ref = mn == -INFINITY ? 0.f : mn;
-        const float alpha = exp2f(m[g] - ref), p = exp2f(s - ref);
+        const float alpha = ex2(m[g] - ref), p = ex2(s - ref);
         float sum = p;
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
@@ -408,12 +465,12 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
     __syncwarp();
     const int tiles = pre[at.b + 1] - pre[at.b];
     const bool head_ends = at.tile + 1 == tiles;
-    if (head_ends || u + 1 == u1) {
+    if (head_ends || it + 1 == count) {
       // the four warps' states of this head group meet
       float *to = merge + warp * d.G * kPart;
       if constexpr (k16) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < kHalves; ++half) {
           l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
           l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
           const int g = r0 + 8 * half;
@@ -440,7 +497,7 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
       const int sub = at.hh % groups, h0 = (at.hh / groups) * (a.Hq / a.Hkv) + sub * kMaxHeads;
       const int n = min(d.G, (a.Hq / a.Hkv) - sub * kMaxHeads);
       // a part that begins with the CTA's run is its slot 0, one that begins later slot 1
-      float *part = d.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (u - (at.tile - first_tile) == u0 ? 0 : 1)) *
+      float *part = d.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (at.tile - first_tile == it ? 0 : 1)) *
                                   d.G * kPart;
       for (int g = tid >> 6; g < n; g += kThreads / 64) {
         const int e = tid & 63;
@@ -464,7 +521,7 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
       }
       __syncthreads();
       advance(at);
-      if (u + 1 < u1) {
+      if (it + 1 < count) {
         begin(at);
         first_tile = 0;
       }
@@ -481,8 +538,8 @@ __global__ void __launch_bounds__(pg::kThreads, 3) paged_decode_kernel(const Pag
 template <typename T>
 __global__ void __launch_bounds__(512) paged_join_kernel(const PagedArgs a, const pg::DecodeArgs d) {
   using namespace pg;
-  constexpr int kRuns = 8;
-  __shared__ float tops[16], sums[kRuns], vals[kRuns][64];
+  constexpr int kRuns = 8, kUnroll = 8;
+  __shared__ float tops[kRuns], sums[kRuns], vals[kRuns][64];
   pdl_wait();
   const int b = blockIdx.y, group = a.Hq / a.Hkv, groups = d.Hh / a.Hkv, tid = threadIdx.x;
   const int h = blockIdx.x, hh = (h / group) * groups + h % group / kMaxHeads, g = h % group % kMaxHeads;
@@ -493,36 +550,53 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const PagedArgs a, cons
     return;
   }
   const int64_t u0 = static_cast<int64_t>(d.plan[b]) * d.Hh + hh * tiles, u1 = u0 + tiles;
-  const int c0 = static_cast<int>(u0 / per), n = static_cast<int>((u1 - 1) / per) - c0 + 1;
+  int c0, n;  // the parts' CTAs
+  if (u1 <= 0x7fffffff) {
+    c0 = static_cast<int>(u0) / static_cast<int>(per);
+    n = static_cast<int>(u1 - 1) / static_cast<int>(per) - c0 + 1;
+  } else {
+    c0 = static_cast<int>(u0 / per);
+    n = static_cast<int>((u1 - 1) / per) - c0 + 1;
+  }
   if (n == 1) return;
   auto part = [&](int i) {
     return d.parts + ((static_cast<int64_t>(c0 + i) * 2 + ((c0 + i) * per < u0 ? 1 : 0)) * d.G + g) * kPart;
   };
-  float top = -INFINITY;  // n <= kCtas <= 512: one part a thread
-  if (tid < n) top = part(tid)[0];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((tid & 31) == 0) tops[tid >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, tops[i]);
   const int run = tid >> 6, e = tid & 63;
   const int i0 = n * run / kRuns, i1 = n * (run + 1) / kRuns;
-  float sum = 0.f, val = 0.f;
-#pragma unroll 8
-  for (int i = i0; i < i1; ++i) {
-    const float *p = part(i);
-    const float f = factor(p[0], top);
-    sum = fmaf(f, p[1], sum);
-    val = fmaf(f, p[2 + e], val);
+  float top = -INFINITY, sum = 0.f, val = 0.f;
+  for (int i = i0; i < i1; i += kUnroll) {
+    float pm[kUnroll], pl[kUnroll], pv[kUnroll], best = top;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const float *p = part(i + u < i1 ? i + u : i);
+      pm[u] = i + u < i1 ? p[0] : -INFINITY, pl[u] = p[1], pv[u] = p[2 + e];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) best = fmaxf(best, pm[u]);
+    const float f0 = factor(top, best);
+    sum *= f0, val *= f0, top = best;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const float f = factor(pm[u], best);
+      sum = fmaf(f, pl[u], sum);
+      val = fmaf(f, pv[u], val);
+    }
   }
+  if (e == 0) tops[run] = top;
   if (e == 0) sums[run] = sum;
   vals[run][e] = val;
   __syncthreads();
   if (tid < 64) {
-    sum = val = 0.f;
+    top = -INFINITY, sum = val = 0.f;
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) sum += sums[i], val += vals[i][e];
+    for (int i = 0; i < kRuns; ++i) top = fmaxf(top, tops[i]);
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+      const float f = factor(tops[i], top);
+      sum = fmaf(f, sums[i], sum);
+      val = fmaf(f, vals[i][e], val);
+    }
     out[e] = from_f<T>(sum == 0.f ? 0.f : val / sum);
   }
 }
@@ -618,7 +692,10 @@ int sd_paged_decode_attention(const void *q, int dtype, int64_t B, int64_t Hq, i
       const unsigned ctas = static_cast<unsigned>(most * d.Hh < pg::kCtas ? most * d.Hh : pg::kCtas);
       const size_t smem = pg::kWarps * pg::kStages * (pg::kWarpBytes + 16) + pg::kWarps * d.G * pg::kPart * 4 +
                           (sizeof(T) == 4 ? d.G * 256 : 0) + (2 * a.B + 1) * 4;
-      auto kern = paged_decode_kernel<T>;
+      const bool whole = page % (pg::kUnit<T> / pg::kWarps) == 0, wide = sizeof(T) == 2 && d.G > 8;
+      auto kern = whole ? wide ? paged_decode_kernel<T, true, true> : paged_decode_kernel<T, true, false>
+                  : wide ? paged_decode_kernel<T, false, true>
+                         : paged_decode_kernel<T, false, false>;
       if (set_max_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
       kern<<<ctas, pg::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a, d);
       rc = check_launch();
