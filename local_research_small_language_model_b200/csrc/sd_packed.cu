@@ -1,5 +1,5 @@
 // Causal grouped-query attention over packed sequences, and its gradients, on
-// CUDA cores with fp32 arithmetic.
+// CUDA cores for fp32 inputs; and the entry points for all types.
 //
 //   O_i = sum_{j <= i} P_ij v_j,  P_ij = exp(scale q_i.k_j - lse_i)
 //   delta_i = dO_i . O_i
@@ -7,11 +7,11 @@
 //   dV_j = sum_i P_ij dO_i,  dK_j = scale sum_i dS_ij q_i,  dQ_i = scale sum_j dS_ij k_j
 //
 // i, j run over the tokens of one sequence; dK and dV also sum over the query
-// heads of their key-value head.  Tiles are 64 x 64; a thread of the 128 owns
-// 8 rows x 4 columns of every product, with all operands row-major in shared
-// memory (row pitch 68 floats: the float4 reads below have no bank conflicts),
-// so 12 16-byte shared loads feed 128 multiply-adds in each of the three forms
-// (row.row, P times rows, P^T times rows).  No atomics: every output element is
+// heads of their key-value head.  Tiles are 64 x 64; a thread of the 256 owns
+// 4 rows x 4 columns of every product, with all operands row-major in shared
+// memory (row pitch 68 floats: the float4 reads below have no bank conflicts).
+// A warp's 16-byte shared loads take 12 cycles of the four schedulers' 16 in
+// each of the three forms (row.row, P times rows, P^T times rows).  No atomics: every output element is
 // summed by one thread in a fixed order.
 #include "sd_packed.cuh"
 
@@ -20,31 +20,18 @@ namespace sd {
 namespace pk {
 
 constexpr int kTile = 64;
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
+constexpr int kR = 4;                        // rows of a thread
 constexpr int kPitch = 68;
 constexpr int kTileFloats = kTile * kPitch;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // 64 rows (rows past `rows` zero) of 64 values from global memory into a tile.
-template <typename T>
-__device__ __forceinline__ void load_tile(float *dst, const T *src, int64_t stride, int rows) {
-  constexpr int kVec = 16 / sizeof(T);
-  constexpr int kChunks = kTile / kVec;
-  for (int e = threadIdx.x; e < kTile * kChunks; e += kThreads) {
-    const int r = e / kChunks, c = (e % kChunks) * kVec;
-    float x[kVec];
-    if (r < rows) {
-      uint4 raw = *reinterpret_cast<const uint4 *>(src + r * stride + c);
-      const T *p = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-      for (int u = 0; u < kVec; ++u) x[u] = to_f(p[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kVec; ++u) x[u] = 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < kVec; u += 4)
-      *reinterpret_cast<float4 *>(dst + r * kPitch + c + u) = make_float4(x[u], x[u + 1], x[u + 2], x[u + 3]);
+__device__ __forceinline__ void load_tile(float *dst, const float *src, int64_t stride, int rows) {
+  for (int e = threadIdx.x; e < kTile * 16; e += kThreads) {
+    const int r = e >> 4, c = (e & 15) * 4;
+    *reinterpret_cast<float4 *>(dst + r * kPitch + c) =
+        r < rows ? *reinterpret_cast<const float4 *>(src + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -53,10 +40,10 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
   return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
 }
 
-// c[i][j] = sum_d A[8 ty + i][d] B[tx + 16 j][d]
-__device__ __forceinline__ void mul_rows(const float *A, const float *B, int ty, int tx, float (&c)[8][4]) {
+// c[i][j] = sum_d A[kR ty + i][d] B[tx + 16 j][d]
+__device__ __forceinline__ void mul_rows(const float *A, const float *B, int ty, int tx, float (&c)[kR][4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < kR; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
 #pragma unroll 4
@@ -65,24 +52,24 @@ __device__ __forceinline__ void mul_rows(const float *A, const float *B, int ty,
 #pragma unroll
     for (int j = 0; j < 4; ++j) b[j] = ld4(B + (tx + 16 * j) * kPitch + d);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 a = ld4(A + (8 * ty + i) * kPitch + d);
+    for (int i = 0; i < kR; ++i) {
+      const float4 a = ld4(A + (kR * ty + i) * kPitch + d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) c[i][j] = dot4(a, b[j], c[i][j]);
     }
   }
 }
 
-// c[i][u] += sum_k P[8 ty + i][k] B[k][4 tx + u]
-__device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, int tx, float (&c)[8][4]) {
+// c[i][u] += sum_k P[kR ty + i][k] B[k][4 tx + u]
+__device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, int tx, float (&c)[kR][4]) {
 #pragma unroll 4
   for (int k = 0; k < kTile; k += 4) {
     float4 b[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) b[e] = ld4(B + (k + e) * kPitch + 4 * tx);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 p = ld4(P + (8 * ty + i) * kPitch + k);
+    for (int i = 0; i < kR; ++i) {
+      const float4 p = ld4(P + (kR * ty + i) * kPitch + k);
       const float pe[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -95,15 +82,15 @@ __device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, in
   }
 }
 
-// c[i][u] += sum_k P[k][8 ty + i] B[k][4 tx + u]
-__device__ __forceinline__ void mul_pt(const float *P, const float *B, int ty, int tx, float (&c)[8][4]) {
+// c[i][u] += sum_k P[k][kR ty + i] B[k][4 tx + u]
+__device__ __forceinline__ void mul_pt(const float *P, const float *B, int ty, int tx, float (&c)[kR][4]) {
 #pragma unroll 4
   for (int k = 0; k < kTile; ++k) {
     const float4 b = ld4(B + k * kPitch + 4 * tx);
-    const float4 p0 = ld4(P + k * kPitch + 8 * ty), p1 = ld4(P + k * kPitch + 8 * ty + 4);
-    const float pe[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+    const float4 p = ld4(P + k * kPitch + kR * ty);
+    const float pe[kR] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kR; ++i) {
       c[i][0] = fmaf(pe[i], b.x, c[i][0]);
       c[i][1] = fmaf(pe[i], b.y, c[i][1]);
       c[i][2] = fmaf(pe[i], b.z, c[i][2]);
@@ -112,14 +99,23 @@ __device__ __forceinline__ void mul_pt(const float *P, const float *B, int ty, i
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T *dst, float a, float b, float c, float d) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4 *>(dst) = make_float4(a, b, c, d);
-  } else {
-    T v[4] = {from_f<T>(a), from_f<T>(b), from_f<T>(c), from_f<T>(d)};
-    *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<uint2 *>(v);
-  }
+__device__ __forceinline__ void store4(float *dst, float a, float b, float c, float d) {
+  *reinterpret_cast<float4 *>(dst) = make_float4(a, b, c, d);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Four values at p's place in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ float4 peer4(const float *p, int rank) {
+  uint32_t addr;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 // The 16 lanes of a row (tx = 0..15).
@@ -136,7 +132,7 @@ __device__ __forceinline__ float row_sum(float x) {
 
 }  // namespace pk
 
-template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) {
+__global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *K = Q + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
@@ -147,28 +143,28 @@ template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_fwd
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int rows = min(kTile, t.len - t.row0);
   const int64_t first = t.start + t.row0;
-  T *out = static_cast<T *>(a.out) + first * a.o_st + h * a.o_sh;
+  float *out = static_cast<float *>(a.out) + first * a.o_st + h * a.o_sh;
   if (t.rest) {
     if (a.zero_rest)
-      for (int i = 0; i < 8; ++i)
-        if (8 * ty + i < rows) store4(out + (8 * ty + i) * a.o_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < kR; ++i)
+        if (kR * ty + i < rows) store4(out + (kR * ty + i) * a.o_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  load_tile(Q, static_cast<const T *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
-  float o[8][4] = {}, m[8], l[8];
+  load_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
+  float o[kR][4] = {}, m[kR], l[kR];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = -INFINITY, l[i] = 0.f;
+  for (int i = 0; i < kR; ++i) m[i] = -INFINITY, l[i] = 0.f;
   for (int k0 = 0; k0 <= t.row0; k0 += kTile) {
     __syncthreads();
     const int keys = min(kTile, t.len - k0);
-    load_tile(K, static_cast<const T *>(a.k) + (t.start + k0) * a.k_st + hk * a.k_sh, a.k_st, keys);
-    load_tile(V, static_cast<const T *>(a.v) + (t.start + k0) * a.v_st + hk * a.v_sh, a.v_st, keys);
+    load_tile(K, static_cast<const float *>(a.k) + (t.start + k0) * a.k_st + hk * a.k_sh, a.k_st, keys);
+    load_tile(V, static_cast<const float *>(a.v) + (t.start + k0) * a.v_st + hk * a.v_sh, a.v_st, keys);
     __syncthreads();
-    float s[8][4];
+    float s[kR][4];
     mul_rows(Q, K, ty, tx, s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = t.row0 + 8 * ty + i;
+    for (int i = 0; i < kR; ++i) {
+      const int row = t.row0 + kR * ty + i;
       float best = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -182,7 +178,7 @@ template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_fwd
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float p = exp2f(s[i][j] - ref);
-        P[(8 * ty + i) * kPitch + tx + 16 * j] = p;
+        P[(kR * ty + i) * kPitch + tx + 16 * j] = p;
         ps += p;
       }
       l[i] = l[i] * alpha + row_sum(ps);
@@ -194,16 +190,16 @@ template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_fwd
     mul_p(P, V, ty, tx, o);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (8 * ty + i >= rows) continue;
+  for (int i = 0; i < kR; ++i) {
+    if (kR * ty + i >= rows) continue;
     const float inv = 1.0f / l[i];
-    store4(out + (8 * ty + i) * a.o_st + 4 * tx, o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
-    if (a.lse && tx == 0) a.lse[h * a.total + first + 8 * ty + i] = m[i] + log2f(l[i]);
+    store4(out + (kR * ty + i) * a.o_st + 4 * tx, o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
+    if (a.lse && tx == 0) a.lse[h * a.total + first + kR * ty + i] = m[i] + log2f(l[i]);
   }
 }
 
 // dQ of a query tile; also delta, which the dK/dV kernel behind it reads.
-template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs a) {
+__global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs a) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *G = Q + kTileFloats, *K = G + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
@@ -214,19 +210,19 @@ template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_bwd
   const int rows = min(kTile, t.len - t.row0);
   const int64_t first = t.start + t.row0;
   const int64_t c_st = static_cast<int64_t>(a.Hq) * kTile;  // dq is contiguous
-  T *dq = static_cast<T *>(a.dq) + first * c_st + h * kTile;
+  float *dq = static_cast<float *>(a.dq) + first * c_st + h * kTile;
   if (t.rest) {
-    for (int i = 0; i < 8; ++i)
-      if (8 * ty + i < rows) store4(dq + (8 * ty + i) * c_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < kR; ++i)
+      if (kR * ty + i < rows) store4(dq + (kR * ty + i) * c_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  load_tile(Q, static_cast<const T *>(a.out) + first * a.o_st + h * a.o_sh, a.o_st, rows);  // O, for delta
-  load_tile(G, static_cast<const T *>(a.dout) + first * a.g_st + h * a.g_sh, a.g_st, rows);
+  load_tile(Q, static_cast<const float *>(a.out) + first * a.o_st + h * a.o_sh, a.o_st, rows);  // O, for delta
+  load_tile(G, static_cast<const float *>(a.dout) + first * a.g_st + h * a.g_sh, a.g_st, rows);
   __syncthreads();
-  float delta[8], lse[8];
+  float delta[kR], lse[kR];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 8 * ty + i;
+  for (int i = 0; i < kR; ++i) {
+    const int r = kR * ty + i;
     delta[i] = row_sum(dot4(ld4(Q + r * kPitch + 4 * tx), ld4(G + r * kPitch + 4 * tx), 0.f));
     lse[i] = 0.f;
     if (r < rows) {
@@ -235,70 +231,73 @@ template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_bwd
     }
   }
   __syncthreads();
-  load_tile(Q, static_cast<const T *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
-  float acc[8][4] = {};
+  load_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
+  float acc[kR][4] = {};
   for (int k0 = 0; k0 <= t.row0; k0 += kTile) {
     __syncthreads();
     const int keys = min(kTile, t.len - k0);
-    load_tile(K, static_cast<const T *>(a.k) + (t.start + k0) * a.k_st + hk * a.k_sh, a.k_st, keys);
-    load_tile(V, static_cast<const T *>(a.v) + (t.start + k0) * a.v_st + hk * a.v_sh, a.v_st, keys);
+    load_tile(K, static_cast<const float *>(a.k) + (t.start + k0) * a.k_st + hk * a.k_sh, a.k_st, keys);
+    load_tile(V, static_cast<const float *>(a.v) + (t.start + k0) * a.v_st + hk * a.v_sh, a.v_st, keys);
     __syncthreads();
-    float s[8][4], dp[8][4];
+    float s[kR][4], dp[kR][4];
     mul_rows(Q, K, ty, tx, s);
     mul_rows(G, V, ty, tx, dp);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kR; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool seen = k0 + tx + 16 * j <= t.row0 + 8 * ty + i;
+        const bool seen = k0 + tx + 16 * j <= t.row0 + kR * ty + i;
         const float p = exp2f(s[i][j] * a.scale_log2 - lse[i]);
-        P[(8 * ty + i) * kPitch + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
+        P[(kR * ty + i) * kPitch + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
       }
     __syncwarp();
     mul_p(P, K, ty, tx, acc);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (8 * ty + i < rows)
-      store4(dq + (8 * ty + i) * c_st + 4 * tx, acc[i][0] * a.scale, acc[i][1] * a.scale, acc[i][2] * a.scale,
+  for (int i = 0; i < kR; ++i)
+    if (kR * ty + i < rows)
+      store4(dq + (kR * ty + i) * c_st + 4 * tx, acc[i][0] * a.scale, acc[i][1] * a.scale, acc[i][2] * a.scale,
              acc[i][3] * a.scale);
 }
 
 // dK and dV of a key tile: every query tile at or behind it, of every query
-// head of the key-value head.
-template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs a) {
+// head of the key-value head.  The heads are shared out over a cluster of CTAs
+// (blockIdx.y = kv head x cluster + rank), which would otherwise walk them one
+// after the other on one SM; rank 0 adds the others' sums, in their order, from
+// their shared memory.
+__global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs a, int ranks) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *K = sm, *V = K + kTileFloats, *Q = V + kTileFloats, *G = Q + kTileFloats, *P = G + kTileFloats,
         *D = P + kTileFloats;
   const PackedTile t = packed_find(a.cu, a.S, a.total, blockIdx.x, kTile);
-  if (!t.valid) return;
-  const int hk = blockIdx.y, group = a.Hq / a.Hkv;
+  if (!t.valid) return;  // the cluster's CTAs share the tile: all return
+  const int hk = blockIdx.y / ranks, rank = blockIdx.y % ranks, group = a.Hq / a.Hkv;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int keys = min(kTile, t.len - t.row0);
   const int64_t first = t.start + t.row0;
   const int64_t c_st = static_cast<int64_t>(a.Hkv) * kTile;
-  T *dk = static_cast<T *>(a.dk) + first * c_st + hk * kTile;
-  T *dv = static_cast<T *>(a.dv) + first * c_st + hk * kTile;
-  float sk[8][4] = {}, sv[8][4] = {};
+  float *dk = static_cast<float *>(a.dk) + first * c_st + hk * kTile;
+  float *dv = static_cast<float *>(a.dv) + first * c_st + hk * kTile;
+  float sk[kR][4] = {}, sv[kR][4] = {};
   if (!t.rest) {
-    load_tile(K, static_cast<const T *>(a.k) + first * a.k_st + hk * a.k_sh, a.k_st, keys);
-    load_tile(V, static_cast<const T *>(a.v) + first * a.v_st + hk * a.v_sh, a.v_st, keys);
-    for (int g = 0; g < group; ++g) {
+    load_tile(K, static_cast<const float *>(a.k) + first * a.k_st + hk * a.k_sh, a.k_st, keys);
+    load_tile(V, static_cast<const float *>(a.v) + first * a.v_st + hk * a.v_sh, a.v_st, keys);
+    for (int g = rank; g < group; g += ranks) {
       const int h = hk * group + g;
       for (int q0 = t.row0; q0 < t.len; q0 += kTile) {
         __syncthreads();
         const int rows = min(kTile, t.len - q0);
         const int64_t at = t.start + q0;
-        load_tile(Q, static_cast<const T *>(a.q) + at * a.q_st + h * a.q_sh, a.q_st, rows);
-        load_tile(G, static_cast<const T *>(a.dout) + at * a.g_st + h * a.g_sh, a.g_st, rows);
+        load_tile(Q, static_cast<const float *>(a.q) + at * a.q_st + h * a.q_sh, a.q_st, rows);
+        load_tile(G, static_cast<const float *>(a.dout) + at * a.g_st + h * a.g_sh, a.g_st, rows);
         __syncthreads();
-        float s[8][4], dp[8][4];
+        float s[kR][4], dp[kR][4];
         mul_rows(Q, K, ty, tx, s);
         mul_rows(G, V, ty, tx, dp);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 8 * ty + i;
+        for (int i = 0; i < kR; ++i) {
+          const int r = kR * ty + i;
           float lse = 0.f, delta = 0.f;
           if (r < rows) {
             lse = a.lse[h * a.total + at + r];
@@ -318,12 +317,34 @@ template <typename T> __global__ void __launch_bounds__(pk::kThreads) packed_bwd
       }
     }
   }
+  if (ranks > 1) {
+    __syncthreads();  // all have read P and D
+    if (rank > 0) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (8 * ty + i < keys) {
-      store4(dk + (8 * ty + i) * c_st + 4 * tx, sk[i][0] * a.scale, sk[i][1] * a.scale, sk[i][2] * a.scale,
+      for (int i = 0; i < kR; ++i) {
+        store4(P + (kR * ty + i) * kPitch + 4 * tx, sk[i][0], sk[i][1], sk[i][2], sk[i][3]);
+        store4(D + (kR * ty + i) * kPitch + 4 * tx, sv[i][0], sv[i][1], sv[i][2], sv[i][3]);
+      }
+    }
+    cluster_sync();
+    if (rank == 0) {
+      for (int c = 1; c < ranks; ++c)
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+          const float4 x = peer4(P + (kR * ty + i) * kPitch + 4 * tx, c), y = peer4(D + (kR * ty + i) * kPitch + 4 * tx, c);
+          sk[i][0] += x.x, sk[i][1] += x.y, sk[i][2] += x.z, sk[i][3] += x.w;
+          sv[i][0] += y.x, sv[i][1] += y.y, sv[i][2] += y.z, sv[i][3] += y.w;
+        }
+    }
+    cluster_sync();  // the others' shared memory stays until it is read
+    if (rank > 0) return;
+  }
+#pragma unroll
+  for (int i = 0; i < kR; ++i)
+    if (kR * ty + i < keys) {
+      store4(dk + (kR * ty + i) * c_st + 4 * tx, sk[i][0] * a.scale, sk[i][1] * a.scale, sk[i][2] * a.scale,
              sk[i][3] * a.scale);
-      store4(dv + (8 * ty + i) * c_st + 4 * tx, sv[i][0], sv[i][1], sv[i][2], sv[i][3]);
+      store4(dv + (kR * ty + i) * c_st + 4 * tx, sv[i][0], sv[i][1], sv[i][2], sv[i][3]);
     }
 }
 
@@ -339,7 +360,7 @@ static int check_packed(const PackedArgs &a, int dtype, int64_t D) {
   if (!dtype_ok(dtype) || a.total <= 0 || a.S < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.Hq % a.Hkv || !a.cu || !a.out ||
       !(a.scale > 0.f) || a.scale > 3.0e38f)
     return SD_ERR_INVALID;
-  if (D != 64 || a.Hq > 65535 || a.total > 0x7fffff00ll || a.S > (1 << 24)) return SD_ERR_UNSUPPORTED;
+  if (D != 64 || a.Hq > 8191 || a.total > 0x7fffff00ll || a.S > (1 << 24)) return SD_ERR_UNSUPPORTED;
   int rc = check_rows(a.q, dtype, a.q_st, a.q_sh);
   if (rc == SD_OK) rc = check_rows(a.k, dtype, a.k_st, a.k_sh);
   if (rc == SD_OK) rc = check_rows(a.v, dtype, a.v_st, a.v_sh);
@@ -370,7 +391,7 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype != SD_DTYPE_F32) return launch_packed_fwd_tc(a, dtype, err, s);
   const size_t smem = 4 * pk::kTileFloats * sizeof(float);
-  auto kern = packed_fwd_kernel<float>;
+  auto kern = packed_fwd_kernel;
   if (set_max_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
   kern<<<dim3(static_cast<unsigned>(packed_slots(total, nseq, pk::kTile)), a.Hq), pk::kThreads, smem, s>>>(a);
   return check_launch();
@@ -403,14 +424,16 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   if (dtype != SD_DTYPE_F32) return launch_packed_bwd_tc(a, dtype, err, s);
   const unsigned slots = static_cast<unsigned>(packed_slots(total, nseq, pk::kTile));
   const size_t smem_q = 5 * pk::kTileFloats * sizeof(float), smem_kv = 6 * pk::kTileFloats * sizeof(float);
-  auto kq = packed_bwd_dq_kernel<float>;
-  auto kkv = packed_bwd_dkv_kernel<float>;
+  auto kq = packed_bwd_dq_kernel;
+  auto kkv = packed_bwd_dkv_kernel;
   if (set_max_smem(kq, smem_q) != SD_OK || set_max_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
   kq<<<dim3(slots, a.Hq), pk::kThreads, smem_q, s>>>(a);
   rc = check_launch();
   if (rc != SD_OK) return rc;
-  kkv<<<dim3(slots, a.Hkv), pk::kThreads, smem_kv, s>>>(a);
-  return check_launch();
+  int ranks = 8;  // CTAs of a cluster: the most that share the group's heads evenly
+  while (a.Hq / a.Hkv % ranks) --ranks;
+  return launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, false, a,
+                        ranks);
 }
 
 }  // extern "C"
