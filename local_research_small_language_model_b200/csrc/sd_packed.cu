@@ -35,6 +35,22 @@ __device__ __forceinline__ void load_tile(float *dst, const float *src, int64_t 
   }
 }
 
+// The same, arriving while the caller computes (one copy group of the thread).
+__device__ __forceinline__ void start_tile(float *dst, const float *src, int64_t stride, int rows) {
+  for (int e = threadIdx.x; e < kTile * 16; e += kThreads) {
+    const int r = e >> 4, c = (e & 15) * 4;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * kPitch + c)),
+                 "l"(r < rows ? src + r * stride + c : src), "r"(r < rows ? 16 : 0)
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void start_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest n groups have arrived, for every thread.
+template <int n> __device__ __forceinline__ void arrived() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+  __syncthreads();
+}
+
 __device__ __forceinline__ float4 ld4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 __device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
   return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
@@ -118,6 +134,20 @@ __device__ __forceinline__ float4 peer4(const float *p, int rank) {
   return v;
 }
 
+// Sums of a tile that a cluster shares: the other ranks put theirs into their
+// own shared memory, rank 0 adds them in their order.
+__device__ __forceinline__ void put(float *P, const float (&c)[kR][4], int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < kR; ++i) store4(P + (kR * ty + i) * kPitch + 4 * tx, c[i][0], c[i][1], c[i][2], c[i][3]);
+}
+__device__ __forceinline__ void add_peer(const float *P, int rank, float (&c)[kR][4], int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < kR; ++i) {
+    const float4 x = peer4(P + (kR * ty + i) * kPitch + 4 * tx, rank);
+    c[i][0] += x.x, c[i][1] += x.y, c[i][2] += x.z, c[i][3] += x.w;
+  }
+}
+
 // The 16 lanes of a row (tx = 0..15).
 __device__ __forceinline__ float row_max(float x) {
 #pragma unroll
@@ -150,18 +180,25 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) 
         if (kR * ty + i < rows) store4(out + (kR * ty + i) * a.o_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  load_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
+  const float *kp = static_cast<const float *>(a.k) + t.start * a.k_st + hk * a.k_sh;
+  const float *vp = static_cast<const float *>(a.v) + t.start * a.v_st + hk * a.v_sh;
+  start_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
+  start_tile(K, kp, a.k_st, min(kTile, t.len));
+  start_group();
+  start_tile(V, vp, a.v_st, min(kTile, t.len));
+  start_group();
   float o[kR][4] = {}, m[kR], l[kR];
 #pragma unroll
   for (int i = 0; i < kR; ++i) m[i] = -INFINITY, l[i] = 0.f;
   for (int k0 = 0; k0 <= t.row0; k0 += kTile) {
-    __syncthreads();
-    const int keys = min(kTile, t.len - k0);
-    load_tile(K, static_cast<const float *>(a.k) + (t.start + k0) * a.k_st + hk * a.k_sh, a.k_st, keys);
-    load_tile(V, static_cast<const float *>(a.v) + (t.start + k0) * a.v_st + hk * a.v_sh, a.v_st, keys);
-    __syncthreads();
+    // a tile's successor comes in as soon as its last product is done
+    const int next = k0 + kTile;
     float s[kR][4];
+    arrived<1>();
     mul_rows(Q, K, ty, tx, s);
+    __syncthreads();
+    if (next <= t.row0) start_tile(K, kp + next * a.k_st, a.k_st, min(kTile, t.len - next));
+    start_group();
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
       const int row = t.row0 + kR * ty + i;
@@ -186,8 +223,11 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) 
 #pragma unroll
       for (int u = 0; u < 4; ++u) o[i][u] *= alpha;
     }
-    __syncwarp();  // a warp reads only the rows of P that it wrote
+    arrived<1>();
     mul_p(P, V, ty, tx, o);
+    __syncthreads();
+    if (next <= t.row0) start_tile(V, vp + next * a.v_st, a.v_st, min(kTile, t.len - next));
+    start_group();
   }
 #pragma unroll
   for (int i = 0; i < kR; ++i) {
@@ -198,21 +238,22 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) 
   }
 }
 
-// dQ of a query tile; also delta, which the dK/dV kernel behind it reads.
-__global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs a) {
+// dQ of a query tile, its key tiles dealt out to the CTAs of a cluster; also
+// delta, which the dK/dV kernel behind it reads.
+__global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs a, int ranks) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *G = Q + kTileFloats, *K = G + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
   const PackedTile t = packed_find(a.cu, a.S, a.total, gridDim.x - 1 - blockIdx.x, kTile);
   if (!t.valid) return;
-  const int h = blockIdx.y, hk = h / (a.Hq / a.Hkv);
+  const int h = blockIdx.y / ranks, rank = blockIdx.y % ranks, hk = h / (a.Hq / a.Hkv);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int rows = min(kTile, t.len - t.row0);
   const int64_t first = t.start + t.row0;
   const int64_t c_st = static_cast<int64_t>(a.Hq) * kTile;  // dq is contiguous
   float *dq = static_cast<float *>(a.dq) + first * c_st + h * kTile;
   if (t.rest) {
-    for (int i = 0; i < kR; ++i)
+    for (int i = 0; i < kR && rank == 0; ++i)
       if (kR * ty + i < rows) store4(dq + (kR * ty + i) * c_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
   }
@@ -227,21 +268,28 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
     lse[i] = 0.f;
     if (r < rows) {
       lse[i] = a.lse[h * a.total + first + r];
-      if (tx == 0) a.delta[h * a.total + first + r] = delta[i];
+      if (rank == 0 && tx == 0) a.delta[h * a.total + first + r] = delta[i];
     }
   }
   __syncthreads();
-  load_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
+  const float *kp = static_cast<const float *>(a.k) + t.start * a.k_st + hk * a.k_sh;
+  const float *vp = static_cast<const float *>(a.v) + t.start * a.v_st + hk * a.v_sh;
+  auto start = [&](float *dst, const float *src, int64_t st, int k0) {
+    if (k0 <= t.row0) start_tile(dst, src + k0 * st, st, min(kTile, t.len - k0));
+    start_group();
+  };
+  start_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
+  start(V, vp, a.v_st, rank * kTile);
+  start(K, kp, a.k_st, rank * kTile);
   float acc[kR][4] = {};
-  for (int k0 = 0; k0 <= t.row0; k0 += kTile) {
-    __syncthreads();
-    const int keys = min(kTile, t.len - k0);
-    load_tile(K, static_cast<const float *>(a.k) + (t.start + k0) * a.k_st + hk * a.k_sh, a.k_st, keys);
-    load_tile(V, static_cast<const float *>(a.v) + (t.start + k0) * a.v_st + hk * a.v_sh, a.v_st, keys);
-    __syncthreads();
+  for (int k0 = rank * kTile; k0 <= t.row0; k0 += ranks * kTile) {
     float s[kR][4], dp[kR][4];
-    mul_rows(Q, K, ty, tx, s);
+    arrived<1>();
     mul_rows(G, V, ty, tx, dp);
+    __syncthreads();
+    start(V, vp, a.v_st, k0 + ranks * kTile);
+    arrived<1>();
+    mul_rows(Q, K, ty, tx, s);
 #pragma unroll
     for (int i = 0; i < kR; ++i)
 #pragma unroll
@@ -250,8 +298,19 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
         const float p = exp2f(s[i][j] * a.scale_log2 - lse[i]);
         P[(kR * ty + i) * kPitch + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
       }
-    __syncwarp();
+    __syncwarp();  // a warp reads only the rows of P that it wrote
     mul_p(P, K, ty, tx, acc);
+    __syncthreads();
+    start(K, kp, a.k_st, k0 + ranks * kTile);
+  }
+  if (ranks > 1) {
+    __syncthreads();
+    if (rank > 0) put(P, acc, ty, tx);
+    cluster_sync();
+    if (rank == 0)
+      for (int c = 1; c < ranks; ++c) add_peer(P, c, acc, ty, tx);
+    cluster_sync();
+    if (rank > 0) return;
   }
 #pragma unroll
   for (int i = 0; i < kR; ++i)
@@ -261,10 +320,9 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
 }
 
 // dK and dV of a key tile: every query tile at or behind it, of every query
-// head of the key-value head.  The heads are shared out over a cluster of CTAs
-// (blockIdx.y = kv head x cluster + rank), which would otherwise walk them one
-// after the other on one SM; rank 0 adds the others' sums, in their order, from
-// their shared memory.
+// head of the key-value head.  These are dealt out in turn to the CTAs of a
+// cluster (blockIdx.y = kv head x ranks + rank): a short batch has few key
+// tiles, and the first of a sequence has them all.
 __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs a, int ranks) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
@@ -281,20 +339,29 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs
   float *dv = static_cast<float *>(a.dv) + first * c_st + hk * kTile;
   float sk[kR][4] = {}, sv[kR][4] = {};
   if (!t.rest) {
-    load_tile(K, static_cast<const float *>(a.k) + first * a.k_st + hk * a.k_sh, a.k_st, keys);
-    load_tile(V, static_cast<const float *>(a.v) + first * a.v_st + hk * a.v_sh, a.v_st, keys);
-    for (int g = rank; g < group; g += ranks) {
-      const int h = hk * group + g;
-      for (int q0 = t.row0; q0 < t.len; q0 += kTile) {
-        __syncthreads();
+    const int per_head = (t.len - t.row0 + kTile - 1) / kTile, items = per_head * group;
+    auto start = [&](float *dst, const void *src, int64_t st, int64_t sh, int item) {
+      if (item < items) {
+        const int q0 = t.row0 + item % per_head * kTile;
+        start_tile(dst, static_cast<const float *>(src) + (t.start + q0) * st + (hk * group + item / per_head) * sh, st,
+                   min(kTile, t.len - q0));
+      }
+      start_group();
+    };
+    start_tile(K, static_cast<const float *>(a.k) + first * a.k_st + hk * a.k_sh, a.k_st, keys);
+    start_tile(V, static_cast<const float *>(a.v) + first * a.v_st + hk * a.v_sh, a.v_st, keys);
+    start(G, a.dout, a.g_st, a.g_sh, rank);
+    start(Q, a.q, a.q_st, a.q_sh, rank);
+    for (int item = rank; item < items; item += ranks) {
+      const int h = hk * group + item / per_head, q0 = t.row0 + item % per_head * kTile;
+      {
         const int rows = min(kTile, t.len - q0);
         const int64_t at = t.start + q0;
-        load_tile(Q, static_cast<const float *>(a.q) + at * a.q_st + h * a.q_sh, a.q_st, rows);
-        load_tile(G, static_cast<const float *>(a.dout) + at * a.g_st + h * a.g_sh, a.g_st, rows);
-        __syncthreads();
         float s[kR][4], dp[kR][4];
-        mul_rows(Q, K, ty, tx, s);
+        arrived<1>();
         mul_rows(G, V, ty, tx, dp);
+        arrived<0>();
+        mul_rows(Q, K, ty, tx, s);
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
           const int r = kR * ty + i;
@@ -313,29 +380,20 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs
         }
         __syncthreads();
         mul_pt(P, G, ty, tx, sv);
+        __syncthreads();
+        start(G, a.dout, a.g_st, a.g_sh, item + ranks);
         mul_pt(D, Q, ty, tx, sk);
+        __syncthreads();
+        start(Q, a.q, a.q_st, a.q_sh, item + ranks);
       }
     }
   }
   if (ranks > 1) {
     __syncthreads();  // all have read P and D
-    if (rank > 0) {
-#pragma unroll
-      for (int i = 0; i < kR; ++i) {
-        store4(P + (kR * ty + i) * kPitch + 4 * tx, sk[i][0], sk[i][1], sk[i][2], sk[i][3]);
-        store4(D + (kR * ty + i) * kPitch + 4 * tx, sv[i][0], sv[i][1], sv[i][2], sv[i][3]);
-      }
-    }
+    if (rank > 0) put(P, sk, ty, tx), put(D, sv, ty, tx);
     cluster_sync();
-    if (rank == 0) {
-      for (int c = 1; c < ranks; ++c)
-#pragma unroll
-        for (int i = 0; i < kR; ++i) {
-          const float4 x = peer4(P + (kR * ty + i) * kPitch + 4 * tx, c), y = peer4(D + (kR * ty + i) * kPitch + 4 * tx, c);
-          sk[i][0] += x.x, sk[i][1] += x.y, sk[i][2] += x.z, sk[i][3] += x.w;
-          sv[i][0] += y.x, sv[i][1] += y.y, sv[i][2] += y.z, sv[i][3] += y.w;
-        }
-    }
+    if (rank == 0)
+      for (int c = 1; c < ranks; ++c) add_peer(P, c, sk, ty, tx), add_peer(D, c, sv, ty, tx);
     cluster_sync();  // the others' shared memory stays until it is read
     if (rank > 0) return;
   }
@@ -427,11 +485,16 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   auto kq = packed_bwd_dq_kernel;
   auto kkv = packed_bwd_dkv_kernel;
   if (set_max_smem(kq, smem_q) != SD_OK || set_max_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
-  kq<<<dim3(slots, a.Hq), pk::kThreads, smem_q, s>>>(a);
-  rc = check_launch();
+  // Clusters as large as it takes to give every SM a few CTAs: two fit an SM.
+  auto ranks_for = [&](int heads) {
+    int ranks = 1;
+    while (ranks < 8 && static_cast<int64_t>(slots) * heads * ranks < 2 * 148) ranks *= 2;
+    return ranks;
+  };
+  int ranks = ranks_for(a.Hq);
+  rc = launch_cluster(kq, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_q, s, false, a, ranks);
   if (rc != SD_OK) return rc;
-  int ranks = 8;  // CTAs of a cluster: the most that share the group's heads evenly
-  while (a.Hq / a.Hkv % ranks) --ranks;
+  ranks = ranks_for(a.Hkv);
   return launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, false, a,
                         ranks);
 }
