@@ -2,6 +2,8 @@
 #include <math.h>
 
 #include <atomic>
+#include <mutex>
+#include <vector>
 
 #include "sd_common.cuh"
 
@@ -34,6 +36,35 @@ int set_max_smem_raw(const void *func, size_t bytes) {
     return SD_ERR_CUDA;
   }
   return SD_OK;
+}
+
+int ensure_smem_raw(const void *func, size_t bytes) {
+  if (bytes <= 48 * 1024) return SD_OK;
+  struct Limit {
+    const void *func;
+    int device;
+    size_t bytes;
+  };
+  static std::mutex lock;
+  static std::vector<Limit> limits;
+  int device = 0;
+  const cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    cudaGetLastError();
+    return SD_ERR_CUDA;
+  }
+  std::lock_guard<std::mutex> hold(lock);
+  for (Limit &l : limits)
+    if (l.func == func && l.device == device) {
+      if (l.bytes >= bytes) return SD_OK;
+      const int rc = set_max_smem_raw(func, bytes);
+      if (rc == SD_OK) l.bytes = bytes;
+      return rc;
+    }
+  const int rc = set_max_smem_raw(func, bytes);
+  if (rc == SD_OK) limits.push_back({func, device, bytes});
+  return rc;
 }
 
 __global__ void advance_len_kernel(int32_t *lens, int n, int delta) {

@@ -26,6 +26,13 @@ template <typename K> int set_max_smem(K *func, size_t bytes) {
   return set_max_smem_raw(reinterpret_cast<const void *>(func), bytes);
 }
 
+// The same where calls are short: remembers, per kernel and device, the limit
+// already raised, and asks the runtime only for more.
+int ensure_smem_raw(const void *func, size_t bytes);
+template <typename K> int ensure_smem(K *func, size_t bytes) {
+  return ensure_smem_raw(reinterpret_cast<const void *>(func), bytes);
+}
+
 // Programmatic dependent launch (sd_set_programmatic_launch): when enabled,
 // the kernels that support it are launched so they may start before the
 // kernel ahead of them on the stream has finished; each waits (pdl_wait) before

@@ -424,7 +424,7 @@ int sd_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t V, in
   if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype)) return SD_ERR_ALIGN;
   SD_DISPATCH_DTYPE(dtype, T, {
     auto run = [&](auto *kern, int threads, size_t smem) {
-      if (set_max_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
+      if (ensure_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
       kern<<<static_cast<unsigned>(rows), threads, smem, static_cast<cudaStream_t>(stream)>>>(
           static_cast<const T *>(logits), rows, V, ld, targets, ignore_index, logprobs, entropy, stats, top_k,
           top_logprobs, top_ids, err);

@@ -450,7 +450,7 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
   if (dtype != SD_DTYPE_F32) return launch_packed_fwd_tc(a, dtype, err, s);
   const size_t smem = 4 * pk::kTileFloats * sizeof(float);
   auto kern = packed_fwd_kernel;
-  if (set_max_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
+  if (ensure_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
   kern<<<dim3(static_cast<unsigned>(packed_slots(total, nseq, pk::kTile)), a.Hq), pk::kThreads, smem, s>>>(a);
   return check_launch();
 }
@@ -484,7 +484,7 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   const size_t smem_q = 5 * pk::kTileFloats * sizeof(float), smem_kv = 6 * pk::kTileFloats * sizeof(float);
   auto kq = packed_bwd_dq_kernel;
   auto kkv = packed_bwd_dkv_kernel;
-  if (set_max_smem(kq, smem_q) != SD_OK || set_max_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
+  if (ensure_smem(kq, smem_q) != SD_OK || ensure_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
   // Clusters as large as it takes to give every SM a few CTAs: two fit an SM.
   auto ranks_for = [&](int heads) {
     int ranks = 1;

@@ -888,7 +888,7 @@ int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
   if (ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
   const size_t smem = pt::FwdSmem::kBytes + 1024;
   auto run = [&](auto *kern) {
-    if (set_max_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
+    if (ensure_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
     kern<<<static_cast<unsigned>(ctas), pt::kFwdThreads, smem, s>>>(a, mk, mv, err);
     return check_launch();
   };
@@ -916,7 +916,7 @@ int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
   }
   const size_t smem = pt::BwdSmem::kBytes + 1024;
   auto run = [&](auto *dq, auto *dkv) {
-    if (set_max_smem(dq, smem) != SD_OK || set_max_smem(dkv, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
+    if (ensure_smem(dq, smem) != SD_OK || ensure_smem(dkv, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
     dq<<<static_cast<unsigned>(slots * a.Hq), pt::kBwdThreads, smem, s>>>(a, mq, mg, mk, mv, top, err);
     const int first = check_launch();
     if (first != SD_OK) return first;

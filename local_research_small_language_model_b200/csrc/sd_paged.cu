@@ -696,7 +696,7 @@ int sd_paged_decode_attention(const void *q, int dtype, int64_t B, int64_t Hq, i
       auto kern = whole ? wide ? paged_decode_kernel<T, true, true> : paged_decode_kernel<T, true, false>
                   : wide ? paged_decode_kernel<T, false, true>
                          : paged_decode_kernel<T, false, false>;
-      if (set_max_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
+      if (ensure_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
       kern<<<ctas, pg::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a, d);
       rc = check_launch();
       if (rc != SD_OK) return rc;

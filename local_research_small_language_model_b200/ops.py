@@ -679,11 +679,11 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     (innermost stride 1, aligned base and strides, no broadcast dimension),
     else a contiguous copy."""
     if not t.data_ptr() & 15:
-        if t.is_contiguous():
+        st = t.stride()
+        if len(st) == 3 and st[2] == 1 and not (st[0] | st[1]) & 7 and st[0] > 0 and st[1] > 0:
             return t
-        *outer, inner = t.stride()
         whole = 16 // t.element_size() - 1
-        if inner == 1 and not any(s & whole for s in outer) and all(s > 0 or n == 1 for s, n in zip(outer, t.shape)):
+        if st[-1] == 1 and not any(s & whole for s in st[:-1]) and all(s > 0 or n == 1 for s, n in zip(st, t.shape)):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -705,13 +705,14 @@ def _scale(scale: Optional[float], d: int) -> float:
 
 
 def _check_packed(q, k, v, cu_seqlens, **like_q):
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise ValueError(f"q must be [total, Hq, D] and k, v [total, Hkv, D], got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    if q.shape[2] != 64:
-        raise ValueError(f"packed attention has head size 64, got {q.shape[2]}")
-    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"query heads ({q.shape[1]}) must be a multiple of kv heads ({k.shape[1]})")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[0] != qs[0] or ks[2] != qs[2]:
+        raise ValueError(f"q must be [total, Hq, D] and k, v [total, Hkv, D], got {tuple(qs)}, {tuple(ks)}, "
+                         f"{tuple(v.shape)}")
+    if qs[2] != 64:
+        raise ValueError(f"packed attention has head size 64, got {qs[2]}")
+    if ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
+        raise ValueError(f"query heads ({qs[1]}) must be a multiple of kv heads ({ks[1]})")
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
         raise ValueError(f"cu_seqlens must hold a bound more than there are sequences, got {tuple(cu_seqlens.shape)}")
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -738,7 +739,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     dev = _device(q, k, v, cu_seqlens, out)
     total, hq, d = q.shape
     sc = _scale(scale, d)
-    cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape)
+    cu = cu_seqlens
+    if cu.dtype is not torch.int32 or cu.stride(0) != 1:
+        cu = _index32("cu_seqlens", cu, cu.shape)
     code = dtype_code(q)
     zero = out is None
     if zero:
@@ -784,17 +787,20 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 def _check_pool(k_pages, v_pages, page_table, seqs, d):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or 0 in k_pages.shape:
-        raise ValueError(f"k_pages and v_pages must be [pages, Hkv, page, D] alike, got {tuple(k_pages.shape)}, "
+    """The pool's (pages, Hkv, page) and its strides, the same for k and v."""
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or not k_pages.numel():
+        raise ValueError(f"k_pages and v_pages must be [pages, Hkv, page, D] alike, got {tuple(shape)}, "
                          f"{tuple(v_pages.shape)}")
-    if d != 64 or k_pages.shape[3] != 64:
-        raise ValueError(f"paged caches have head size 64, got {d} and {k_pages.shape[3]}")
-    if k_pages.dtype != v_pages.dtype or k_pages.stride() != v_pages.stride():
+    if d != 64 or shape[3] != 64:
+        raise ValueError(f"paged caches have head size 64, got {d} and {shape[3]}")
+    if k_pages.dtype != v_pages.dtype or strides != v_pages.stride():
         raise ValueError("k_pages and v_pages must share dtype and strides")
-    if _rows16(k_pages) is not k_pages or _rows16(v_pages) is not v_pages:
+    if _rows16(k_pages) is not k_pages or v_pages.data_ptr() & 15:
         raise ValueError("pages must have 16-byte aligned rows and innermost stride 1")
-    if page_table.dim() != 2 or page_table.shape[0] != seqs or page_table.shape[1] == 0:
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or not page_table.shape[1]:
         raise ValueError(f"page_table must be [{seqs}, width], got {tuple(page_table.shape)}")
+    return shape[:3], strides[:3]
 
 
 def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -811,9 +817,9 @@ def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pa
                          f"{tuple(xv.shape)}, {tuple(lens.shape)}")
     n, hkv, d = xk.shape
     b = lens.shape[0]
-    _check_pool(k_pages, v_pages, page_table, b, d)
-    if k_pages.shape[1] != hkv:
-        raise ValueError(f"the pool has {k_pages.shape[1]} kv heads, the rows {hkv}")
+    (pages, held, page), pool_strides = _check_pool(k_pages, v_pages, page_table, b, d)
+    if held != hkv:
+        raise ValueError(f"the pool has {held} kv heads, the rows {hkv}")
     if xk.dtype != k_pages.dtype or xv.dtype != k_pages.dtype:
         raise TypeError(f"rows of {xk.dtype} do not fit pages of {k_pages.dtype}")
     if cu_seqlens is None and n != b:
@@ -827,8 +833,7 @@ def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pa
         return
     xk, xv = _rows16(xk), _rows16(xv)
     _launch("sd_paged_append", dev, xk.data_ptr(), xv.data_ptr(), code, n, hkv, d, *xk.stride()[:2],
-            *xv.stride()[:2], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], k_pages.shape[2],
-            *k_pages.stride()[:3], table.data_ptr(), table.stride(0), table.shape[1], ln.data_ptr(), b,
+            *xv.stride()[:2], k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *pool_strides, table.data_ptr(), table.stride(0), table.shape[1], ln.data_ptr(), b,
             cu.data_ptr() if cu is not None else None, _err_ptr(dev))
 
 
@@ -849,8 +854,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if q.dim() != 3 or lens.dim() != 1 or q.shape[0] != lens.shape[0]:
         raise ValueError(f"q must be [B, Hq, D] and lens [B], got {tuple(q.shape)}, {tuple(lens.shape)}")
     b, hq, d = q.shape
-    _check_pool(k_pages, v_pages, page_table, b, d)
-    pages, hkv, page, _ = k_pages.shape
+    (pages, hkv, page), pool_strides = _check_pool(k_pages, v_pages, page_table, b, d)
     if hq == 0 or hq % hkv:
         raise ValueError(f"query heads ({hq}) must be a multiple of kv heads ({hkv})")
     if q.dtype != k_pages.dtype or (out is not None and out.dtype != q.dtype):
@@ -873,8 +877,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     need = _decode_workspace(b, hq, hkv)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     _launch("sd_paged_decode_attention", dev, q.data_ptr(), code, b, hq, hkv, d, *q.stride()[:2],
-            k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *k_pages.stride()[:3], table.data_ptr(),
-            table.stride(0), table.shape[1], ln.data_ptr(), sc, out.data_ptr(), *out.stride()[:2], ws.data_ptr(),
+            k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *pool_strides, table.data_ptr(), table.stride(0), table.shape[1], ln.data_ptr(), sc, out.data_ptr(), *out.stride()[:2], ws.data_ptr(),
             need, _err_ptr(dev))
     return out
 
