@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) 
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *K = Q + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
-  // the last tiles of a sequence see the most keys: they start first
-  const PackedTile t = packed_find(a.cu, a.S, a.total, gridDim.x - 1 - blockIdx.x, kTile);
+  // the tiles that see the most keys start first
+  const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x, gridDim.x, kTile, true);
   if (!t.valid) return;
   const int h = blockIdx.y, hk = h / (a.Hq / a.Hkv);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *G = Q + kTileFloats, *K = G + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
-  const PackedTile t = packed_find(a.cu, a.S, a.total, gridDim.x - 1 - blockIdx.x, kTile);
+  const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x, gridDim.x, kTile, true);
   if (!t.valid) return;
   const int h = blockIdx.y / ranks, rank = blockIdx.y % ranks, hk = h / (a.Hq / a.Hkv);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs
   extern __shared__ __align__(16) float sm[];
   float *K = sm, *V = K + kTileFloats, *Q = V + kTileFloats, *G = Q + kTileFloats, *P = G + kTileFloats,
         *D = P + kTileFloats;
-  const PackedTile t = packed_find(a.cu, a.S, a.total, blockIdx.x, kTile);
+  const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x, gridDim.x, kTile, false);
   if (!t.valid) return;  // the cluster's CTAs share the tile: all return
   const int hk = blockIdx.y / ranks, rank = blockIdx.y % ranks, group = a.Hq / a.Hkv;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;

@@ -77,6 +77,79 @@ __device__ __forceinline__ PackedTile packed_find(const int32_t *cu, int S, int6
   return t;
 }
 
+// The nth tile in order of falling work, for up to 128 sequences: CTAs start in
+// launch order, and a long tile that starts late is what the others wait for
+// (11 prompts, 16384 tokens: a fifth of the forward's time).  A tile with i
+// tiles before it in its sequence (last_first: query tiles, which see the keys
+// before them) or behind it (key tiles, seen by the queries behind them) has
+// level i; f(i) = sum_s max(0, T_s - i) tiles have level i or more, so the nth
+// tile's level is the largest i with f(i) > n, found by bisection with the
+// counts T_s in registers.  Tiles of the rows outside every sequence follow.
+// With more sequences than that: the slots above, in their order.
+__device__ __forceinline__ PackedTile packed_nth(const int32_t *cu, int S, int64_t total, int64_t n, int64_t slots,
+                                                 int tile, bool last_first) {
+  constexpr int kEach = 4;  // sequences a lane
+  if (S > 32 * kEach) return packed_find(cu, S, total, last_first ? slots - 1 - n : n, tile);
+  const int lane = threadIdx.x & 31;
+  int tiles[kEach], most = 0, all = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int s = lane + 32 * e;
+    tiles[e] = 0;
+    if (s < S) {
+      const int64_t len = packed_bound(cu, S, total, s + 2) - packed_bound(cu, S, total, s + 1);
+      tiles[e] = len > 0 ? static_cast<int>((len + tile - 1) / tile) : 0;
+    }
+    most = max(most, tiles[e]);
+    all += tiles[e];
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  all = __reduce_add_sync(0xffffffffu, all);
+  PackedTile t = {};
+  if (n >= all) {  // the rows before cu[0], then those from cu[S] on
+    n -= all;
+    const int64_t first = packed_bound(cu, S, total, 1), last = packed_bound(cu, S, total, S + 1);
+    const int64_t before = (first + tile - 1) / tile;
+    t.rest = true;
+    t.start = n < before ? 0 : last;
+    t.len = static_cast<int>(n < before ? first : total - last);
+    if (n >= before) n -= before;
+    t.valid = n * tile < t.len;
+    t.row0 = t.valid ? static_cast<int>(n * tile) : 0;
+    return t;
+  }
+  auto from = [&](int i) {
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) c += max(0, tiles[e] - i);
+    return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
+  };
+  int lo = 0, hi = most;  // f(lo) > n >= f(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (from(mid) > n) lo = mid; else hi = mid;
+  }
+  int rank = static_cast<int>(n) - from(hi);  // among the sequences with more than lo tiles
+  int seq = 0, held = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const unsigned has = __ballot_sync(0xffffffffu, tiles[e] > lo);
+    const int c = __popc(has);
+    if (rank >= 0 && rank < c) {
+      const int l = __fns(has, 0, rank + 1);
+      seq = 32 * e + l;
+      held = __shfl_sync(0xffffffffu, tiles[e], l);
+    }
+    rank -= c;
+  }
+  const int64_t b = packed_bound(cu, S, total, seq + 1), e = packed_bound(cu, S, total, seq + 2);
+  t.start = b;
+  t.len = static_cast<int>(e - b);
+  t.row0 = (last_first ? lo : held - 1 - lo) * tile;
+  t.valid = true;
+  return t;
+}
+
 // The tensor-core kernels (16-bit types).
 int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s);
 int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s);

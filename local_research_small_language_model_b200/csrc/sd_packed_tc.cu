@@ -198,10 +198,10 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
                          const __grid_constant__ CUtensorMap tmv, int32_t *err) {
   using namespace pt;
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  // heads fastest; the last tiles, which see the most keys, first
+  // heads fastest; the tiles that see the most keys first
   const int h = blockIdx.x % a.Hq;
   const int64_t slots = gridDim.x / a.Hq;
-  const PackedTile t = packed_find(a.cu, a.S, a.total, slots - 1 - blockIdx.x / a.Hq, 2 * kRows);
+  const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x / a.Hq, slots, 2 * kRows, true);
   if (!t.valid) return;
   const int rows = min(2 * kRows, t.len - t.row0);
   const int64_t first = t.start + t.row0;
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   constexpr uint32_t fmt = kHalf ? 0u : 1u;
   const int h = blockIdx.x % a.Hq;
   const int64_t slots = gridDim.x / a.Hq;
-  const PackedTile t = packed_find(a.cu, a.S, a.total, slots - 1 - blockIdx.x / a.Hq, kRows);
+  const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x / a.Hq, slots, kRows, true);
   if (!t.valid) return;
   const int rows = min(kRows, t.len - t.row0);
   const int64_t first = t.start + t.row0, c_st = static_cast<int64_t>(a.Hq) * 64;
@@ -731,8 +731,8 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr uint32_t fmt = kHalf ? 0u : 1u;
   const int hk = blockIdx.x % a.Hkv, group = a.Hq / a.Hkv;
-  // a sequence's first keys are seen by the most queries: they start first
-  const PackedTile t = packed_find(a.cu, a.S, a.total, blockIdx.x / a.Hkv, kRows);
+  // the keys that are seen by the most queries first
+  const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x / a.Hkv, gridDim.x / a.Hkv, kRows, false);
   if (!t.valid) return;
   const int keys = min(kRows, t.len - t.row0);
   const int64_t first = t.start + t.row0, c_st = static_cast<int64_t>(a.Hkv) * 64;

@@ -45,6 +45,7 @@ LENGTHS = {
     "ragged": [300, 1, 0, 77, 513, 2],
     "long": [1100],
     "many": [5] * 70 + [0] * 7 + [40],
+    "crowd": [3, 0, 130] * 60,
 }
 
 
