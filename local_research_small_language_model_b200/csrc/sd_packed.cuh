@@ -91,21 +91,33 @@ __device__ __forceinline__ PackedTile packed_nth(const int32_t *cu, int S, int64
   constexpr int kEach = 4;  // sequences a lane
   if (S > 32 * kEach) return packed_find(cu, S, total, last_first ? slots - 1 - n : n, tile);
   const int lane = threadIdx.x & 31;
-  int tiles[kEach], most = 0, all = 0;
+  int start[kEach], len[kEach], tiles[kEach], most = 0, all = 0;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int s = lane + 32 * e;
-    tiles[e] = 0;
+    start[e] = len[e] = tiles[e] = 0;
     if (s < S) {
-      const int64_t len = packed_bound(cu, S, total, s + 2) - packed_bound(cu, S, total, s + 1);
-      tiles[e] = len > 0 ? static_cast<int>((len + tile - 1) / tile) : 0;
+      start[e] = static_cast<int>(packed_bound(cu, S, total, s + 1));
+      len[e] = max(0, static_cast<int>(packed_bound(cu, S, total, s + 2)) - start[e]);
+      tiles[e] = static_cast<int>((static_cast<unsigned>(len[e]) + tile - 1) / tile);
     }
     most = max(most, tiles[e]);
     all += tiles[e];
   }
-  most = __reduce_max_sync(0xffffffffu, most);
-  all = __reduce_add_sync(0xffffffffu, all);
   PackedTile t = {};
+  t.valid = true;
+  if (S == 1) {
+    all = __shfl_sync(0xffffffffu, tiles[0], 0);
+    if (n < all) {
+      t.start = __shfl_sync(0xffffffffu, start[0], 0);
+      t.len = __shfl_sync(0xffffffffu, len[0], 0);
+      t.row0 = (last_first ? all - 1 - static_cast<int>(n) : static_cast<int>(n)) * tile;
+      return t;
+    }
+  } else {
+    most = __reduce_max_sync(0xffffffffu, most);
+    all = __reduce_add_sync(0xffffffffu, all);
+  }
   if (n >= all) {  // the rows before cu[0], then those from cu[S] on
     n -= all;
     const int64_t first = packed_bound(cu, S, total, 1), last = packed_bound(cu, S, total, S + 1);
@@ -119,34 +131,36 @@ __device__ __forceinline__ PackedTile packed_nth(const int32_t *cu, int S, int64
     return t;
   }
   auto from = [&](int i) {
-    int c = 0;
+    int c = max(0, tiles[0] - i);
+    if (S > 32) {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) c += max(0, tiles[e] - i);
+      for (int e = 1; e < kEach; ++e) c += max(0, tiles[e] - i);
+    }
     return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
   };
-  int lo = 0, hi = most;  // f(lo) > n >= f(hi)
+  int lo = 0, hi = most, above = 0;  // f(lo) > n >= f(hi) = above
   while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (from(mid) > n) lo = mid; else hi = mid;
+    const int mid = (lo + hi) / 2, f = from(mid);
+    if (f > n)
+      lo = mid;
+    else
+      hi = mid, above = f;
   }
-  int rank = static_cast<int>(n) - from(hi);  // among the sequences with more than lo tiles
-  int seq = 0, held = 0;
+  int rank = static_cast<int>(n) - above;  // among the sequences with more than lo tiles
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const unsigned has = __ballot_sync(0xffffffffu, tiles[e] > lo);
-    const int c = __popc(has);
-    if (rank >= 0 && rank < c) {
-      const int l = __fns(has, 0, rank + 1);
-      seq = 32 * e + l;
-      held = __shfl_sync(0xffffffffu, tiles[e], l);
+    const bool mine = tiles[e] > lo;
+    const unsigned has = __ballot_sync(0xffffffffu, mine);
+    const unsigned hit = __ballot_sync(0xffffffffu, mine && __popc(has & ((1u << lane) - 1u)) == rank);
+    if (hit) {
+      const int l = __ffs(hit) - 1, held = __shfl_sync(0xffffffffu, tiles[e], l);
+      t.start = __shfl_sync(0xffffffffu, start[e], l);
+      t.len = __shfl_sync(0xffffffffu, len[e], l);
+      t.row0 = (last_first ? lo : held - 1 - lo) * tile;
+      break;
     }
-    rank -= c;
+    rank -= __popc(has);
   }
-  const int64_t b = packed_bound(cu, S, total, seq + 1), e = packed_bound(cu, S, total, seq + 2);
-  t.start = b;
-  t.len = static_cast<int>(e - b);
-  t.row0 = (last_first ? lo : held - 1 - lo) * tile;
-  t.valid = true;
   return t;
 }
 

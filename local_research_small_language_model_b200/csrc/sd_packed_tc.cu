@@ -787,16 +787,16 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     float next_l, next_d;
     auto fetch = [&](bool more) {
       const bool held = more && qn + lane < span;
-      next_l = held ? -a.lse[at + qn] : 0.f;
-      next_d = held ? -a.delta[at + qn] : 0.f;
+      next_l = next_d = 0.f;
+      if (held) next_l = a.lse[at + qn], next_d = a.delta[at + qn];  // negated when stored: nothing waits for them here
       qn += kRows;
       if (qn >= span + 32 * wg) qn = 0, at += a.total;
     };
     fetch(true);
     for (int i = 0; i < blocks; ++i) {
       __syncwarp();
-      mine[lane] = next_l;
-      mine[32 + lane] = next_d;
+      mine[lane] = -next_l;
+      mine[32 + lane] = -next_d;
       const bool nan = __any_sync(0xffffffffu, next_l != next_l);
       __syncwarp();
       const int q0 = qn == 0 ? (span + 32 * wg - 1) / kRows * kRows : qn - kRows;  // this block's
