@@ -25,7 +25,7 @@ namespace lp {
 constexpr int64_t kManyRows = 4 * 148;
 constexpr int kGroups = 128;            // of threads: their maxima bound the top_k-th value (top_k <= 64)
 constexpr int kAbove = 4096;            // room for the values above that bound,
-constexpr int kTies = 8192 + 64;        // and for those equal to it: a step's and fewer than top_k before
+constexpr int kTies = 512;              // and for those equal to it
 constexpr int kCandidates = kAbove + kTies;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e4f;         // stands for -inf: its exponential is 0 and 0 * kFloor is 0
@@ -179,9 +179,9 @@ template <typename T> struct Row {
 //
 // top_k: the top_k-th largest of the 128 thread groups' maxima bounds the
 // top_k-th largest value from below, so a second pass (the row is in L2, 64 KB
-// for 32000 16-bit logits) collects the values above that bound, and as many of
-// those equal to it, in index order, as can be needed; a candidate's rank among
-// them is its place in the answer.
+// for 32000 16-bit logits) collects the values above that bound and those equal
+// to it (only the first top_k of these, in index order, where they are many); a
+// candidate's rank among them is its place in the answer.
 template <typename T, bool kTop, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     token_logprobs_kernel(const T *x, int64_t rows, int64_t V, int64_t ld, const int64_t *targets,
@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     __shared__ float group[kGroups];
     __shared__ float bound;
     __shared__ int above, ties;  // values above the bound, and equal to it
+    __shared__ int count[kWarps];
     constexpr int kGroup = kThreads / kGroups;  // threads of a group
 #pragma unroll
     for (int o = 1; o < kGroup; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -269,42 +270,81 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     __syncthreads();
     const float low = bound;
     // candidates above the bound fill the buffer from its start, equal ones from
-    // its end; equal ones are taken in index order, piece by piece of the row,
-    // until there are top_k of them
-    auto take = [&](float v, int64_t j, bool equal_too) {
+    // its end
+    auto take = [&](float v, int64_t j) {
       if (v < low) return;
       if (v == low) {
-        if (!equal_too) return;
         const int at = atomicAdd(&ties, 1);
-        cand[kCandidates - 1 - at] = key_of(v, j);
+        if (at < kTies) cand[kCandidates - 1 - at] = key_of(v, j);
       } else {
         const int at = atomicAdd(&above, 1);
         if (at < kAbove) cand[at] = key_of(v, j);
       }
     };
-    if (tid < row.head) take(to_f(row.p[tid]), tid, true);
-    __syncthreads();
     const uint4 *body = row.body();
-    for (int64_t i0 = 0; i0 < row.vecs; i0 += kThreads) {
-      const bool equal_too = ties < top_k;
-      __syncthreads();  // all have read ties before any adds to it
-      if (i0 + tid < row.vecs) {
-        float y[kN];
-        Vec<T>::unpack(__ldg(body + i0 + tid), y);
-        bool any = false;
+    auto take_vec = [&](const uint4 &raw, int64_t i) {
+      float y[kN];
+      Vec<T>::unpack(raw, y);
+      bool any = false;
 #pragma unroll
-        for (int e = 0; e < kN; ++e) any = any || !(y[e] < low);
-        if (any) {
+      for (int e = 0; e < kN; ++e) any = any || !(y[e] < low);
+      if (any) {
 #pragma unroll
-          for (int e = 0; e < kN; ++e) take(y[e], row.head + (i0 + tid) * kN + e, equal_too);
-        }
+        for (int e = 0; e < kN; ++e) take(y[e], row.head + i * kN + e);
       }
-      __syncthreads();
+    };
+    if (tid < row.head) take(to_f(row.p[tid]), tid);
+    if (row.tail + tid < V) take(to_f(row.p[row.tail + tid]), row.tail + tid);
+    for (int64_t i = tid; i < row.vecs; i += kUnroll * kThreads) {
+      uint4 raw[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i + u * kThreads < row.vecs) raw[u] = __ldg(body + i + u * kThreads);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i + u * kThreads < row.vecs) take_vec(raw[u], i + u * kThreads);
     }
-    {
-      const bool equal_too = ties < top_k;
+    __syncthreads();
+    if (ties > kTies) {  // (a masked vocabulary, a flat row) keep the first top_k of the equal ones, in index order
+      int found = 0;
       __syncthreads();
-      if (row.tail + tid < V) take(to_f(row.p[row.tail + tid]), row.tail + tid, equal_too);
+      // pieces in order: the head, the body's, the tail; a thread's equal values and how many lie before them
+      const int64_t steps = (row.vecs + kThreads - 1) / kThreads + 2;
+      for (int64_t step = 0; step < steps && found < top_k; ++step) {
+        const bool head = step == 0, tail = step == steps - 1;
+        const int64_t i = (step - 1) * kThreads + tid;
+        int64_t j = head ? tid : tail ? row.tail + tid : row.head + i * kN;
+        uint32_t equal = 0;
+        if (head || tail) {
+          equal = j < (head ? row.head : V) && to_f(row.p[j]) == low;
+        } else if (i < row.vecs) {
+          float y[kN];
+          Vec<T>::unpack(__ldg(body + i), y);
+#pragma unroll
+          for (int e = 0; e < kN; ++e) equal |= static_cast<uint32_t>(y[e] == low) << e;
+        }
+        int before = __popc(equal);
+        const int own = before;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += y;
+        }
+        if (lane == 31) count[warp] = before;
+        __syncthreads();
+        before += found - own;
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) before += count[w];
+          all += count[w];
+        }
+        for (; equal && before < top_k; equal &= equal - 1, ++before)
+          cand[kCandidates - 1 - before] = key_of(low, j + __ffs(equal) - 1);
+        found += all;
+        __syncthreads();
+      }
+      if (tid == 0) ties = min(found, top_k);
       __syncthreads();
     }
     const int na = above, nt = ties, n = na + nt;

@@ -46,43 +46,64 @@ __device__ __forceinline__ int64_t row_of(const PagedArgs &a, int b, int h, int 
 
 }  // namespace pg
 
-// One 16-byte chunk of K and of V a thread.  cu (nullable): token rows
-// [cu[b], cu[b + 1]) belong to sequence b; without it row b is sequence b's
-// one token.  Rows outside every sequence are not written anywhere.
-template <typename T>
+// The append: kTok rows a CTA, whose places the first kTok threads look up; then
+// all threads move 16-byte chunks of K and V, several in flight each.  cu
+// (nullable): token rows [cu[b], cu[b + 1]) belong to sequence b; without it row
+// b is sequence b's one token.  Rows outside every sequence are not written
+// anywhere.
+template <typename T, int kTok>
 __global__ void __launch_bounds__(256)
     paged_append_kernel(PagedArgs a, const int32_t *cu, int64_t N, const T *xk, const T *xv, int64_t k_sn,
                         int64_t k_sh, int64_t v_sn, int64_t v_sh, T *k_pages, T *v_pages) {
-  constexpr int kVec = 16 / sizeof(T), kChunks = 64 / kVec;
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int c = static_cast<int>(e % kChunks) * kVec;
-  const int h = static_cast<int>(e / kChunks % a.Hkv);
-  const int64_t n = e / (kChunks * a.Hkv);
-  if (n >= N) return;
-  int b = static_cast<int>(n);
-  int64_t t = 0;
-  if (cu) {
-    int lo = 0, hi = a.B;  // the last b with cu[b] <= n, if n < cu[b + 1]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (cu[mid] <= n) lo = mid; else hi = mid;
+  constexpr int kVec = 16 / sizeof(T), kChunks = 64 / kVec, kUnroll = 4;
+  __shared__ int64_t place[kTok];  // element offset of the row in the pool, head 0; -1: dropped
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTok;
+  const int rows = static_cast<int>(N - n0 < kTok ? N - n0 : kTok), tid = threadIdx.x;
+  if (tid < rows) {
+    const int64_t n = n0 + tid;
+    int b = static_cast<int>(n);
+    int64_t t = 0, off = -1;
+    bool held = true;
+    if (cu) {
+      int lo = 0, hi = a.B;  // the last b with cu[b] <= n, if n < cu[b + 1]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (cu[mid] <= n) lo = mid; else hi = mid;
+      }
+      b = lo;
+      held = n >= cu[b] && n < cu[b + 1];
+      t = n - cu[b];
     }
-    b = lo;
-    if (n < cu[b] || n >= cu[b + 1]) return;
-    t = n - cu[b];
+    if (held) {
+      t += a.lens[b];
+      if (t >= 0 && t < static_cast<int64_t>(a.width) * a.page) off = pg::row_of(a, b, 0, static_cast<int>(t));
+      if (off < 0) pg::report(a.err, SD_KERR_BOUNDS);
+    }
+    place[tid] = off;
   }
-  t += a.lens[b];
-  if (t < 0 || t >= static_cast<int64_t>(a.width) * a.page) {
-    pg::report(a.err, SD_KERR_BOUNDS);
-    return;
+  __syncthreads();
+  const int chunks = rows * a.Hkv * kChunks;
+  for (int e0 = tid; e0 < chunks; e0 += 256 * kUnroll) {
+    uint4 k[kUnroll], v[kUnroll];
+    int64_t to[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int e = e0 + 256 * u;
+      to[u] = -1;
+      if (e >= chunks) continue;
+      const int c = e % kChunks * kVec, hr = e / kChunks, r = hr / a.Hkv, h = hr - r * a.Hkv;
+      if (place[r] < 0) continue;
+      to[u] = place[r] + h * a.p_sh + c;
+      k[u] = *reinterpret_cast<const uint4 *>(xk + (n0 + r) * k_sn + h * k_sh + c);
+      v[u] = *reinterpret_cast<const uint4 *>(xv + (n0 + r) * v_sn + h * v_sh + c);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (to[u] >= 0) {
+        *reinterpret_cast<uint4 *>(k_pages + to[u]) = k[u];
+        *reinterpret_cast<uint4 *>(v_pages + to[u]) = v[u];
+      }
   }
-  const int64_t off = pg::row_of(a, b, h, static_cast<int>(t));
-  if (off < 0) {
-    pg::report(a.err, SD_KERR_BOUNDS);
-    return;
-  }
-  *reinterpret_cast<uint4 *>(k_pages + off + c) = *reinterpret_cast<const uint4 *>(xk + n * k_sn + h * k_sh + c);
-  *reinterpret_cast<uint4 *>(v_pages + off + c) = *reinterpret_cast<const uint4 *>(xv + n * v_sn + h * v_sh + c);
 }
 
 // ---------------------------------------------------------------- decode
@@ -629,10 +650,13 @@ int sd_paged_append(const void *xk, const void *xv, int dtype, int64_t N, int64_
   if (!aligned16(xk) || !aligned16(xv) || (k_sn * size) % 16 || (k_sh * size) % 16 || (v_sn * size) % 16 ||
       (v_sh * size) % 16)
     return SD_ERR_ALIGN;
-  const int64_t threads = N * Hkv * (64 * size / 16);
-  if ((threads + 255) / 256 > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
+  // a decode step's few rows go to more CTAs
+  const bool many = N >= 32 * 148;
+  const int64_t ctas = many ? (N + 31) / 32 : (N + 3) / 4;
+  if (ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
   SD_DISPATCH_DTYPE(dtype, T, {
-    paged_append_kernel<T><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    auto kern = many ? paged_append_kernel<T, 32> : paged_append_kernel<T, 4>;
+    kern<<<static_cast<unsigned>(ctas), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         a, cu_seqlens, N, static_cast<const T *>(xk), static_cast<const T *>(xv), k_sn, k_sh, v_sn, v_sh,
         static_cast<T *>(k_pages), static_cast<T *>(v_pages));
   });

@@ -94,6 +94,24 @@ def test_ties_and_signed_zeros(dev, dtype):
     assert torch.equal(got.top_ids[3], torch.arange(2, 122, 3, device=dev))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+def test_many_candidates(dev, dtype):
+    """Rows that leave the quick search too much: thousands of equal values at
+    the bound (also all of them: a masked vocabulary), and thousands of large
+    values in a few threads' shares."""
+    x, t = make(dev, dtype, 6, 32003, seed=12)
+    x[0] = 0.25
+    x[1, 7:] = -math.inf
+    x[2, 100:] = -math.inf
+    x[3, ::3] = 9.0
+    x[4].clamp_(max=1.0)
+    piece = torch.arange(32003, device=dev) // (16 // x.element_size())
+    x[5] = x[5] * 0.01 + torch.where(piece % 512 < 200, 5.0, 0.0).to(dtype)
+    for k in (1, 8, 63, 64):
+        same_order(sd.token_logprobs(x, t, top_k=k).top_ids, x, k)
+        same_order(sd.token_logprobs(x[:, 3:], t.clamp(max=100), top_k=k).top_ids, x[:, 3:], k)
+
+
 def grads(x, t, g, ge):
     leaf = x.detach().requires_grad_()
     got = sd.token_logprobs(leaf, t)
