@@ -419,26 +419,28 @@ SD_API int sd_decode_layer_offload(const void *qkv, int dtype, int64_t qkv_sb, c
  * = softmax(scale q k^T over the sequence's tokens up to the query's own) v.
  * Rows outside every sequence: zeros with zero_rest, else left as they are.
  * lse (nullable): fp32 [Hq,total], log2 of each row's sum of exponentials, for
- * the backward.  16-bit inputs run on the tensor cores, fp32 on CUDA cores.
+ * the backward.  rest (nullable, 16-bit types): contiguous [total,Hq,64], what
+ * rounding took from out, for the backward.  16-bit inputs run on the tensor cores, fp32 on CUDA cores.
  * scale > 0. */
 SD_API int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, int64_t total, int64_t Hq,
                                int64_t Hkv, int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
                                int64_t v_st, int64_t v_sh, const int32_t *cu_seqlens, int nseq, float scale,
-                               void *out, int64_t o_st, int64_t o_sh, float *lse, int zero_rest, int32_t *err,
-                               void *stream);
+                               void *out, int64_t o_st, int64_t o_sh, float *lse, void *rest, int zero_rest,
+                               int32_t *err, void *stream);
 
 /* Its gradients for the output gradient dout [total,Hq,64]: dq [total,Hq,64],
  * dk and dv [total,Hkv,64], contiguous, in the inputs' dtype (dk and dv summed
- * over the query heads of their kv head; zeros outside every sequence).  out
- * and lse are the forward's.  delta: workspace of this call, fp32 [Hq*total + 1].
+ * over the query heads of their kv head; zeros outside every sequence).  out,
+ * lse and rest (nullable: dq and dk are then a little less exact) are the
+ * forward's.  delta: workspace of this call, fp32 [Hq*total + 1].
  * Sums have a fixed order: equal inputs give equal bits. */
 SD_API int sd_packed_attention_backward(const void *q, const void *k, const void *v, const void *out,
                                         const void *dout, int dtype, int64_t total, int64_t Hq, int64_t Hkv,
                                         int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
                                         int64_t v_st, int64_t v_sh, int64_t o_st, int64_t o_sh, int64_t g_st,
                                         int64_t g_sh, const int32_t *cu_seqlens, int nseq, float scale,
-                                        const float *lse, float *delta, void *dq, void *dk, void *dv, int32_t *err,
-                                        void *stream);
+                                        const float *lse, const void *rest, float *delta, void *dq, void *dk,
+                                        void *dv, int32_t *err, void *stream);
 
 /* Paged KV append.  k_pages, v_pages: pools of `pages` pages [page][64] per kv
  * head with element strides (p_sp, p_sh, p_st) for (page, head, token), the

@@ -77,12 +77,12 @@ _SIGS = {
                                 _i64, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _c_void_p, _i64, _c_void_p,
                                 _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p],
     "sd_packed_attention": [_c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-                            _i64, _i64, _c_void_p, _i32, _f32, _c_void_p, _i64, _i64, _c_void_p, _i32, _c_void_p,
-                            _c_void_p],
+                            _i64, _i64, _c_void_p, _i32, _f32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i32,
+                            _c_void_p, _c_void_p],
     "sd_packed_attention_backward": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, _i64,
                                      _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p,
                                      _i32, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-                                     _c_void_p],
+                                     _c_void_p, _c_void_p],
     "sd_paged_append": [_c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p,
                         _i64, _i32, _i64, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p, _i32, _c_void_p, _c_void_p,
                         _c_void_p],

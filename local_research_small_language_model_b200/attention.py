@@ -65,16 +65,18 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, scale):
-        out, lse = ops.packed_attention(q, k, v, cu_seqlens, scale, return_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        # 16-bit types: the output's low bits too, for the backward's rowsum(dout * out)
+        rest = None if q.dtype == torch.float32 else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out, lse = ops.packed_attention(q, k, v, cu_seqlens, scale, return_lse=True, rest=rest)
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens, rest)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
-        dq, dk, dv = ops.packed_attention_backward(q, k, v, out, gout, lse, cu_seqlens, ctx.scale)
+        q, k, v, out, lse, cu_seqlens, rest = ctx.saved_tensors
+        dq, dk, dv = ops.packed_attention_backward(q, k, v, out, gout, lse, cu_seqlens, ctx.scale, rest)
         return dq, dk, dv, None, None
 
 

@@ -433,7 +433,7 @@ extern "C" {
 int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, int64_t total, int64_t Hq,
                         int64_t Hkv, int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
                         int64_t v_sh, const int32_t *cu_seqlens, int nseq, float scale, void *out, int64_t o_st,
-                        int64_t o_sh, float *lse, int zero_rest, int32_t *err, void *stream) {
+                        int64_t o_sh, float *lse, void *rest, int zero_rest, int32_t *err, void *stream) {
   using namespace sd;
   PackedArgs a = {};
   a.q = q, a.k = k, a.v = v;
@@ -443,9 +443,10 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
   a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv);
   a.scale = scale, a.scale_log2 = scale * pk::kLog2e;
   a.out = out, a.o_st = o_st, a.o_sh = o_sh;
-  a.lse = lse, a.zero_rest = zero_rest;
+  a.lse = lse, a.rest = rest, a.zero_rest = zero_rest;
   int rc = check_packed(a, dtype, D);
   if (rc != SD_OK) return rc;
+  if (!aligned16(rest)) return SD_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype != SD_DTYPE_F32) return launch_packed_fwd_tc(a, dtype, err, s);
   const size_t smem = 4 * pk::kTileFloats * sizeof(float);
@@ -459,8 +460,8 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
                                  int dtype, int64_t total, int64_t Hq, int64_t Hkv, int64_t D, int64_t q_st,
                                  int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t o_st,
                                  int64_t o_sh, int64_t g_st, int64_t g_sh, const int32_t *cu_seqlens, int nseq,
-                                 float scale, const float *lse, float *delta, void *dq, void *dk, void *dv,
-                                 int32_t *err, void *stream) {
+                                 float scale, const float *lse, const void *rest, float *delta, void *dq, void *dk,
+                                 void *dv, int32_t *err, void *stream) {
   using namespace sd;
   PackedArgs a = {};
   a.q = q, a.k = k, a.v = v;
@@ -470,14 +471,14 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv);
   a.scale = scale, a.scale_log2 = scale * pk::kLog2e;
   a.out = const_cast<void *>(out), a.o_st = o_st, a.o_sh = o_sh;
-  a.lse = const_cast<float *>(lse), a.delta = delta;
+  a.lse = const_cast<float *>(lse), a.rest = const_cast<void *>(rest), a.delta = delta;
   a.dout = dout, a.g_st = g_st, a.g_sh = g_sh;
   a.dq = dq, a.dk = dk, a.dv = dv;
   int rc = check_packed(a, dtype, D);
   if (rc == SD_OK) rc = check_rows(dout, dtype, g_st, g_sh);
   if (rc != SD_OK) return rc;
   if (!lse || !delta || !dq || !dk || !dv) return SD_ERR_INVALID;
-  if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return SD_ERR_ALIGN;
+  if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(rest)) return SD_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype != SD_DTYPE_F32) return launch_packed_bwd_tc(a, dtype, err, s);
   const unsigned slots = static_cast<unsigned>(packed_slots(total, nseq, pk::kTile));

@@ -17,6 +17,7 @@ struct PackedArgs {
   void *out;                            // forward output, row strides o_st, o_sh
   int64_t o_st, o_sh;
   float *lse;                           // [Hq][total] log2 of the row's exponential sum (nullable in the forward)
+  void *rest;                           // nullable, contiguous [total][Hq][64]: what rounding took from out (16-bit)
   int zero_rest;                        // write zeros to the rows outside every sequence
   // backward
   const void *dout;

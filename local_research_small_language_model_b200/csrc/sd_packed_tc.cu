@@ -164,8 +164,10 @@ __device__ __forceinline__ void clear_rows(char *tile, int first, int rows) {
   __syncwarp();
 }
 
-// 64 fp32 values of one row, scaled, to 16-bit memory.
-template <typename T> __device__ __forceinline__ void store_row(T *dst, uint32_t taddr, float scale, bool write) {
+// 64 fp32 values of one row, scaled, to 16-bit memory; with `rest` also what the
+// rounding took from them.
+template <typename T>
+__device__ __forceinline__ void store_row(T *dst, uint32_t taddr, float scale, bool write, T *rest = nullptr) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float v[32];
@@ -173,10 +175,20 @@ template <typename T> __device__ __forceinline__ void store_row(T *dst, uint32_t
     tmem_wait_ld();
     if (!write) continue;
 #pragma unroll
-    for (int c = 0; c < 32; c += 8)
-      *reinterpret_cast<uint4 *>(dst + 32 * h + c) =
-          make_uint4(pack2<T>(v[c] * scale, v[c + 1] * scale), pack2<T>(v[c + 2] * scale, v[c + 3] * scale),
-                     pack2<T>(v[c + 4] * scale, v[c + 5] * scale), pack2<T>(v[c + 6] * scale, v[c + 7] * scale));
+    for (int c = 0; c < 32; c += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c + e] *= scale;
+      *reinterpret_cast<uint4 *>(dst + 32 * h + c) = make_uint4(
+          pack2<T>(v[c], v[c + 1]), pack2<T>(v[c + 2], v[c + 3]), pack2<T>(v[c + 4], v[c + 5]),
+          pack2<T>(v[c + 6], v[c + 7]));
+      if (rest) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[c + e] -= round_to<T>(v[c + e]);
+        *reinterpret_cast<uint4 *>(rest + 32 * h + c) = make_uint4(
+            pack2<T>(v[c], v[c + 1]), pack2<T>(v[c + 2], v[c + 3]), pack2<T>(v[c + 4], v[c + 5]),
+            pack2<T>(v[c + 6], v[c + 7]));
+      }
+    }
   }
 }
 
@@ -420,7 +432,8 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
   if (warp < 8 && (x == 0 || n1 > 0)) {
     const int row = x * kRows + r;
     fence_after_sync();
-    store_row(out + row * a.o_st, tmem + lane_base + kFwdO + 64 * x, 1.0f / l, row < rows);
+    T *rest = a.rest ? static_cast<T *>(a.rest) + ((first + row) * a.Hq + h) * 64 : nullptr;
+    store_row(out + row * a.o_st, tmem + lane_base + kFwdO + 64 * x, 1.0f / l, row < rows, rest);
     if (row < rows && a.lse) a.lse[h * a.total + first + row] = m + log2f(l);
   }
   fence_before_sync();
@@ -626,6 +639,13 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
         for (int u = 0; u < 8; ++u) {
           delta = fmaf(to_f(po[u]), to_f(pg[u]), delta);
           if (kHalf) big = fmaxf(big, fabsf(to_f(pg[u])));
+        }
+        if (a.rest) {  // out in twice its bits: delta's error is the same for a whole row of dS, and would add up
+          const uint4 z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.rest) +
+                                                           ((first + r) * a.Hq + h) * 64 + 8 * e);
+          const T *pz = reinterpret_cast<const T *>(&z);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) delta = fmaf(to_f(pz[u]), to_f(pg[u]), delta);
         }
       }
       a.delta[h * a.total + first + r] = delta;

@@ -728,15 +728,16 @@ def _check_packed(q, k, v, cu_seqlens, **like_q):
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-                     return_lse: bool = False):
+                     return_lse: bool = False, rest: Optional[torch.Tensor] = None):
     """Causal GQA attention over sequences packed back to back
     (sd_packed_attention).  q [total,Hq,64], k, v [total,Hkv,64] (any strides);
     sequence s holds rows cu_seqlens[s] .. cu_seqlens[s+1]-1 (device int32).
     Returns [total,Hq,64]; rows outside every sequence are zero, or left as
     they are in a caller's ``out``.  With ``return_lse`` also the fp32 [Hq,total]
-    the backward needs."""
-    _check_packed(q, k, v, cu_seqlens, out=out)
-    dev = _device(q, k, v, cu_seqlens, out)
+    the backward needs.  ``rest`` (16-bit types, contiguous, like out) receives
+    what rounding took from the output, for a more exact backward."""
+    _check_packed(q, k, v, cu_seqlens, out=out, rest=rest)
+    dev = _device(q, k, v, cu_seqlens, out, rest)
     total, hq, d = q.shape
     sc = _scale(scale, d)
     cu = cu_seqlens
@@ -748,28 +749,33 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         out = q.new_empty((total, hq, d))
     elif _rows16(out) is not out:
         raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
+    if rest is not None and not rest.is_contiguous():
+        raise ValueError("rest must be contiguous")
     lse = torch.empty(hq, total, dtype=torch.float32, device=q.device) if return_lse else None
     if total:
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
         _launch("sd_packed_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, total, hq, k.shape[1], d,
                 *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, sc,
-                out.data_ptr(), *out.stride()[:2], lse.data_ptr() if return_lse else None, zero, _err_ptr(dev))
+                out.data_ptr(), *out.stride()[:2], lse.data_ptr() if return_lse else None,
+                rest.data_ptr() if rest is not None else None, zero, _err_ptr(dev))
     return (out, lse) if return_lse else out
 
 
 def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                               dout: torch.Tensor, lse: torch.Tensor, cu_seqlens: torch.Tensor,
-                              scale: Optional[float] = None
+                              scale: Optional[float] = None, rest: Optional[torch.Tensor] = None
                               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv, contiguous, in q's dtype) of packed_attention for
-    the output gradient dout; out and lse are the forward's
+    the output gradient dout; out, lse and rest (optional) are the forward's
     (sd_packed_attention_backward).  Equal inputs give equal bits."""
-    _check_packed(q, k, v, cu_seqlens, out=out, dout=dout)
-    dev = _device(q, k, v, out, dout, lse, cu_seqlens)
+    _check_packed(q, k, v, cu_seqlens, out=out, dout=dout, rest=rest)
+    dev = _device(q, k, v, out, dout, lse, cu_seqlens, rest)
     total, hq, d = q.shape
     hkv = k.shape[1]
     if lse.shape != (hq, total) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError(f"lse must be the forward's fp32 [{hq}, {total}], got {tuple(lse.shape)} of {lse.dtype}")
+    if rest is not None and not rest.is_contiguous():
+        raise ValueError("rest must be contiguous")
     sc = _scale(scale, d)
     cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape)
     code = dtype_code(q)
@@ -782,7 +788,7 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         _launch("sd_packed_attention_backward", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                 dout.data_ptr(), code, total, hq, hkv, d, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
                 *out.stride()[:2], *dout.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, sc, lse.data_ptr(),
-                delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _err_ptr(dev))
+                rest.data_ptr() if rest is not None else None, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _err_ptr(dev))
     return dq, dk, dv
 
 

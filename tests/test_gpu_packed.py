@@ -137,6 +137,15 @@ def test_packed_attention_and_gradients(dev, dtype, heads, name):
     val, err = exact(q, k, v, dout, cu, 0.125)
     for x, y in zip(("out", "dq", "dk", "dv"), got):
         check(y, val[x], err[x], x)
+    # the output's low bits: out and rest together are nearer (the weights' rounding remains); without them the
+    # gradients hold the same bounds
+    rest = torch.empty(q.shape, dtype=dtype, device=dev) if dtype != torch.float32 else None
+    out, lse = ops.packed_attention(q, k, v, dcu, return_lse=True, rest=rest)
+    assert torch.equal(out, got[0])
+    if rest is not None:
+        check(out.double() + rest.double(), val["out"], err["out"] - U[dtype] * val["out"].abs() * 0.9, "out + rest")
+        for x, y in zip(("dq", "dk", "dv"), ops.packed_attention_backward(q, k, v, out, dout, lse, dcu)):
+            check(y, val[x], err[x], x + " without rest")
     # without autograd, and again: the same bits
     assert torch.equal(sd.packed_attention(q, k, v, dcu), got[0])
     for x, y in zip(got, run(q, k, v, dout, dcu)):

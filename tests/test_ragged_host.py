@@ -17,7 +17,7 @@ INVALID, UNSUPPORTED, ALIGN = -1, -2, -4
 
 def packed(lib, **kw):
     a = dict(q=P, k=P, v=P, dtype=1, total=10, hq=4, hkv=2, d=64, q_st=256, q_sh=64, k_st=128, k_sh=64, v_st=128,
-             v_sh=64, cu=P, nseq=1, scale=0.125, out=P, o_st=256, o_sh=64, lse=P, zero=1)
+             v_sh=64, cu=P, nseq=1, scale=0.125, out=P, o_st=256, o_sh=64, lse=P, rest=P, zero=1)
     a.update(kw)
     return lib.sd_packed_attention(*a.values(), None, None)
 
@@ -25,7 +25,7 @@ def packed(lib, **kw):
 def backward(lib, **kw):
     a = dict(q=P, k=P, v=P, out=P, dout=P, dtype=1, total=10, hq=4, hkv=2, d=64, q_st=256, q_sh=64, k_st=128,
              k_sh=64, v_st=128, v_sh=64, o_st=256, o_sh=64, g_st=256, g_sh=64, cu=P, nseq=1, scale=0.125, lse=P,
-             delta=P, dq=P, dk=P, dv=P)
+             rest=P, delta=P, dq=P, dk=P, dv=P)
     a.update(kw)
     return lib.sd_packed_attention_backward(*a.values(), None, None)
 
@@ -64,7 +64,7 @@ REFUSED = [
     (packed, dict(scale=float("nan")), INVALID), (packed, dict(scale=float("inf")), INVALID),
     (packed, dict(nseq=-1), INVALID), (packed, dict(d=128), UNSUPPORTED), (packed, dict(hq=131072), UNSUPPORTED),
     (packed, dict(total=2 ** 31), UNSUPPORTED), (packed, dict(k=ODD), ALIGN), (packed, dict(v_st=129), ALIGN),
-    (packed, dict(o_sh=60), ALIGN),
+    (packed, dict(o_sh=60), ALIGN), (packed, dict(rest=ODD), ALIGN), (backward, dict(rest=ODD), ALIGN),
     (backward, dict(dout=None), INVALID), (backward, dict(lse=None), INVALID), (backward, dict(delta=None), INVALID),
     (backward, dict(dk=None), INVALID), (backward, dict(dv=ODD), ALIGN), (backward, dict(g_st=4), ALIGN),
     (backward, dict(d=32), UNSUPPORTED),
