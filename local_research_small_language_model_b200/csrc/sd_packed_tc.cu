@@ -58,7 +58,7 @@ constexpr int kTileBytes = kRows * 128;
 constexpr float kMostSum = 16384.f;          // of a block's weights against a row's reference
 
 struct FwdBars {
-  uint64_t full[kStages], empty[kStages], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full, full[kStages], empty[kStages], s_full[2], p_full[2], o_full[2];
   uint32_t tmem;
 };
 
@@ -164,30 +164,41 @@ __device__ __forceinline__ void clear_rows(char *tile, int first, int rows) {
   __syncwarp();
 }
 
-// 64 fp32 values of one row, scaled, to 16-bit memory; with `rest` also what the
-// rounding took from them.
+// A warp's 32 accumulator rows of 64 values, scaled, to 16-bit rows `stride`
+// apart, the first `rows` of them; with `rest` also what the rounding took from
+// them.  Through 4 KB of the warp's own shared memory, so that eight lanes write
+// a row's 128 bytes together.
 template <typename T>
-__device__ __forceinline__ void store_row(T *dst, uint32_t taddr, float scale, bool write, T *rest = nullptr) {
+__device__ __forceinline__ void store_rows(T *dst, int64_t stride, int rows, uint32_t taddr, float scale, char *sm,
+                                           T *rest = nullptr, int64_t rest_stride = 0) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int pass = 0; pass < (rest == nullptr ? 1 : 2); ++pass) {
+    __syncwarp();
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float v[32];
-    tmem_ld32(taddr + 32 * h, v);
-    tmem_wait_ld();
-    if (!write) continue;
+    for (int h = 0; h < 2; ++h) {
+      float v[32];
+      tmem_ld32(taddr + 32 * h, v);
+      tmem_wait_ld();
 #pragma unroll
-    for (int c = 0; c < 32; c += 8) {
+      for (int c = 0; c < 32; c += 8) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[c + e] *= scale;
-      *reinterpret_cast<uint4 *>(dst + 32 * h + c) = make_uint4(
-          pack2<T>(v[c], v[c + 1]), pack2<T>(v[c + 2], v[c + 3]), pack2<T>(v[c + 4], v[c + 5]),
-          pack2<T>(v[c + 6], v[c + 7]));
-      if (rest) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[c + e] -= round_to<T>(v[c + e]);
-        *reinterpret_cast<uint4 *>(rest + 32 * h + c) = make_uint4(
+        for (int e = 0; e < 8; ++e) {
+          v[c + e] *= scale;
+          if (pass == 1) v[c + e] -= round_to<T>(v[c + e]);
+        }
+        *reinterpret_cast<uint4 *>(sm + sw128(lane, 4 * h + (c >> 3))) = make_uint4(
             pack2<T>(v[c], v[c + 1]), pack2<T>(v[c + 2], v[c + 3]), pack2<T>(v[c + 4], v[c + 5]),
             pack2<T>(v[c + 6], v[c + 7]));
       }
+    }
+    __syncwarp();
+    T *to = pass == 0 ? dst : rest;
+    const int64_t st = pass == 0 ? stride : rest_stride;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3), c = lane & 7;
+      if (r < rows) *reinterpret_cast<uint4 *>(to + r * st + 8 * c) = *reinterpret_cast<const uint4 *>(sm + sw128(r, c));
     }
   }
 }
@@ -206,8 +217,9 @@ template <typename T> __device__ __forceinline__ void zero_rows(T *dst, int64_t 
 
 template <typename T>
 __global__ void __launch_bounds__(pt::kFwdThreads, 2)
-    packed_fwd_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmk,
-                         const __grid_constant__ CUtensorMap tmv, int32_t *err) {
+    packed_fwd_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
+                         const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                         int32_t *err) {
   using namespace pt;
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   // heads fastest; the tiles that see the most keys first
@@ -233,6 +245,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
   const int blocks = max(n0, n1);
   if (warp == 8) tmem_alloc(&bars->tmem, kFwdCols);
   if (tid == 288) {
+    mbar_init(&bars->q_full, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
@@ -259,26 +272,15 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
     tma_load_4d(sm + FwdSmem::kK + s * kBlockBytes, &tmk, 0, row, hk, 0, &bars->full[s]);
     tma_load_4d(sm + FwdSmem::kV + s * kBlockBytes, &tmv, 0, row, hk, 0, &bars->full[s]);
   };
-  if (warp == 9 && lane == 0)
-    for (int i = 0; i < min(blocks, kStages); ++i) load(i);
-  if (warp < 8 && (x == 0 || n1 > 0)) {
-    // this thread's row of Q, swizzled as the copies swizzle (zeros behind the sequence)
-    const T *src = static_cast<const T *>(a.q) + (first + x * kRows + r) * a.q_st + h * a.q_sh;
-    const bool held = x * kRows + r < rows;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      *reinterpret_cast<uint4 *>(sm + FwdSmem::kQ + x * kTileBytes + sw128(r, e)) =
-          held ? *reinterpret_cast<const uint4 *>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
-    fence_async_smem();
-  }
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
-
   if (warp == 9) {
     if (lane == 0) {
-      for (int i = kStages; i < blocks; ++i) {
-        ok = mbar_wait(&bars->empty[i % kStages], (i / kStages - 1) & 1);
+      // Q rows behind the sequence are others' (their results go nowhere)
+      mbar_arrive_expect_tx(&bars->q_full, (n1 > 0 ? 2 : 1) * kTileBytes);
+      for (int i = 0; i < (n1 > 0 ? 4 : 2); ++i)
+        tma_load_4d(sm + FwdSmem::kQ + i * kBlockBytes, &tmq, 0, static_cast<int>(first) + i * kBlock, h, 0,
+                    &bars->q_full);
+      for (int i = 0; i < blocks; ++i) {
+        if (i >= kStages) ok = mbar_wait(&bars->empty[i % kStages], (i / kStages - 1) & 1);
         if (!ok) break;
         load(i);
       }
@@ -303,6 +305,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
       }
       __syncwarp();
     };
+    ok = mbar_wait(&bars->q_full, 0);
     issue_s(0, 0);
     if (u1 > 0) issue_s(1, 0);
     const int tail = shared_value(t.len) / kBlock;  // the block that holds the sequence's end, if it ends inside one
@@ -333,6 +336,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
     }
   } else {
     const int n = x ? n1 : n0, row = t.row0 + x * kRows + r;
+    const bool held = x * kRows + r < rows;  // the others' sums move no reference
     const uint32_t t_s = tmem + lane_base + 64 * x, t_o = tmem + lane_base + kFwdO + 64 * x;
     const float c = a.scale_log2;
     for (int i = 0; i < n; ++i) {
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
         // masked and first blocks, and what the polynomial's range does not hold (a NaN, an infinity, a weight
         // past 2^127: the sum tells), take the special-function unit for all
         sum = raise || edge ? weights(std::false_type()) : weights(std::true_type());
-        if (raise || !__any_sync(0xffffffffu, !(sum <= kMostSum))) break;
+        if (raise || !__any_sync(0xffffffffu, held && !(sum <= kMostSum))) break;
         raise = true;
       }
       l += sum;
@@ -424,16 +428,20 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
   }
   const bool failed = __syncthreads_or(!ok);
   if (failed) {  // a bounded wait expired: let copies in flight land, poison the rows
-    if (tid == 288)
+    if (tid == 288) {
+      mbar_wait(&bars->q_full, 0, 1000000ull);
       for (int s = 0; s < kStages; ++s) mbar_wait(&bars->full[s], 0, 1000000ull);
+    }
     l = __int_as_float(0x7fc00000);
     if (tid == 0 && err) *err = SD_KERR_TIMEOUT;
   }
   if (warp < 8 && (x == 0 || n1 > 0)) {
-    const int row = x * kRows + r;
     fence_after_sync();
-    T *rest = a.rest ? static_cast<T *>(a.rest) + ((first + row) * a.Hq + h) * 64 : nullptr;
-    store_row(out + row * a.o_st, tmem + lane_base + kFwdO + 64 * x, 1.0f / l, row < rows, rest);
+    const int row0 = 32 * warp, row = row0 + lane;  // of the CTA's rows
+    T *rest = a.rest ? static_cast<T *>(a.rest) + ((first + row0) * a.Hq + h) * 64 : nullptr;
+    // the tile's own Q is read no more
+    store_rows(out + row0 * a.o_st, a.o_st, rows - row0, tmem + lane_base + kFwdO + 64 * x, 1.0f / l,
+               sm + FwdSmem::kQ + warp * 4096, rest, static_cast<int64_t>(a.Hq) * 64);
     if (row < rows && a.lse) a.lse[h * a.total + first + row] = m + log2f(l);
   }
   fence_before_sync();
@@ -626,37 +634,47 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (tid == 32 * kBwdCopy) bwd_init(bars);
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  if (warp < 4) {  // delta, and for fp16 the largest |dout|, of row r
-    float delta = 0.f, big = 0.f;
-    if (r < rows) {
-      const T *o = static_cast<const T *>(a.out) + (first + r) * a.o_st + h * a.o_sh;
-      const T *g = static_cast<const T *>(a.dout) + (first + r) * a.g_st + h * a.g_sh;
+  if (warp < 16) {  // delta, and for fp16 the largest |dout|: eight lanes a row, eight rows a warp
+    float delta[2], big[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(o + 8 * e), y = *reinterpret_cast<const uint4 *>(g + 8 * e);
-        const T *po = reinterpret_cast<const T *>(&x), *pg = reinterpret_cast<const T *>(&y);
+    for (int i = 0; i < 2; ++i) {
+      const int row = 8 * warp + 4 * i + (lane >> 3), c = 8 * (lane & 7);
+      delta[i] = big[i] = 0.f;
+      if (row < rows) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.out) + (first + row) * a.o_st +
+                                                         h * a.o_sh + c);
+        const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.dout) + (first + row) * a.g_st +
+                                                         h * a.g_sh + c);
+        uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        // out in twice its bits: delta's error is the same for a whole row of dS, and would add up
+        if (a.rest)
+          z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.rest) + ((first + row) * a.Hq + h) * 64 + c);
+        const T *po = reinterpret_cast<const T *>(&x), *pg = reinterpret_cast<const T *>(&y),
+                *pz = reinterpret_cast<const T *>(&z);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          delta = fmaf(to_f(po[u]), to_f(pg[u]), delta);
-          if (kHalf) big = fmaxf(big, fabsf(to_f(pg[u])));
-        }
-        if (a.rest) {  // out in twice its bits: delta's error is the same for a whole row of dS, and would add up
-          const uint4 z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.rest) +
-                                                           ((first + r) * a.Hq + h) * 64 + 8 * e);
-          const T *pz = reinterpret_cast<const T *>(&z);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) delta = fmaf(to_f(pz[u]), to_f(pg[u]), delta);
+          delta[i] = fmaf(to_f(po[u]), to_f(pg[u]), delta[i]);
+          delta[i] = fmaf(to_f(pz[u]), to_f(pg[u]), delta[i]);
+          if (kHalf) big[i] = fmaxf(big[i], fabsf(to_f(pg[u])));
         }
       }
-      a.delta[h * a.total + first + r] = delta;
-    }
-    vec[r] = delta;
-    if (kHalf) {
-      big = big < INFINITY ? big : 0.f;
-      vec[128 + r] = big;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-      if (lane == 0) atomicMax(top, __float_as_uint(big));
+      for (int o = 4; o > 0; o >>= 1) {
+        delta[i] += __shfl_xor_sync(0xffffffffu, delta[i], o);
+        if (kHalf) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], o));
+      }
+      if (kHalf && !(big[i] < INFINITY)) big[i] = 0.f;
+      if ((lane & 7) == 0) {
+        vec[row] = delta[i];
+        if (row < rows) a.delta[h * a.total + first + row] = delta[i];
+        if (kHalf) vec[128 + row] = big[i];
+      }
+    }
+    if (kHalf) {
+      float most = fmaxf(big[0], big[1]);
+#pragma unroll
+      for (int o = 16; o >= 8; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (lane == 0) atomicMax(top, __float_as_uint(most));
     }
   }
   fence_before_sync();
@@ -732,7 +750,8 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (warp < 4) {
     fence_after_sync();
     const float back = failed ? __int_as_float(0x7fc00000) : a.scale / (kHalf ? unit_scale(vec[128 + r]) : 1.f);
-    store_row(dq + r * c_st, tmem + lane_base + kDqAcc, back, r < rows);
+    store_rows(dq + 32 * warp * c_st, c_st, rows - 32 * warp, tmem + lane_base + kDqAcc, back,
+               sm + BwdSmem::kRowsA + warp * 4096);
   }
   fence_before_sync();
   __syncthreads();
@@ -881,7 +900,9 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (warp < 8) {
     fence_after_sync();
     const float back = failed ? __int_as_float(0x7fc00000) : wg == 0 ? 1.f : a.scale / f;
-    store_row((wg == 0 ? dv : dk) + r * c_st, tmem + lane_base + (wg == 0 ? kDkvAcc : kDkvAcc2), back, r < keys);
+    const int row0 = 32 * (warp & 3);
+    store_rows((wg == 0 ? dv : dk) + row0 * c_st, c_st, keys - row0,
+               tmem + lane_base + (wg == 0 ? kDkvAcc : kDkvAcc2), back, sm + BwdSmem::kRowsA + warp * 4096);
   }
   fence_before_sync();
   __syncthreads();
@@ -900,8 +921,9 @@ static int packed_map(CUtensorMap *map, const void *p, int dtype, int64_t total,
 }
 
 int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s) {
-  CUtensorMap mk, mv;
-  int rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kBlock);
+  CUtensorMap mq, mk, mv;
+  int rc = packed_map(&mq, a.q, dtype, a.total, a.Hq, a.q_st, a.q_sh, pt::kBlock);
+  if (rc == SD_OK) rc = packed_map(&mk, a.k, dtype, a.total, a.Hkv, a.k_st, a.k_sh, pt::kBlock);
   if (rc == SD_OK) rc = packed_map(&mv, a.v, dtype, a.total, a.Hkv, a.v_st, a.v_sh, pt::kBlock);
   if (rc != SD_OK) return rc;
   const int64_t ctas = packed_slots(a.total, a.S, 2 * pt::kRows) * a.Hq;
@@ -909,7 +931,7 @@ int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
   const size_t smem = pt::FwdSmem::kBytes + 1024;
   auto run = [&](auto *kern) {
     if (ensure_smem(kern, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
-    kern<<<static_cast<unsigned>(ctas), pt::kFwdThreads, smem, s>>>(a, mk, mv, err);
+    kern<<<static_cast<unsigned>(ctas), pt::kFwdThreads, smem, s>>>(a, mq, mk, mv, err);
     return check_launch();
   };
   return dtype == SD_DTYPE_BF16 ? run(packed_fwd_tc_kernel<__nv_bfloat16>) : run(packed_fwd_tc_kernel<__half>);
