@@ -843,50 +843,61 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
       ok = mbar_wait(&bars->sd_full, i & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
-      float s[32], d[32];
-      tmem_ld32(t_s, s);
-      tmem_ld32(t_s + kColDp, d);
-      tmem_wait_ld();
-      warp_arrive(&bars->sd_free);
-      auto weights = [&](auto poly) {
-#pragma unroll
-        for (int u = 0; u < 32; u += 4) {
-          const float4 l4 = *reinterpret_cast<const float4 *>(mine + u);
-          const float4 d4 = *reinterpret_cast<const float4 *>(mine + 32 + u);
-          fma2v(s[u], s[u + 1], a.scale_log2, l4.x, l4.y);
-          fma2v(s[u + 2], s[u + 3], a.scale_log2, l4.z, l4.w);
-          add2(d[u], d[u + 1], d4.x, d4.y);
-          add2(d[u + 2], d[u + 3], d4.z, d4.w);
-          s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
-          if (decltype(poly)::value && u % 8 == 4)
-            exp2_fma<false>(s[u + 2], s[u + 3]);
-          else
-            s[u + 2] = ex2(s[u + 2]), s[u + 3] = ex2(s[u + 3]);
-          if (kHalf) {
-            mul2(d[u], d[u + 1], f, f);
-            mul2(d[u + 2], d[u + 3], f, f);
-          }
-          mul2(d[u], d[u + 1], s[u], s[u + 1]);
-          mul2(d[u + 2], d[u + 3], s[u + 2], s[u + 3]);
-        }
-      };
       const int from = r - q0 - 32 * wg, to = span - q0;  // visible columns: from .. to - 1
-      if (q0 > 0 && to >= 32 && !nan) {
-        weights(std::true_type());
-      } else {
-        weights(std::false_type());
+      const bool plain = q0 > 0 && to >= 32 && !nan;
+      // 16 columns at a time: the two weights' 32-bit halves take over the scores' registers
+      float wp[16], wd[16];
 #pragma unroll
-        for (int u = 0; u < 32; ++u) {
-          const bool seen = u >= from && u < to;
-          s[u] = seen ? s[u] : 0.f;
-          d[u] = seen ? d[u] : 0.f;
+      for (int half = 0; half < 2; ++half) {
+        float s[16], d[16];
+        tmem_ld16(t_s + 16 * half, s);
+        tmem_ld16(t_s + kColDp + 16 * half, d);
+        tmem_wait_ld();
+        if (half == 1) warp_arrive(&bars->sd_free);
+        auto weights = [&](auto poly) {
+#pragma unroll
+          for (int u = 0; u < 16; u += 4) {
+            const float4 l4 = *reinterpret_cast<const float4 *>(mine + 16 * half + u);
+            const float4 d4 = *reinterpret_cast<const float4 *>(mine + 32 + 16 * half + u);
+            fma2v(s[u], s[u + 1], a.scale_log2, l4.x, l4.y);
+            fma2v(s[u + 2], s[u + 3], a.scale_log2, l4.z, l4.w);
+            add2(d[u], d[u + 1], d4.x, d4.y);
+            add2(d[u + 2], d[u + 3], d4.z, d4.w);
+            s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
+            if (decltype(poly)::value && u % 8 == 4)
+              exp2_fma<false>(s[u + 2], s[u + 3]);
+            else
+              s[u + 2] = ex2(s[u + 2]), s[u + 3] = ex2(s[u + 3]);
+            if (kHalf) {
+              mul2(d[u], d[u + 1], f, f);
+              mul2(d[u + 2], d[u + 3], f, f);
+            }
+            mul2(d[u], d[u + 1], s[u], s[u + 1]);
+            mul2(d[u + 2], d[u + 3], s[u + 2], s[u + 3]);
+          }
+        };
+        if (plain) {
+          weights(std::true_type());
+        } else {
+          weights(std::false_type());
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            const bool seen = 16 * half + u >= from && 16 * half + u < to;
+            s[u] = seen ? s[u] : 0.f;
+            d[u] = seen ? d[u] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          wp[8 * half + u] = __uint_as_float(pack2<T>(s[2 * u], s[2 * u + 1]));
+          wd[8 * half + u] = __uint_as_float(pack2<T>(d[2 * u], d[2 * u + 1]));
         }
       }
       if (i > 0) ok = mbar_wait(&bars->w_free, (i - 1) & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
-      store_weights<T>(tmem + lane_base + kColW + 16 * wg, s);
-      store_weights<T>(tmem + lane_base + kColW2 + 16 * wg, d);
+      tmem_st16(tmem + lane_base + kColW + 16 * wg, wp);
+      tmem_st16(tmem + lane_base + kColW2 + 16 * wg, wd);
       tmem_wait_st();
       warp_arrive(&bars->w_full);
     }
