@@ -640,18 +640,18 @@ def swiglu_weight(w_gate: torch.Tensor, w_up: torch.Tensor) -> torch.Tensor:
 _err_ptrs = {}
 
 
-def _device(*ts) -> int:
+def _device(first, *ts) -> int:
     """The one CUDA device index of the tensors (None is skipped)."""
-    dev = -1
+    dev = first.get_device()
     for t in ts:
-        if t is not None:
-            i = t.get_device()
-            if i < 0:
-                raise ValueError("the B200 kernels need CUDA tensors (this library has no CPU path)")
-            if dev < 0:
-                dev = i
-            elif dev != i:
-                raise ValueError(f"tensors on cuda:{dev} and cuda:{i}: one call needs one device")
+        if t is not None and t.get_device() != dev:
+            other = t.get_device()
+            if dev >= 0 and other >= 0:
+                raise ValueError(f"tensors on cuda:{dev} and cuda:{other}: one call needs one device")
+            dev = -1
+            break
+    if dev < 0:
+        raise ValueError("the B200 kernels need CUDA tensors (this library has no CPU path)")
     return dev
 
 
@@ -662,11 +662,16 @@ def _err_ptr(dev: int) -> int:
     return ptr
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(L.load(), name)
+
+
 def _launch(name: str, dev: int, *args) -> None:
     """L.call on the current stream of device ``dev``, which a launch needs as
     the current device."""
     if torch._C._cuda_getDevice() == dev:
-        code = getattr(L.load(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+        code = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
         if code != L.SD_OK:
             L.check(name, code)
         return
@@ -682,18 +687,31 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
         st = t.stride()
         if len(st) == 3 and st[2] == 1 and not (st[0] | st[1]) & 7 and st[0] > 0 and st[1] > 0:
             return t
+        if t.is_contiguous():
+            return t
         whole = 16 // t.element_size() - 1
         if st[-1] == 1 and not any(s & whole for s in st[:-1]) and all(s > 0 or n == 1 for s, n in zip(st, t.shape)):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _index32(name: str, t: torch.Tensor, shape) -> torch.Tensor:
-    if t.shape != shape or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must be {list(shape)} of int32, got {tuple(t.shape)} of {t.dtype}")
+def _index32(name: str, t: torch.Tensor, rows: int) -> torch.Tensor:
+    """A vector (rows values) of int32 for a kernel."""
+    if t.dtype is torch.int32 and t.shape == (rows,) and (t.stride(0) == 1 or rows == 1):
+        return t
+    if t.shape != (rows,) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be [{rows}] of int32, got {tuple(t.shape)} of {t.dtype}")
+    return t.to(torch.int32).contiguous()
+
+
+def _table32(t: torch.Tensor, rows: int) -> torch.Tensor:
+    """A page table [rows, width >= 1] of int32 for a kernel."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or not shape[1] or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"page_table must be [{rows}, width] of int32, got {tuple(shape)} of {t.dtype}")
     if t.dtype is not torch.int32:
         t = t.to(torch.int32)
-    return t if t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
 def _scale(scale: Optional[float], d: int) -> float:
@@ -704,7 +722,7 @@ def _scale(scale: Optional[float], d: int) -> float:
     return float(scale)
 
 
-def _check_packed(q, k, v, cu_seqlens, **like_q):
+def _check_packed(q, k, v, cu_seqlens):
     qs, ks = q.shape, k.shape
     if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError(f"q must be [total, Hq, D] and k, v [total, Hkv, D], got {tuple(qs)}, {tuple(ks)}, "
@@ -715,12 +733,15 @@ def _check_packed(q, k, v, cu_seqlens, **like_q):
         raise ValueError(f"query heads ({qs[1]}) must be a multiple of kv heads ({ks[1]})")
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
         raise ValueError(f"cu_seqlens must hold a bound more than there are sequences, got {tuple(cu_seqlens.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError(f"q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    for name, t in like_q.items():
+
+
+def _check_like_q(q, **ts):
+    for name, t in ts.items():
         if t is None:
             continue
-        if t.dtype != q.dtype:
+        if t.dtype is not q.dtype:
             raise TypeError(f"{name} must have q's dtype {q.dtype}, got {t.dtype}")
         if t.shape != q.shape:
             raise ValueError(f"{name} must have q's shape {tuple(q.shape)}, got {tuple(t.shape)}")
@@ -736,17 +757,17 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     they are in a caller's ``out``.  With ``return_lse`` also the fp32 [Hq,total]
     the backward needs.  ``rest`` (16-bit types, contiguous, like out) receives
     what rounding took from the output, for a more exact backward."""
-    _check_packed(q, k, v, cu_seqlens, out=out, rest=rest)
+    _check_packed(q, k, v, cu_seqlens)
+    if out is not None or rest is not None:
+        _check_like_q(q, out=out, rest=rest)
     dev = _device(q, k, v, cu_seqlens, out, rest)
     total, hq, d = q.shape
     sc = _scale(scale, d)
-    cu = cu_seqlens
-    if cu.dtype is not torch.int32 or cu.stride(0) != 1:
-        cu = _index32("cu_seqlens", cu, cu.shape)
+    cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape[0])
     code = dtype_code(q)
     zero = out is None
     if zero:
-        out = q.new_empty((total, hq, d))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif _rows16(out) is not out:
         raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
     if rest is not None and not rest.is_contiguous():
@@ -754,9 +775,13 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     lse = torch.empty(hq, total, dtype=torch.float32, device=q.device) if return_lse else None
     if total:
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        q_st, q_sh, _ = q.stride()
+        k_st, k_sh, _ = k.stride()
+        v_st, v_sh, _ = v.stride()
+        o_st, o_sh, _ = out.stride()
         _launch("sd_packed_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, total, hq, k.shape[1], d,
-                *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, sc,
-                out.data_ptr(), *out.stride()[:2], lse.data_ptr() if return_lse else None,
+                q_st, q_sh, k_st, k_sh, v_st, v_sh, cu.data_ptr(), cu.shape[0] - 1, sc, out.data_ptr(), o_st, o_sh,
+                lse.data_ptr() if return_lse else None,
                 rest.data_ptr() if rest is not None else None, zero, _err_ptr(dev))
     return (out, lse) if return_lse else out
 
@@ -768,7 +793,8 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """Gradients (dq, dk, dv, contiguous, in q's dtype) of packed_attention for
     the output gradient dout; out, lse and rest (optional) are the forward's
     (sd_packed_attention_backward).  Equal inputs give equal bits."""
-    _check_packed(q, k, v, cu_seqlens, out=out, dout=dout, rest=rest)
+    _check_packed(q, k, v, cu_seqlens)
+    _check_like_q(q, out=out, dout=dout, rest=rest)
     dev = _device(q, k, v, out, dout, lse, cu_seqlens, rest)
     total, hq, d = q.shape
     hkv = k.shape[1]
@@ -777,7 +803,7 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if rest is not None and not rest.is_contiguous():
         raise ValueError("rest must be contiguous")
     sc = _scale(scale, d)
-    cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape)
+    cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape[0])
     code = dtype_code(q)
     dq = q.new_empty((total, hq, d))
     dk = q.new_empty((total, hkv, d))
@@ -792,21 +818,19 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return dq, dk, dv
 
 
-def _check_pool(k_pages, v_pages, page_table, seqs, d):
+def _check_pool(k_pages, v_pages, d):
     """The pool's (pages, Hkv, page) and its strides, the same for k and v."""
     shape, strides = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or shape != v_pages.shape or not k_pages.numel():
+    if len(shape) != 4 or shape != v_pages.shape or 0 in shape:
         raise ValueError(f"k_pages and v_pages must be [pages, Hkv, page, D] alike, got {tuple(shape)}, "
                          f"{tuple(v_pages.shape)}")
     if d != 64 or shape[3] != 64:
         raise ValueError(f"paged caches have head size 64, got {d} and {shape[3]}")
-    if k_pages.dtype != v_pages.dtype or strides != v_pages.stride():
+    if k_pages.dtype is not v_pages.dtype or strides != v_pages.stride():
         raise ValueError("k_pages and v_pages must share dtype and strides")
     if _rows16(k_pages) is not k_pages or v_pages.data_ptr() & 15:
         raise ValueError("pages must have 16-byte aligned rows and innermost stride 1")
-    if page_table.dim() != 2 or page_table.shape[0] != seqs or not page_table.shape[1]:
-        raise ValueError(f"page_table must be [{seqs}, width], got {tuple(page_table.shape)}")
-    return shape[:3], strides[:3]
+    return shape, strides
 
 
 def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -818,29 +842,33 @@ def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pa
     cu_seqlens[b+1]-1 go to positions lens[b], lens[b]+1, ..; without
     cu_seqlens row b is sequence b's one new token.  A row whose place is out
     of range is dropped and check_device_errors reports it."""
-    if xk.dim() != 3 or xk.shape != xv.shape or lens.dim() != 1:
-        raise ValueError(f"xk, xv must be [N, Hkv, D] alike and lens [B], got {tuple(xk.shape)}, "
-                         f"{tuple(xv.shape)}, {tuple(lens.shape)}")
-    n, hkv, d = xk.shape
+    rows = xk.shape
+    if len(rows) != 3 or rows != xv.shape or lens.dim() != 1:
+        raise ValueError(f"xk, xv must be [N, Hkv, D] alike and lens [B], got {tuple(rows)}, {tuple(xv.shape)}, "
+                         f"{tuple(lens.shape)}")
+    n, hkv, d = rows
     b = lens.shape[0]
-    (pages, held, page), pool_strides = _check_pool(k_pages, v_pages, page_table, b, d)
+    (pages, held, page, _), (p_sp, p_sh, p_st, _) = _check_pool(k_pages, v_pages, d)
+    table = _table32(page_table, b)
     if held != hkv:
         raise ValueError(f"the pool has {held} kv heads, the rows {hkv}")
-    if xk.dtype != k_pages.dtype or xv.dtype != k_pages.dtype:
-        raise TypeError(f"rows of {xk.dtype} do not fit pages of {k_pages.dtype}")
+    dtype = k_pages.dtype
+    if xk.dtype is not dtype or xv.dtype is not dtype:
+        raise TypeError(f"rows of {xk.dtype} do not fit pages of {dtype}")
     if cu_seqlens is None and n != b:
         raise ValueError(f"without cu_seqlens every one of the {b} sequences has one row, got {n}")
     dev = _device(xk, xv, k_pages, v_pages, page_table, lens, cu_seqlens)
-    table = _index32("page_table", page_table, page_table.shape)
-    ln = _index32("lens", lens, (b,))
-    cu = _index32("cu_seqlens", cu_seqlens, (b + 1,)) if cu_seqlens is not None else None
+    ln = _index32("lens", lens, b)
+    cu = _index32("cu_seqlens", cu_seqlens, b + 1) if cu_seqlens is not None else None
     code = dtype_code(k_pages)
     if n == 0 or b == 0:
         return
     xk, xv = _rows16(xk), _rows16(xv)
-    _launch("sd_paged_append", dev, xk.data_ptr(), xv.data_ptr(), code, n, hkv, d, *xk.stride()[:2],
-            *xv.stride()[:2], k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *pool_strides, table.data_ptr(), table.stride(0), table.shape[1], ln.data_ptr(), b,
-            cu.data_ptr() if cu is not None else None, _err_ptr(dev))
+    k_sn, k_sh, _ = xk.stride()
+    v_sn, v_sh, _ = xv.stride()
+    _launch("sd_paged_append", dev, xk.data_ptr(), xv.data_ptr(), code, n, hkv, d, k_sn, k_sh, v_sn, v_sh,
+            k_pages.data_ptr(), v_pages.data_ptr(), pages, page, p_sp, p_sh, p_st, table.data_ptr(), table.stride(0),
+            table.shape[1], ln.data_ptr(), b, cu.data_ptr() if cu is not None else None, _err_ptr(dev))
 
 
 @functools.lru_cache(maxsize=256)
@@ -857,23 +885,24 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     lens[b] positions of its pages (the new token's own included, once
     appended); layout as paged_append (sd_paged_decode_attention).  Returns
     [B,Hq,64]; a sequence without tokens gives zeros."""
-    if q.dim() != 3 or lens.dim() != 1 or q.shape[0] != lens.shape[0]:
-        raise ValueError(f"q must be [B, Hq, D] and lens [B], got {tuple(q.shape)}, {tuple(lens.shape)}")
-    b, hq, d = q.shape
-    (pages, hkv, page), pool_strides = _check_pool(k_pages, v_pages, page_table, b, d)
+    shape = q.shape
+    if len(shape) != 3 or lens.dim() != 1 or shape[0] != lens.shape[0]:
+        raise ValueError(f"q must be [B, Hq, D] and lens [B], got {tuple(shape)}, {tuple(lens.shape)}")
+    b, hq, d = shape
+    (pages, hkv, page, _), (p_sp, p_sh, p_st, _) = _check_pool(k_pages, v_pages, d)
+    table = _table32(page_table, b)
     if hq == 0 or hq % hkv:
         raise ValueError(f"query heads ({hq}) must be a multiple of kv heads ({hkv})")
-    if q.dtype != k_pages.dtype or (out is not None and out.dtype != q.dtype):
+    if q.dtype is not k_pages.dtype or (out is not None and out.dtype is not q.dtype):
         raise TypeError(f"q of {q.dtype} does not fit pages of {k_pages.dtype}")
-    if out is not None and out.shape != q.shape:
-        raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
     dev = _device(q, k_pages, v_pages, page_table, lens, out)
-    table = _index32("page_table", page_table, page_table.shape)
-    ln = _index32("lens", lens, (b,))
+    ln = _index32("lens", lens, b)
     code = dtype_code(q)
     sc = _scale(scale, d)
     if out is None:
-        out = q.new_empty((b, hq, d))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != shape:
+        raise ValueError(f"out must have q's shape {tuple(shape)}, got {tuple(out.shape)}")
     elif _rows16(out) is not out:
         raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
     if b == 0:
@@ -882,9 +911,11 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     # from the caching allocator, so that calls on other streams and captured graphs have their own
     need = _decode_workspace(b, hq, hkv)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _launch("sd_paged_decode_attention", dev, q.data_ptr(), code, b, hq, hkv, d, *q.stride()[:2],
-            k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *pool_strides, table.data_ptr(), table.stride(0), table.shape[1], ln.data_ptr(), sc, out.data_ptr(), *out.stride()[:2], ws.data_ptr(),
-            need, _err_ptr(dev))
+    q_sb, q_sh, _ = q.stride()
+    o_sb, o_sh, _ = out.stride()
+    _launch("sd_paged_decode_attention", dev, q.data_ptr(), code, b, hq, hkv, d, q_sb, q_sh, k_pages.data_ptr(),
+            v_pages.data_ptr(), pages, page, p_sp, p_sh, p_st, table.data_ptr(), table.stride(0), table.shape[1],
+            ln.data_ptr(), sc, out.data_ptr(), o_sb, o_sh, ws.data_ptr(), need, _err_ptr(dev))
     return out
 
 
