@@ -341,15 +341,17 @@ class RaggedBatch:
         self.cos, self.sin, self.cu_seqlens, self.lens_after = cos, sin, cu_seqlens, lens_after
 
     @classmethod
-    def prompts(cls, cu_seqlens: torch.Tensor, total: int, rotary_emb) -> "RaggedBatch":
+    def prompts(cls, cu_seqlens: torch.Tensor, total: int, rotary_emb, longest: Optional[int] = None) -> "RaggedBatch":
         """Packed prompts: the token at row r of sequence s has position
-        r - cu_seqlens[s].  Bounds stay on the device; no position can reach
-        ``total``, which the tables are grown to."""
-        rotary_emb.ensure(total)
+        r - cu_seqlens[s].  Bounds stay on the device; the RoPE tables are
+        grown to ``longest``, the longest sequence where the host knows it
+        (else ``total``)."""
+        longest = total if longest is None else longest
+        rotary_emb.ensure(longest)
         rows = torch.arange(total, device=cu_seqlens.device)
         bounds = cu_seqlens.to(torch.int64)
         seq = torch.searchsorted(bounds, rows, right=True) - 1
-        pos = (rows - bounds[seq.clamp_min(0)]).clamp(0, max(total - 1, 0))
+        pos = (rows - bounds[seq.clamp_min(0)]).clamp(0, max(longest - 1, 0))
         return cls(rotary_emb.cos[pos], rotary_emb.sin[pos], cu_seqlens=cu_seqlens)
 
     @classmethod
@@ -406,7 +408,7 @@ class B200DenseAttention(BaseAttention):
                 ragged = RaggedBatch.step(kv_cache.pages.lens, kv_cache.pages.capacity, rotary_emb)
             else:
                 bounds = torch.arange(0, (b + 1) * t, t, dtype=torch.int32, device=xq.device)
-                ragged = RaggedBatch.prompts(bounds, b * t, rotary_emb)
+                ragged = RaggedBatch.prompts(bounds, b * t, rotary_emb, t)
         if not step and b != 1 and ragged.cu_seqlens.numel() != b + 1:
             raise ValueError(f"{ragged.cu_seqlens.numel() - 1} packed sequences do not fit {b} rows of {t} tokens")
         rope = _RopeQK.apply if grad else ops.rope_qk

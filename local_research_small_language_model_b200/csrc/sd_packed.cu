@@ -162,7 +162,7 @@ __device__ __forceinline__ float row_sum(float x) {
 
 }  // namespace pk
 
-__global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) {
+__global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_constant__ PackedArgs a) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *K = Q + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
@@ -231,10 +231,28 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(PackedArgs a) 
   }
 #pragma unroll
   for (int i = 0; i < kR; ++i) {
-    if (kR * ty + i >= rows) continue;
     const float inv = 1.0f / l[i];
-    store4(out + (kR * ty + i) * a.o_st + 4 * tx, o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
-    if (a.lse && tx == 0) a.lse[h * a.total + first + kR * ty + i] = m[i] + log2f(l[i]);
+    bool finite = true;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      o[i][u] *= inv;
+      finite = finite && fabsf(o[i][u]) < INFINITY;
+    }
+    const bool held = kR * ty + i < rows;
+    if (held) {
+      store4(out + (kR * ty + i) * a.o_st + 4 * tx, o[i][0], o[i][1], o[i][2], o[i][3]);
+      if (a.lse && tx == 0) a.lse[h * a.total + first + kR * ty + i] = m[i] + log2f(l[i]);
+    }
+    // the warp's two rows in turn
+    const unsigned bad = __ballot_sync(0xffffffffu, held && !finite);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      if (bad >> (16 * half) & 0xffffu) {
+        __syncwarp();
+        const int row = __shfl_sync(0xffffffffu, t.row0 + kR * ty + i, 16 * half);
+        packed_row<float>(a, t.start, row, h, __shfl_sync(0xffffffffu, m[i], 16 * half),
+                          __shfl_sync(0xffffffffu, l[i], 16 * half));
+      }
   }
 }
 

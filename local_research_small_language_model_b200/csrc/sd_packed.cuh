@@ -165,6 +165,43 @@ __device__ __forceinline__ PackedTile packed_nth(const int32_t *cu, int S, int64
   return t;
 }
 
+// One row of the forward again, by a warp and without matrix products, for a
+// result that is not finite: there a masked weight of 0 met a NaN or an infinity
+// of a later token's v, which the row does not see; or it does see one, and the
+// result stays what it is.  Row `row` (of the sequence) of head h, with its
+// reference m and sum l from the fast path.
+template <typename T>
+__device__ __forceinline__ void packed_row(const PackedArgs &a, int64_t start, int row, int h, float m, float l) {
+  const int lane = threadIdx.x & 31, hk = h / (a.Hq / a.Hkv);
+  const T *q = static_cast<const T *>(a.q) + (start + row) * a.q_st + h * a.q_sh;
+  const T *k = static_cast<const T *>(a.k) + start * a.k_st + hk * a.k_sh;
+  const T *v = static_cast<const T *>(a.v) + start * a.v_st + hk * a.v_sh;
+  float o0 = 0.f, o1 = 0.f;
+  for (int j0 = 0; j0 <= row; j0 += 32) {
+    float p = 0.f;
+    if (j0 + lane <= row) {
+      const T *kj = k + (j0 + lane) * a.k_st;
+      float s = 0.f;
+      for (int d = 0; d < 64; ++d) s = fmaf(to_f(q[d]), to_f(kj[d]), s);
+      p = exp2f(fmaf(s, a.scale_log2, m == -INFINITY ? 0.f : -m));
+    }
+    const int n = min(32, row + 1 - j0);
+    for (int t = 0; t < n; ++t) {
+      const float w = __shfl_sync(0xffffffffu, p, t);
+      const T *vj = v + (j0 + t) * a.v_st + 2 * lane;
+      o0 = fmaf(w, to_f(vj[0]), o0);
+      o1 = fmaf(w, to_f(vj[1]), o1);
+    }
+  }
+  o0 /= l, o1 /= l;
+  T *out = static_cast<T *>(a.out) + (start + row) * a.o_st + h * a.o_sh + 2 * lane;
+  out[0] = from_f<T>(o0), out[1] = from_f<T>(o1);
+  if (a.rest) {
+    T *rest = static_cast<T *>(a.rest) + ((start + row) * a.Hq + h) * 64 + 2 * lane;
+    rest[0] = from_f<T>(o0 - round_to<T>(o0)), rest[1] = from_f<T>(o1 - round_to<T>(o1));
+  }
+}
+
 // The tensor-core kernels (16-bit types).
 int launch_packed_fwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s);
 int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStream_t s);

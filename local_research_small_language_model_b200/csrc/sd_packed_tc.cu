@@ -167,11 +167,13 @@ __device__ __forceinline__ void clear_rows(char *tile, int first, int rows) {
 // A warp's 32 accumulator rows of 64 values, scaled, to 16-bit rows `stride`
 // apart, the first `rows` of them; with `rest` also what the rounding took from
 // them.  Through 4 KB of the warp's own shared memory, so that eight lanes write
-// a row's 128 bytes together.
+// a row's 128 bytes together.  Returns the lanes whose row holds a value that is
+// not finite.
 template <typename T>
-__device__ __forceinline__ void store_rows(T *dst, int64_t stride, int rows, uint32_t taddr, float scale, char *sm,
+__device__ __forceinline__ unsigned store_rows(T *dst, int64_t stride, int rows, uint32_t taddr, float scale, char *sm,
                                            T *rest = nullptr, int64_t rest_stride = 0) {
   const int lane = threadIdx.x & 31;
+  bool finite = true;
 #pragma unroll 1
   for (int pass = 0; pass < (rest == nullptr ? 1 : 2); ++pass) {
     __syncwarp();
@@ -185,6 +187,7 @@ __device__ __forceinline__ void store_rows(T *dst, int64_t stride, int rows, uin
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           v[c + e] *= scale;
+          finite = finite && fabsf(v[c + e]) < INFINITY;
           if (pass == 1) v[c + e] -= round_to<T>(v[c + e]);
         }
         *reinterpret_cast<uint4 *>(sm + sw128(lane, 4 * h + (c >> 3))) = make_uint4(
@@ -201,6 +204,7 @@ __device__ __forceinline__ void store_rows(T *dst, int64_t stride, int rows, uin
       if (r < rows) *reinterpret_cast<uint4 *>(to + r * st + 8 * c) = *reinterpret_cast<const uint4 *>(sm + sw128(r, c));
     }
   }
+  return __ballot_sync(0xffffffffu, !finite && lane < rows);
 }
 
 // A value that the warp's lanes share, in a form the compiler knows to be shared:
@@ -217,7 +221,7 @@ template <typename T> __device__ __forceinline__ void zero_rows(T *dst, int64_t 
 
 template <typename T>
 __global__ void __launch_bounds__(pt::kFwdThreads, 2)
-    packed_fwd_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
+    packed_fwd_tc_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ CUtensorMap tmq,
                          const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                          int32_t *err) {
   using namespace pt;
@@ -354,9 +358,10 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
         }
       };
       uint32_t w[32];
-      auto weights = [&](auto poly) {
+      auto weights = [&](auto poly, bool raise) {
         constexpr bool kPoly = decltype(poly)::value;
-        const float neg = m == -INFINITY ? 0.f : -m;
+        // without a reference yet: the sum is to say so, unless the block has none to give
+        const float neg = m == -INFINITY ? (raise ? 0.f : INFINITY) : -m;
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
         }
         // masked and first blocks, and what the polynomial's range does not hold (a NaN, an infinity, a weight
         // past 2^127: the sum tells), take the special-function unit for all
-        sum = raise || edge ? weights(std::false_type()) : weights(std::true_type());
+        sum = raise || edge ? weights(std::false_type(), raise) : weights(std::true_type(), false);
         if (raise || !__any_sync(0xffffffffu, held && !(sum <= kMostSum))) break;
         raise = true;
       }
@@ -440,8 +445,18 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
     const int row0 = 32 * warp, row = row0 + lane;  // of the CTA's rows
     T *rest = a.rest ? static_cast<T *>(a.rest) + ((first + row0) * a.Hq + h) * 64 : nullptr;
     // the tile's own Q is read no more
-    store_rows(out + row0 * a.o_st, a.o_st, rows - row0, tmem + lane_base + kFwdO + 64 * x, 1.0f / l,
-               sm + FwdSmem::kQ + warp * 4096, rest, static_cast<int64_t>(a.Hq) * 64);
+    unsigned again = store_rows(out + row0 * a.o_st, a.o_st, rows - row0, tmem + lane_base + kFwdO + 64 * x, 1.0f / l,
+                                sm + FwdSmem::kQ + warp * 4096, rest, static_cast<int64_t>(a.Hq) * 64);
+    if (again && !failed) {
+      __syncwarp();  // a row's first result is written by other lanes than its second
+      // the tile is looked up again: nothing is kept for this in the loop's registers
+      const PackedTile u = packed_nth(a.cu, a.S, a.total, blockIdx.x / a.Hq, gridDim.x / a.Hq, 2 * kRows, true);
+      for (; again; again &= again - 1) {
+        const int i = __ffs(again) - 1;
+        packed_row<T>(a, u.start, u.row0 + 32 * warp + i, blockIdx.x % a.Hq, __shfl_sync(0xffffffffu, m, i),
+                      __shfl_sync(0xffffffffu, l, i));
+      }
+    }
     if (row < rows && a.lse) a.lse[h * a.total + first + row] = m + log2f(l);
   }
   fence_before_sync();

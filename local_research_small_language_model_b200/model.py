@@ -422,7 +422,8 @@ class SparDAB200Model(nn.Module):
                 raise ValueError("packed prompts into a cache need their lengths on the host too, "
                                  "with the sum of the row's tokens")
             pages.reserve(counts)
-        return RaggedBatch.prompts(cu_seqlens, b * t, self.rotary_emb), pages, counts
+        longest = max(counts) if counts else None
+        return RaggedBatch.prompts(cu_seqlens, b * t, self.rotary_emb, longest), pages, counts
 
     def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
                 kv_caches: Optional[List] = None, return_forecasts: bool = False,

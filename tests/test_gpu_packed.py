@@ -183,6 +183,44 @@ def test_rows_outside_every_sequence(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf], ids=str)
+def test_later_tokens_do_not_show(dev, dtype, bad):
+    """A NaN or an infinity in k or v of a later token of the same sequence, in
+    the same tile or another, changes no bound of the rows before it; the rows
+    from it on are what the formula makes of it."""
+    cu = bounds([70, 300])
+    dcu = torch.tensor(cu, dtype=torch.int32, device=dev)
+    for token in (71, 70 + 130, 70 + 299):
+        q, k, v, dout = inputs(dev, dtype, 370, 4, 2, seed=21)
+        val, err = exact(q, k, v, dout, cu, 0.125)
+        for kind in ("k", "v"):
+            q2, k2, v2 = q.clone(), k.clone(), v.clone()
+            (k2 if kind == "k" else v2)[token, 1, 5] = bad
+            got = ops.packed_attention(q2, k2, v2, dcu)
+            check(got[:token], val["out"][:token], err["out"][:token], f"{kind} {token}")
+            assert torch.isfinite(got[:, :2]).all()  # the other kv head's rows
+            if kind == "v":
+                seen = got[token:, 2:, 5].double()
+                assert (seen.isnan() if math.isnan(bad) else (seen == bad) | seen.isnan()).all()
+                keep = [c for c in range(64) if c != 5]
+                check(got[token:, 2:][..., keep], val["out"][token:, 2:][..., keep], err["out"][token:, 2:][..., keep], "v")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+def test_rows_whose_first_scores_are_infinite(dev, dtype):
+    """Keys with a score of -inf weigh nothing, also where a whole first block
+    has no other; a row that sees nothing else is NaN, as softmax of -inf is."""
+    q, k, v, dout = inputs(dev, dtype, 260, 2, 2, seed=22)
+    q = (q.abs() + 0.5).to(dtype)
+    k = k.clone()
+    k[:150] = -math.inf
+    got, lse = ops.packed_attention(q, k, v, torch.tensor([0, 260], dtype=torch.int32, device=dev), return_lse=True)
+    val, err = exact(q[150:], k[150:], v[150:], dout[150:], [0, 110], 0.125)
+    check(got[150:], val["out"], err["out"], "out")
+    assert got[:150].isnan().all() and torch.isfinite(lse[:, 150:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
 def test_strides_views_and_broadcast(dev, dtype):
     """Head-major storage, an unaligned base, an int64 cu, and k and v shared by
     expanding one head: the gradient of the one head is the heads' sum."""
