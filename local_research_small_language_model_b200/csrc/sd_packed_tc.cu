@@ -348,13 +348,13 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
       if (__any_sync(0xffffffffu, !ok)) break;
       fence_after_sync();
       const bool edge = i * kBlock + kBlock - 1 > row - r;  // the diagonal's two blocks
-      auto scores = [&](int half, float (&s)[32]) {
-        tmem_ld32(t_s + 32 * half, s);
+      auto scores = [&](int part, float (&s)[16]) {
+        tmem_ld16(t_s + 16 * part, s);
         tmem_wait_ld();
         if (edge) {
-          const int seen = row + 1 - i * kBlock - 32 * half;
+          const int seen = row + 1 - i * kBlock - 16 * part;
 #pragma unroll
-          for (int u = 0; u < 32; ++u) s[u] = u < seen ? s[u] : -INFINITY;
+          for (int u = 0; u < 16; ++u) s[u] = u < seen ? s[u] : -INFINITY;
         }
       };
       uint32_t w[32];
@@ -364,11 +364,11 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
         const float neg = m == -INFINITY ? (raise ? 0.f : INFINITY) : -m;
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float s[32];
-          scores(half, s);
+        for (int q = 0; q < 4; ++q) {
+          float s[16];
+          scores(q, s);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 8; ++e) {
             float y0 = s[2 * e], y1 = s[2 * e + 1];
             fma2(y0, y1, c, neg);
             // every fourth pair's exponentials on the FMA pipe: the special-function unit is the bound
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
             else
               y0 = ex2(y0), y1 = ex2(y1);
             add2(part[2 * (e & 1)], part[2 * (e & 1) + 1], y0, y1);
-            w[16 * half + e] = pack2<T>(y0, y1);
+            w[8 * q + e] = pack2<T>(y0, y1);
           }
         }
         return (part[0] + part[1]) + (part[2] + part[3]);
@@ -387,11 +387,11 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
         if (raise) {  // the reference moves to this block's maximum, what is summed so far with it
           float best = -INFINITY;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float s[32];
-            scores(half, s);
+          for (int q = 0; q < 4; ++q) {
+            float s[16];
+            scores(q, s);
 #pragma unroll
-            for (int u = 0; u < 32; ++u) best = fmaxf(best, s[u]);
+            for (int u = 0; u < 16; ++u) best = fmaxf(best, s[u]);
           }
           best *= c;
           float alpha = 1.f;
