@@ -194,6 +194,36 @@ def test_append(dev, dtype, page):
     ops.check_device_errors(dev)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+def test_append_of_many_rows(dev, dtype):
+    """Thousands of rows (the larger CTAs), token-major pages, strided rows."""
+    new = [4000, 0, 1500, 1, 700]
+    k, v, table = pool(dev, dtype, [n + 9 for n in new], 2, 16, seed=8)
+    k, v = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (k, v))
+    wk, wv = k.clone(), v.clone()
+    g = torch.Generator(device=dev).manual_seed(5)
+    rows = torch.randn(sum(new), 7, 64, generator=g, device=dev).to(dtype)
+    ends = torch.tensor([0, *new], device=dev).cumsum(0)
+    lens = torch.full((5,), 9, dtype=torch.int32, device=dev)
+    sd.paged_append(rows[:, 1:3], rows[:, 4:6], k, v, table, lens, ends.to(torch.int32))
+    for b, n in enumerate(new):
+        t = torch.arange(9, 9 + n, device=dev)
+        wk[table[b].long()[t // 16], :, t % 16] = rows[ends[b]:ends[b] + n, 1:3]
+        wv[table[b].long()[t // 16], :, t % 16] = rows[ends[b]:ends[b] + n, 4:6]
+    assert torch.equal(k, wk) and torch.equal(v, wv)
+    ops.check_device_errors(dev)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+def test_more_sequences_than_one_launch_plans(dev, dtype):
+    lens = [(7 * b) % 90 for b in range(2100)]
+    k, v, table = pool(dev, dtype, lens, 2, 16, seed=9)
+    q = query(dev, dtype, 2100, 4)
+    got = sd.paged_decode_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device=dev))
+    check(got, *exact(q, k, v, table, lens))
+    ops.check_device_errors(dev)
+
+
 def test_append_out_of_range_is_dropped_and_reported(dev):
     k, v, table = pool(dev, torch.bfloat16, [40, 40], 2, 16, seed=6)
     wk, wv = k.clone(), v.clone()

@@ -62,7 +62,7 @@ def same_order(got, x, k):
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("shape", [(1, 1), (3, 2), (5, 7), (2, 63), (130, 257), (64, 32000), (9, 32003), (3, 100001)],
+@pytest.mark.parametrize("shape", [(1, 1), (3, 2), (5, 7), (2, 63), (130, 257), (700, 1031), (64, 32000), (9, 32003), (3, 100001)],
                          ids=str)
 @pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
 def test_scores(dev, dtype, shape):
@@ -145,7 +145,7 @@ def exact_grad(x, t, g, ge):
 
 
 @pytest.mark.parametrize("which", ["logprobs", "entropy", "both"])
-@pytest.mark.parametrize("shape", [(1, 1), (5, 7), (130, 257), (33, 32000), (9, 32003)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (5, 7), (130, 257), (700, 1031), (33, 32000), (9, 32003)], ids=str)
 @pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
 def test_gradient(dev, dtype, shape, which):
     x, t = make(dev, dtype, *shape, seed=shape[0])
