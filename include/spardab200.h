@@ -497,6 +497,19 @@ SD_API int sd_token_logprobs_backward(const void *logits, int dtype, int64_t row
                                       const float *g_logprobs, const float *g_entropy, void *dlogits, int64_t d_ld,
                                       void *stream);
 
+/* The launches of ragged batches by number, with their arguments in one array
+ * of n 64-bit words in the declared order (integers and pointers as they are,
+ * a float as the bits of a double): for bindings whose foreign-function
+ * interface pays for every argument (ctypes: 2.8 us for 25, 0.8 us this way).
+ * n other than the entry point's number of arguments: SD_ERR_INVALID. */
+#define SD_CALL_PACKED_ATTENTION 0
+#define SD_CALL_PACKED_ATTENTION_BACKWARD 1
+#define SD_CALL_PAGED_APPEND 2
+#define SD_CALL_PAGED_DECODE_ATTENTION 3
+#define SD_CALL_TOKEN_LOGPROBS 4
+#define SD_CALL_TOKEN_LOGPROBS_BACKWARD 5
+SD_API int sd_invoke(int call, const int64_t *words, int n);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,9 @@ library is missing, every op raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -96,6 +98,12 @@ _SIGS = {
                                    _c_void_p, _c_void_p, _i64, _c_void_p],
 }
 
+_SIGS["sd_invoke"] = [_i32, ctypes.c_char_p, _i32]
+
+# launches that sd_invoke takes as one block of 64-bit words (SD_CALL_*)
+_BLOCK_CALLS = {"sd_packed_attention": 0, "sd_packed_attention_backward": 1, "sd_paged_append": 2,
+                "sd_paged_decode_attention": 3, "sd_token_logprobs": 4, "sd_token_logprobs_backward": 5}
+
 # entry points that return something other than an int status
 _RESTYPES = {}
 
@@ -133,6 +141,21 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+@functools.lru_cache(maxsize=None)
+def block_call(name: str):
+    """A function of an entry point's arguments (0 for a null pointer) that
+    returns its status, by way of sd_invoke: one conversion instead of one an
+    argument, which is what a call of 25 arguments spends most on."""
+    number, sig = _BLOCK_CALLS[name], _SIGS[name]
+    pack = struct.Struct("=" + "".join("d" if t is _f32 else "q" for t in sig)).pack
+    invoke, n = load().sd_invoke, len(sig)
+
+    def run(*args) -> int:
+        return invoke(number, pack(*args), n)
+
+    return run
 
 
 def call(name: str, *args) -> None:

@@ -1,8 +1,11 @@
 // Library-wide entry points: error text, version, last CUDA error, length bump.
 #include <math.h>
+#include <string.h>
 
 #include <atomic>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "sd_common.cuh"
@@ -73,9 +76,44 @@ __global__ void advance_len_kernel(int32_t *lens, int n, int delta) {
   if (i < n) lens[i] += delta;
 }
 
+// One word of sd_invoke as an argument of type A.
+template <typename A> static A from_word(int64_t word) {
+  if constexpr (std::is_pointer<A>::value) {
+    return reinterpret_cast<A>(static_cast<intptr_t>(word));
+  } else if constexpr (std::is_same<A, float>::value) {
+    double d;
+    memcpy(&d, &word, sizeof(d));
+    return static_cast<float>(d);
+  } else {
+    return static_cast<A>(word);
+  }
+}
+
+template <typename... A, size_t... I>
+static int call_words(int (*f)(A...), const int64_t *words, std::index_sequence<I...>) {
+  return f(from_word<A>(words[I])...);
+}
+template <typename... A> static int invoke(int (*f)(A...), const int64_t *words, int n) {
+  if (n != static_cast<int>(sizeof...(A))) return SD_ERR_INVALID;
+  return call_words(f, words, std::index_sequence_for<A...>());
+}
+
 }  // namespace sd
 
 extern "C" {
+
+int sd_invoke(int call, const int64_t *words, int n) {
+  if (!words) return SD_ERR_INVALID;
+  switch (call) {
+    case SD_CALL_PACKED_ATTENTION: return sd::invoke(sd_packed_attention, words, n);
+    case SD_CALL_PACKED_ATTENTION_BACKWARD: return sd::invoke(sd_packed_attention_backward, words, n);
+    case SD_CALL_PAGED_APPEND: return sd::invoke(sd_paged_append, words, n);
+    case SD_CALL_PAGED_DECODE_ATTENTION: return sd::invoke(sd_paged_decode_attention, words, n);
+    case SD_CALL_TOKEN_LOGPROBS: return sd::invoke(sd_token_logprobs, words, n);
+    case SD_CALL_TOKEN_LOGPROBS_BACKWARD: return sd::invoke(sd_token_logprobs_backward, words, n);
+    default: return SD_ERR_INVALID;
+  }
+}
 
 const char *sd_strerror(int code) {
   switch (code) {

@@ -662,21 +662,16 @@ def _err_ptr(dev: int) -> int:
     return ptr
 
 
-@functools.lru_cache(maxsize=None)
-def _entry(name: str):
-    return getattr(L.load(), name)
-
-
 def _launch(name: str, dev: int, *args) -> None:
-    """L.call on the current stream of device ``dev``, which a launch needs as
-    the current device."""
+    """An entry point on the current stream of device ``dev``, which a launch
+    needs as the current device."""
     if torch._C._cuda_getDevice() == dev:
-        code = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
-        if code != L.SD_OK:
-            L.check(name, code)
-        return
-    with torch.cuda.device(dev):
-        L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+        code = L.block_call(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            code = L.block_call(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if code != L.SD_OK:
+        L.check(name, code)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -781,8 +776,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         o_st, o_sh, _ = out.stride()
         _launch("sd_packed_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, total, hq, k.shape[1], d,
                 q_st, q_sh, k_st, k_sh, v_st, v_sh, cu.data_ptr(), cu.shape[0] - 1, sc, out.data_ptr(), o_st, o_sh,
-                lse.data_ptr() if return_lse else None,
-                rest.data_ptr() if rest is not None else None, zero, _err_ptr(dev))
+                lse.data_ptr() if return_lse else 0,
+                rest.data_ptr() if rest is not None else 0, zero, _err_ptr(dev))
     return (out, lse) if return_lse else out
 
 
@@ -814,7 +809,7 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         _launch("sd_packed_attention_backward", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                 dout.data_ptr(), code, total, hq, hkv, d, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
                 *out.stride()[:2], *dout.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, sc, lse.data_ptr(),
-                rest.data_ptr() if rest is not None else None, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _err_ptr(dev))
+                rest.data_ptr() if rest is not None else 0, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _err_ptr(dev))
     return dq, dk, dv
 
 
@@ -868,7 +863,7 @@ def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pa
     v_sn, v_sh, _ = xv.stride()
     _launch("sd_paged_append", dev, xk.data_ptr(), xv.data_ptr(), code, n, hkv, d, k_sn, k_sh, v_sn, v_sh,
             k_pages.data_ptr(), v_pages.data_ptr(), pages, page, p_sp, p_sh, p_st, table.data_ptr(), table.stride(0),
-            table.shape[1], ln.data_ptr(), b, cu.data_ptr() if cu is not None else None, _err_ptr(dev))
+            table.shape[1], ln.data_ptr(), b, cu.data_ptr() if cu is not None else 0, _err_ptr(dev))
 
 
 @functools.lru_cache(maxsize=256)
@@ -949,8 +944,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=where)
     if rows:
         _launch("sd_token_logprobs", dev, logits.data_ptr(), code, rows, vocab, logits.stride(0), targets.data_ptr(),
-                ignore_index, logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr() if return_stats else None,
-                top_k, top_lp.data_ptr() if top_k else None, top_ids.data_ptr() if top_k else None, _err_ptr(dev))
+                ignore_index, logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr() if return_stats else 0,
+                top_k, top_lp.data_ptr() if top_k else 0, top_ids.data_ptr() if top_k else 0, _err_ptr(dev))
     found = (logprobs, entropy, top_lp, top_ids)
     return found + (stats,) if return_stats else found
 
@@ -974,6 +969,6 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: 
     d = logits.new_empty((rows, vocab))
     if rows:
         _launch("sd_token_logprobs_backward", dev, logits.data_ptr(), code, rows, vocab, logits.stride(0),
-                targets.data_ptr(), ignore_index, stats.data_ptr(), gl.data_ptr() if gl is not None else None,
-                ge.data_ptr() if ge is not None else None, d.data_ptr(), d.stride(0))
+                targets.data_ptr(), ignore_index, stats.data_ptr(), gl.data_ptr() if gl is not None else 0,
+                ge.data_ptr() if ge is not None else 0, d.data_ptr(), d.stride(0))
     return d

@@ -90,6 +90,32 @@ def test_entry_points_refuse(case):
     assert call(sd.load_library(), **wrong) == code
 
 
+def test_argument_blocks_reach_the_same_entry_points():
+    """sd_invoke with the declared number of words gives the entry point's own
+    status; another number of words, or call, is refused."""
+    from local_research_small_language_model_b200 import _lib
+    lib = sd.load_library()
+    for call, wrong, code in REFUSED:
+        name = {packed: "sd_packed_attention", backward: "sd_packed_attention_backward", append: "sd_paged_append",
+                decode: "sd_paged_decode_attention", scores: "sd_token_logprobs",
+                scores_backward: "sd_token_logprobs_backward"}[call]
+
+        class Spy:
+            def __getattr__(self, entry):
+                def run(*args):
+                    assert entry == name and len(args) == len(_lib._SIGS[name])
+                    plain = [a.value if isinstance(a, ctypes.c_void_p) else a for a in args]
+                    return _lib.block_call(name)(*[0 if a is None else a for a in plain])
+                return run
+
+        assert call(Spy(), **wrong) == code, (name, wrong)
+    words = (ctypes.c_int64 * 40)()
+    block = ctypes.cast(words, ctypes.c_char_p)
+    for number in range(6):
+        assert lib.sd_invoke(number, block, 3) == INVALID
+    assert lib.sd_invoke(6, block, 13) == INVALID and lib.sd_invoke(0, None, 24) == INVALID
+
+
 def test_workspace_sizes():
     lib = sd.load_library()
     n = ctypes.c_int64(-1)
