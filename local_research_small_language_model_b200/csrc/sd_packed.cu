@@ -11,8 +11,16 @@
 // 4 rows x 4 columns of every product, with all operands row-major in shared
 // memory (row pitch 68 floats: the float4 reads below have no bank conflicts).
 // A warp's 16-byte shared loads take 12 cycles of the four schedulers' 16 in
-// each of the three forms (row.row, P times rows, P^T times rows).  No atomics: every output element is
-// summed by one thread in a fixed order.
+// each of the three forms (row.row, P times rows, P^T times rows).  No atomics:
+// every sum has a fixed order.
+//
+// With few sequences there are few tiles, and the longest decides: so the CTAs of
+// a cluster deal out a tile's other axis until every SM has its two CTAs, and
+// rank 0 joins their parts.  1023 tokens in 3 sequences, 12 query and 4 key-value
+// heads: forward 54 us (62 with one CTA a tile), dQ 75 us, dK/dV 101 us; the
+// three in a graph 221 us (36 us at the fp32 pipe's rate).  What bounds them: the
+// fp32 pipe is about half busy, the rest is the barriers between a tile's
+// products and the join of unequal CTAs.
 #include "sd_packed.cuh"
 
 namespace sd {
@@ -55,13 +63,22 @@ __device__ __forceinline__ float4 ld4(const float *p) { return *reinterpret_cast
 __device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
   return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
 }
+// Two multiply-adds in one instruction (the same 128 a cycle and SM, in half the
+// issue slots, which the shared loads need): {x, y} += {a, b} * {c, d}.
+__device__ __forceinline__ void fma2(float &x, float &y, float a, float b, float c, float d) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+}
 
-// c[i][j] = sum_d A[kR ty + i][d] B[tx + 16 j][d]
+// c[i][j] = sum_d A[kR ty + i][d] B[tx + 16 j][d], even and odd d apart
 __device__ __forceinline__ void mul_rows(const float *A, const float *B, int ty, int tx, float (&c)[kR][4]) {
+  float even[kR][4], odd[kR][4];
 #pragma unroll
   for (int i = 0; i < kR; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) even[i][j] = odd[i][j] = 0.f;
 #pragma unroll 4
   for (int d = 0; d < kTile; d += 4) {
     float4 b[4];
@@ -71,9 +88,22 @@ __device__ __forceinline__ void mul_rows(const float *A, const float *B, int ty,
     for (int i = 0; i < kR; ++i) {
       const float4 a = ld4(A + (kR * ty + i) * kPitch + d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[i][j] = dot4(a, b[j], c[i][j]);
+      for (int j = 0; j < 4; ++j) {
+        fma2(even[i][j], odd[i][j], a.x, a.y, b[j].x, b[j].y);
+        fma2(even[i][j], odd[i][j], a.z, a.w, b[j].z, b[j].w);
+      }
     }
   }
+#pragma unroll
+  for (int i = 0; i < kR; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[i][j] = even[i][j] + odd[i][j];
+}
+
+// c[i][u] += w b[u]
+__device__ __forceinline__ void add_row(float (&c)[4], float w, float4 b) {
+  fma2(c[0], c[1], w, w, b.x, b.y);
+  fma2(c[2], c[3], w, w, b.z, b.w);
 }
 
 // c[i][u] += sum_k P[kR ty + i][k] B[k][4 tx + u]
@@ -86,14 +116,10 @@ __device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, in
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
       const float4 p = ld4(P + (kR * ty + i) * kPitch + k);
-      const float pe[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        c[i][0] = fmaf(pe[e], b[e].x, c[i][0]);
-        c[i][1] = fmaf(pe[e], b[e].y, c[i][1]);
-        c[i][2] = fmaf(pe[e], b[e].z, c[i][2]);
-        c[i][3] = fmaf(pe[e], b[e].w, c[i][3]);
-      }
+      add_row(c[i], p.x, b[0]);
+      add_row(c[i], p.y, b[1]);
+      add_row(c[i], p.z, b[2]);
+      add_row(c[i], p.w, b[3]);
     }
   }
 }
@@ -102,16 +128,11 @@ __device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, in
 __device__ __forceinline__ void mul_pt(const float *P, const float *B, int ty, int tx, float (&c)[kR][4]) {
 #pragma unroll 4
   for (int k = 0; k < kTile; ++k) {
-    const float4 b = ld4(B + k * kPitch + 4 * tx);
-    const float4 p = ld4(P + k * kPitch + kR * ty);
-    const float pe[kR] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-    for (int i = 0; i < kR; ++i) {
-      c[i][0] = fmaf(pe[i], b.x, c[i][0]);
-      c[i][1] = fmaf(pe[i], b.y, c[i][1]);
-      c[i][2] = fmaf(pe[i], b.z, c[i][2]);
-      c[i][3] = fmaf(pe[i], b.w, c[i][3]);
-    }
+    const float4 b = ld4(B + k * kPitch + 4 * tx), p = ld4(P + k * kPitch + kR * ty);
+    add_row(c[0], p.x, b);
+    add_row(c[1], p.y, b);
+    add_row(c[2], p.z, b);
+    add_row(c[3], p.w, b);
   }
 }
 
@@ -148,6 +169,13 @@ __device__ __forceinline__ void add_peer(const float *P, int rank, float (&c)[kR
   }
 }
 
+// CTAs that share a tile: as many as give every SM its two.
+static int cluster_ranks(int64_t slots, int heads) {
+  int ranks = 1;
+  while (ranks < 8 && slots * heads * ranks < 2 * 148) ranks *= 2;
+  return ranks;
+}
+
 // The 16 lanes of a row (tx = 0..15).
 __device__ __forceinline__ float row_max(float x) {
 #pragma unroll
@@ -162,20 +190,20 @@ __device__ __forceinline__ float row_sum(float x) {
 
 }  // namespace pk
 
-__global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_constant__ PackedArgs a) {
+__global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_constant__ PackedArgs a, int ranks) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *K = Q + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
   // the tiles that see the most keys start first
   const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x, gridDim.x, kTile, true);
   if (!t.valid) return;
-  const int h = blockIdx.y, hk = h / (a.Hq / a.Hkv);
+  const int h = blockIdx.y / ranks, rank = blockIdx.y % ranks, hk = h / (a.Hq / a.Hkv);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int rows = min(kTile, t.len - t.row0);
   const int64_t first = t.start + t.row0;
   float *out = static_cast<float *>(a.out) + first * a.o_st + h * a.o_sh;
   if (t.rest) {
-    if (a.zero_rest)
+    if (a.zero_rest && rank == 0)
       for (int i = 0; i < kR; ++i)
         if (kR * ty + i < rows) store4(out + (kR * ty + i) * a.o_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
@@ -183,22 +211,23 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
   const float *kp = static_cast<const float *>(a.k) + t.start * a.k_st + hk * a.k_sh;
   const float *vp = static_cast<const float *>(a.v) + t.start * a.v_st + hk * a.v_sh;
   start_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
-  start_tile(K, kp, a.k_st, min(kTile, t.len));
-  start_group();
-  start_tile(V, vp, a.v_st, min(kTile, t.len));
-  start_group();
+  auto start = [&](float *dst, const float *src, int64_t st, int k0) {
+    if (k0 <= t.row0) start_tile(dst, src + k0 * st, st, min(kTile, t.len - k0));
+    start_group();
+  };
+  start(K, kp, a.k_st, rank * kTile);
+  start(V, vp, a.v_st, rank * kTile);
   float o[kR][4] = {}, m[kR], l[kR];
 #pragma unroll
   for (int i = 0; i < kR; ++i) m[i] = -INFINITY, l[i] = 0.f;
-  for (int k0 = 0; k0 <= t.row0; k0 += kTile) {
+  for (int k0 = rank * kTile; k0 <= t.row0; k0 += ranks * kTile) {
     // a tile's successor comes in as soon as its last product is done
-    const int next = k0 + kTile;
+    const int next = k0 + ranks * kTile;
     float s[kR][4];
     arrived<1>();
     mul_rows(Q, K, ty, tx, s);
     __syncthreads();
-    if (next <= t.row0) start_tile(K, kp + next * a.k_st, a.k_st, min(kTile, t.len - next));
-    start_group();
+    start(K, kp, a.k_st, next);
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
       const int row = t.row0 + kR * ty + i;
@@ -226,8 +255,34 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
     arrived<1>();
     mul_p(P, V, ty, tx, o);
     __syncthreads();
-    if (next <= t.row0) start_tile(V, vp + next * a.v_st, a.v_st, min(kTile, t.len - next));
-    start_group();
+    start(V, vp, a.v_st, next);
+  }
+  if (ranks > 1) {  // the ranks' parts, in their order; maximum and sum beside the 64 columns
+    __syncthreads();
+    if (rank > 0) {
+      put(P, o, ty, tx);
+      if (tx == 0) {
+#pragma unroll
+        for (int i = 0; i < kR; ++i) P[(kR * ty + i) * kPitch + 64] = m[i], P[(kR * ty + i) * kPitch + 65] = l[i];
+      }
+    }
+    cluster_sync();
+    if (rank == 0) {
+      for (int c = 1; c < ranks; ++c)
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+          const float *row = P + (kR * ty + i) * kPitch;
+          const float4 ml = peer4(row + 64, c), x = peer4(row + 4 * tx, c);
+          const float mn = fmaxf(m[i], ml.x), ref = mn == -INFINITY ? 0.f : mn;
+          const float f0 = exp2f(m[i] - ref), f1 = exp2f(ml.x - ref);
+          m[i] = mn;
+          l[i] = l[i] * f0 + ml.y * f1;
+          o[i][0] = o[i][0] * f0 + x.x * f1, o[i][1] = o[i][1] * f0 + x.y * f1;
+          o[i][2] = o[i][2] * f0 + x.z * f1, o[i][3] = o[i][3] * f0 + x.w * f1;
+        }
+    }
+    cluster_sync();
+    if (rank > 0) return;
   }
 #pragma unroll
   for (int i = 0; i < kR; ++i) {
@@ -468,10 +523,11 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype != SD_DTYPE_F32) return launch_packed_fwd_tc(a, dtype, err, s);
   const size_t smem = 4 * pk::kTileFloats * sizeof(float);
-  auto kern = packed_fwd_kernel;
-  if (ensure_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
-  kern<<<dim3(static_cast<unsigned>(packed_slots(total, nseq, pk::kTile)), a.Hq), pk::kThreads, smem, s>>>(a);
-  return check_launch();
+  if (ensure_smem(packed_fwd_kernel, smem) != SD_OK) return SD_ERR_CUDA;
+  const unsigned slots = static_cast<unsigned>(packed_slots(total, nseq, pk::kTile));
+  const int ranks = pk::cluster_ranks(slots, a.Hq);
+  return launch_cluster(packed_fwd_kernel, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem, s,
+                        false, a, ranks);
 }
 
 int sd_packed_attention_backward(const void *q, const void *k, const void *v, const void *out, const void *dout,
@@ -504,16 +560,10 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   auto kq = packed_bwd_dq_kernel;
   auto kkv = packed_bwd_dkv_kernel;
   if (ensure_smem(kq, smem_q) != SD_OK || ensure_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
-  // Clusters as large as it takes to give every SM a few CTAs: two fit an SM.
-  auto ranks_for = [&](int heads) {
-    int ranks = 1;
-    while (ranks < 8 && static_cast<int64_t>(slots) * heads * ranks < 2 * 148) ranks *= 2;
-    return ranks;
-  };
-  int ranks = ranks_for(a.Hq);
+  int ranks = pk::cluster_ranks(slots, a.Hq);
   rc = launch_cluster(kq, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_q, s, false, a, ranks);
   if (rc != SD_OK) return rc;
-  ranks = ranks_for(a.Hkv);
+  ranks = pk::cluster_ranks(slots, a.Hkv);
   return launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, false, a,
                         ranks);
 }
