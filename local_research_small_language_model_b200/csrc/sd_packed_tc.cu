@@ -35,6 +35,16 @@
 // S and dP are computed in both (7 products and 2 exponentials a pair instead
 // of 5 and 1): in return every gradient is summed in tensor memory in a fixed
 // order, with no atomics and no fp32 buffer to add into and convert.
+//
+// Measured, 12 query and 4 key-value heads, bf16.  One sequence of 32768 tokens:
+// forward 1.74 ms (945 TFLOP/s; 1.00 ms of products, 1.43 ms of exponentials if
+// all ran on the special-function units), backward 6.0 ms (690 TFLOP/s of the 5
+// products a gradient needs, 965 of the 7 it computes).  Training on 16000 tokens
+// in 9 sequences: 0.48 ms, forward and backward.  Of one 8192-token sequence's
+// cycles the forward keeps the special-function units busy for 56 %, instruction
+// issue for 56 % and the tensor pipe for 37 %, dQ 42, 55 and 41 %, dK/dV 38, 62
+// and 50 %: the backward's bound is issue, and its warps' waits for one another
+// between the phases of a block.
 #include <type_traits>
 
 #include "sd_packed.cuh"

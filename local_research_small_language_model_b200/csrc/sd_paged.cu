@@ -50,7 +50,9 @@ __device__ __forceinline__ int64_t row_of(const PagedArgs &a, int b, int h, int 
 // all threads move 16-byte chunks of K and V, several in flight each.  cu
 // (nullable): token rows [cu[b], cu[b + 1]) belong to sequence b; without it row
 // b is sequence b's one token.  Rows outside every sequence are not written
-// anywhere.
+// anywhere.  HBM-bound: 32768 rows of 4 bf16 heads into pages of 64 tokens in
+// 12.4 us (67 MB, 5.4 TB/s with the launch); 64 single tokens 4.2 us, the launch
+// and three loads that depend on one another (length, page, value).
 template <typename T, int kTok>
 __global__ void __launch_bounds__(256)
     paged_append_kernel(PagedArgs a, const int32_t *cu, int64_t N, const T *xk, const T *xv, int64_t k_sn,
@@ -123,6 +125,12 @@ __global__ void __launch_bounds__(256)
 // states meet at the end of a head.  16-bit products are mma.sync m16n8k16 with
 // up to 16 query heads as the rows (a kv head has few: a 128-row tcgen05 tile
 // would be mostly padding, and the tensor pipe is not what bounds this).
+//
+// Measured, 12 query and 4 key-value heads: 64 sequences up to 16384 tokens, bf16,
+// 738 MB in 121 us (6.1 TB/s); one of 32768 tokens 14.4 us (33.5 MB, 5.1 us of
+// reading: start-up of the copies, the join and its launch are the rest); 5 up to
+// 1100 tokens in fp32 with pages of 24 tokens 12.5 us (nearly all latency: a
+// unit's length, page and rows depend on one another).
 namespace pg {
 
 constexpr int kThreads = 128, kWarps = 4, kStages = 4;
