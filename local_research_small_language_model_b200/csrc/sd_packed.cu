@@ -7,20 +7,22 @@
 //   dV_j = sum_i P_ij dO_i,  dK_j = scale sum_i dS_ij q_i,  dQ_i = scale sum_j dS_ij k_j
 //
 // i, j run over the tokens of one sequence; dK and dV also sum over the query
-// heads of their key-value head.  Tiles are 64 x 64; a thread of the 256 owns
-// 4 rows x 4 columns of every product, with all operands row-major in shared
+// heads of their key-value head.  Tiles are 64 x 64; a thread of the 128 owns
+// 8 rows x 4 columns of every product, with all operands row-major in shared
 // memory (row pitch 68 floats: the float4 reads below have no bank conflicts).
-// A warp's 16-byte shared loads take 12 cycles of the four schedulers' 16 in
-// each of the three forms (row.row, P times rows, P^T times rows).  No atomics:
+// A warp's 16-byte shared loads take 16 cycles of the four schedulers' 32 in each
+// of the three forms (row.row, P times rows, P^T times rows); 4 x 4 a thread with
+// 256 threads, 12 of 16, was up to 13 % slower where tiles are many.  No atomics:
 // every sum has a fixed order.
 //
-// With few sequences there are few tiles, and the longest decides: so the CTAs of
-// a cluster deal out a tile's other axis until every SM has its two CTAs, and
-// rank 0 joins their parts.  1023 tokens in 3 sequences, 12 query and 4 key-value
-// heads: forward 54 us (62 with one CTA a tile), dQ 75 us, dK/dV 101 us; the
-// three in a graph 221 us (36 us at the fp32 pipe's rate).  What bounds them: the
-// fp32 pipe is about half busy, the rest is the barriers between a tile's
-// products and the join of unequal CTAs.
+// With few sequences there are few tiles, and the longest decide: so the CTAs of
+// a cluster deal out a tile's other axis, and rank 0 joins their parts.
+// Measured, 12 query and 4 key-value heads: 1023 tokens in 3 sequences, forward
+// 50 us (62 with one CTA a tile), backward 170 us (36 us for all of it at the fp32
+// pipe's rate); 8096 tokens, the longest sequence 4096, forward 1.21 ms (34
+// TFLOP/s), dQ 1.85 ms (34), dK/dV 2.46 ms (34): half of the 69 that its pipe
+// reaches.  What bounds them: the latency of shared loads behind each barrier
+// between a tile's products, with 8 warps an SM to cover it.
 #include "sd_packed.cuh"
 
 namespace sd {
@@ -28,8 +30,8 @@ namespace sd {
 namespace pk {
 
 constexpr int kTile = 64;
-constexpr int kThreads = 256;
-constexpr int kR = 4;                        // rows of a thread
+constexpr int kThreads = 128;
+constexpr int kR = 8;                        // rows of a thread
 constexpr int kPitch = 68;
 constexpr int kTileFloats = kTile * kPitch;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -59,6 +61,10 @@ template <int n> __device__ __forceinline__ void arrived() {
   __syncthreads();
 }
 
+// The rows of a thread: fours, 32 apart, so that the two that a warp reads at a
+// time lie in different banks.
+__device__ __forceinline__ int row_of(int ty, int i) { return 4 * ty + (i & 3) + 8 * (i & ~3); }
+
 __device__ __forceinline__ float4 ld4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 __device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
   return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
@@ -72,7 +78,7 @@ __device__ __forceinline__ void fma2(float &x, float &y, float a, float b, float
       : "f"(a), "f"(b), "f"(c), "f"(d));
 }
 
-// c[i][j] = sum_d A[kR ty + i][d] B[tx + 16 j][d], even and odd d apart
+// c[i][j] = sum_d A[row i][d] B[tx + 16 j][d], even and odd d apart
 __device__ __forceinline__ void mul_rows(const float *A, const float *B, int ty, int tx, float (&c)[kR][4]) {
   float even[kR][4], odd[kR][4];
 #pragma unroll
@@ -86,7 +92,7 @@ __device__ __forceinline__ void mul_rows(const float *A, const float *B, int ty,
     for (int j = 0; j < 4; ++j) b[j] = ld4(B + (tx + 16 * j) * kPitch + d);
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
-      const float4 a = ld4(A + (kR * ty + i) * kPitch + d);
+      const float4 a = ld4(A + row_of(ty, i) * kPitch + d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         fma2(even[i][j], odd[i][j], a.x, a.y, b[j].x, b[j].y);
@@ -106,7 +112,7 @@ __device__ __forceinline__ void add_row(float (&c)[4], float w, float4 b) {
   fma2(c[2], c[3], w, w, b.z, b.w);
 }
 
-// c[i][u] += sum_k P[kR ty + i][k] B[k][4 tx + u]
+// c[i][u] += sum_k P[row i][k] B[k][4 tx + u]
 __device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, int tx, float (&c)[kR][4]) {
 #pragma unroll 4
   for (int k = 0; k < kTile; k += 4) {
@@ -115,7 +121,7 @@ __device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, in
     for (int e = 0; e < 4; ++e) b[e] = ld4(B + (k + e) * kPitch + 4 * tx);
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
-      const float4 p = ld4(P + (kR * ty + i) * kPitch + k);
+      const float4 p = ld4(P + row_of(ty, i) * kPitch + k);
       add_row(c[i], p.x, b[0]);
       add_row(c[i], p.y, b[1]);
       add_row(c[i], p.z, b[2]);
@@ -124,15 +130,19 @@ __device__ __forceinline__ void mul_p(const float *P, const float *B, int ty, in
   }
 }
 
-// c[i][u] += sum_k P[k][kR ty + i] B[k][4 tx + u]
+// c[i][u] += sum_k P[k][row i] B[k][4 tx + u]
 __device__ __forceinline__ void mul_pt(const float *P, const float *B, int ty, int tx, float (&c)[kR][4]) {
 #pragma unroll 4
   for (int k = 0; k < kTile; ++k) {
-    const float4 b = ld4(B + k * kPitch + 4 * tx), p = ld4(P + k * kPitch + kR * ty);
-    add_row(c[0], p.x, b);
-    add_row(c[1], p.y, b);
-    add_row(c[2], p.z, b);
-    add_row(c[3], p.w, b);
+    const float4 b = ld4(B + k * kPitch + 4 * tx);
+#pragma unroll
+    for (int i = 0; i < kR; i += 4) {
+      const float4 p = ld4(P + k * kPitch + row_of(ty, i));
+      add_row(c[i], p.x, b);
+      add_row(c[i + 1], p.y, b);
+      add_row(c[i + 2], p.z, b);
+      add_row(c[i + 3], p.w, b);
+    }
   }
 }
 
@@ -159,20 +169,26 @@ __device__ __forceinline__ float4 peer4(const float *p, int rank) {
 // own shared memory, rank 0 adds them in their order.
 __device__ __forceinline__ void put(float *P, const float (&c)[kR][4], int ty, int tx) {
 #pragma unroll
-  for (int i = 0; i < kR; ++i) store4(P + (kR * ty + i) * kPitch + 4 * tx, c[i][0], c[i][1], c[i][2], c[i][3]);
+  for (int i = 0; i < kR; ++i) store4(P + row_of(ty, i) * kPitch + 4 * tx, c[i][0], c[i][1], c[i][2], c[i][3]);
 }
 __device__ __forceinline__ void add_peer(const float *P, int rank, float (&c)[kR][4], int ty, int tx) {
 #pragma unroll
   for (int i = 0; i < kR; ++i) {
-    const float4 x = peer4(P + (kR * ty + i) * kPitch + 4 * tx, rank);
+    const float4 x = peer4(P + row_of(ty, i) * kPitch + 4 * tx, rank);
     c[i][0] += x.x, c[i][1] += x.y, c[i][2] += x.z, c[i][3] += x.w;
   }
 }
 
-// CTAs that share a tile: as many as give every SM its two.
-static int cluster_ranks(int64_t slots, int heads) {
+// CTAs that share a tile: as many as make `ctas` in all, so that the longest rows
+// of tiles do not outlast the rest, but no more than twice the tiles of an average
+// sequence, which would find nothing to do.  Two CTAs fit an SM.  12 query
+// and 4 key-value heads, for 2, 3, 4 and 6 times 148: one sequence of 2048 tokens,
+// forward 277, 226, 227 us, dQ 408, 363, 350 us, dK/dV (from 3) 474, 440, 439 us;
+// 1023 tokens in 3 sequences, forward 58, 57, 64 us, dQ 80, 79, 90 us.
+static int cluster_ranks(const PackedArgs &a, int64_t slots, int heads, int ctas) {
+  const int64_t most = 2 * ((a.total + kTile * int64_t(a.S) - 1) / (kTile * int64_t(a.S > 0 ? a.S : 1)));
   int ranks = 1;
-  while (ranks < 8 && slots * heads * ranks < 2 * 148) ranks *= 2;
+  while (ranks < 8 && 2 * ranks <= most && slots * heads * ranks < ctas) ranks *= 2;
   return ranks;
 }
 
@@ -190,7 +206,7 @@ __device__ __forceinline__ float row_sum(float x) {
 
 }  // namespace pk
 
-__global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_constant__ PackedArgs a, int ranks) {
+__global__ void __launch_bounds__(pk::kThreads, 2) packed_fwd_kernel(const __grid_constant__ PackedArgs a, int ranks) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *K = Q + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
@@ -205,7 +221,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
   if (t.rest) {
     if (a.zero_rest && rank == 0)
       for (int i = 0; i < kR; ++i)
-        if (kR * ty + i < rows) store4(out + (kR * ty + i) * a.o_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
+        if (row_of(ty, i) < rows) store4(out + row_of(ty, i) * a.o_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
   }
   const float *kp = static_cast<const float *>(a.k) + t.start * a.k_st + hk * a.k_sh;
@@ -230,7 +246,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
     start(K, kp, a.k_st, next);
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
-      const int row = t.row0 + kR * ty + i;
+      const int row = t.row0 + row_of(ty, i);
       float best = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -244,7 +260,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float p = exp2f(s[i][j] - ref);
-        P[(kR * ty + i) * kPitch + tx + 16 * j] = p;
+        P[row_of(ty, i) * kPitch + tx + 16 * j] = p;
         ps += p;
       }
       l[i] = l[i] * alpha + row_sum(ps);
@@ -263,7 +279,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
       put(P, o, ty, tx);
       if (tx == 0) {
 #pragma unroll
-        for (int i = 0; i < kR; ++i) P[(kR * ty + i) * kPitch + 64] = m[i], P[(kR * ty + i) * kPitch + 65] = l[i];
+        for (int i = 0; i < kR; ++i) P[row_of(ty, i) * kPitch + 64] = m[i], P[row_of(ty, i) * kPitch + 65] = l[i];
       }
     }
     cluster_sync();
@@ -271,7 +287,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
       for (int c = 1; c < ranks; ++c)
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
-          const float *row = P + (kR * ty + i) * kPitch;
+          const float *row = P + row_of(ty, i) * kPitch;
           const float4 ml = peer4(row + 64, c), x = peer4(row + 4 * tx, c);
           const float mn = fmaxf(m[i], ml.x), ref = mn == -INFINITY ? 0.f : mn;
           const float f0 = exp2f(m[i] - ref), f1 = exp2f(ml.x - ref);
@@ -293,10 +309,10 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
       o[i][u] *= inv;
       finite = finite && fabsf(o[i][u]) < INFINITY;
     }
-    const bool held = kR * ty + i < rows;
+    const bool held = row_of(ty, i) < rows;
     if (held) {
-      store4(out + (kR * ty + i) * a.o_st + 4 * tx, o[i][0], o[i][1], o[i][2], o[i][3]);
-      if (a.lse && tx == 0) a.lse[h * a.total + first + kR * ty + i] = m[i] + log2f(l[i]);
+      store4(out + row_of(ty, i) * a.o_st + 4 * tx, o[i][0], o[i][1], o[i][2], o[i][3]);
+      if (a.lse && tx == 0) a.lse[h * a.total + first + row_of(ty, i)] = m[i] + log2f(l[i]);
     }
     // the warp's two rows in turn
     const unsigned bad = __ballot_sync(0xffffffffu, held && !finite);
@@ -304,7 +320,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
     for (int half = 0; half < 2; ++half)
       if (bad >> (16 * half) & 0xffffu) {
         __syncwarp();
-        const int row = __shfl_sync(0xffffffffu, t.row0 + kR * ty + i, 16 * half);
+        const int row = __shfl_sync(0xffffffffu, t.row0 + row_of(ty, i), 16 * half);
         packed_row<float>(a, t.start, row, h, __shfl_sync(0xffffffffu, m[i], 16 * half),
                           __shfl_sync(0xffffffffu, l[i], 16 * half));
       }
@@ -313,7 +329,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_fwd_kernel(const __grid_c
 
 // dQ of a query tile, its key tiles dealt out to the CTAs of a cluster; also
 // delta, which the dK/dV kernel behind it reads.
-__global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs a, int ranks) {
+__global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dq_kernel(PackedArgs a, int ranks) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *G = Q + kTileFloats, *K = G + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
@@ -327,7 +343,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
   float *dq = static_cast<float *>(a.dq) + first * c_st + h * kTile;
   if (t.rest) {
     for (int i = 0; i < kR && rank == 0; ++i)
-      if (kR * ty + i < rows) store4(dq + (kR * ty + i) * c_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
+      if (row_of(ty, i) < rows) store4(dq + row_of(ty, i) * c_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
   }
   load_tile(Q, static_cast<const float *>(a.out) + first * a.o_st + h * a.o_sh, a.o_st, rows);  // O, for delta
@@ -336,7 +352,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
   float delta[kR], lse[kR];
 #pragma unroll
   for (int i = 0; i < kR; ++i) {
-    const int r = kR * ty + i;
+    const int r = row_of(ty, i);
     delta[i] = row_sum(dot4(ld4(Q + r * kPitch + 4 * tx), ld4(G + r * kPitch + 4 * tx), 0.f));
     lse[i] = 0.f;
     if (r < rows) {
@@ -367,9 +383,9 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
     for (int i = 0; i < kR; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool seen = k0 + tx + 16 * j <= t.row0 + kR * ty + i;
+        const bool seen = k0 + tx + 16 * j <= t.row0 + row_of(ty, i);
         const float p = exp2f(s[i][j] * a.scale_log2 - lse[i]);
-        P[(kR * ty + i) * kPitch + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
+        P[row_of(ty, i) * kPitch + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
       }
     __syncwarp();  // a warp reads only the rows of P that it wrote
     mul_p(P, K, ty, tx, acc);
@@ -387,8 +403,8 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
   }
 #pragma unroll
   for (int i = 0; i < kR; ++i)
-    if (kR * ty + i < rows)
-      store4(dq + (kR * ty + i) * c_st + 4 * tx, acc[i][0] * a.scale, acc[i][1] * a.scale, acc[i][2] * a.scale,
+    if (row_of(ty, i) < rows)
+      store4(dq + row_of(ty, i) * c_st + 4 * tx, acc[i][0] * a.scale, acc[i][1] * a.scale, acc[i][2] * a.scale,
              acc[i][3] * a.scale);
 }
 
@@ -396,7 +412,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dq_kernel(PackedArgs 
 // head of the key-value head.  These are dealt out in turn to the CTAs of a
 // cluster (blockIdx.y = kv head x ranks + rank): a short batch has few key
 // tiles, and the first of a sequence has them all.
-__global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs a, int ranks) {
+__global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dkv_kernel(PackedArgs a, int ranks) {
   using namespace pk;
   extern __shared__ __align__(16) float sm[];
   float *K = sm, *V = K + kTileFloats, *Q = V + kTileFloats, *G = Q + kTileFloats, *P = G + kTileFloats,
@@ -437,7 +453,7 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs
         mul_rows(Q, K, ty, tx, s);
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
-          const int r = kR * ty + i;
+          const int r = row_of(ty, i);
           float lse = 0.f, delta = 0.f;
           if (r < rows) {
             lse = a.lse[h * a.total + at + r];
@@ -472,10 +488,10 @@ __global__ void __launch_bounds__(pk::kThreads) packed_bwd_dkv_kernel(PackedArgs
   }
 #pragma unroll
   for (int i = 0; i < kR; ++i)
-    if (kR * ty + i < keys) {
-      store4(dk + (kR * ty + i) * c_st + 4 * tx, sk[i][0] * a.scale, sk[i][1] * a.scale, sk[i][2] * a.scale,
+    if (row_of(ty, i) < keys) {
+      store4(dk + row_of(ty, i) * c_st + 4 * tx, sk[i][0] * a.scale, sk[i][1] * a.scale, sk[i][2] * a.scale,
              sk[i][3] * a.scale);
-      store4(dv + (kR * ty + i) * c_st + 4 * tx, sv[i][0], sv[i][1], sv[i][2], sv[i][3]);
+      store4(dv + row_of(ty, i) * c_st + 4 * tx, sv[i][0], sv[i][1], sv[i][2], sv[i][3]);
     }
 }
 
@@ -525,7 +541,7 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
   const size_t smem = 4 * pk::kTileFloats * sizeof(float);
   if (ensure_smem(packed_fwd_kernel, smem) != SD_OK) return SD_ERR_CUDA;
   const unsigned slots = static_cast<unsigned>(packed_slots(total, nseq, pk::kTile));
-  const int ranks = pk::cluster_ranks(slots, a.Hq);
+  const int ranks = pk::cluster_ranks(a, slots, a.Hq, 3 * 148);
   return launch_cluster(packed_fwd_kernel, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem, s,
                         false, a, ranks);
 }
@@ -560,10 +576,10 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   auto kq = packed_bwd_dq_kernel;
   auto kkv = packed_bwd_dkv_kernel;
   if (ensure_smem(kq, smem_q) != SD_OK || ensure_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
-  int ranks = pk::cluster_ranks(slots, a.Hq);
+  int ranks = pk::cluster_ranks(a, slots, a.Hq, 3 * 148);
   rc = launch_cluster(kq, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_q, s, false, a, ranks);
   if (rc != SD_OK) return rc;
-  ranks = pk::cluster_ranks(slots, a.Hkv);
+  ranks = pk::cluster_ranks(a, slots, a.Hkv, 4 * 148);
   return launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, false, a,
                         ranks);
 }
