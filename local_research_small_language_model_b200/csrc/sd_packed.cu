@@ -17,12 +17,15 @@
 //
 // With few sequences there are few tiles, and the longest decide: so the CTAs of
 // a cluster deal out a tile's other axis, and rank 0 joins their parts.
+// dK/dV's CTAs start as dQ's last ones leave SMs free (one after the other: 235
+// instead of 208 us for the training call below).
+//
 // Measured, 12 query and 4 key-value heads: 1023 tokens in 3 sequences, forward
-// 50 us (62 with one CTA a tile), backward 170 us (36 us for all of it at the fp32
-// pipe's rate); 8096 tokens, the longest sequence 4096, forward 1.21 ms (34
-// TFLOP/s), dQ 1.85 ms (34), dK/dV 2.46 ms (34): half of the 69 that its pipe
-// reaches.  What bounds them: the latency of shared loads behind each barrier
-// between a tile's products, with 8 warps an SM to cover it.
+// 50 us (62 with one CTA a tile), backward 151 us, both from a graph 192 us (36 us
+// at the fp32 pipe's rate); 8096 tokens, the longest sequence 4096, forward 1.22
+// ms (34 TFLOP/s), dQ 1.86 ms (33), dQ and dK/dV together 4.05 ms (36): half of
+// the 69 that the pipe reaches.  What bounds them: the latency of shared loads
+// behind each barrier between a tile's products, with 8 warps an SM to cover it.
 #include "sd_packed.cuh"
 
 namespace sd {
@@ -36,16 +39,8 @@ constexpr int kPitch = 68;
 constexpr int kTileFloats = kTile * kPitch;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// 64 rows (rows past `rows` zero) of 64 values from global memory into a tile.
-__device__ __forceinline__ void load_tile(float *dst, const float *src, int64_t stride, int rows) {
-  for (int e = threadIdx.x; e < kTile * 16; e += kThreads) {
-    const int r = e >> 4, c = (e & 15) * 4;
-    *reinterpret_cast<float4 *>(dst + r * kPitch + c) =
-        r < rows ? *reinterpret_cast<const float4 *>(src + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-}
-
-// The same, arriving while the caller computes (one copy group of the thread).
+// 64 rows (rows past `rows` zero) of 64 values from global memory into a tile,
+// arriving while the caller computes (one copy group of the thread).
 __device__ __forceinline__ void start_tile(float *dst, const float *src, int64_t stride, int rows) {
   for (int e = threadIdx.x; e < kTile * 16; e += kThreads) {
     const int r = e >> 4, c = (e & 15) * 4;
@@ -327,10 +322,25 @@ __global__ void __launch_bounds__(pk::kThreads, 2) packed_fwd_kernel(const __gri
   }
 }
 
-// dQ of a query tile, its key tiles dealt out to the CTAs of a cluster; also
-// delta, which the dK/dV kernel behind it reads.
+// delta, 16 lanes a row.  A kernel of its own, so that both gradients' kernels can
+// read it and the second may start while the first ends.
+__global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a) {
+  using namespace pk;
+  const int64_t n = blockIdx.x * 16ll + (threadIdx.x >> 4);  // row x head
+  const int64_t row = n / a.Hq;
+  const int h = static_cast<int>(n - row * a.Hq), c = 4 * (threadIdx.x & 15);
+  float d = 0.f;
+  if (row < a.total)
+    d = dot4(ld4(static_cast<const float *>(a.out) + row * a.o_st + h * a.o_sh + c),
+             ld4(static_cast<const float *>(a.dout) + row * a.g_st + h * a.g_sh + c), 0.f);
+  d = row_sum(d);
+  if (row < a.total && c == 0) a.delta[h * a.total + row] = d;
+}
+
+// dQ of a query tile, its key tiles dealt out to the CTAs of a cluster.
 __global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dq_kernel(PackedArgs a, int ranks) {
   using namespace pk;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // dK/dV's CTAs take the SMs that this one's leave
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *G = Q + kTileFloats, *K = G + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
   const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x, gridDim.x, kTile, true);
@@ -346,27 +356,20 @@ __global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dq_kernel(PackedAr
       if (row_of(ty, i) < rows) store4(dq + row_of(ty, i) * c_st + 4 * tx, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  load_tile(Q, static_cast<const float *>(a.out) + first * a.o_st + h * a.o_sh, a.o_st, rows);  // O, for delta
-  load_tile(G, static_cast<const float *>(a.dout) + first * a.g_st + h * a.g_sh, a.g_st, rows);
-  __syncthreads();
   float delta[kR], lse[kR];
 #pragma unroll
   for (int i = 0; i < kR; ++i) {
     const int r = row_of(ty, i);
-    delta[i] = row_sum(dot4(ld4(Q + r * kPitch + 4 * tx), ld4(G + r * kPitch + 4 * tx), 0.f));
-    lse[i] = 0.f;
-    if (r < rows) {
-      lse[i] = a.lse[h * a.total + first + r];
-      if (rank == 0 && tx == 0) a.delta[h * a.total + first + r] = delta[i];
-    }
+    delta[i] = r < rows ? a.delta[h * a.total + first + r] : 0.f;
+    lse[i] = r < rows ? a.lse[h * a.total + first + r] : 0.f;
   }
-  __syncthreads();
   const float *kp = static_cast<const float *>(a.k) + t.start * a.k_st + hk * a.k_sh;
   const float *vp = static_cast<const float *>(a.v) + t.start * a.v_st + hk * a.v_sh;
   auto start = [&](float *dst, const float *src, int64_t st, int k0) {
     if (k0 <= t.row0) start_tile(dst, src + k0 * st, st, min(kTile, t.len - k0));
     start_group();
   };
+  start_tile(G, static_cast<const float *>(a.dout) + first * a.g_st + h * a.g_sh, a.g_st, rows);
   start_tile(Q, static_cast<const float *>(a.q) + first * a.q_st + h * a.q_sh, a.q_st, rows);
   start(V, vp, a.v_st, rank * kTile);
   start(K, kp, a.k_st, rank * kTile);
@@ -414,6 +417,9 @@ __global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dq_kernel(PackedAr
 // tiles, and the first of a sequence has them all.
 __global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dkv_kernel(PackedArgs a, int ranks) {
   using namespace pk;
+  // Starts while dQ's last CTAs run, of which it reads nothing; what follows on the
+  // stream follows both, as one CTA here ends after all of dQ's.
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) pdl_wait();
   extern __shared__ __align__(16) float sm[];
   float *K = sm, *V = K + kTileFloats, *Q = V + kTileFloats, *G = Q + kTileFloats, *P = G + kTileFloats,
         *D = P + kTileFloats;
@@ -576,11 +582,16 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   auto kq = packed_bwd_dq_kernel;
   auto kkv = packed_bwd_dkv_kernel;
   if (ensure_smem(kq, smem_q) != SD_OK || ensure_smem(kkv, smem_kv) != SD_OK) return SD_ERR_CUDA;
+  const int64_t delta_ctas = (total * a.Hq + 15) / 16;
+  if (delta_ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
+  packed_delta_kernel<<<static_cast<unsigned>(delta_ctas), 256, 0, s>>>(a);
+  rc = check_launch();
+  if (rc != SD_OK) return rc;
   int ranks = pk::cluster_ranks(a, slots, a.Hq, 3 * 148);
   rc = launch_cluster(kq, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_q, s, false, a, ranks);
   if (rc != SD_OK) return rc;
   ranks = pk::cluster_ranks(a, slots, a.Hkv, 4 * 148);
-  return launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, false, a,
+  return launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, true, a,
                         ranks);
 }
 
