@@ -35,12 +35,16 @@
 // S and dP are computed in both (7 products and 2 exponentials a pair instead
 // of 5 and 1): in return every gradient is summed in tensor memory in a fixed
 // order, with no atomics and no fp32 buffer to add into and convert.
+// A small kernel ahead of them computes delta, so that neither needs the other:
+// dK/dV, whose CTAs are longer, goes first, and dQ's CTAs take the SMs that its
+// last ones leave (one after the other: 457 instead of 416 us at 8192 tokens, 100
+// instead of 78 at 2048).
 //
 // Measured, 12 query and 4 key-value heads, bf16.  One sequence of 32768 tokens:
 // forward 1.74 ms (945 TFLOP/s; 1.00 ms of products, 1.43 ms of exponentials if
-// all ran on the special-function units), backward 6.0 ms (690 TFLOP/s of the 5
-// products a gradient needs, 965 of the 7 it computes).  Training on 16000 tokens
-// in 9 sequences: 0.48 ms, forward and backward.  Of one 8192-token sequence's
+// all ran on the special-function units), backward 5.9 ms (700 TFLOP/s of the 5
+// products a gradient needs, 985 of the 7 it computes).  Training on 16000 tokens
+// in 9 sequences: 0.41 ms, forward and backward.  Of one 8192-token sequence's
 // cycles the forward keeps the special-function units busy for 56 %, instruction
 // issue for 56 % and the tensor pipe for 37 %, dQ 42, 55 and 41 %, dK/dV 38, 62
 // and 50 %: the backward's bound is issue, and its warps' waits for one another
@@ -489,7 +493,7 @@ struct BwdSmem {
   static constexpr int kRowsB = kRowsA + kTileBytes;            // dO or V
   static constexpr int kA = kRowsB + kTileBytes;                // the other side's blocks: K or Q
   static constexpr int kB = kA + kBwdStages * kTileBytes;       // V or dO
-  static constexpr int kVec = kB + kBwdStages * kTileBytes;     // dQ: [128] delta, [128] max |dout|;
+  static constexpr int kVec = kB + kBwdStages * kTileBytes;     // dQ: [128] max |dout|;
   static constexpr int kBar = kVec + 4096;                      // dK/dV: 16 warps x (32 lse, 32 delta)
   static constexpr int kBytes = kBar + 256;
 };
@@ -627,14 +631,76 @@ template <typename T> __device__ __forceinline__ void store_weights(uint32_t tad
   tmem_st16(taddr, w);
 }
 
+// The largest magnitude of eight values; a NaN counts as an infinity.
+template <typename T> __device__ __forceinline__ float largest8(const T *p) {
+  const uint4 x = *reinterpret_cast<const uint4 *>(p);
+  const T *v = reinterpret_cast<const T *>(&x);
+  float big = 0.f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const float y = fabsf(to_f(v[u]));
+    big = y <= big ? big : (y < INFINITY ? y : INFINITY);
+  }
+  return big;
+}
+
 }  // namespace pt
+
+// delta = rowsum(dout out), for fp16 also the largest |dout| of all sequences' rows;
+// eight lanes a row and head.  A kernel of its own, so that both gradients'
+// kernels can read it and the second may start while the first ends.
+template <typename T> __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const PackedArgs a, unsigned *top) {
+  using namespace pt;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  const int64_t n = blockIdx.x * 32ll + (threadIdx.x >> 3), row = n / a.Hq;
+  const int h = static_cast<int>(n - row * a.Hq), c = 8 * (threadIdx.x & 7);
+  float delta = 0.f;
+  const bool in = row < a.total;
+  if (in) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.out) + row * a.o_st + h * a.o_sh + c);
+    const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.dout) + row * a.g_st + h * a.g_sh + c);
+    uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    // out in twice its bits: delta's error is the same for a whole row of dS, and would add up
+    if (a.rest) z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.rest) + (row * a.Hq + h) * 64 + c);
+    const T *po = reinterpret_cast<const T *>(&x), *pg = reinterpret_cast<const T *>(&y),
+            *pz = reinterpret_cast<const T *>(&z);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      delta = fmaf(to_f(po[u]), to_f(pg[u]), delta);
+      delta = fmaf(to_f(pz[u]), to_f(pg[u]), delta);
+    }
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, o);
+  if (in && c == 0) a.delta[h * a.total + row] = delta;
+  if (kHalf) {
+    const bool counts = in && row >= packed_bound(a.cu, a.S, a.total, 1) && row < packed_bound(a.cu, a.S, a.total, a.S + 1);
+    float big = counts ? largest8(static_cast<const T *>(a.dout) + row * a.g_st + h * a.g_sh + c) : 0.f;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    if (!(big < INFINITY)) big = 0.f;  // such a row's gradients are not finite whatever the scale
+    __shared__ unsigned most[8];
+    const unsigned warp_most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = warp_most;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const unsigned all = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? most[threadIdx.x] : 0u);
+      // few CTAs find a larger one than is known already: the maximum is the same in any order
+      if (threadIdx.x == 0 && all > *static_cast<volatile unsigned *>(top)) atomicMax(top, all);
+    }
+  }
+}
+
 
 template <typename T>
 __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     packed_bwd_dq_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
                             const __grid_constant__ CUtensorMap tmg, const __grid_constant__ CUtensorMap tmk,
-                            const __grid_constant__ CUtensorMap tmv, unsigned *top, int32_t *err) {
+                            const __grid_constant__ CUtensorMap tmv, int32_t *err) {
   using namespace pt;
+  // Starts while dK/dV's last CTAs run, of which it reads nothing; what follows on
+  // the stream follows both, as one CTA here ends after all of theirs.
+  if (blockIdx.x == gridDim.x - 1) pdl_wait();
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr uint32_t fmt = kHalf ? 0u : 1u;
   const int h = blockIdx.x % a.Hq;
@@ -650,7 +716,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
   extern __shared__ __align__(1024) char smem_raw[];
   char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float *vec = reinterpret_cast<float *>(sm + BwdSmem::kVec);
+  float *most = reinterpret_cast<float *>(sm + BwdSmem::kVec);
   BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = h / (a.Hq / a.Hkv);
@@ -659,47 +725,15 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (tid == 32 * kBwdCopy) bwd_init(bars);
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  if (warp < 16) {  // delta, and for fp16 the largest |dout|: eight lanes a row, eight rows a warp
-    float delta[2], big[2];
+  if (kHalf && warp < 16) {  // the rows' largest |dout|: eight lanes a row, eight rows a warp
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = 8 * warp + 4 * i + (lane >> 3), c = 8 * (lane & 7);
-      delta[i] = big[i] = 0.f;
-      if (row < rows) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.out) + (first + row) * a.o_st +
-                                                         h * a.o_sh + c);
-        const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.dout) + (first + row) * a.g_st +
-                                                         h * a.g_sh + c);
-        uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        // out in twice its bits: delta's error is the same for a whole row of dS, and would add up
-        if (a.rest)
-          z = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.rest) + ((first + row) * a.Hq + h) * 64 + c);
-        const T *po = reinterpret_cast<const T *>(&x), *pg = reinterpret_cast<const T *>(&y),
-                *pz = reinterpret_cast<const T *>(&z);
+      float big = 0.f;
+      if (row < rows) big = largest8(static_cast<const T *>(a.dout) + (first + row) * a.g_st + h * a.g_sh + c);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          delta[i] = fmaf(to_f(po[u]), to_f(pg[u]), delta[i]);
-          delta[i] = fmaf(to_f(pz[u]), to_f(pg[u]), delta[i]);
-          if (kHalf) big[i] = fmaxf(big[i], fabsf(to_f(pg[u])));
-        }
-      }
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        delta[i] += __shfl_xor_sync(0xffffffffu, delta[i], o);
-        if (kHalf) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], o));
-      }
-      if (kHalf && !(big[i] < INFINITY)) big[i] = 0.f;
-      if ((lane & 7) == 0) {
-        vec[row] = delta[i];
-        if (row < rows) a.delta[h * a.total + first + row] = delta[i];
-        if (kHalf) vec[128 + row] = big[i];
-      }
-    }
-    if (kHalf) {
-      float most = fmaxf(big[0], big[1]);
-#pragma unroll
-      for (int o = 16; o >= 8; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (lane == 0) atomicMax(top, __float_as_uint(most));
+      for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      if ((lane & 7) == 0) most[row] = big < INFINITY ? big : 0.f;
     }
   }
   fence_before_sync();
@@ -724,8 +758,9 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     });
   } else {
     const uint32_t t_s = tmem + lane_base + kColS + 32 * wg;
-    const float delta = vec[r], lse = r < rows ? a.lse[h * a.total + first + r] : 0.f;
-    const float f = kHalf ? unit_scale(vec[128 + r]) : 1.f;
+    const float delta = r < rows ? a.delta[h * a.total + first + r] : 0.f;
+    const float lse = r < rows ? a.lse[h * a.total + first + r] : 0.f;
+    const float f = kHalf ? unit_scale(most[r]) : 1.f;
     for (int i = 0; i < blocks; ++i) {
       ok = mbar_wait(&bars->sd_full, i & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
@@ -774,7 +809,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (failed) bwd_failed(bars, err);
   if (warp < 4) {
     fence_after_sync();
-    const float back = failed ? __int_as_float(0x7fc00000) : a.scale / (kHalf ? unit_scale(vec[128 + r]) : 1.f);
+    const float back = failed ? __int_as_float(0x7fc00000) : a.scale / (kHalf ? unit_scale(most[r]) : 1.f);
     store_rows(dq + 32 * warp * c_st, c_st, rows - 32 * warp, tmem + lane_base + kDqAcc, back,
                sm + BwdSmem::kRowsA + warp * 4096);
   }
@@ -792,6 +827,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
                              const __grid_constant__ CUtensorMap tmg, const __grid_constant__ CUtensorMap tmk,
                              const __grid_constant__ CUtensorMap tmv, const unsigned *top, int32_t *err) {
   using namespace pt;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // dQ's CTAs take the SMs that this one's leave
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr uint32_t fmt = kHalf ? 0u : 1u;
   const int hk = blockIdx.x % a.Hkv, group = a.Hq / a.Hkv;
@@ -993,17 +1029,24 @@ int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
     }
   }
   const size_t smem = pt::BwdSmem::kBytes + 1024;
-  auto run = [&](auto *dq, auto *dkv) {
+  const int64_t delta_ctas = (a.total * a.Hq + 31) / 32;
+  if (delta_ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
+  auto run = [&](auto *delta, auto *dq, auto *dkv) {
     if (ensure_smem(dq, smem) != SD_OK || ensure_smem(dkv, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
-    dq<<<static_cast<unsigned>(slots * a.Hq), pt::kBwdThreads, smem, s>>>(a, mq, mg, mk, mv, top, err);
-    const int first = check_launch();
-    if (first != SD_OK) return first;
+    delta<<<static_cast<unsigned>(delta_ctas), 256, 0, s>>>(a, top);
+    int rc = check_launch();
+    if (rc != SD_OK) return rc;
+    // the kernel with the longer CTAs first: the other's fill the SMs that its last ones leave
     dkv<<<static_cast<unsigned>(slots * a.Hkv), pt::kBwdThreads, smem, s>>>(a, mq, mg, mk, mv, top, err);
-    return check_launch();
+    rc = check_launch();
+    if (rc != SD_OK) return rc;
+    return launch(dq, dim3(static_cast<unsigned>(slots * a.Hq)), dim3(pt::kBwdThreads), smem, s, true, a, mq, mg, mk,
+                  mv, err);
   };
-  return dtype == SD_DTYPE_BF16
-             ? run(packed_bwd_dq_tc_kernel<__nv_bfloat16>, packed_bwd_dkv_tc_kernel<__nv_bfloat16>)
-             : run(packed_bwd_dq_tc_kernel<__half>, packed_bwd_dkv_tc_kernel<__half>);
+  return dtype == SD_DTYPE_BF16 ? run(packed_delta_tc_kernel<__nv_bfloat16>, packed_bwd_dq_tc_kernel<__nv_bfloat16>,
+                                      packed_bwd_dkv_tc_kernel<__nv_bfloat16>)
+                                : run(packed_delta_tc_kernel<__half>, packed_bwd_dq_tc_kernel<__half>,
+                                      packed_bwd_dkv_tc_kernel<__half>);
 }
 
 }  // namespace sd
