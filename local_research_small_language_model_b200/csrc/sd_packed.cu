@@ -17,15 +17,16 @@
 //
 // With few sequences there are few tiles, and the longest decide: so the CTAs of
 // a cluster deal out a tile's other axis, and rank 0 joins their parts.
-// dK/dV's CTAs start as dQ's last ones leave SMs free (one after the other: 235
-// instead of 208 us for the training call below).
+// dK/dV goes before dQ, whose CTAs are shorter and start as the first's last ones
+// leave SMs free (8096 tokens: 4.35 ms one after the other, 4.06 ms with dQ first,
+// 3.83 ms so).
 //
 // Measured, 12 query and 4 key-value heads: 1023 tokens in 3 sequences, forward
-// 50 us (62 with one CTA a tile), backward 151 us, both from a graph 192 us (36 us
-// at the fp32 pipe's rate); 8096 tokens, the longest sequence 4096, forward 1.22
-// ms (34 TFLOP/s), dQ 1.86 ms (33), dQ and dK/dV together 4.05 ms (36): half of
-// the 69 that the pipe reaches.  What bounds them: the latency of shared loads
-// behind each barrier between a tile's products, with 8 warps an SM to cover it.
+// 50 us (62 with one CTA a tile), backward 146 us (36 us for all of it at the fp32
+// pipe's rate); 8096 tokens, the longest sequence 4096, forward 1.22 ms (34
+// TFLOP/s), backward 3.83 ms (38): half of the 69 that the pipe reaches.  What
+// bounds them: the latency of shared loads behind each barrier between a tile's
+// products, with 8 warps an SM to cover it.
 #include "sd_packed.cuh"
 
 namespace sd {
@@ -340,7 +341,9 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a) {
 // dQ of a query tile, its key tiles dealt out to the CTAs of a cluster.
 __global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dq_kernel(PackedArgs a, int ranks) {
   using namespace pk;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // dK/dV's CTAs take the SMs that this one's leave
+  // Starts while dK/dV's last CTAs run, of which it reads nothing; what follows on
+  // the stream follows both, as one CTA here ends after all of theirs.
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) pdl_wait();
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *G = Q + kTileFloats, *K = G + kTileFloats, *V = K + kTileFloats, *P = V + kTileFloats;
   const PackedTile t = packed_nth(a.cu, a.S, a.total, blockIdx.x, gridDim.x, kTile, true);
@@ -417,9 +420,7 @@ __global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dq_kernel(PackedAr
 // tiles, and the first of a sequence has them all.
 __global__ void __launch_bounds__(pk::kThreads, 2) packed_bwd_dkv_kernel(PackedArgs a, int ranks) {
   using namespace pk;
-  // Starts while dQ's last CTAs run, of which it reads nothing; what follows on the
-  // stream follows both, as one CTA here ends after all of dQ's.
-  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) pdl_wait();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // dQ's CTAs take the SMs that this one's leave
   extern __shared__ __align__(16) float sm[];
   float *K = sm, *V = K + kTileFloats, *Q = V + kTileFloats, *G = Q + kTileFloats, *P = G + kTileFloats,
         *D = P + kTileFloats;
@@ -587,12 +588,12 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   packed_delta_kernel<<<static_cast<unsigned>(delta_ctas), 256, 0, s>>>(a);
   rc = check_launch();
   if (rc != SD_OK) return rc;
-  int ranks = pk::cluster_ranks(a, slots, a.Hq, 3 * 148);
-  rc = launch_cluster(kq, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_q, s, false, a, ranks);
+  int ranks = pk::cluster_ranks(a, slots, a.Hkv, 4 * 148);
+  rc = launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, false, a,
+                      ranks);
   if (rc != SD_OK) return rc;
-  ranks = pk::cluster_ranks(a, slots, a.Hkv, 4 * 148);
-  return launch_cluster(kkv, dim3(slots, a.Hkv * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_kv, s, true, a,
-                        ranks);
+  ranks = pk::cluster_ranks(a, slots, a.Hq, 3 * 148);
+  return launch_cluster(kq, dim3(slots, a.Hq * ranks), dim3(pk::kThreads), dim3(1, ranks, 1), smem_q, s, true, a, ranks);
 }
 
 }  // extern "C"
