@@ -355,6 +355,53 @@ def test_streams_and_graph_replay(dev, dtype):
                 assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("lengths", [[1], [700, 5, 40], [2500], [90] * 12], ids=["one", "mixed", "long", "equal"])
+def test_what_follows_the_backward_waits_for_all_of_it(dev, dtype, lengths):
+    """Inputs overwritten and gradients read right behind the call on its stream,
+    and calls one behind the other, give the bits of calls that stand alone."""
+    total = sum(lengths)
+    cu = torch.tensor(bounds(lengths), dtype=torch.int32, device=dev)
+    sets = [inputs(dev, dtype, total, 12, 4, seed=20 + i) for i in range(3)]
+    want = []
+    for q, k, v, dout in sets:
+        out, lse = ops.packed_attention(q, k, v, cu, return_lse=True)
+        torch.cuda.synchronize()
+        want.append(ops.packed_attention_backward(q, k, v, out, dout, lse, cu))
+        torch.cuda.synchronize()
+    got = []
+    for q, k, v, dout in sets:
+        q, k, v, dout = (x.clone() for x in (q, k, v, dout))
+        out, lse = ops.packed_attention(q, k, v, cu, return_lse=True)
+        grads = ops.packed_attention_backward(q, k, v, out, dout, lse, cu)
+        for x in (q, k, v, dout, out, lse):
+            x.fill_(7.0)
+        copies = [x.clone() for x in grads]
+        for x in grads:
+            x.fill_(7.0)
+        got.append(copies)
+    for g, w in zip(got, want):
+        for x, y in zip(g, w):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t)[6:])
+def test_gradients_outside_the_sequences_do_not_count(dev, dtype):
+    """dout's rows outside every sequence change no bit of a gradient, be they
+    large (they take no part in fp16's common scale), infinite or NaN."""
+    total, cu = 200, torch.tensor([40, 130, 170], dtype=torch.int32, device=dev)
+    q, k, v, dout = inputs(dev, dtype, total, 4, 2, seed=31)
+    out, lse = ops.packed_attention(q, k, v, cu, return_lse=True)
+    want = ops.packed_attention_backward(q, k, v, out, dout, lse, cu)
+    for bad in (3.0e4, math.inf, math.nan):
+        other = dout.clone()
+        other[:40] = bad
+        other[170:] = bad
+        got = ops.packed_attention_backward(q, k, v, out, other, lse, cu)
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
 def test_malformed_bounds_stay_inside(dev):
     """Bounds that descend or leave the rows give wrong rows, not faults: the
     memory around the output is untouched."""
