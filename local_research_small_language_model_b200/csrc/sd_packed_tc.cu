@@ -674,7 +674,8 @@ template <typename T> __global__ void __launch_bounds__(256) packed_delta_tc_ker
   for (int o = 4; o > 0; o >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, o);
   if (in && c == 0) a.delta[h * a.total + row] = delta;
   if (kHalf) {
-    const bool counts = in && row >= packed_bound(a.cu, a.S, a.total, 1) && row < packed_bound(a.cu, a.S, a.total, a.S + 1);
+    const bool counts = in && row >= packed_bound(a.cu, a.S, a.total, 1) &&
+                        row < packed_bound(a.cu, a.S, a.total, a.S + 1);
     float big = counts ? largest8(static_cast<const T *>(a.dout) + row * a.g_st + h * a.g_sh + c) : 0.f;
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
