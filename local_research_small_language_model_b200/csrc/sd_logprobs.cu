@@ -34,7 +34,7 @@ constexpr int kAbove = 4096;            // room for the values above that bound,
 constexpr int kTies = 512;              // and for those equal to it
 constexpr int kCandidates = kAbove + kTies;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFloor = -1e4f;         // stands for -inf: its exponential is 0 and 0 * kFloor is 0
+constexpr float kFloor = -1e4f;         // stands for what is below it: its exponential is 0 and 0 * kFloor is 0
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -59,7 +59,8 @@ __device__ __forceinline__ void raise(Stat &a, float top) {
     a.m = top;
     return;  // s and w are 0, or NaN
   }
-  const float d = a.m - top, c = ex2(d * kLog2e);
+  // a sum of masked values (the type's lowest, or far below) times their distance would pass the range of fp32
+  const float d = fmaxf(a.m - top, kFloor), c = ex2(d * kLog2e);
   a.w = c * fmaf(a.s, d, a.w);
   a.s *= c;
   a.m = top;
@@ -84,13 +85,14 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 // N values (N even) with their largest and smallest (NaNs left out).  Nearly
-// always none is -inf, and its guard is left out for all.
+// always none is -inf or so far below that its distance could overflow, and the
+// guard is left out for all.
 template <int N> __device__ __forceinline__ void add(Stat &a, const float (&x)[N], float top, float least) {
   raise(a, top);
   const float ref = a.m == -INFINITY ? 0.f : a.m;
   const float2 neg = {-ref, -ref}, log2e = {kLog2e, kLog2e}, zero = {0.f, 0.f};
   float2 s[2] = {}, w[2] = {};
-  const bool guard = least == -INFINITY;
+  const bool guard = least - ref < kFloor;
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
     float2 d = add2({x[i], x[i + 1]}, neg);
