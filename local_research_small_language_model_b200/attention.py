@@ -381,9 +381,10 @@ class B200DenseAttention(BaseAttention):
                 ragged: Optional[RaggedBatch] = None, **kwargs):
         b, t, _ = x.shape
         # gradients reach wq, wk and wv through their own products
-        grad = torch.is_grad_enabled() and (x.requires_grad or self.wq.weight.requires_grad)
+        proj = (self.wq, self.wk, self.wv)
+        grad = torch.is_grad_enabled() and (x.requires_grad or any(w.weight.requires_grad for w in proj))
         if grad:
-            heads = [w(x).view(b * t, -1, self.head_dim) for w in (self.wq, self.wk, self.wv)]
+            heads = [w(x).view(b * t, -1, self.head_dim) for w in proj]
         else:
             rows = F.linear(x, self.qkv_weight()).view(b * t, -1, self.head_dim)
             heads = rows.split([self.n_head, self.n_kv_head, self.n_kv_head], dim=1)
