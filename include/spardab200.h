@@ -450,8 +450,11 @@ SD_API int sd_packed_attention_backward(const void *q, const void *k, const void
  * With cu_seqlens (device int32 [B + 1]) rows cu_seqlens[b] .. of sequence b
  * take positions lens[b], lens[b] + 1, ..; without it N == B and row b is
  * sequence b's one new token.  lens is not changed.  A row whose position or
- * page is out of range is dropped and SD_KERR_BOUNDS is written to *err.  Two
- * rows that name the same place leave either one's values there. */
+ * page is out of range is dropped and SD_KERR_BOUNDS is written to *err; with
+ * lens[b] == SD_LEN_ABSENT sequence b takes no part and its rows are dropped
+ * without a report.  Two rows that name the same place leave either one's
+ * values there. */
+#define SD_LEN_ABSENT (-2147483647 - 1)
 SD_API int sd_paged_append(const void *xk, const void *xv, int dtype, int64_t N, int64_t Hkv, int64_t D,
                            int64_t k_sn, int64_t k_sh, int64_t v_sn, int64_t v_sh, void *k_pages, void *v_pages,
                            int64_t pages, int page, int64_t p_sp, int64_t p_sh, int64_t p_st, const int32_t *table,

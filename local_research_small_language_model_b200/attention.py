@@ -3,7 +3,7 @@ whose hot path runs on the sm_100a kernels of libspardab200.so."""
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 import torch.nn as nn
@@ -11,7 +11,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from .cache import B200KVCache, B200PagedKVCache
+from .cache import B200KVCache, B200PagedKVCache, PageTable
 from .offload import B200OffloadKVCache
 from .forecast import ForecastBlockSelector, KVBlockCompressor
 from .rope import apply_rotary_emb
@@ -333,34 +333,42 @@ class B200SparseAttention(BaseAttention):
 
 class RaggedBatch:
     """What every layer of one ragged forward shares: the bounds of the packed
-    sequences, or for a decode step of one token each the lengths with that
-    token; and the RoPE rows of the tokens' own positions, fp32 [tokens, D/2]."""
+    sequences, or for a decode step of one token each the lengths with and
+    without that token; and the RoPE rows of the tokens' own positions, fp32
+    [tokens, D/2].  lengths: of packed prompts, where the host knows them."""
 
     def __init__(self, cos: torch.Tensor, sin: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
-                 lens_after: Optional[torch.Tensor] = None):
+                 lens_after: Optional[torch.Tensor] = None, lens_before: Optional[torch.Tensor] = None,
+                 lengths: Optional[Sequence[int]] = None):
         self.cos, self.sin, self.cu_seqlens, self.lens_after = cos, sin, cu_seqlens, lens_after
+        self.lens_before, self.lengths = lens_before, lengths
 
     @classmethod
-    def prompts(cls, cu_seqlens: torch.Tensor, total: int, rotary_emb, longest: Optional[int] = None) -> "RaggedBatch":
+    def prompts(cls, cu_seqlens: torch.Tensor, total: int, rotary_emb, longest: Optional[int] = None,
+                lengths: Optional[Sequence[int]] = None) -> "RaggedBatch":
         """Packed prompts: the token at row r of sequence s has position
         r - cu_seqlens[s].  Bounds stay on the device; the RoPE tables are
         grown to ``longest``, the longest sequence where the host knows it
-        (else ``total``)."""
+        (else ``total``).  ``lengths`` on the host allow a cache in which other
+        sequences hold tokens."""
         longest = total if longest is None else longest
         rotary_emb.ensure(longest)
         rows = torch.arange(total, device=cu_seqlens.device)
         bounds = cu_seqlens.to(torch.int64)
         seq = torch.searchsorted(bounds, rows, right=True) - 1
         pos = (rows - bounds[seq.clamp_min(0)]).clamp(0, max(longest - 1, 0))
-        return cls(rotary_emb.cos[pos], rotary_emb.sin[pos], cu_seqlens=cu_seqlens)
+        return cls(rotary_emb.cos[pos], rotary_emb.sin[pos], cu_seqlens=cu_seqlens, lengths=lengths)
 
     @classmethod
-    def step(cls, lens: torch.Tensor, capacity: int, rotary_emb) -> "RaggedBatch":
+    def step(cls, lens: torch.Tensor, capacity: int, rotary_emb,
+             pages: Optional[PageTable] = None) -> "RaggedBatch":
         """One new token per sequence, at the positions lens (device int32,
-        each below ``capacity``)."""
+        each below ``capacity``).  With ``pages``, their released sequences
+        (length 0) take no part: no token is written, and none attended to."""
         rotary_emb.ensure(capacity)
         pos = lens.to(torch.int64).clamp(0, capacity - 1)
-        return cls(rotary_emb.cos[pos], rotary_emb.sin[pos], lens_after=lens + 1)
+        after, before = (lens + 1, lens) if pages is None else (lens + pages.active, lens + pages.absent)
+        return cls(rotary_emb.cos[pos], rotary_emb.sin[pos], lens_after=after, lens_before=before)
 
 
 class B200DenseAttention(BaseAttention):
@@ -372,9 +380,10 @@ class B200DenseAttention(BaseAttention):
 
     x is [B,T,C]: B sequences of T tokens, or with ``ragged`` (a RaggedBatch
     with bounds) one row [1,total,C] of packed sequences.  ``kv_cache`` is a
-    B200PagedKVCache whose PageTable has the pages reserved: prompts (its
-    sequences empty so far) or, with T == 1 and no bounds, one decode step of
-    every sequence.  The caller advances the PageTable after the last layer."""
+    B200PagedKVCache whose PageTable has the pages reserved: prompts (of
+    sequences that are empty so far) or, with T == 1 and no bounds, one decode
+    step of every sequence.  The caller advances the PageTable after the last
+    layer."""
 
     def forward(self, x: torch.Tensor, rotary_emb, kv_cache=None, mask: Optional[torch.Tensor] = None,
                 is_causal: bool = True, forecast_vector: Optional[torch.Tensor] = None,
@@ -406,10 +415,11 @@ class B200DenseAttention(BaseAttention):
                                                     else ragged.cu_seqlens is None)
         if ragged is None:
             if step:
-                ragged = RaggedBatch.step(kv_cache.pages.lens, kv_cache.pages.capacity, rotary_emb)
+                pages = kv_cache.pages
+                ragged = RaggedBatch.step(pages.lens, pages.capacity, rotary_emb, pages)
             else:
                 bounds = torch.arange(0, (b + 1) * t, t, dtype=torch.int32, device=xq.device)
-                ragged = RaggedBatch.prompts(bounds, b * t, rotary_emb, t)
+                ragged = RaggedBatch.prompts(bounds, b * t, rotary_emb, t, [t] * b)
         if not step and b != 1 and ragged.cu_seqlens.numel() != b + 1:
             raise ValueError(f"{ragged.cu_seqlens.numel() - 1} packed sequences do not fit {b} rows of {t} tokens")
         rope = _RopeQK.apply if grad else ops.rope_qk
@@ -417,9 +427,9 @@ class B200DenseAttention(BaseAttention):
         if kv_cache is None:
             return packed_attention(xq, xk, xv, ragged.cu_seqlens)
         pages = kv_cache.pages
-        if not step and any(pages.held):
+        if not step and pages.fills(ragged.lengths):
             raise NotImplementedError("prefill into a non-empty cache")
-        kv_cache.append(xk, xv, ragged.cu_seqlens)
+        kv_cache.append(xk, xv, ragged.cu_seqlens, ragged.lens_before)
         if step:
             return ops.paged_decode_attention(xq, kv_cache.k_pages, kv_cache.v_pages, pages.table,
                                               ragged.lens_after)

@@ -80,10 +80,14 @@ class PageTable:
 
       table  int32 [max_seqs, width] on the device: position t of sequence b
              lies in page table[b, t // page_size]; -1 where none is held;
-      lens   int32 [max_seqs] on the device, tokens cached so far.
+      lens   int32 [max_seqs] on the device, tokens cached so far;
+      active int32 [max_seqs] on the device: 0 for a released sequence, which
+             takes no part in decode steps until a prompt takes its place, else 1
+             (absent: 0 where active is 1, else ops.LEN_ABSENT).
 
-    The host keeps the same lengths (``held``), each sequence's pages and the
-    free pages; ``reserve`` before a forward, ``advance`` after it."""
+    The host keeps the same lengths (``held``), each sequence's pages, the
+    released sequences and the free pages; ``reserve`` before a forward,
+    ``advance`` after it."""
 
     def __init__(self, max_seqs: int, max_seq_len: int, num_pages: int, device: torch.device, page_size: int = 64):
         if min(max_seqs, max_seq_len, num_pages, page_size) < 1:
@@ -93,23 +97,30 @@ class PageTable:
         self.capacity = self.width * page_size
         self.table = torch.full((max_seqs, self.width), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self.active = torch.ones(max_seqs, dtype=torch.int32, device=device)
+        self.absent = torch.zeros(max_seqs, dtype=torch.int32, device=device)
         self.reset_host()
 
     def reset_host(self) -> None:
         self.held: List[int] = [0] * self.max_seqs
         self.owned: List[List[int]] = [[] for _ in range(self.max_seqs)]
         self.free: List[int] = list(range(self.num_pages - 1, -1, -1))
+        self.released: List[bool] = [False] * self.max_seqs
 
     def _counts(self, counts) -> List[int]:
-        counts = [int(counts)] * self.max_seqs if isinstance(counts, int) else [int(c) for c in counts]
+        if isinstance(counts, int):
+            counts = [min(counts, 0) if out else counts for out in self.released]
+        else:
+            counts = [int(c) for c in counts]
         if len(counts) != self.max_seqs or min(counts) < 0:
             raise ValueError(f"need {self.max_seqs} non-negative token counts, got {counts}")
         return counts
 
     def reserve(self, counts) -> None:
-        """Pages for counts[b] more tokens of every sequence b (or the same
-        number for all).  Raises, with nothing changed, when a sequence would
-        pass its longest or the pool has too few pages."""
+        """Pages for counts[b] more tokens of every sequence b, or the same
+        number for all but the released ones.  A list's tokens for a released
+        sequence take its place up again.  Raises, with nothing changed, when a
+        sequence would pass its longest or the pool has too few pages."""
         counts = self._counts(counts)
         need = []
         for b, c in enumerate(counts):
@@ -128,10 +139,26 @@ class PageTable:
         if pages:
             where = torch.tensor([rows, cols, pages], dtype=torch.int64).to(self.table.device)
             self.table[where[0], where[1]] = where[2].to(torch.int32)
+        for b, c in enumerate(counts):
+            if c and self.released[b]:
+                self._take_part(b, True)
+
+    def _take_part(self, seq: int, yes: bool) -> None:
+        self.released[seq] = not yes
+        self.active[seq] = int(yes)
+        self.absent[seq] = 0 if yes else ops.LEN_ABSENT
+
+    def fills(self, lengths) -> bool:
+        """Whether prompts of these lengths (None: unknown) would reach a
+        sequence that holds tokens."""
+        if lengths is None:
+            return any(self.held)
+        return any(n and h for n, h in zip(lengths, self.held))
 
     def advance(self, counts, device: bool = True) -> None:
-        """Counts the tokens of a finished forward: on the host and, unless a
-        captured step does that itself, on the device."""
+        """Counts the tokens of a finished forward (counts as in reserve): on
+        the host and, unless a captured step does that itself, on the device."""
+        same = counts if isinstance(counts, int) else None
         counts = self._counts(counts)
         for b, c in enumerate(counts):
             if self.held[b] + c > len(self.owned[b]) * self.page_size:
@@ -139,24 +166,31 @@ class PageTable:
         for b, c in enumerate(counts):
             self.held[b] += c
         if device:
-            if len(set(counts)) == 1:
+            if same is not None:  # a captured step follows later releases
+                self.lens.add_(self.active, alpha=same)
+            elif len(set(counts)) == 1:
                 self.lens.add_(counts[0])
             else:
                 self.lens.add_(torch.tensor(counts, dtype=torch.int32).to(self.lens.device))
 
     def release(self, seq: int) -> None:
-        """Frees a finished sequence's pages; its row starts empty again."""
+        """Frees a finished sequence's pages.  It takes no part in the steps
+        that follow (its row of their results is that of no context); a prompt
+        may take its place."""
         if not 0 <= seq < self.max_seqs:
             raise ValueError(f"no sequence {seq} of {self.max_seqs}")
         self.free.extend(reversed(self.owned[seq]))
         self.owned[seq], self.held[seq] = [], 0
         self.table[seq].fill_(-1)
         self.lens[seq] = 0
+        self._take_part(seq, False)
 
     def reset(self) -> None:
         self.reset_host()
         self.table.fill_(-1)
         self.lens.zero_()
+        self.active.fill_(1)
+        self.absent.zero_()
 
 
 class B200PagedKVCache:
@@ -172,9 +206,11 @@ class B200PagedKVCache:
         self.k_pages = torch.zeros(shape, device=device, dtype=dtype)
         self.v_pages = torch.zeros(shape, device=device, dtype=dtype)
 
-    def append(self, xk: torch.Tensor, xv: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    def append(self, xk: torch.Tensor, xv: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+               lens: Optional[torch.Tensor] = None) -> None:
         """Writes rows xk, xv [N,H,D] behind the cached tokens of their
-        sequences (one row each, or packed by cu_seqlens); lengths are
-        advanced on the PageTable, once for all layers."""
+        sequences (one row each, or packed by cu_seqlens; ``lens`` in place of
+        the PageTable's, ops.LEN_ABSENT for a sequence whose row is not
+        written); lengths are advanced on the PageTable, once for all layers."""
         ops.paged_append(xk.to(self.k_pages.dtype), xv.to(self.v_pages.dtype), self.k_pages, self.v_pages,
-                         self.pages.table, self.pages.lens, cu_seqlens)
+                         self.pages.table, self.pages.lens if lens is None else lens, cu_seqlens)

@@ -49,8 +49,8 @@ __device__ __forceinline__ int64_t row_of(const PagedArgs &a, int b, int h, int 
 // The append: kTok rows a CTA, whose places the first kTok threads look up; then
 // all threads move 16-byte chunks of K and V, several in flight each.  cu
 // (nullable): token rows [cu[b], cu[b + 1]) belong to sequence b; without it row
-// b is sequence b's one token.  Rows outside every sequence are not written
-// anywhere.  HBM-bound: 32768 rows of 4 bf16 heads into pages of 64 tokens in
+// b is sequence b's one token.  Rows outside every sequence, and those of an
+// absent one, are not written anywhere.  HBM-bound: 32768 rows of 4 bf16 heads into pages of 64 tokens in
 // 12.4 us (67 MB, 5.4 TB/s with the launch); 64 single tokens 4.2 us, the launch
 // and three loads that depend on one another (length, page, value).
 template <typename T, int kTok>
@@ -76,8 +76,9 @@ __global__ void __launch_bounds__(256)
       held = n >= cu[b] && n < cu[b + 1];
       t = n - cu[b];
     }
-    if (held) {
-      t += a.lens[b];
+    const int before = held ? a.lens[b] : SD_LEN_ABSENT;
+    if (before != SD_LEN_ABSENT) {
+      t += before;
       if (t >= 0 && t < static_cast<int64_t>(a.width) * a.page) off = pg::row_of(a, b, 0, static_cast<int>(t));
       if (off < 0) pg::report(a.err, SD_KERR_BOUNDS);
     }

@@ -407,9 +407,7 @@ class SparDAB200Model(nn.Module):
             raise ValueError(f"{b} rows for a cache of {pages.max_seqs} sequences")
         if pages is not None and cu_seqlens is None and t == 1 and any(pages.held):
             pages.reserve(1)
-            return RaggedBatch.step(pages.lens, pages.capacity, self.rotary_emb), pages, 1
-        if pages is not None and any(pages.held):
-            raise NotImplementedError("prefill into a non-empty cache")
+            return RaggedBatch.step(pages.lens, pages.capacity, self.rotary_emb, pages), pages, 1
         if cu_seqlens is None:
             cu_seqlens = torch.arange(0, (b + 1) * t, t, dtype=torch.int32, device=input_ids.device)
             counts = [t] * b
@@ -421,9 +419,11 @@ class SparDAB200Model(nn.Module):
             if counts is None or sum(counts) != b * t:
                 raise ValueError("packed prompts into a cache need their lengths on the host too, "
                                  "with the sum of the row's tokens")
+            if pages.fills(counts):
+                raise NotImplementedError("prefill into a non-empty cache")
             pages.reserve(counts)
         longest = max(counts) if counts else None
-        return RaggedBatch.prompts(cu_seqlens, b * t, self.rotary_emb, longest), pages, counts
+        return RaggedBatch.prompts(cu_seqlens, b * t, self.rotary_emb, longest, counts), pages, counts
 
     def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
                 kv_caches: Optional[List] = None, return_forecasts: bool = False,
@@ -431,7 +431,8 @@ class SparDAB200Model(nn.Module):
                 lengths: Optional[List[int]] = None) -> Dict[str, torch.Tensor]:
         """``cu_seqlens`` (device int32, "b200_dense" backend): input_ids
         [1,total] holds sequences packed back to back; with paged caches also
-        their ``lengths`` as host numbers."""
+        their ``lengths`` as host numbers, one a sequence of the cache (0 for
+        those that go on: prompts may take the place of released ones)."""
         b, t = input_ids.shape
         if self.config.attention_backend == "b200_dense":
             return self._forward_dense(input_ids, targets, kv_caches, cu_seqlens, lengths)

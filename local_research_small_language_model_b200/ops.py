@@ -635,6 +635,8 @@ def swiglu_weight(w_gate: torch.Tensor, w_up: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- ragged batches
+LEN_ABSENT = -2 ** 31  # SD_LEN_ABSENT: in lens of paged_append, the sequence takes no part
+
 # These calls are a few microseconds on the device, so their wrappers look at
 # each tensor once and keep to the cheap accessors.
 _err_ptrs = {}
@@ -836,7 +838,8 @@ def paged_append(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, v_pa
     lens [B] int32, tokens cached before (not changed).  Rows cu_seqlens[b] ..
     cu_seqlens[b+1]-1 go to positions lens[b], lens[b]+1, ..; without
     cu_seqlens row b is sequence b's one new token.  A row whose place is out
-    of range is dropped and check_device_errors reports it."""
+    of range is dropped and check_device_errors reports it; lens[b] ==
+    LEN_ABSENT drops the rows of sequence b without a report."""
     rows = xk.shape
     if len(rows) != 3 or rows != xv.shape or lens.dim() != 1:
         raise ValueError(f"xk, xv must be [N, Hkv, D] alike and lens [B], got {tuple(rows)}, {tuple(xv.shape)}, "
