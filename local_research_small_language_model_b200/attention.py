@@ -382,8 +382,9 @@ class B200DenseAttention(BaseAttention):
     with bounds) one row [1,total,C] of packed sequences.  ``kv_cache`` is a
     B200PagedKVCache whose PageTable has the pages reserved: prompts (of
     sequences that are empty so far) or, with T == 1 and no bounds, one decode
-    step of every sequence.  The caller advances the PageTable after the last
-    layer."""
+    step of every sequence.  A cache of another dtype than x holds rows rounded
+    to it; prompts attend to what they computed, steps in the cache's type.
+    The caller advances the PageTable after the last layer."""
 
     def forward(self, x: torch.Tensor, rotary_emb, kv_cache=None, mask: Optional[torch.Tensor] = None,
                 is_causal: bool = True, forecast_vector: Optional[torch.Tensor] = None,
@@ -431,6 +432,8 @@ class B200DenseAttention(BaseAttention):
             raise NotImplementedError("prefill into a non-empty cache")
         kv_cache.append(xk, xv, ragged.cu_seqlens, ragged.lens_before)
         if step:
-            return ops.paged_decode_attention(xq, kv_cache.k_pages, kv_cache.v_pages, pages.table,
-                                              ragged.lens_after)
+            # in the cache's type, as the sparse backend's steps
+            out = ops.paged_decode_attention(xq.to(kv_cache.k_pages.dtype), kv_cache.k_pages, kv_cache.v_pages,
+                                             pages.table, ragged.lens_after)
+            return out.to(xq.dtype)
         return packed_attention(xq, xk, xv, ragged.cu_seqlens)

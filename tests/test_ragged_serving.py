@@ -7,7 +7,7 @@ import torch
 
 import local_research_small_language_model_b200 as sd
 from local_research_small_language_model_b200 import model, ops
-from tests.test_ragged_layers import CONFIG, on_cpu  # noqa: F401
+from tests.test_ragged_layers import CONFIG, on_cpu, plain_rope  # noqa: F401
 
 
 def plain_append(xk, xv, k_pages, v_pages, page_table, lens, cu_seqlens=None):
