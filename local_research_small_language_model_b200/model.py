@@ -158,25 +158,26 @@ class TransformerBlock(nn.Module):
         gu = F.linear(self.ffn_norm(x2), self.packed_ffn_weight())
         return torch.addmm(x2, ops.silu_mul(gu), self.ffn.w_down.weight.t())
 
-    def _forward_dense(self, x, rotary_emb, kv_cache, mask, is_causal, ragged):
-        """The block around exact attention: no forecast (nothing selects
-        blocks by it)."""
+    def _forward_dense(self, x, rotary_emb, kv_cache, mask, is_causal, ragged, forecast):
+        """The block around exact attention, with its forecast where it is
+        asked for (nothing selects blocks by it)."""
         a = self.attention
         normed = self.attn_norm(x)
+        current = self.forecast(normed) if forecast else None
         if _records_grad(x, self):
             x = x + a(normed, rotary_emb, kv_cache, mask, is_causal, ragged=ragged)
-            return x + self.ffn(self.ffn_norm(x))
+            return x + self.ffn(self.ffn_norm(x)), current
         b, t, c = x.shape
         rows = F.linear(normed.reshape(b * t, c), a.qkv_weight()).unflatten(1, (-1, a.head_dim))
         xq, xk, xv = rows.split([a.n_head, a.n_kv_head, a.n_kv_head], dim=1)
         out = a.core(xq, xk, xv, b, t, rotary_emb, kv_cache, mask, is_causal, ragged)
-        return self._ffn_decode(x.reshape(b * t, c), out.flatten(1), False).view(b, t, c)
+        return self._ffn_decode(x.reshape(b * t, c), out.flatten(1), False).view(b, t, c), current
 
     def forward(self, x, rotary_emb, kv_cache=None, mask=None, is_causal=True, prev_layer_forecast=None,
-                next_layer_block=None, next_kv_cache=None, ragged=None):
+                next_layer_block=None, next_kv_cache=None, ragged=None, forecast=False):
         b, t, c = x.shape
         if isinstance(self.attention, B200DenseAttention):
-            return self._forward_dense(x, rotary_emb, kv_cache, mask, is_causal, ragged), None
+            return self._forward_dense(x, rotary_emb, kv_cache, mask, is_causal, ragged, forecast)
         if isinstance(kv_cache, (B200KVCache, B200OffloadKVCache)) and t == 1:
             # decode step: 8 launches per layer by default (norm, [wq;wk;wv;wf]
             # GEMM, fused attention kernel, wo GEMM with the residual add folded
@@ -435,7 +436,7 @@ class SparDAB200Model(nn.Module):
         those that go on: prompts may take the place of released ones)."""
         b, t = input_ids.shape
         if self.config.attention_backend == "b200_dense":
-            return self._forward_dense(input_ids, targets, kv_caches, cu_seqlens, lengths)
+            return self._forward_dense(input_ids, targets, kv_caches, return_forecasts, cu_seqlens, lengths)
         if cu_seqlens is not None:
             raise NotImplementedError('packed sequences need attention_backend="b200_dense"')
         x = self.embeddings.embed(input_ids)
@@ -468,18 +469,23 @@ class SparDAB200Model(nn.Module):
                                           ignore_index=-100)
         return out
 
-    def _forward_dense(self, input_ids, targets, kv_caches, cu_seqlens, lengths) -> Dict[str, torch.Tensor]:
+    def _forward_dense(self, input_ids, targets, kv_caches, return_forecasts, cu_seqlens,
+                       lengths) -> Dict[str, torch.Tensor]:
         if kv_caches is not None and not all(isinstance(c, B200PagedKVCache) for c in kv_caches):
             raise NotImplementedError("the dense backend caches in a B200PagedKVCache")
         ragged, pages, counts = self._ragged(input_ids, kv_caches, cu_seqlens, lengths)
         x = self.embeddings.embed(input_ids)
+        forecasts = []
         for i, layer in enumerate(self.layers):
-            x, _ = layer(x=x, rotary_emb=self.rotary_emb, kv_cache=kv_caches[i] if kv_caches is not None else None,
-                         ragged=ragged)
+            x, current = layer(x=x, rotary_emb=self.rotary_emb, ragged=ragged, forecast=return_forecasts,
+                               kv_cache=kv_caches[i] if kv_caches is not None else None)
+            forecasts.append(current)
         if pages is not None:
             pages.advance(counts)
         logits = self.embeddings.project(self.final_norm(x))
         out = {"logits": logits}
+        if return_forecasts:
+            out["forecasts"] = forecasts
         if targets is not None:
             # the mean over the scored tokens, as F.cross_entropy(ignore_index=-100)
             flat = targets.reshape(-1)

@@ -82,3 +82,21 @@ def test_training_some_projections_of_a_model_trains_its_first_layer(on_cpu):
     m(ids, targets=ids)["loss"].backward()
     for name, p in m.named_parameters():
         assert (p.grad is not None and bool(p.grad.any())) == p.requires_grad, name
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forecasts_are_returned_where_they_are_asked_for(on_cpu, grad):
+    """The projection of every layer's normed input, as the reference's block
+    computes it whatever attends (model/transformer.py:104-107)."""
+    torch.manual_seed(2)
+    m = model.SparDAB200Model(sd.ModelConfig(**CONFIG))
+    ids = torch.randint(0, 50, (2, 6))
+    inputs = []
+    for layer in m.layers:
+        layer.attn_norm.register_forward_hook(lambda mod, args, out: inputs.append(out))
+    with torch.set_grad_enabled(grad):
+        got = m(ids, return_forecasts=True)
+    assert len(got["forecasts"]) == 2
+    for f, x, layer in zip(got["forecasts"], inputs, m.layers):
+        assert torch.equal(f, layer.forecast(x)) and f.requires_grad == grad
+    assert "forecasts" not in m(ids)
