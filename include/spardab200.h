@@ -419,9 +419,9 @@ SD_API int sd_decode_layer_offload(const void *qkv, int dtype, int64_t qkv_sb, c
  * = softmax(scale q k^T over the sequence's tokens up to the query's own) v.
  * Rows outside every sequence: zeros with zero_rest, else left as they are.
  * lse (nullable): fp32 [Hq,total], log2 of each row's sum of exponentials, for
- * the backward.  rest (nullable, 16-bit types): contiguous [total,Hq,64], what
- * rounding took from out, for the backward.  16-bit inputs run on the tensor cores, fp32 on CUDA cores.
- * scale > 0. */
+ * the backward.  rest (nullable; 16-bit types only, SD_ERR_INVALID with fp32):
+ * contiguous [total,Hq,64], what rounding took from out, for the backward.
+ * 16-bit inputs run on the tensor cores, fp32 on CUDA cores.  scale > 0. */
 SD_API int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, int64_t total, int64_t Hq,
                                int64_t Hkv, int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
                                int64_t v_st, int64_t v_sh, const int32_t *cu_seqlens, int nseq, float scale,

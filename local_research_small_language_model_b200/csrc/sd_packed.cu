@@ -542,6 +542,7 @@ int sd_packed_attention(const void *q, const void *k, const void *v, int dtype, 
   a.lse = lse, a.rest = rest, a.zero_rest = zero_rest;
   int rc = check_packed(a, dtype, D);
   if (rc != SD_OK) return rc;
+  if (rest && dtype == SD_DTYPE_F32) return SD_ERR_INVALID;
   if (!aligned16(rest)) return SD_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype != SD_DTYPE_F32) return launch_packed_fwd_tc(a, dtype, err, s);
@@ -574,7 +575,7 @@ int sd_packed_attention_backward(const void *q, const void *k, const void *v, co
   int rc = check_packed(a, dtype, D);
   if (rc == SD_OK) rc = check_rows(dout, dtype, g_st, g_sh);
   if (rc != SD_OK) return rc;
-  if (!lse || !delta || !dq || !dk || !dv) return SD_ERR_INVALID;
+  if (!lse || !delta || !dq || !dk || !dv || (rest && dtype == SD_DTYPE_F32)) return SD_ERR_INVALID;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(rest)) return SD_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype != SD_DTYPE_F32) return launch_packed_bwd_tc(a, dtype, err, s);

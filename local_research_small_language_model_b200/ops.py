@@ -744,6 +744,14 @@ def _check_like_q(q, **ts):
             raise ValueError(f"{name} must have q's shape {tuple(q.shape)}, got {tuple(t.shape)}")
 
 
+def _check_rest(rest):
+    if rest is not None:
+        if rest.dtype is torch.float32:
+            raise TypeError("rest holds what rounding to 16 bits takes from the output: fp32 has none")
+        if not rest.is_contiguous():
+            raise ValueError("rest must be contiguous")
+
+
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                      return_lse: bool = False, rest: Optional[torch.Tensor] = None):
@@ -757,6 +765,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     _check_packed(q, k, v, cu_seqlens)
     if out is not None or rest is not None:
         _check_like_q(q, out=out, rest=rest)
+        _check_rest(rest)
     dev = _device(q, k, v, cu_seqlens, out, rest)
     total, hq, d = q.shape
     sc = _scale(scale, d)
@@ -767,8 +776,6 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif _rows16(out) is not out:
         raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
-    if rest is not None and not rest.is_contiguous():
-        raise ValueError("rest must be contiguous")
     lse = torch.empty(hq, total, dtype=torch.float32, device=q.device) if return_lse else None
     if total:
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
@@ -792,13 +799,12 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     (sd_packed_attention_backward).  Equal inputs give equal bits."""
     _check_packed(q, k, v, cu_seqlens)
     _check_like_q(q, out=out, dout=dout, rest=rest)
+    _check_rest(rest)
     dev = _device(q, k, v, out, dout, lse, cu_seqlens, rest)
     total, hq, d = q.shape
     hkv = k.shape[1]
     if lse.shape != (hq, total) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError(f"lse must be the forward's fp32 [{hq}, {total}], got {tuple(lse.shape)} of {lse.dtype}")
-    if rest is not None and not rest.is_contiguous():
-        raise ValueError("rest must be contiguous")
     sc = _scale(scale, d)
     cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape[0])
     code = dtype_code(q)
