@@ -678,18 +678,29 @@ def _launch(name: str, dev: int, *args) -> None:
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t itself where its rows of 64 values suit 16-byte loads and tensor copies
-    (innermost stride 1, aligned base and strides, no broadcast dimension),
-    else a contiguous copy."""
+    (innermost stride 1, aligned base and strides, no broadcast dimension), a
+    view of it where only a dimension of one has another stride, else a
+    contiguous copy."""
     if not t.data_ptr() & 15:
         st = t.stride()
         if len(st) == 3 and st[2] == 1 and not (st[0] | st[1]) & 7 and st[0] > 0 and st[1] > 0:
             return t
-        if t.is_contiguous():
-            return t
+        if 1 in t.shape:  # a stride that nothing steps by
+            steps = tuple(64 if n == 1 else s for s, n in zip(st, t.shape))
+            if steps != st:
+                t, st = t.as_strided(t.shape, steps), steps
         whole = 16 // t.element_size() - 1
-        if st[-1] == 1 and not any(s & whole for s in st[:-1]) and all(s > 0 or n == 1 for s, n in zip(st, t.shape)):
+        if st[-1] == 1 and not any(s & whole for s in st[:-1]) and min(st) > 0 or not t.numel():
             return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _rows16_of(what: str, t: torch.Tensor) -> torch.Tensor:
+    """_rows16 of a tensor that a kernel writes, or reads where a copy would not do."""
+    rows = _rows16(t)
+    if rows.data_ptr() != t.data_ptr():
+        raise ValueError(f"{what} must have 16-byte aligned rows and innermost stride 1")
+    return rows
 
 
 def _index32(name: str, t: torch.Tensor, rows: int) -> torch.Tensor:
@@ -772,17 +783,15 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu = _index32("cu_seqlens", cu_seqlens, cu_seqlens.shape[0])
     code = dtype_code(q)
     zero = out is None
-    if zero:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif _rows16(out) is not out:
-        raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if zero else out
+    to = out if zero else _rows16_of("out", out)
     lse = torch.empty(hq, total, dtype=torch.float32, device=q.device) if return_lse else None
     if total:
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
         q_st, q_sh, _ = q.stride()
         k_st, k_sh, _ = k.stride()
         v_st, v_sh, _ = v.stride()
-        o_st, o_sh, _ = out.stride()
+        o_st, o_sh, _ = to.stride()
         _launch("sd_packed_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, total, hq, k.shape[1], d,
                 q_st, q_sh, k_st, k_sh, v_st, v_sh, cu.data_ptr(), cu.shape[0] - 1, sc, out.data_ptr(), o_st, o_sh,
                 lse.data_ptr() if return_lse else 0,
@@ -823,16 +832,18 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 def _check_pool(k_pages, v_pages, d):
     """The pool's (pages, Hkv, page) and its strides, the same for k and v."""
-    shape, strides = k_pages.shape, k_pages.stride()
+    shape = k_pages.shape
     if len(shape) != 4 or shape != v_pages.shape or 0 in shape:
         raise ValueError(f"k_pages and v_pages must be [pages, Hkv, page, D] alike, got {tuple(shape)}, "
                          f"{tuple(v_pages.shape)}")
     if d != 64 or shape[3] != 64:
         raise ValueError(f"paged caches have head size 64, got {d} and {shape[3]}")
-    if k_pages.dtype is not v_pages.dtype or strides != v_pages.stride():
-        raise ValueError("k_pages and v_pages must share dtype and strides")
-    if _rows16(k_pages) is not k_pages or v_pages.data_ptr() & 15:
-        raise ValueError("pages must have 16-byte aligned rows and innermost stride 1")
+    strides, alike = k_pages.stride(), k_pages.dtype is v_pages.dtype
+    if not alike or strides != v_pages.stride() or strides[3] != 1 or (strides[0] | strides[1] | strides[2]) & 7 \
+            or min(strides) < 1 or (k_pages.data_ptr() | v_pages.data_ptr()) & 15:
+        strides = _rows16_of("pages", k_pages).stride()
+        if not alike or strides != _rows16_of("pages", v_pages).stride():
+            raise ValueError("k_pages and v_pages must share dtype and strides")
     return shape, strides
 
 
@@ -904,11 +915,11 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     code = dtype_code(q)
     sc = _scale(scale, d)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        to = out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape:
         raise ValueError(f"out must have q's shape {tuple(shape)}, got {tuple(out.shape)}")
-    elif _rows16(out) is not out:
-        raise ValueError("out must have 16-byte aligned rows and innermost stride 1")
+    else:
+        to = _rows16_of("out", out)
     if b == 0:
         return out
     q = _rows16(q)
@@ -916,7 +927,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     need = _decode_workspace(b, hq, hkv)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     q_sb, q_sh, _ = q.stride()
-    o_sb, o_sh, _ = out.stride()
+    o_sb, o_sh, _ = to.stride()
     _launch("sd_paged_decode_attention", dev, q.data_ptr(), code, b, hq, hkv, d, q_sb, q_sh, k_pages.data_ptr(),
             v_pages.data_ptr(), pages, page, p_sp, p_sh, p_st, table.data_ptr(), table.stride(0), table.shape[1],
             ln.data_ptr(), sc, out.data_ptr(), o_sb, o_sh, ws.data_ptr(), need, _err_ptr(dev))
