@@ -310,16 +310,19 @@ __global__ void __launch_bounds__(pk::kThreads, 2) packed_fwd_kernel(const __gri
       store4(out + row_of(ty, i) * a.o_st + 4 * tx, o[i][0], o[i][1], o[i][2], o[i][3]);
       if (a.lse && tx == 0) a.lse[h * a.total + first + row_of(ty, i)] = m[i] + log2f(l[i]);
     }
-    // the warp's two rows in turn
+    // the warp's two rows, where one is not finite
     const unsigned bad = __ballot_sync(0xffffffffu, held && !finite);
+    if (bad) {
+      __syncwarp();
+      PackedRows<2> g;
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
-      if (bad >> (16 * half) & 0xffffu) {
-        __syncwarp();
+      for (int half = 0; half < 2; ++half) {
         const int row = __shfl_sync(0xffffffffu, t.row0 + row_of(ty, i), 16 * half);
-        packed_row<float>(a, t.start, row, h, __shfl_sync(0xffffffffu, m[i], 16 * half),
-                          __shfl_sync(0xffffffffu, l[i], 16 * half));
+        g.row[half] = bad >> (16 * half) & 0xffffu ? row : -1;
+        g.m[half] = __shfl_sync(0xffffffffu, m[i], 16 * half), g.l[half] = __shfl_sync(0xffffffffu, l[i], 16 * half);
       }
+      packed_again<float>(a, t.start, min(t.len, t.row0 + kTile), h, g);
+    }
   }
 }
 

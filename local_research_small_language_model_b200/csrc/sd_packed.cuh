@@ -165,40 +165,118 @@ __device__ __forceinline__ PackedTile packed_nth(const int32_t *cu, int S, int64
   return t;
 }
 
-// One row of the forward again, by a warp and without matrix products, for a
-// result that is not finite: there a masked weight of 0 met a NaN or an infinity
-// of a later token's v, which the row does not see; or it does see one, and the
-// result stays what it is.  Row `row` (of the sequence) of head h, with its
-// reference m and sum l from the fast path.
+// The columns in which rows from .. to - 1 of v hold a NaN or an infinity, by a
+// warp from the last row down until all of `want` are found: bit e of lane n
+// stands for column (64 / kLanes) (n % kLanes) + e.
 template <typename T>
-__device__ __forceinline__ void packed_row(const PackedArgs &a, int64_t start, int row, int h, float m, float l) {
+__device__ __forceinline__ unsigned packed_not_finite(const T *v, int64_t stride, int from, int to, unsigned want) {
+  constexpr int kCols = 16 / sizeof(T), kLanes = 64 / kCols, kAtOnce = 32 / kLanes, kUnroll = 8;
+  const int lane = threadIdx.x & 31;
+  unsigned found = 0;
+  for (int r1 = to; r1 > from; r1 -= kAtOnce * kUnroll) {
+    uint4 x[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int r = r1 - 1 - kAtOnce * u - lane / kLanes;
+      x[u] = r >= from ? *reinterpret_cast<const uint4 *>(v + r * stride + lane % kLanes * kCols)
+                       : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const T *p = reinterpret_cast<const T *>(&x[u]);
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) found |= static_cast<unsigned>(!(fabsf(to_f(p[e])) < INFINITY)) << e;
+    }
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1) found |= __shfl_xor_sync(0xffffffffu, found, o);
+    if (!__any_sync(0xffffffffu, want & ~found)) break;
+  }
+  return found;
+}
+
+// Rows of the forward again, by a warp and without matrix products, where a masked
+// weight of 0 met a NaN or an infinity of a later token's v, which the row does
+// not see.  Rows `row` (of the sequence; below 0: none) of head h, with their
+// references m and sums l from the fast path, whose blocks held the sequence's
+// keys up to `end`.  Only columns are computed that hold such a value behind the
+// row and none up to it: with one up to it, or a sum that is not finite, the
+// result is not finite whatever is computed.  So a tensor full of NaN costs two
+// looks at a few rows of v (32768 tokens: 2.2 ms instead of 1.7, 2.5 with one NaN
+// in the first token); it is the rows before a column's first such value, fewer
+// than a tile's, that walk over their keys (the worst: it is the last of 8192
+// tokens, 17 ms, of 32768, 68 ms).  Two rows at a time: 24 ms with one; four, or a
+// function that is not inlined, make the kernels' loops spill.
+template <int R> struct PackedRows {
+  int row[R];
+  float m[R], l[R];
+};
+template <typename T, int R>
+__device__ __forceinline__ void packed_again(const PackedArgs &a, int64_t start, int end, int h, const PackedRows<R> &g) {
+  constexpr int kCols = 16 / sizeof(T), kLanes = 64 / kCols, kAtOnce = 32 / kLanes;
   const int lane = threadIdx.x & 31, hk = h / (a.Hq / a.Hkv);
-  const T *q = static_cast<const T *>(a.q) + (start + row) * a.q_st + h * a.q_sh;
+  const T *q = static_cast<const T *>(a.q) + start * a.q_st + h * a.q_sh;
   const T *k = static_cast<const T *>(a.k) + start * a.k_st + hk * a.k_sh;
   const T *v = static_cast<const T *>(a.v) + start * a.v_st + hk * a.v_sh;
-  float o0 = 0.f, o1 = 0.f;
-  for (int j0 = 0; j0 <= row; j0 += 32) {
-    float p = 0.f;
-    if (j0 + lane <= row) {
-      const T *kj = k + (j0 + lane) * a.k_st;
-      float s = 0.f;
-      for (int d = 0; d < 64; ++d) s = fmaf(to_f(q[d]), to_f(kj[d]), s);
-      p = exp2f(fmaf(s, a.scale_log2, m == -INFINITY ? 0.f : -m));
+  const int c = lane % kLanes * kCols;  // this lane's columns; it reads every kAtOnce-th row of v
+  unsigned again[R];                    // those of them to be computed
+  int row[R], last = -1;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    row[r] = -1, again[r] = 0;
+    if (g.row[r] < 0 || !(g.l[r] > 0.f && g.l[r] < INFINITY)) continue;
+    again[r] = packed_not_finite(v, a.v_st, g.row[r] + 1, end, (1u << kCols) - 1);
+    if (__any_sync(0xffffffffu, again[r])) again[r] &= ~packed_not_finite(v, a.v_st, 0, g.row[r] + 1, again[r]);
+    if (__any_sync(0xffffffffu, again[r])) row[r] = g.row[r], last = max(last, row[r]);
+  }
+  if (last < 0) return;
+  float o[R][kCols] = {};
+  for (int j0 = 0; j0 <= last; j0 += 32) {
+    float p[R] = {};
+    const T *kj = k + min(j0 + lane, last) * a.k_st;
+#pragma unroll 4
+    for (int d = 0; d < 64; d += kCols) {
+      const uint4 y = *reinterpret_cast<const uint4 *>(kj + d);
+      const T *py = reinterpret_cast<const T *>(&y);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(q + max(row[r], 0) * a.q_st + d);
+        const T *px = reinterpret_cast<const T *>(&x);
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) p[r] = fmaf(to_f(px[e]), to_f(py[e]), p[r]);
+      }
     }
-    const int n = min(32, row + 1 - j0);
-    for (int t = 0; t < n; ++t) {
-      const float w = __shfl_sync(0xffffffffu, p, t);
-      const T *vj = v + (j0 + t) * a.v_st + 2 * lane;
-      o0 = fmaf(w, to_f(vj[0]), o0);
-      o1 = fmaf(w, to_f(vj[1]), o1);
+#pragma unroll
+    for (int r = 0; r < R; ++r) p[r] = exp2f(fmaf(p[r], a.scale_log2, g.m[r] == -INFINITY ? 0.f : -g.m[r]));
+#pragma unroll 4
+    for (int t0 = 0; t0 < 32; t0 += kAtOnce) {
+      const int t = t0 + lane / kLanes;
+      const uint4 x = *reinterpret_cast<const uint4 *>(v + min(j0 + t, last) * a.v_st + c);
+      const T *px = reinterpret_cast<const T *>(&x);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float w = __shfl_sync(0xffffffffu, p[r], t);
+        if (j0 + t > row[r]) continue;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) o[r][e] = fmaf(w, to_f(px[e]), o[r][e]);
+      }
     }
   }
-  o0 /= l, o1 /= l;
-  T *out = static_cast<T *>(a.out) + (start + row) * a.o_st + h * a.o_sh + 2 * lane;
-  out[0] = from_f<T>(o0), out[1] = from_f<T>(o1);
-  if (a.rest) {
-    T *rest = static_cast<T *>(a.rest) + ((start + row) * a.Hq + h) * 64 + 2 * lane;
-    rest[0] = from_f<T>(o0 - round_to<T>(o0)), rest[1] = from_f<T>(o1 - round_to<T>(o1));
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int e = 0; e < kCols; ++e)
+#pragma unroll
+      for (int n = kLanes; n < 32; n <<= 1) o[r][e] += __shfl_xor_sync(0xffffffffu, o[r][e], n);
+    if (row[r] < 0 || lane >= kLanes) continue;
+    const int64_t at = start + row[r];
+    T *out = static_cast<T *>(a.out) + at * a.o_st + h * a.o_sh + c;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) {
+      if (!(again[r] >> e & 1)) continue;
+      const float x = o[r][e] / g.l[r];
+      out[e] = from_f<T>(x);
+      if (a.rest) static_cast<T *>(a.rest)[(at * a.Hq + h) * 64 + c + e] = from_f<T>(x - round_to<T>(x));
+    }
   }
 }
 

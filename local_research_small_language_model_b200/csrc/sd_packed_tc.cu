@@ -465,10 +465,17 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
       __syncwarp();  // a row's first result is written by other lanes than its second
       // the tile is looked up again: nothing is kept for this in the loop's registers
       const PackedTile u = packed_nth(a.cu, a.S, a.total, blockIdx.x / a.Hq, gridDim.x / a.Hq, 2 * kRows, true);
-      for (; again; again &= again - 1) {
-        const int i = __ffs(again) - 1;
-        packed_row<T>(a, u.start, u.row0 + 32 * warp + i, blockIdx.x % a.Hq, __shfl_sync(0xffffffffu, m, i),
-                      __shfl_sync(0xffffffffu, l, i));
+      const int at = u.row0 + 32 * warp, end = min(u.len, (at / kRows + 1) * kRows);  // the tile's keys end with its rows
+      while (again) {
+        PackedRows<2> g;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = again ? __ffs(again) - 1 : 0;
+          g.row[i] = again ? at + n : -1;
+          g.m[i] = __shfl_sync(0xffffffffu, m, n), g.l[i] = __shfl_sync(0xffffffffu, l, n);
+          again &= again - 1;
+        }
+        packed_again<T>(a, u.start, end, blockIdx.x % a.Hq, g);
       }
     }
     if (row < rows && a.lse) a.lse[h * a.total + first + row] = m + log2f(l);
