@@ -432,7 +432,7 @@ SD_API int sd_packed_attention(const void *q, const void *k, const void *v, int 
  * dk and dv [total,Hkv,64], contiguous, in the inputs' dtype (dk and dv summed
  * over the query heads of their kv head; zeros outside every sequence).  out,
  * lse and rest (nullable: dq and dk are then a little less exact) are the
- * forward's.  delta: workspace of this call, fp32 [Hq*total + 1].
+ * forward's.  delta: workspace of this call, fp32 [Hq,total].
  * Sums have a fixed order: equal inputs give equal bits. */
 SD_API int sd_packed_attention_backward(const void *q, const void *k, const void *v, const void *out,
                                         const void *dout, int dtype, int64_t total, int64_t Hq, int64_t Hkv,

@@ -22,7 +22,7 @@ struct PackedArgs {
   // backward
   const void *dout;
   int64_t g_st, g_sh;
-  float *delta;                         // [Hq][total] rowsum(dout * out), and one word more
+  float *delta;                         // [Hq][total] rowsum(dout * out)
   void *dq, *dk, *dv;                   // contiguous
 };
 

@@ -500,8 +500,9 @@ struct BwdSmem {
   static constexpr int kRowsB = kRowsA + kTileBytes;            // dO or V
   static constexpr int kA = kRowsB + kTileBytes;                // the other side's blocks: K or Q
   static constexpr int kB = kA + kBwdStages * kTileBytes;       // V or dO
-  static constexpr int kVec = kB + kBwdStages * kTileBytes;     // dQ: [128] max |dout|;
-  static constexpr int kBar = kVec + 4096;                      // dK/dV: 16 warps x (32 lse, 32 delta)
+  static constexpr int kVec = kB + kBwdStages * kTileBytes;     // dK/dV: 16 warps x (32 lse, 32 delta)
+  static constexpr int kTop = kVec + 4096;                      // fp16: the largest |dout|, |v|, |delta| of rows
+  static constexpr int kBar = kTop + 2048;
   static constexpr int kBytes = kBar + 256;
 };
 
@@ -559,9 +560,31 @@ __device__ __forceinline__ void bwd_failed(BwdBars *bars, int32_t *err) {
   if (threadIdx.x == 0 && err) *err = SD_KERR_TIMEOUT;
 }
 
-// The power of two that takes x into [1/2, 1) (1 for 0): fp16 holds dS scaled
-// by it, so that small output gradients (a loss averaged over many tokens)
-// keep their digits.
+// fp16's range is narrow: weights fall as 1 / n, a loss averaged over many tokens
+// has small output gradients, a scaled one large ones, and values add up.  So dS is
+// held scaled by a power of two per accumulator row, from the pairs of that row
+// alone: neither what else is packed beside its sequence nor what the row does not
+// see costs it digits.  |dP - delta| is at most 64 max|dout| max|v| + max|delta|,
+// which the power takes into [2^14, 2^15): twice that fits.  A look at the other
+// side's rows ahead of the loop (the compute warps', while the first products run)
+// finds the maxima: 16-bit magnitudes in pairs as integers, whose order is theirs.
+__device__ __forceinline__ unsigned top2(uint4 x) {
+  constexpr unsigned kAbs = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(x.x & kAbs, x.y & kAbs), __vmaxu2(x.z & kAbs, x.w & kAbs));
+}
+__device__ __forceinline__ unsigned top1(unsigned pair) { return max(pair & 0xffffu, pair >> 16); }
+// What is not finite counts as the largest number: its own rows' gradients are not finite whatever the scale.
+__device__ __forceinline__ float top_value(unsigned bits) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(min(bits, 0x7bffu))));
+}
+__device__ __forceinline__ float range_scale(float bound) {
+  const int e = 268 - static_cast<int>(__float_as_uint(bound) >> 23);  // 2^(14 - floor(log2 bound))
+  return __uint_as_float(static_cast<uint32_t>(min(max(e, 27), 227)) << 23);
+}
+constexpr int kComputeThreads = 512;
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+
+// The power of two that takes x into [1/2, 1) (1 for 0).
 __device__ __forceinline__ float unit_scale(float x) {
   const int e = static_cast<int>(__float_as_uint(x) >> 23) - 126;
   return x > 0.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 1.f;
@@ -653,12 +676,10 @@ template <typename T> __device__ __forceinline__ float largest8(const T *p) {
 
 }  // namespace pt
 
-// delta = rowsum(dout out), for fp16 also the largest |dout| of all sequences' rows;
-// eight lanes a row and head.  A kernel of its own, so that both gradients'
-// kernels can read it and the second may start while the first ends.
-template <typename T> __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const PackedArgs a, unsigned *top) {
-  using namespace pt;
-  constexpr bool kHalf = std::is_same<T, __half>::value;
+// delta = rowsum(dout out), eight lanes a row and head.  A kernel of its own, so
+// that both gradients' kernels can read it and the second may start while the first
+// ends.
+template <typename T> __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const PackedArgs a) {
   const int64_t n = blockIdx.x * 32ll + (threadIdx.x >> 3), row = n / a.Hq;
   const int h = static_cast<int>(n - row * a.Hq), c = 8 * (threadIdx.x & 7);
   float delta = 0.f;
@@ -680,23 +701,6 @@ template <typename T> __global__ void __launch_bounds__(256) packed_delta_tc_ker
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, o);
   if (in && c == 0) a.delta[h * a.total + row] = delta;
-  if (kHalf) {
-    const bool counts = in && row >= packed_bound(a.cu, a.S, a.total, 1) &&
-                        row < packed_bound(a.cu, a.S, a.total, a.S + 1);
-    float big = counts ? largest8(static_cast<const T *>(a.dout) + row * a.g_st + h * a.g_sh + c) : 0.f;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-    if (!(big < INFINITY)) big = 0.f;  // such a row's gradients are not finite whatever the scale
-    __shared__ unsigned most[8];
-    const unsigned warp_most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = warp_most;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      const unsigned all = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? most[threadIdx.x] : 0u);
-      // few CTAs find a larger one than is known already: the maximum is the same in any order
-      if (threadIdx.x == 0 && all > *static_cast<volatile unsigned *>(top)) atomicMax(top, all);
-    }
-  }
 }
 
 
@@ -724,7 +728,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
   extern __shared__ __align__(1024) char smem_raw[];
   char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float *most = reinterpret_cast<float *>(sm + BwdSmem::kVec);
+  float *most = reinterpret_cast<float *>(sm + BwdSmem::kTop);
   BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = h / (a.Hq / a.Hkv);
@@ -833,7 +837,7 @@ template <typename T>
 __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     packed_bwd_dkv_tc_kernel(const PackedArgs a, const __grid_constant__ CUtensorMap tmq,
                              const __grid_constant__ CUtensorMap tmg, const __grid_constant__ CUtensorMap tmk,
-                             const __grid_constant__ CUtensorMap tmv, const unsigned *top, int32_t *err) {
+                             const __grid_constant__ CUtensorMap tmv, int32_t *err) {
   using namespace pt;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // dQ's CTAs take the SMs that this one's leave
   constexpr bool kHalf = std::is_same<T, __half>::value;
@@ -864,7 +868,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   const uint32_t tmem = bars->tmem;
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  const float f = kHalf ? unit_scale(__uint_as_float(*top)) : 1.f;
+  float f = 1.f;  // of this thread's key
   bool ok = true;
   if (warp == kBwdCopy) {
     if (lane == 0)
@@ -901,6 +905,59 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
       if (qn >= span + 32 * wg) qn = 0, at += a.total;
     };
     fetch(true);
+    if (kHalf) {
+      // largest |v| of each key; |dout| and |delta| of each query of the tile's own rows, and of all behind them
+      unsigned *vals = reinterpret_cast<unsigned *>(sm + BwdSmem::kTop), *grads = vals + kRows, *grads_on = grads + kRows;
+      float *deltas = reinterpret_cast<float *>(grads_on + 16), *deltas_on = deltas + kRows;
+      const int len = t.len - t.row0, part = lane >> 3, c = 8 * (lane & 7);
+      const T *v = static_cast<const T *>(a.v) + first * a.v_st + hk * a.v_sh + c;
+      const T *g = static_cast<const T *>(a.dout) + first * a.g_st + hk * group * a.g_sh + c;
+      auto row_top = [&](const T *p) { return top2(*reinterpret_cast<const uint4 *>(p)); };
+      for (int row = 4 * warp + part; row < kRows; row += 64) {
+        unsigned big_v = 0, big_g = 0;
+        if (row < keys) {
+          big_v = row_top(v + row * a.v_st);
+          for (int h = 0; h < group; ++h) big_g = __vmaxu2(big_g, row_top(g + row * a.g_st + h * a.g_sh));
+        }
+        unsigned both = top1(big_v) << 16 | top1(big_g);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+        if ((lane & 7) == 0) vals[row] = both >> 16, grads[row] = both & 0xffffu;
+      }
+      auto size = [](float x) { return fminf(fabsf(x), 3.0e38f); };  // a NaN as well
+      const float *d = a.delta + static_cast<int64_t>(hk) * group * a.total + first;
+      if (tid < kRows) {
+        float big = 0.f;
+        for (int h = 0; h < group; ++h)
+          if (tid < keys) big = fmaxf(big, size(d[h * a.total + tid]));
+        deltas[tid] = big;
+      }
+      unsigned on = 0;
+      float d_on = 0.f;
+      for (int h = 0; h < group; ++h) {
+#pragma unroll 8
+        for (int row = kRows + 4 * warp + part; row < len; row += 64)
+          on = __vmaxu2(on, row_top(g + row * a.g_st + h * a.g_sh));
+#pragma unroll 4
+        for (int row = kRows + tid; row < len; row += kComputeThreads) d_on = fmaxf(d_on, size(d[h * a.total + row]));
+      }
+      on = __reduce_max_sync(0xffffffffu, top1(on));
+      const unsigned d_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(d_on));
+      if (lane == 0) grads_on[warp] = on, deltas_on[warp] = __uint_as_float(d_bits);
+      compute_sync();
+      // over the queries from this thread's key on: the key's 32 rows by a scan, those behind them whole
+      unsigned top_g = grads_on[lane & 15], top_d = __float_as_uint(deltas_on[lane & 15]);
+      for (int w = (warp & 3) + 1; w < 4; ++w)
+        top_g = max(top_g, grads[32 * w + lane]), top_d = max(top_d, __float_as_uint(deltas[32 * w + lane]));
+      top_g = __reduce_max_sync(0xffffffffu, top_g), top_d = __reduce_max_sync(0xffffffffu, top_d);
+      unsigned own_g = grads[r], own_d = __float_as_uint(deltas[r]);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_down_sync(0xffffffffu, own_g, o), y = __shfl_down_sync(0xffffffffu, own_d, o);
+        if (lane + o < 32) own_g = max(own_g, x), own_d = max(own_d, y);
+      }
+      f = range_scale(64.f * top_value(max(top_g, own_g)) * top_value(vals[r]) + __uint_as_float(max(top_d, own_d)));
+    }
     for (int i = 0; i < blocks; ++i) {
       __syncwarp();
       mine[lane] = -next_l;
@@ -979,7 +1036,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (failed) bwd_failed(bars, err);
   if (warp < 8) {
     fence_after_sync();
-    const float back = failed ? __int_as_float(0x7fc00000) : wg == 0 ? 1.f : a.scale / f;
+    const float back = failed ? __int_as_float(0x7fc00000) : wg == 0 ? 1.f : a.scale / f;  // f: of row r for every wg
     const int row0 = 32 * (warp & 3);
     store_rows((wg == 0 ? dv : dk) + row0 * c_st, c_st, keys - row0,
                tmem + lane_base + (wg == 0 ? kDkvAcc : kDkvAcc2), back, sm + BwdSmem::kRowsA + warp * 4096);
@@ -1026,26 +1083,16 @@ int launch_packed_bwd_tc(const PackedArgs &a, int dtype, int32_t *err, cudaStrea
   if (rc != SD_OK) return rc;
   const int64_t slots = packed_slots(a.total, a.S, pt::kRows);
   if (slots * a.Hq > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
-  // fp16: the largest |dout|, in the word behind delta
-  unsigned *top = reinterpret_cast<unsigned *>(a.delta + a.Hq * a.total);
-  if (dtype == SD_DTYPE_F16) {
-    const cudaError_t e = cudaMemsetAsync(top, 0, sizeof(*top), s);
-    if (e != cudaSuccess) {
-      set_cuda_error(e);
-      cudaGetLastError();
-      return SD_ERR_CUDA;
-    }
-  }
   const size_t smem = pt::BwdSmem::kBytes + 1024;
   const int64_t delta_ctas = (a.total * a.Hq + 31) / 32;
   if (delta_ctas > 0x7fffffffll) return SD_ERR_UNSUPPORTED;
   auto run = [&](auto *delta, auto *dq, auto *dkv) {
     if (ensure_smem(dq, smem) != SD_OK || ensure_smem(dkv, smem) != SD_OK) return static_cast<int>(SD_ERR_CUDA);
-    delta<<<static_cast<unsigned>(delta_ctas), 256, 0, s>>>(a, top);
+    delta<<<static_cast<unsigned>(delta_ctas), 256, 0, s>>>(a);
     int rc = check_launch();
     if (rc != SD_OK) return rc;
     // the kernel with the longer CTAs first: the other's fill the SMs that its last ones leave
-    dkv<<<static_cast<unsigned>(slots * a.Hkv), pt::kBwdThreads, smem, s>>>(a, mq, mg, mk, mv, top, err);
+    dkv<<<static_cast<unsigned>(slots * a.Hkv), pt::kBwdThreads, smem, s>>>(a, mq, mg, mk, mv, err);
     rc = check_launch();
     if (rc != SD_OK) return rc;
     return launch(dq, dim3(static_cast<unsigned>(slots * a.Hq)), dim3(pt::kBwdThreads), smem, s, true, a, mq, mg, mk,

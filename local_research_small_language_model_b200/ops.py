@@ -822,7 +822,7 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     dv = q.new_empty((total, hkv, d))
     if total:
         q, k, v, out, dout = _rows16(q), _rows16(k), _rows16(v), _rows16(out), _rows16(dout)
-        delta = lse.new_empty(hq * total + 1)
+        delta = lse.new_empty(hq * total)
         _launch("sd_packed_attention_backward", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                 dout.data_ptr(), code, total, hq, hkv, d, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
                 *out.stride()[:2], *dout.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, sc, lse.data_ptr(),
