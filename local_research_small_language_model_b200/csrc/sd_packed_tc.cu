@@ -584,12 +584,6 @@ __device__ __forceinline__ float range_scale(float bound) {
 constexpr int kComputeThreads = 512;
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
-// The power of two that takes x into [1/2, 1) (1 for 0).
-__device__ __forceinline__ float unit_scale(float x) {
-  const int e = static_cast<int>(__float_as_uint(x) >> 23) - 126;
-  return x > 0.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 1.f;
-}
-
 // The MMA warp's loop, the same for both kernels: the products of block i + 1
 // as soon as block i's are read, then the accumulation of block i once its
 // weights are there.  Blocks come in runs of per_head, each over
@@ -661,19 +655,6 @@ template <typename T> __device__ __forceinline__ void store_weights(uint32_t tad
   tmem_st16(taddr, w);
 }
 
-// The largest magnitude of eight values; a NaN counts as an infinity.
-template <typename T> __device__ __forceinline__ float largest8(const T *p) {
-  const uint4 x = *reinterpret_cast<const uint4 *>(p);
-  const T *v = reinterpret_cast<const T *>(&x);
-  float big = 0.f;
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const float y = fabsf(to_f(v[u]));
-    big = y <= big ? big : (y < INFINITY ? y : INFINITY);
-  }
-  return big;
-}
-
 }  // namespace pt
 
 // delta = rowsum(dout out), eight lanes a row and head.  A kernel of its own, so
@@ -728,7 +709,6 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   }
   extern __shared__ __align__(1024) char smem_raw[];
   char *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float *most = reinterpret_cast<float *>(sm + BwdSmem::kTop);
   BwdBars *bars = reinterpret_cast<BwdBars *>(sm + BwdSmem::kBar);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = h / (a.Hq / a.Hkv);
@@ -737,21 +717,11 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (tid == 32 * kBwdCopy) bwd_init(bars);
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  if (kHalf && warp < 16) {  // the rows' largest |dout|: eight lanes a row, eight rows a warp
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = 8 * warp + 4 * i + (lane >> 3), c = 8 * (lane & 7);
-      float big = 0.f;
-      if (row < rows) big = largest8(static_cast<const T *>(a.dout) + (first + row) * a.g_st + h * a.g_sh + c);
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-      if ((lane & 7) == 0) most[row] = big < INFINITY ? big : 0.f;
-    }
-  }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = bars->tmem;
+  float f = 1.f;  // of this thread's query
   bool ok = true;
   if (warp == kBwdCopy) {
     if (lane == 0)
@@ -772,7 +742,37 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
     const uint32_t t_s = tmem + lane_base + kColS + 32 * wg;
     const float delta = r < rows ? a.delta[h * a.total + first + r] : 0.f;
     const float lse = r < rows ? a.lse[h * a.total + first + r] : 0.f;
-    const float f = kHalf ? unit_scale(most[r]) : 1.f;
+    if (kHalf) {
+      // largest |dout| of each query; |v| of each key of the tile's own rows, and of all before them
+      unsigned *grads = reinterpret_cast<unsigned *>(sm + BwdSmem::kTop), *vals = grads + kRows, *vals_on = vals + kRows;
+      const int part = lane >> 3, c = 8 * (lane & 7);
+      const T *v = static_cast<const T *>(a.v) + t.start * a.v_st + hk * a.v_sh + c;
+      const T *g = static_cast<const T *>(a.dout) + first * a.g_st + h * a.g_sh + c;
+      auto row_top = [&](const T *p) { return top2(*reinterpret_cast<const uint4 *>(p)); };
+      for (int row = 4 * warp + part; row < kRows; row += 64) {
+        unsigned both = 0;
+        if (row < rows) both = top1(row_top(v + (t.row0 + row) * a.v_st)) << 16 | top1(row_top(g + row * a.g_st));
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+        if ((lane & 7) == 0) vals[row] = both >> 16, grads[row] = both & 0xffffu;
+      }
+      unsigned on = 0;
+#pragma unroll 8
+      for (int row = 4 * warp + part; row < t.row0; row += 64) on = __vmaxu2(on, row_top(v + row * a.v_st));
+      on = __reduce_max_sync(0xffffffffu, top1(on));
+      if (lane == 0) vals_on[warp] = on;
+      compute_sync();
+      // over the keys up to this thread's query: the query's 32 rows by a scan, those before them whole
+      unsigned top_v = vals_on[lane & 15], own_v = vals[r];
+      for (int w = 0; w < (warp & 3); ++w) top_v = max(top_v, vals[32 * w + lane]);
+      top_v = __reduce_max_sync(0xffffffffu, top_v);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, own_v, o);
+        if (lane >= o) own_v = max(own_v, x);
+      }
+      f = range_scale(64.f * top_value(grads[r]) * top_value(max(top_v, own_v)) + fminf(fabsf(delta), 3.0e38f));
+    }
     for (int i = 0; i < blocks; ++i) {
       ok = mbar_wait(&bars->sd_full, i & 1);
       if (__any_sync(0xffffffffu, !ok)) break;
@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (failed) bwd_failed(bars, err);
   if (warp < 4) {
     fence_after_sync();
-    const float back = failed ? __int_as_float(0x7fc00000) : a.scale / (kHalf ? unit_scale(most[r]) : 1.f);
+    const float back = failed ? __int_as_float(0x7fc00000) : a.scale / f;
     store_rows(dq + 32 * warp * c_st, c_st, rows - 32 * warp, tmem + lane_base + kDqAcc, back,
                sm + BwdSmem::kRowsA + warp * 4096);
   }

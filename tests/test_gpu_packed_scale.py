@@ -116,3 +116,26 @@ def test_a_key_depends_on_what_sees_it(dev, dtype):
         got = run(q, k, v, dout, cu)
         val, err = exact(q, k, v, dout, causal_step=True)
         check_all(got, val, err, what)
+
+
+@pytest.mark.parametrize("size", [4000.0, 30000.0])
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+def test_large_values(dev, dtype, size):
+    """Values of v in the thousands, in one head of one size with a sign a token
+    (so that dout.v adds up over the columns and differs between the tokens):
+    dS passes 65504 unless its scale takes v into account."""
+    lengths = [200, 330]
+    cu = bounds(lengths)
+    q, k, v, dout = inputs(dev, dtype, 530, 6, 2, seed=43)
+    v = (v.float().clamp(-2, 2) * size).to(dtype)
+    v[:, 1] = torch.where(v[:, 1, :1] > 0, size, -size).to(dtype)
+    dout = (dout.float().clamp(-3, 3) / 4).to(dtype)
+    dout[:, 3:] = 0.75
+    # queries and keys so small that the gradients stay in fp16's range
+    k = (k.float() / 64).to(dtype)
+    q = (q.float() / 64).to(dtype)
+    got = run(q, k, v, dout, torch.tensor(cu, dtype=torch.int32, device=dev))
+    for a, b in zip(cu, cu[1:]):
+        val, err = exact(*(x[a:b] for x in (q, k, v, dout)))
+        assert max(float(x.abs().max()) for x in val.values()) <= 60000.0
+        check_all([x[a:b] for x in got], val, err, f"rows {a}")
