@@ -55,7 +55,14 @@ def error_buffer(device) -> torch.Tensor:
     key = device.index if device.index is not None else torch.cuda.current_device()
     buf = _err_bufs.get(key)
     if buf is None:
-        buf = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+        where = torch.device("cuda", key)
+        if torch.cuda.is_current_stream_capturing():
+            # zeroed now, on a stream that is not captured, and not by every replay
+            buf = torch.empty(1, dtype=torch.int32, device=where)
+            with torch.cuda.stream(torch.cuda.Stream(where)):
+                buf.zero_()
+        else:
+            buf = torch.zeros(1, dtype=torch.int32, device=where)
         _err_bufs[key] = buf
     return buf
 
