@@ -68,13 +68,15 @@ def error_buffer(device) -> torch.Tensor:
 
 
 def check_device_errors(device=None) -> None:
-    """Synchronises and raises if any kernel reported a device-side timeout."""
+    """Synchronises and raises if any kernel reported a device-side timeout, or
+    an index, length or page out of range."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     buf = error_buffer(device)
     if int(buf.item()) != 0:
         code = int(buf.item())
         buf.zero_()
-        raise L.SparDAError(f"a kernel gave up a bounded wait (device error code {code})")
+        what = "met an index, length or page out of range" if code == L.SD_KERR_BOUNDS else "gave up a bounded wait"
+        raise L.SparDAError(f"a kernel {what} (device error code {code})")
 
 
 def num_blocks(t: int, bs: int) -> int:

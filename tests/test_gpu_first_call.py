@@ -42,3 +42,14 @@ print("fine")
 def test_first_call_in_a_capture(dev):
     done = subprocess.run([sys.executable, "-c", PROGRAM], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
+
+
+def test_reports_say_what_happened(dev):
+    import torch
+
+    import local_research_small_language_model_b200 as sd
+    from local_research_small_language_model_b200 import ops
+
+    sd.token_logprobs(torch.zeros(2, 9, device=dev), torch.full((2,), 9, dtype=torch.int64, device=dev))
+    with pytest.raises(sd.SparDAError, match="out of range .device error code 2"):
+        ops.check_device_errors(dev)
