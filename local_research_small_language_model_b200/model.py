@@ -416,6 +416,11 @@ class SparDAB200Model(nn.Module):
             raise ValueError(f"packed sequences are one row of tokens, got {b}")
         else:
             counts = lengths
+            if counts is not None:
+                counts = [int(n) for n in counts]
+                if len(counts) != cu_seqlens.numel() - 1 or min(counts) < 0 or sum(counts) > t:
+                    raise ValueError(f"lengths must be those of the {cu_seqlens.numel() - 1} sequences in {t} "
+                                     f"tokens, got {counts}")
         if pages is not None:
             if counts is None or sum(counts) != b * t:
                 raise ValueError("packed prompts into a cache need their lengths on the host too, "
@@ -431,9 +436,10 @@ class SparDAB200Model(nn.Module):
                 cu_seqlens: Optional[torch.Tensor] = None,
                 lengths: Optional[List[int]] = None) -> Dict[str, torch.Tensor]:
         """``cu_seqlens`` (device int32, "b200_dense" backend): input_ids
-        [1,total] holds sequences packed back to back; with paged caches also
-        their ``lengths`` as host numbers, one a sequence of the cache (0 for
-        those that go on: prompts may take the place of released ones)."""
+        [1,total] holds sequences packed back to back, ``lengths`` (optional)
+        the same as host numbers; needed with paged caches, one a sequence of the
+        cache (0 for those that go on: prompts may take the place of released
+        ones)."""
         b, t = input_ids.shape
         if self.config.attention_backend == "b200_dense":
             return self._forward_dense(input_ids, targets, kv_caches, return_forecasts, cu_seqlens, lengths)

@@ -100,3 +100,20 @@ def test_forecasts_are_returned_where_they_are_asked_for(on_cpu, grad):
     for f, x, layer in zip(got["forecasts"], inputs, m.layers):
         assert torch.equal(f, layer.forecast(x)) and f.requires_grad == grad
     assert "forecasts" not in m(ids)
+
+
+def test_lengths_have_to_be_those_of_the_bounds(on_cpu):
+    """They bound the tokens' positions: wrong ones would rotate tokens wrongly."""
+    m = model.SparDAB200Model(sd.ModelConfig(**CONFIG)).eval()
+    ids = torch.randint(0, 50, (1, 12))
+    cu = torch.tensor([0, 8, 11], dtype=torch.int32)
+    with torch.no_grad():
+        want = m(ids, cu_seqlens=cu)["logits"]
+        assert torch.equal(m(ids, cu_seqlens=cu, lengths=[8, 3])["logits"], want)
+        for wrong in ([3], [8, 3, 1], [9, 4], [-1, 3], []):
+            with pytest.raises(ValueError, match="lengths"):
+                m(ids, cu_seqlens=cu, lengths=wrong)
+        caches = m.allocate_paged_caches(3, 64)
+        with pytest.raises(ValueError, match="lengths"):
+            m(ids, kv_caches=caches, cu_seqlens=cu, lengths=[8, 4, 0])
+        assert not any(caches[0].pages.owned)  # nothing was reserved
