@@ -421,6 +421,8 @@ class B200DenseAttention(BaseAttention):
             else:
                 bounds = torch.arange(0, (b + 1) * t, t, dtype=torch.int32, device=xq.device)
                 ragged = RaggedBatch.prompts(bounds, b * t, rotary_emb, t, [t] * b)
+        if not step and ragged.cu_seqlens is None:
+            raise ValueError("a decode step needs a paged cache and one token per sequence")
         if not step and b != 1 and ragged.cu_seqlens.numel() != b + 1:
             raise ValueError(f"{ragged.cu_seqlens.numel() - 1} packed sequences do not fit {b} rows of {t} tokens")
         rope = _RopeQK.apply if grad else ops.rope_qk

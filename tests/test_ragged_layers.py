@@ -117,3 +117,11 @@ def test_lengths_have_to_be_those_of_the_bounds(on_cpu):
         with pytest.raises(ValueError, match="lengths"):
             m(ids, kv_caches=caches, cu_seqlens=cu, lengths=[8, 4, 0])
         assert not any(caches[0].pages.owned)  # nothing was reserved
+
+
+def test_a_step_without_a_cache_is_refused(on_cpu):
+    layer = sd.B200DenseAttention(sd.ModelConfig(**CONFIG), 0)
+    rope = sd.RotaryEmbedding(64, 64)
+    step = sd.RaggedBatch.step(torch.tensor([3, 4], dtype=torch.int32), 64, rope)
+    with torch.no_grad(), pytest.raises(ValueError, match="paged cache"):
+        layer(torch.randn(2, 1, 128), rope, ragged=step)
