@@ -6,7 +6,6 @@
 #include <mutex>
 #include <type_traits>
 #include <utility>
-#include <vector>
 
 #include "sd_common.cuh"
 
@@ -49,7 +48,8 @@ int ensure_smem_raw(const void *func, size_t bytes) {
     size_t bytes;
   };
   static std::mutex lock;
-  static std::vector<Limit> limits;
+  static Limit limits[1024];  // no allocation: nothing may be thrown through a C entry point
+  static int known = 0;
   int device = 0;
   const cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) {
@@ -58,16 +58,17 @@ int ensure_smem_raw(const void *func, size_t bytes) {
     return SD_ERR_CUDA;
   }
   std::lock_guard<std::mutex> hold(lock);
-  for (Limit &l : limits)
-    if (l.func == func && l.device == device) {
-      if (l.bytes >= bytes) return SD_OK;
-      const int rc = set_max_smem_raw(func, bytes);
-      if (rc == SD_OK) l.bytes = bytes;
-      return rc;
-    }
+  Limit *at = nullptr;
+  for (int i = 0; i < known && !at; ++i)
+    if (limits[i].func == func && limits[i].device == device) at = &limits[i];
+  if (at && at->bytes >= bytes) return SD_OK;
   const int rc = set_max_smem_raw(func, bytes);
-  if (rc == SD_OK) limits.push_back({func, device, bytes});
-  return rc;
+  if (rc != SD_OK) return rc;
+  if (at)
+    at->bytes = bytes;
+  else if (known < static_cast<int>(sizeof(limits) / sizeof(limits[0])))
+    limits[known++] = {func, device, bytes};
+  return SD_OK;
 }
 
 __global__ void advance_len_kernel(int32_t *lens, int n, int delta) {
