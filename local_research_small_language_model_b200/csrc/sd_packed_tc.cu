@@ -869,6 +869,8 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
   float f = 1.f;  // of this thread's key
+  // fp16: P, at most 1, is held as 2^15 P, so that keys with little weight keep the digits of dV
+  constexpr float kWeight = kHalf ? 15.f : 0.f, kUnweight = kHalf ? 1.f / 32768.f : 1.f;
   bool ok = true;
   if (warp == kBwdCopy) {
     if (lane == 0)
@@ -958,9 +960,10 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
       }
       f = range_scale(64.f * top_value(max(top_g, own_g)) * top_value(vals[r]) + __uint_as_float(max(top_d, own_d)));
     }
+    const float fw = f * kUnweight;  // dP - delta's share: dS = (2^15 P) (fw (dP - delta))
     for (int i = 0; i < blocks; ++i) {
       __syncwarp();
-      mine[lane] = -next_l;
+      mine[lane] = kWeight - next_l;
       mine[32 + lane] = -next_d;
       const bool nan = __any_sync(0xffffffffu, next_l != next_l);
       __syncwarp();
@@ -995,8 +998,8 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
             else
               s[u + 2] = ex2(s[u + 2]), s[u + 3] = ex2(s[u + 3]);
             if (kHalf) {
-              mul2(d[u], d[u + 1], f, f);
-              mul2(d[u + 2], d[u + 3], f, f);
+              mul2(d[u], d[u + 1], fw, fw);
+              mul2(d[u + 2], d[u + 3], fw, fw);
             }
             mul2(d[u], d[u + 1], s[u], s[u + 1]);
             mul2(d[u + 2], d[u + 3], s[u + 2], s[u + 3]);
@@ -1036,7 +1039,7 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
   if (failed) bwd_failed(bars, err);
   if (warp < 8) {
     fence_after_sync();
-    const float back = failed ? __int_as_float(0x7fc00000) : wg == 0 ? 1.f : a.scale / f;  // f: of row r for every wg
+    const float back = failed ? __int_as_float(0x7fc00000) : wg == 0 ? kUnweight : a.scale / f;
     const int row0 = 32 * (warp & 3);
     store_rows((wg == 0 ? dv : dk) + row0 * c_st, c_st, keys - row0,
                tmem + lane_base + (wg == 0 ? kDkvAcc : kDkvAcc2), back, sm + BwdSmem::kRowsA + warp * 4096);

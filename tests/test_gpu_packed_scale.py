@@ -22,9 +22,10 @@ from tests.test_gpu_packed import DTYPES, U, U32, bounds, check, inputs, run
 pytestmark = pytest.mark.gpu
 
 
-def exact(q, k, v, dout, scale=0.125, causal_step=False):
+def exact(q, k, v, dout, scale=0.125, causal_step=False, tiny_p=None):
     """(out, dq, dk, dv) of one sequence and their bounds.  causal_step: the
-    sum above over the pairs that a row sees, not over the whole sequence."""
+    sum above over the pairs that a row sees, not over the whole sequence.
+    tiny_p: fp16's least step of P in dV (2^-24 unless given)."""
     dtype, u = q.dtype, U[q.dtype]
     half = dtype == torch.float16
     tiny = 2.0 ** -24 if half else 0.0
@@ -58,7 +59,7 @@ def exact(q, k, v, dout, scale=0.125, causal_step=False):
             mk = ((seen_g * big_v + seen_gv) / 2)[None, :]
         else:
             mq = mk = (heads[:, j].max() * big_v.max()).expand(1, 1)
-        ep = (u + eps) * p + (tiny + 2.0 ** -126) * ~late
+        ep = (u + eps) * p + ((tiny if tiny_p is None else tiny_p) + 2.0 ** -126) * ~late
         val["dq"][:, h] = ds @ kh * scale
         err["dq"][:, h] = scale * ((eds + step * mq * ~late + n * U32 * ds.abs()) @ kh.abs())
         val["dk"][:, j] += ds.t() @ qh * scale
@@ -139,3 +140,20 @@ def test_large_values(dev, dtype, size):
         val, err = exact(*(x[a:b] for x in (q, k, v, dout)))
         assert max(float(x.abs().max()) for x in val.values()) <= 60000.0
         check_all([x[a:b] for x in got], val, err, f"rows {a}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+def test_keys_that_get_little_weight(dev, dtype):
+    """Keys whose every weight is far below fp16's smallest normal number, 2^-14:
+    their dV keeps its digits.  fp16 holds P scaled by 2^15, so a rounding is off
+    by half a step relative, or by 2^-40 at the least."""
+    n = 400
+    q, k, v, dout = inputs(dev, dtype, n, 4, 2, seed=44, scale_out=512.0)
+    q, k = q.clone(), k.clone()
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    few = torch.arange(n, device=dev) % 3 == 1
+    k[few, :, 0] = -12.0  # scores lower by 12: e^-12 / n
+    got = run(q, k, v, dout, torch.tensor([0, n], dtype=torch.int32, device=dev))
+    val, err = exact(q, k, v, dout, tiny_p=2.0 ** -40 if dtype == torch.float16 else 0.0)
+    check_all(got, val, err, "little weight")
+    assert float(val["dv"][few].abs().max()) < 0.1 < float(val["dv"].abs().max())  # the case is what it says
