@@ -114,6 +114,16 @@ template <> __device__ __forceinline__ __half from_f<__half>(float x) { return _
 // Round a float to T's precision and back (identity for float).
 template <typename T> __device__ __forceinline__ float round_to(float x) { return to_f<T>(from_f<T>(x)); }
 
+// 2^x with the SFU's approximate base-2 exponential (one instruction;
+// 2^-inf = +0, so masked keys need no select): the attention and scoring kernels
+// are bound by instruction issue or by this unit, so the cheapest form per element
+// wins.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // One rotated element with the reference's rounding sequence
 // (model/rope.py:58-63): the fp32 tables cast to T, then x*cos and
 // rotate_half(x)*sin and their sum each rounded to T.  rot is the element of

@@ -36,11 +36,6 @@ constexpr int kCandidates = kAbove + kTies;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e4f;         // stands for what is below it: its exponential is 0 and 0 * kFloor is 0
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // max that keeps a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;

@@ -171,12 +171,6 @@ __device__ __forceinline__ int page_of(int t, int page, uint32_t inv) {
   return t - p * page >= page ? p + 1 : p;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // What a part with maximum m weighs under the common maximum.
 __device__ __forceinline__ float factor(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
 
@@ -726,8 +720,9 @@ int sd_paged_decode_attention(const void *q, int dtype, int64_t B, int64_t Hq, i
       const size_t smem = pg::kWarps * pg::kStages * (pg::kWarpBytes + 16) + pg::kWarps * d.G * pg::kPart * 4 +
                           (sizeof(T) == 4 ? d.G * 256 : 0) + (2 * a.B + 1) * 4;
       const bool whole = page % (pg::kUnit<T> / pg::kWarps) == 0, wide = sizeof(T) == 2 && d.G > 8;
-      auto kern = whole ? wide ? paged_decode_kernel<T, true, true> : paged_decode_kernel<T, true, false>
-                  : wide ? paged_decode_kernel<T, false, true>
+      constexpr bool k16 = sizeof(T) == 2;  // fp32 has no wide form
+      auto kern = whole ? wide ? paged_decode_kernel<T, true, k16> : paged_decode_kernel<T, true, false>
+                  : wide ? paged_decode_kernel<T, false, k16>
                          : paged_decode_kernel<T, false, false>;
       if (ensure_smem(kern, smem) != SD_OK) return SD_ERR_CUDA;
       kern<<<ctas, pg::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a, d);

@@ -17,11 +17,10 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr, uint32_t lbo
 }
 
 // Instruction descriptor, kind::f16: fp32 accumulator, A/B 16-bit format
-// (0 = f16, 1 = bf16), A and B K-major or MN-major, M = 128, N = 64 unless given.
-__host__ __device__ constexpr uint32_t idesc_f16(uint32_t fmt, bool b_mn_major, uint32_t n = 64u,
-                                                 bool a_mn_major = false) {
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
-         ((n >> 3) << 17) | ((128u >> 4) << 24);
+// (0 = f16, 1 = bf16), A K-major, B K-major or MN-major, M = 128, N = 64 unless given.
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t fmt, bool b_mn_major, uint32_t n = 64u) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) |
+         ((128u >> 4) << 24);
 }
 
 __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -74,15 +73,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
       : "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// 2^x with the SFU's approximate base-2 exponential (one instruction;
-// 2^-inf = +0, so masked keys need no select): the attention kernels are bound
-// by instruction issue or by this unit, so the cheapest form per element wins.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
