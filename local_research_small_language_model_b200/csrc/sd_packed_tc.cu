@@ -792,8 +792,10 @@ __global__ void __launch_bounds__(pt::kBwdThreads, 1)
             exp2_fma<false>(s[u], s[u + 1]);
           else
             s[u] = ex2(s[u]), s[u + 1] = ex2(s[u + 1]);
-          add2(d[u], d[u + 1], -delta, -delta);
-          if (kHalf) mul2(d[u], d[u + 1], f, f);
+          if (kHalf)
+            fma2(d[u], d[u + 1], f, -delta * f);
+          else
+            add2(d[u], d[u + 1], -delta, -delta);
           mul2(d[u], d[u + 1], s[u], s[u + 1]);
         }
       };
