@@ -433,7 +433,9 @@ SD_API int sd_packed_attention(const void *q, const void *k, const void *v, int 
  * over the query heads of their kv head; zeros outside every sequence).  out,
  * lse and rest (nullable: dq and dk are then a little less exact) are the
  * forward's.  delta: workspace of this call, fp32 [Hq,total].
- * Sums have a fixed order: equal inputs give equal bits. */
+ * Sums have a fixed order: equal inputs give equal bits.  A NaN or an infinity
+ * may show in the gradients of its own sequence's 128 rows around it (64 in
+ * fp32), also where the formula's are finite; never in another sequence's. */
 SD_API int sd_packed_attention_backward(const void *q, const void *k, const void *v, const void *out,
                                         const void *dout, int dtype, int64_t total, int64_t Hq, int64_t Hkv,
                                         int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,

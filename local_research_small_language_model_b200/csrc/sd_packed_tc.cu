@@ -11,9 +11,10 @@
 //   O_x += P_x V     4 MMAs, A from tensor memory
 // Warp 8 issues all MMAs, warp 9 all copies (K and V in a ring of 4 stages).
 // The four tiles of an SM take turns: while one's products run, the others
-// compute exponentials, which are the bound (64 a row and block at 16 a cycle
-// and SM; the products need 320 of those 512 cycles).  S_x(i + 1) is issued right
-// behind O_x(i), so its arrival also says that O_x(i) is done.
+// compute exponentials (64 a row and block: at 16 a cycle and SM 512 cycles, 384
+// with the quarter of them that is computed elsewhere; the products need 320).
+// S_x(i + 1) is issued right behind O_x(i), so its arrival also says that O_x(i)
+// is done.
 // A row's reference m is its first block's maximum, and stays while a block's
 // weights sum to at most 2^14 (16-bit weights and fp32 sums have the same
 // relative precision there), so the common path looks for no maximum: the sum,
@@ -35,20 +36,26 @@
 // S and dP are computed in both (7 products and 2 exponentials a pair instead
 // of 5 and 1): in return every gradient is summed in tensor memory in a fixed
 // order, with no atomics and no fp32 buffer to add into and convert.
+// P and dS are rounded to 16 bits, as P is in the forward: the products that take
+// them have 16-bit operands, and splitting them in two would double four products.
 // A small kernel ahead of them computes delta, so that neither needs the other:
 // dK/dV, whose CTAs are longer, goes first, and dQ's CTAs take the SMs that its
 // last ones leave (one after the other: 457 instead of 416 us at 8192 tokens, 100
 // instead of 78 at 2048).
 //
 // Measured, 12 query and 4 key-value heads, bf16.  One sequence of 32768 tokens:
-// forward 1.74 ms (945 TFLOP/s; 1.00 ms of products, 1.43 ms of exponentials if
-// all ran on the special-function units), backward 5.9 ms (700 TFLOP/s of the 5
-// products a gradient needs, 985 of the 7 it computes).  Training on 16000 tokens
-// in 9 sequences: 0.41 ms, forward and backward.  Of one 8192-token sequence's
-// cycles the forward keeps the special-function units busy for 56 %, instruction
-// issue for 56 % and the tensor pipe for 37 %, dQ 42, 55 and 41 %, dK/dV 38, 62
-// and 50 %: the backward's bound is issue, and its warps' waits for one another
-// between the phases of a block.
+// forward 1.74 ms as the best of five runs of ten (945 TFLOP/s), 2.0 ms called for
+// longer, under the power cap (820); 1.00 ms of products, 1.07 ms of exponentials
+// on the special-function units (1.43 if all were there).  Backward 5.9 ms (700
+// TFLOP/s of the 5 products a gradient needs, 985 of the 7 it computes).  Training
+// on 16000 tokens in 9 sequences: 0.40 to 0.45 ms, forward and backward (f16 0.46).
+// Of a sequence's cycles the forward keeps the special-function units, instruction
+// issue and the tensor pipe busy for 67, 65 and 44 % at 32768 tokens, 57, 57 and
+// 36 % at 8192, 31, 34 and 18 % at 2048: no unit is its bound, but the chain of a
+// block's steps, and in short batches the longest tiles.  dQ at 8192: 44, 55 and
+// 43 %, dK/dV 38, 62 and 50 %: issue, and its warps' waits for one another between
+// the phases of a block.  f16's look at the other side's rows costs a tenth of its
+// backward there (435 us; 362 in bf16).  The forward spills 32 bytes a thread.
 #include <type_traits>
 
 #include "sd_packed.cuh"
@@ -385,7 +392,8 @@ __global__ void __launch_bounds__(pt::kFwdThreads, 2)
           for (int e = 0; e < 8; ++e) {
             float y0 = s[2 * e], y1 = s[2 * e + 1];
             fma2(y0, y1, c, neg);
-            // every fourth pair's exponentials on the FMA pipe: the special-function unit is the bound
+            // every fourth pair's exponentials on the FMA pipe: the special-function unit is the busiest (1.90 -> 1.82
+            // ms at 32768 tokens)
             if (kPoly && (e & 3) == 3)
               exp2_fma<true>(y0, y1);
             else

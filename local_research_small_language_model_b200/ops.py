@@ -814,7 +814,9 @@ def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv, contiguous, in q's dtype) of packed_attention for
     the output gradient dout; out, lse and rest (optional) are the forward's
-    (sd_packed_attention_backward).  Equal inputs give equal bits."""
+    (sd_packed_attention_backward).  Equal inputs give equal bits.  A NaN or an
+    infinity may show in all gradients of its own sequence's 128-row block (64
+    rows in fp32)."""
     _check_packed(q, k, v, cu_seqlens)
     _check_like_q(q, out=out, dout=dout, rest=rest)
     _check_rest(rest)
