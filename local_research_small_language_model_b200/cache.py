@@ -211,6 +211,10 @@ class B200PagedKVCache:
         """Writes rows xk, xv [N,H,D] behind the cached tokens of their
         sequences (one row each, or packed by cu_seqlens; ``lens`` in place of
         the PageTable's, ops.LEN_ABSENT for a sequence whose row is not
-        written); lengths are advanced on the PageTable, once for all layers."""
-        ops.paged_append(xk.to(self.k_pages.dtype), xv.to(self.v_pages.dtype), self.k_pages, self.v_pages,
-                         self.pages.table, self.pages.lens if lens is None else lens, cu_seqlens)
+        written, as for the released ones without it); lengths are advanced on
+        the PageTable, once for all layers."""
+        pages = self.pages
+        if lens is None:
+            lens = pages.lens + pages.absent if any(pages.released) else pages.lens
+        ops.paged_append(xk.to(self.k_pages.dtype), xv.to(self.v_pages.dtype), self.k_pages, self.v_pages, pages.table,
+                         lens, cu_seqlens)

@@ -111,3 +111,20 @@ def test_steps_after_a_release_and_a_prompt_in_its_place(paged):
     for _ in range(2):
         step()
     assert pages.held == [21, 22, 10] == pages.lens.tolist()
+
+
+def test_append_leaves_released_sequences_out(paged):
+    """A step's rows written by hand, without the model."""
+    t = sd.PageTable(3, 64, 6, torch.device("cpu"), page_size=16)
+    cache = sd.B200PagedKVCache(t, 1, 64, torch.device("cpu"), torch.float32)
+    t.reserve([3, 4, 5])
+    t.advance([3, 4, 5])
+    t.release(1)
+    t.reserve(1)
+    x = torch.randn(3, 1, 64)
+    cache.append(x, x)
+    t.advance(1)
+    assert t.lens.tolist() == [4, 0, 6]
+    want = torch.zeros_like(cache.k_pages)
+    want[t.owned[0][0], :, 3], want[t.owned[2][0], :, 5] = x[0], x[2]
+    assert torch.equal(cache.k_pages, want)
