@@ -1,6 +1,7 @@
 """The first call of a process made inside a graph capture: the word in which
 kernels report errors belongs to the library, not to the graph.  Needs a B200."""
 
+import os
 import subprocess
 import sys
 
@@ -40,7 +41,8 @@ print("fine")
 
 
 def test_first_call_in_a_capture(dev):
-    done = subprocess.run([sys.executable, "-c", PROGRAM], capture_output=True, text=True, timeout=300)
+    done = subprocess.run([sys.executable, "-c", PROGRAM], capture_output=True, text=True, timeout=300,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
 
 
